@@ -21,6 +21,10 @@
  *   xs_keep_confident           keep_confident                 src/generate.rs:3898-3905
  *   xs_select_option            select_option                  src/batch.rs:1545-1588
  *
+ * Beside them stands a speculative step whose drafts are a tree of tokens over
+ * a bounded cache (no counterpart in the reference, which verifies one chain):
+ * xs_tree_attend, xs_verify_tree, xs_cache_commit and xs_cache_evict.
+ *
  * Randomness: the reference draws from a seeded StdRng inside the sampler.  Here
  * the caller supplies one uniform per sampled row, u = j * 2^-23 with j in
  * [0, 2^23) -- exactly the f32 rand 0.9's UniformFloat derives from 23 random
@@ -65,7 +69,9 @@ extern "C" {
  *                      otherwise hands sub-records off through memory, so
  *                      this is not seen in practice; xs_test_xcd forces it
  *   XS_ROW_ID_OOR      a scored id (score_ids) outside the encodable ids
- *                      (last_logprobs_for, generate.rs:1874-1879)           */
+ *                      (last_logprobs_for, generate.rs:1874-1879)
+ *   XS_ROW_CACHE_FULL  a sequence's cache has no room for its accepted path
+ *                      (xs_cache_commit; no reference counterpart)          */
 #define XS_ROW_OK 0
 #define XS_ROW_NAN 1
 #define XS_ROW_NO_FINITE 2
@@ -76,6 +82,7 @@ extern "C" {
 #define XS_ROW_BAD_PARAM 7
 #define XS_ROW_INTERNAL 8
 #define XS_ROW_ID_OOR 9
+#define XS_ROW_CACHE_FULL 10
 
 /* Largest top_k the streaming selection serves (it keeps top_k + 1 entries).
  * A context created with k_max above it serves every top_k up to k_max --
@@ -321,6 +328,214 @@ typedef struct {
 } xs_verify_args;
 
 int xs_verify(xs_context* ctx, const xs_verify_args* args);
+
+/* ---------------------------------------------------------------------------
+ * A tree of drafted tokens: the speculative step whose drafts branch.
+ *
+ * A sequence's tree has up to XS_TREE_MAX nodes.  Node 0 is the last committed
+ * token (its keys and values are not in the cache yet), the others are drafts;
+ * parent[i] < i is the node that node i follows.  One step is
+ *
+ *   xs_tree_attend    per layer: the nodes attend to the cache and to their
+ *                     own ancestors
+ *   xs_verify_tree    once: every node's row of logits is sampled, and the
+ *                     walk goes down the tree while the sampled token is a
+ *                     drafted child
+ *   xs_cache_commit   per layer: the accepted nodes' keys and values are
+ *                     appended to the cache, which holds committed tokens only
+ *                     (a rejected branch needs no roll-back), and, if asked,
+ *                     the attention weight they gave to each slot is added up
+ *   xs_cache_evict    per layer, for a cache over its budget: keeps the slots
+ *                     with the most weight
+ *
+ * xs_verify_tree runs on an xs_context, the others on an xs_cache_context. */
+#define XS_TREE_MAX 64
+
+/* xs_verify for trees.  Rows are laid out [seqs, nodes, ld]; row i of a
+ * sequence holds the logits after node i.  Every row is sampled as xs_sample
+ * would, with its own uniform (rows past n_nodes too; nothing reads those).
+ * The walk starts at node 0 and, at each node: stops before it once `budget`
+ * tokens are committed; stops, with the row's status as the sequence's, where
+ * the row failed; commits the row's token; stops after an end-of-generation id
+ * or where the token is the token of no child; else goes on to the child with
+ * that token (the lowest such node; counted as accepted).  A node follows
+ * parent[i] where parent[i] < i; any other value (the root's own is -1) leaves
+ * it out of the walk.  For a chain (parent[i] = i - 1, tokens[i] =
+ * drafts[i - 1]) this is xs_verify. */
+typedef struct {
+  const float* logits;   /* [seqs * nodes, ld] */
+  int64_t seqs;
+  int64_t nodes;         /* rows per sequence, 1..XS_TREE_MAX */
+  int64_t ld, width, enc;
+  const xs_row_params* params;  /* [seqs * nodes] */
+  const float* uniforms;        /* [seqs * nodes] */
+  const uint32_t* allowed;      /* [seqs * nodes, allowed_ld] or NULL (per-node masks) */
+  int64_t allowed_words, allowed_ld;
+  const int32_t* tokens;        /* [seqs, nodes] each node's token (node 0's is not read) */
+  const int32_t* parent;        /* [seqs, nodes] */
+  const int32_t* n_nodes;       /* [seqs] nodes of each tree (0: nothing is committed), or NULL for
+                                   `nodes`; outside [0, nodes] is XS_ROW_BAD_PARAM */
+  const int32_t* budget;        /* [seqs] max committed tokens, or NULL = unbounded */
+  int32_t n_eog;
+  const int32_t* eog;           /* [n_eog] */
+  /* outputs */
+  int32_t* row_token;    /* [seqs * nodes] every row's sampled id */
+  int32_t* row_status;   /* [seqs * nodes] */
+  int32_t* accepted;     /* [seqs] drafted children that were sampled */
+  int32_t* path;         /* [seqs, nodes] the nodes whose tokens were drawn, root first: n_committed
+                            entries, then -1.  These are the nodes to append to the caches; the last
+                            committed token is the next tree's node 0 */
+  int32_t* committed;    /* [seqs, nodes] committed ids (committed[r] was drawn at path[r]), then -1 */
+  int32_t* n_committed;  /* [seqs] */
+  int32_t* seq_status;   /* [seqs] the first row error the walk reached, else XS_ROW_OK */
+  /* per-node controls [seqs * nodes] as in xs_sample_args, or NULL */
+  const xs_row_control* controls;
+  const uint32_t* ctl_ids;
+  const float* ctl_delta;
+  /* [seqs * nodes] or NULL: nonzero at node j when committing tokens[j]
+   * completes the grammar: the walk counts j as accepted and ends there */
+  const uint8_t* done_after;
+  /* as xs_sample_args.k_max */
+  int32_t k_max;
+} xs_verify_tree_args;
+
+int xs_verify_tree(xs_context* ctx, const xs_verify_tree_args* args);
+
+/* The workspace of the cache calls, sized for the largest call.  Allocates
+ * once; calls allocate nothing afterwards and may be captured.  Owned by one
+ * thread at a time, its calls serialised on its stream, like an xs_context;
+ * graphs captured from one context are not to run at the same time. */
+typedef struct xs_cache_context xs_cache_context;
+typedef struct {
+  int64_t max_seqs;
+  int64_t max_nodes;     /* 1..XS_TREE_MAX */
+  int64_t q_heads, kv_heads, head_dim, capacity;  /* the largest of each */
+} xs_cache_dims;
+int xs_cache_create(int device, const xs_cache_dims* dims, xs_cache_context** out);
+int xs_cache_destroy(xs_cache_context* ctx);
+int xs_cache_set_stream(xs_cache_context* ctx, void* hip_stream);
+
+/* Element types of keys, values and queries. */
+#define XS_BF16 0
+#define XS_F16 1
+
+/* Keys and values of one layer, [seqs, slots, kv_heads, head_dim] in any order
+ * of the first three: head_dim is contiguous, the strides (in elements, shared
+ * by k and v) are multiples of 8, the pointers 16-byte aligned. */
+typedef struct {
+  void* k;
+  void* v;
+  int64_t seq_stride, slot_stride, head_stride;
+} xs_kv;
+
+/* Attention of a tree's nodes.  Node i sees the sequence's cache slots
+ * [0, len) and, of the tree, itself and its ancestors:
+ *   out = sum_j softmax_j(scale q.k_j) v_j,  lse = ln sum_j exp(scale q.k_j)
+ * with q head h reading kv head h / (q_heads / kv_heads).  Sums and softmax
+ * statistics are f32; the weights are rounded to the inputs' type before they
+ * multiply the values, and out once at the end.  nodes = 1 is plain decoding.
+ * parent[i] is -1 (node i follows the cache) or a node below i; any other
+ * value makes i and what follows it see nothing: out 0, lse -inf, as for a
+ * row whose every score is -inf.  A score of NaN or +inf makes its row NaN;
+ * what a node does not see never reaches it, whatever it holds.  Rows past
+ * n_nodes are left as they were, and a sequence whose len is outside
+ * [0, max_len] or n_nodes outside [0, nodes] gets XS_ROW_BAD_PARAM and nothing
+ * else. */
+typedef struct {
+  int32_t dtype;         /* XS_BF16 or XS_F16: q, k, v and out */
+  int32_t head_dim;      /* a multiple of 8, 8..256 */
+  int64_t seqs, nodes;   /* nodes 1..XS_TREE_MAX */
+  int64_t q_heads, kv_heads;  /* q_heads a multiple of kv_heads */
+  const void* q;         /* [seqs, nodes, q_heads, head_dim] by strides like xs_kv's */
+  int64_t q_seq_stride, q_node_stride, q_head_stride;
+  xs_kv cache;
+  int64_t capacity;      /* slots of the cache */
+  int64_t max_len;       /* a bound on every len of this call, or 0 for capacity: sizes the launch */
+  const int32_t* len;    /* [seqs] slots in use */
+  xs_kv fresh;           /* the nodes' own keys and values, [seqs, nodes, kv_heads, head_dim] */
+  const int32_t* parent; /* [seqs, nodes] */
+  const int32_t* n_nodes;  /* [seqs], or NULL for `nodes` */
+  float scale;
+  void* out;             /* [seqs, nodes, q_heads, head_dim] by strides like xs_kv's; not q itself */
+  int64_t out_seq_stride, out_node_stride, out_head_stride;
+  float* lse;            /* [seqs, nodes, q_heads] or NULL */
+  int32_t* seq_status;   /* [seqs] */
+} xs_tree_attend_args;
+
+int xs_tree_attend(xs_cache_context* ctx, const xs_tree_attend_args* args);
+
+/* Appends the accepted nodes: slot len + r takes the keys and values of node
+ * path[r], for r < n_path, and new_len = len + n_path.  Optionally
+ *   positions  pos[kv head][len + r] = next_pos + r, new_next_pos =
+ *              next_pos + n_path (the slots' places in the sequence, which
+ *              eviction moves along);
+ *   weights    new_mass[kv head][s] = mass[s] + sum over the path's nodes and
+ *              the kv head's q heads of exp(scale q.k_s - lse), s < len, and
+ *              the same without mass for the appended slots (which a node sees
+ *              from its own rank on).  q, lse and scale are xs_tree_attend's.
+ * Per-slot arrays are [seqs, kv_heads, slot_ld].  new_mass may be mass.  The
+ * sums are f32, in an order fixed by the sizes.  A sequence whose len is
+ * outside [0, max_len], whose n_path is outside [0, nodes] or whose path holds
+ * a node outside [0, nodes) gets XS_ROW_BAD_PARAM, one without room
+ * XS_ROW_CACHE_FULL; its new_len and new_next_pos are len and next_pos, and
+ * nothing else of it is written. */
+typedef struct {
+  int32_t dtype, head_dim;
+  int64_t seqs, nodes, q_heads, kv_heads;
+  xs_kv cache;
+  int64_t capacity, max_len;  /* as in xs_tree_attend_args */
+  const int32_t* len;    /* [seqs] */
+  xs_kv fresh;
+  const int32_t* path;   /* [seqs, path_ld], xs_verify_tree's */
+  int64_t path_ld;       /* >= nodes */
+  const int32_t* n_path; /* [seqs], xs_verify_tree's n_committed */
+  int32_t* new_len;      /* [seqs], not len itself */
+  int64_t slot_ld;       /* >= capacity */
+  /* positions: all three or none */
+  const int32_t* next_pos;  /* [seqs] */
+  int32_t* pos;
+  int32_t* new_next_pos;    /* [seqs], not next_pos itself */
+  /* weights: all of q, lse, mass and new_mass, or none */
+  const void* q;
+  int64_t q_seq_stride, q_node_stride, q_head_stride;
+  const float* lse;      /* [seqs, nodes, q_heads] */
+  float scale;
+  const float* mass;
+  float* new_mass;
+  int32_t* seq_status;   /* [seqs] */
+} xs_cache_commit_args;
+
+int xs_cache_commit(xs_cache_context* ctx, const xs_cache_commit_args* args);
+
+/* Cuts every sequence of more than `keep` slots to `keep`, each kv head on its
+ * own.  A head keeps first the slots with pos < sinks or pos >= next_pos -
+ * recent, the lowest positions first, then the others by mass, the largest
+ * first (NaN last); ties go to the lower position, then to the lower slot.
+ * The kept slots below `keep` stay where they are, and the i-th free one
+ * among them takes the keys, values, mass and position of the i-th kept slot
+ * at or past `keep` (attention does not depend on the slots' order).  new_len
+ * = min(len, keep).  new_mass and new_pos may be mass and pos, both or
+ * neither; entries past new_len are left as they were.  A sequence whose len is
+ * outside [0, max_len] gets XS_ROW_BAD_PARAM and new_len = len. */
+typedef struct {
+  int32_t dtype, head_dim;
+  int64_t seqs, kv_heads;
+  xs_kv cache;
+  int64_t capacity, max_len;
+  const int32_t* len;    /* [seqs] */
+  const float* mass;     /* [seqs, kv_heads, slot_ld] */
+  float* new_mass;
+  const int32_t* pos;    /* [seqs, kv_heads, slot_ld] */
+  int32_t* new_pos;
+  int64_t slot_ld;       /* >= capacity */
+  const int32_t* next_pos;  /* [seqs] */
+  int64_t keep;          /* >= 1 */
+  int64_t sinks, recent; /* sinks + recent <= keep */
+  int32_t* new_len;      /* [seqs], not len itself */
+  int32_t* seq_status;   /* [seqs] */
+} xs_cache_evict_args;
+
+int xs_cache_evict(xs_cache_context* ctx, const xs_cache_evict_args* args);
 
 /* ---------------------------------------------------------------------------
  * Drafter confidence: argmax_probs_device / draft_argmax_probs

@@ -16,7 +16,7 @@ HEADER = os.path.join(ROOT, "include", "xsamp.h")
 
 XS_OK, XS_ERR_ARG, XS_ERR_HIP, XS_ERR_CAPACITY = 0, -1, -2, -3
 ROW_OK, ROW_NAN, ROW_NO_FINITE, ROW_MASK_SHORT, ROW_FORCE_OOR, ROW_ZERO_WEIGHT, ROW_NARROW, \
-    ROW_BAD_PARAM, ROW_INTERNAL, ROW_ID_OOR = range(10)
+    ROW_BAD_PARAM, ROW_INTERNAL, ROW_ID_OOR, ROW_CACHE_FULL = range(11)
 K_MAX = 127
 SCORE_MAX = 4096
 CLASS_MAX = 8
@@ -26,6 +26,8 @@ ORDER_MAX = 1024
 NOALLOC_ROWS = 64
 NOALLOC_VOCAB = 262144
 NOALLOC_BYTES = 15030784
+TREE_MAX = 64
+BF16, F16 = 0, 1
 
 _vp = C.c_void_p
 _i64 = C.c_int64
@@ -83,6 +85,61 @@ class ArgmaxArgs(C.Structure):
                 ("ids", _vp), ("probs", _vp)]
 
 
+class VerifyTreeArgs(C.Structure):
+    _fields_ = [
+        ("logits", _vp), ("seqs", _i64), ("nodes", _i64), ("ld", _i64), ("width", _i64),
+        ("enc", _i64), ("params", _vp), ("uniforms", _vp),
+        ("allowed", _vp), ("allowed_words", _i64), ("allowed_ld", _i64),
+        ("tokens", _vp), ("parent", _vp), ("n_nodes", _vp), ("budget", _vp), ("n_eog", _i32), ("eog", _vp),
+        ("row_token", _vp), ("row_status", _vp), ("accepted", _vp), ("path", _vp), ("committed", _vp),
+        ("n_committed", _vp), ("seq_status", _vp),
+        ("controls", _vp), ("ctl_ids", _vp), ("ctl_delta", _vp), ("done_after", _vp),
+        ("k_max", _i32),
+    ]
+
+
+class CacheDims(C.Structure):
+    _fields_ = [("max_seqs", _i64), ("max_nodes", _i64), ("q_heads", _i64), ("kv_heads", _i64),
+                ("head_dim", _i64), ("capacity", _i64)]
+
+
+class Kv(C.Structure):
+    """xs_kv: keys and values of one layer and their strides in elements."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("seq_stride", _i64), ("slot_stride", _i64), ("head_stride", _i64)]
+
+
+class TreeAttendArgs(C.Structure):
+    _fields_ = [
+        ("dtype", _i32), ("head_dim", _i32), ("seqs", _i64), ("nodes", _i64), ("q_heads", _i64), ("kv_heads", _i64),
+        ("q", _vp), ("q_seq_stride", _i64), ("q_node_stride", _i64), ("q_head_stride", _i64),
+        ("cache", Kv), ("capacity", _i64), ("max_len", _i64), ("len", _vp), ("fresh", Kv),
+        ("parent", _vp), ("n_nodes", _vp), ("scale", C.c_float),
+        ("out", _vp), ("out_seq_stride", _i64), ("out_node_stride", _i64), ("out_head_stride", _i64),
+        ("lse", _vp), ("seq_status", _vp),
+    ]
+
+
+class CacheCommitArgs(C.Structure):
+    _fields_ = [
+        ("dtype", _i32), ("head_dim", _i32), ("seqs", _i64), ("nodes", _i64), ("q_heads", _i64), ("kv_heads", _i64),
+        ("cache", Kv), ("capacity", _i64), ("max_len", _i64), ("len", _vp), ("fresh", Kv),
+        ("path", _vp), ("path_ld", _i64), ("n_path", _vp), ("new_len", _vp), ("slot_ld", _i64),
+        ("next_pos", _vp), ("pos", _vp), ("new_next_pos", _vp),
+        ("q", _vp), ("q_seq_stride", _i64), ("q_node_stride", _i64), ("q_head_stride", _i64),
+        ("lse", _vp), ("scale", C.c_float), ("mass", _vp), ("new_mass", _vp), ("seq_status", _vp),
+    ]
+
+
+class CacheEvictArgs(C.Structure):
+    _fields_ = [
+        ("dtype", _i32), ("head_dim", _i32), ("seqs", _i64), ("kv_heads", _i64),
+        ("cache", Kv), ("capacity", _i64), ("max_len", _i64), ("len", _vp),
+        ("mass", _vp), ("new_mass", _vp), ("pos", _vp), ("new_pos", _vp), ("slot_ld", _i64), ("next_pos", _vp),
+        ("keep", _i64), ("sinks", _i64), ("recent", _i64), ("new_len", _vp), ("seq_status", _vp),
+    ]
+
+
 class XsError(RuntimeError):
     pass
 
@@ -112,6 +169,20 @@ def load() -> C.CDLL:
     L.xs_sample_noalloc.argtypes = [C.POINTER(SampleArgs), _vp]
     L.xs_verify.restype = C.c_int
     L.xs_verify.argtypes = [_vp, C.POINTER(VerifyArgs)]
+    L.xs_verify_tree.restype = C.c_int
+    L.xs_verify_tree.argtypes = [_vp, C.POINTER(VerifyTreeArgs)]
+    L.xs_cache_create.restype = C.c_int
+    L.xs_cache_create.argtypes = [C.c_int, C.POINTER(CacheDims), C.POINTER(_vp)]
+    L.xs_cache_destroy.restype = C.c_int
+    L.xs_cache_destroy.argtypes = [_vp]
+    L.xs_cache_set_stream.restype = C.c_int
+    L.xs_cache_set_stream.argtypes = [_vp, _vp]
+    L.xs_tree_attend.restype = C.c_int
+    L.xs_tree_attend.argtypes = [_vp, C.POINTER(TreeAttendArgs)]
+    L.xs_cache_commit.restype = C.c_int
+    L.xs_cache_commit.argtypes = [_vp, C.POINTER(CacheCommitArgs)]
+    L.xs_cache_evict.restype = C.c_int
+    L.xs_cache_evict.argtypes = [_vp, C.POINTER(CacheEvictArgs)]
     L.xs_argmax_probs.restype = C.c_int
     L.xs_argmax_probs.argtypes = [_vp, C.POINTER(ArgmaxArgs)]
     L.xs_select_option.restype = _i32

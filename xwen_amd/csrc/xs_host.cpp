@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <utility>
 #include <vector>
 
 namespace {
@@ -29,6 +30,60 @@ int check_common(const xs_host_limits* lim, const float* logits, int64_t rows, i
   if (allowed && (allowed_ld < allowed_words || allowed_words < 0)) return XS_ERR_ARG;
   if (xs_host::chunks_for(enc) > lim->max_chunks) return XS_ERR_CAPACITY;
   return XS_OK;
+}
+
+// The last element of [n0, n1, n2, head_dim] by these strides lies within a
+// 64-bit offset (of elements of 8 bytes at most).
+bool spans_fit(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2, int64_t s2) {
+  int64_t a, b, c, d;
+  if (__builtin_mul_overflow(n0, s0, &a) || __builtin_mul_overflow(n1, s1, &b) || __builtin_mul_overflow(n2, s2, &c))
+    return false;
+  return !__builtin_add_overflow(a, b, &d) && !__builtin_add_overflow(d, c, &d) && d < (INT64_MAX >> 4);
+}
+
+// Strides of rows of head_dim elements that 16-byte loads reach.  Rows that
+// the call writes may not overlap: taken from the smallest stride up, each
+// passes over all that the smaller ones span (an input may repeat its rows,
+// stride 0).
+bool strides_ok(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t head_dim, bool written) {
+  if (s0 < 0 || s1 < 0 || s2 < 0 || s0 % 8 || s1 % 8 || s2 % 8) return false;
+  if (!spans_fit(n0, s0, n1, s1, n2, s2)) return false;
+  if (!written) return true;
+  std::pair<int64_t, int64_t> d[3] = {{s0, n0}, {s1, n1}, {s2, n2}};
+  std::sort(d, d + 3);
+  int64_t extent = head_dim;
+  for (const auto& [s, n] : d) {
+    if (n <= 1) continue;
+    if (s < extent) return false;
+    extent += s * (n - 1);
+  }
+  return true;
+}
+
+bool kv_ok(const xs_kv& kv, int64_t seqs, int64_t slots, int64_t kv_heads, int64_t head_dim, bool written) {
+  return kv.k && kv.v && aligned16(kv.k) && aligned16(kv.v) &&
+         strides_ok(seqs, kv.seq_stride, slots, kv.slot_stride, kv_heads, kv.head_stride, head_dim, written);
+}
+
+// Per-slot arrays [seqs, kv_heads, slot_ld] lie within a 64-bit offset.
+bool slots_fit(int64_t seqs, int64_t kv_heads, int64_t slot_ld) {
+  return slot_ld <= (INT64_MAX >> 4) / kv_heads / (seqs > 0 ? seqs : 1);
+}
+
+// The sizes every cache call shares, against what its context holds.
+int check_sizes(const xs_cache_dims* dims, int32_t dtype, int64_t head_dim, int64_t seqs, int64_t kv_heads,
+                int64_t capacity, int64_t max_len) {
+  if (dtype != XS_BF16 && dtype != XS_F16) return XS_ERR_ARG;
+  if (head_dim < 8 || head_dim > 256 || head_dim % 8) return XS_ERR_ARG;
+  if (seqs < 0 || kv_heads < 1 || capacity < 1 || max_len < 0 || max_len > capacity) return XS_ERR_ARG;
+  if (seqs > dims->max_seqs || kv_heads > dims->kv_heads || head_dim > dims->head_dim || capacity > dims->capacity)
+    return XS_ERR_CAPACITY;
+  return XS_OK;
+}
+
+int check_queries(const xs_cache_dims* dims, int64_t nodes, int64_t q_heads, int64_t kv_heads) {
+  if (nodes < 1 || nodes > XS_TREE_MAX || q_heads < 1 || q_heads % kv_heads) return XS_ERR_ARG;
+  return nodes > dims->max_nodes || q_heads > dims->q_heads ? XS_ERR_CAPACITY : XS_OK;
 }
 
 }  // namespace
@@ -89,6 +144,78 @@ int xs_host_check_verify(const xs_host_limits* lim, const xs_verify_args* in) {
   if (in->seqs > INT64_MAX / in->span) return XS_ERR_CAPACITY;
   return check_common(lim, in->logits, in->seqs * in->span, in->ld, in->width, in->enc, in->params,
                       in->uniforms, in->allowed, in->allowed_words, in->allowed_ld);
+}
+
+int xs_host_check_verify_tree(const xs_host_limits* lim, const xs_verify_tree_args* in) {
+  if (!lim || !in) return XS_ERR_ARG;
+  if (in->seqs < 0 || in->nodes < 1 || in->nodes > XS_TREE_MAX || in->n_eog < 0 || in->k_max < 0) return XS_ERR_ARG;
+  if (in->seqs == 0) return XS_OK;
+  if (!in->row_token || !in->row_status || !in->accepted || !in->path || !in->committed || !in->n_committed ||
+      !in->seq_status || !in->tokens || !in->parent)
+    return XS_ERR_ARG;
+  if (in->n_eog > 0 && !in->eog) return XS_ERR_ARG;
+  if (in->seqs > INT64_MAX / in->nodes) return XS_ERR_CAPACITY;
+  return check_common(lim, in->logits, in->seqs * in->nodes, in->ld, in->width, in->enc, in->params,
+                      in->uniforms, in->allowed, in->allowed_words, in->allowed_ld);
+}
+
+int xs_host_check_dims(const xs_cache_dims* d) {
+  if (!d || d->max_seqs < 1 || d->max_nodes < 1 || d->max_nodes > XS_TREE_MAX || d->q_heads < 1 || d->kv_heads < 1 ||
+      d->head_dim < 8 || d->head_dim > 256 || d->capacity < 1)
+    return XS_ERR_ARG;
+  // slots and rows are counted in 32 bits, and so are the workgroups of a launch
+  if (d->max_seqs > 65536 || d->q_heads > 4096 || d->kv_heads > d->q_heads || d->capacity > (1 << 28)) return XS_ERR_CAPACITY;
+  return XS_OK;
+}
+
+int xs_host_check_attend(const xs_cache_dims* dims, const xs_tree_attend_args* in) {
+  if (!dims || !in) return XS_ERR_ARG;
+  int rc = check_sizes(dims, in->dtype, in->head_dim, in->seqs, in->kv_heads, in->capacity, in->max_len);
+  if (rc == XS_OK) rc = check_queries(dims, in->nodes, in->q_heads, in->kv_heads);
+  if (rc != XS_OK || in->seqs == 0) return rc;
+  if (!in->len || !in->parent || !in->seq_status || !in->q || !in->out || in->q == in->out) return XS_ERR_ARG;
+  if (!aligned16(in->q) || !aligned16(in->out) ||
+      !kv_ok(in->cache, in->seqs, in->capacity, in->kv_heads, in->head_dim, false) ||
+      !kv_ok(in->fresh, in->seqs, in->nodes, in->kv_heads, in->head_dim, false) ||
+      !strides_ok(in->seqs, in->q_seq_stride, in->nodes, in->q_node_stride, in->q_heads, in->q_head_stride, in->head_dim, false) ||
+      !strides_ok(in->seqs, in->out_seq_stride, in->nodes, in->out_node_stride, in->q_heads, in->out_head_stride, in->head_dim, true))
+    return XS_ERR_ARG;
+  return XS_OK;
+}
+
+int xs_host_check_commit(const xs_cache_dims* dims, const xs_cache_commit_args* in) {
+  if (!dims || !in) return XS_ERR_ARG;
+  int rc = check_sizes(dims, in->dtype, in->head_dim, in->seqs, in->kv_heads, in->capacity, in->max_len);
+  if (rc == XS_OK) rc = check_queries(dims, in->nodes, in->q_heads, in->kv_heads);
+  if (rc != XS_OK || in->seqs == 0) return rc;
+  if (!in->len || !in->path || !in->n_path || !in->new_len || !in->seq_status || in->new_len == in->len) return XS_ERR_ARG;
+  if (in->path_ld < in->nodes || in->slot_ld < in->capacity) return XS_ERR_ARG;
+  if (!slots_fit(in->seqs, in->kv_heads, in->slot_ld) || in->path_ld > INT32_MAX) return XS_ERR_ARG;
+  const int positions = (in->next_pos != nullptr) + (in->pos != nullptr) + (in->new_next_pos != nullptr);
+  if ((positions != 0 && positions != 3) || (positions == 3 && in->new_next_pos == in->next_pos)) return XS_ERR_ARG;
+  const int weights = (in->q != nullptr) + (in->lse != nullptr) + (in->mass != nullptr) + (in->new_mass != nullptr);
+  if (weights != 0 && weights != 4) return XS_ERR_ARG;
+  if (!kv_ok(in->cache, in->seqs, in->capacity, in->kv_heads, in->head_dim, true) ||
+      !kv_ok(in->fresh, in->seqs, in->nodes, in->kv_heads, in->head_dim, false))
+    return XS_ERR_ARG;
+  if (weights && (!aligned16(in->q) || !strides_ok(in->seqs, in->q_seq_stride, in->nodes, in->q_node_stride, in->q_heads,
+                                                   in->q_head_stride, in->head_dim, false)))
+    return XS_ERR_ARG;
+  return XS_OK;
+}
+
+int xs_host_check_evict(const xs_cache_dims* dims, const xs_cache_evict_args* in) {
+  if (!dims || !in) return XS_ERR_ARG;
+  const int rc = check_sizes(dims, in->dtype, in->head_dim, in->seqs, in->kv_heads, in->capacity, in->max_len);
+  if (rc != XS_OK || in->seqs == 0) return rc;
+  if (!in->len || !in->mass || !in->new_mass || !in->pos || !in->new_pos || !in->next_pos || !in->new_len ||
+      !in->seq_status || in->new_len == in->len)
+    return XS_ERR_ARG;
+  if ((in->new_mass == in->mass) != (in->new_pos == in->pos)) return XS_ERR_ARG;
+  if (in->keep < 1 || in->sinks < 0 || in->recent < 0 || in->sinks > in->keep || in->recent > in->keep - in->sinks)
+    return XS_ERR_ARG;
+  if (in->slot_ld < in->capacity || !slots_fit(in->seqs, in->kv_heads, in->slot_ld)) return XS_ERR_ARG;
+  return kv_ok(in->cache, in->seqs, in->capacity, in->kv_heads, in->head_dim, true) ? XS_OK : XS_ERR_ARG;
 }
 
 int xs_host_check_argmax(const xs_host_limits* lim, const xs_argmax_args* in) {

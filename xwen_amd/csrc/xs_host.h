@@ -26,6 +26,12 @@ typedef struct {
 int xs_host_check_sample(const xs_host_limits* lim, const xs_sample_args* in);
 int xs_host_check_verify(const xs_host_limits* lim, const xs_verify_args* in);
 int xs_host_check_argmax(const xs_host_limits* lim, const xs_argmax_args* in);
+int xs_host_check_verify_tree(const xs_host_limits* lim, const xs_verify_tree_args* in);
+// The same for the calls of a cache context, and for the sizes it is made for.
+int xs_host_check_dims(const xs_cache_dims* dims);
+int xs_host_check_attend(const xs_cache_dims* dims, const xs_tree_attend_args* in);
+int xs_host_check_commit(const xs_cache_dims* dims, const xs_cache_commit_args* in);
+int xs_host_check_evict(const xs_cache_dims* dims, const xs_cache_evict_args* in);
 // Whether a sample call needs the rows' held_row lse (any held_row or scoring
 // output), and whether it asks for the scoring reads that score_kernel writes.
 bool xs_host_wants_lse(const xs_sample_args* in);

@@ -4852,6 +4852,72 @@ __global__ void fill_verify_kernel(const xs_verify_args a, int32_t st) {
   }
 }
 
+// The walk of xs_verify_tree, one wave per sequence, after every row is
+// sampled.  Lane j holds node j; a step is one ballot over the children of the
+// current node.  The walk only goes to higher nodes, so it ends within n steps
+// whatever parent holds.  st: a call-level data error (a narrow row, a short
+// mask), which fails every row.
+__global__ __launch_bounds__(64) void tree_walk_kernel(const xs_verify_tree_args a, int32_t st) {
+  const int seq = blockIdx.x, lane = threadIdx.x;
+  const int64_t r0 = (int64_t)seq * a.nodes;
+  const int nodes = (int)a.nodes;
+  const int n_raw = a.n_nodes ? a.n_nodes[seq] : nodes;
+  const bool bad = n_raw < 0 || n_raw > nodes;
+  const int n = bad ? 0 : n_raw;
+  const int bud = a.budget ? a.budget[seq] : 0x7FFFFFFF;
+  const bool in = lane < nodes;
+  int rs = XS_ROW_OK, s = -1, tok = -1, par = -1;
+  bool end = false, fin = false;
+  if (in) {
+    if (st != XS_ROW_OK) {
+      rs = st;
+      a.row_token[r0 + lane] = -1;
+      a.row_status[r0 + lane] = st;
+    } else {
+      rs = a.row_status[r0 + lane];
+      s = a.row_token[r0 + lane];
+    }
+    tok = a.tokens[r0 + lane];
+    par = a.parent[r0 + lane];
+    if (par < 0 || par >= lane) par = -1;
+    fin = a.done_after != nullptr && a.done_after[r0 + lane] != 0;
+    for (int e = 0; e < a.n_eog; e++) end |= (s == a.eog[e]);
+  }
+  int cur = 0, ncom = 0, acc = 0, sst = bad ? XS_ROW_BAD_PARAM : XS_ROW_OK;
+  int path = -1, com = -1;  // lane r: the r-th entry
+  const uint64_t ended = __ballot(end), finished = __ballot(fin);
+  bool more = n > 0;
+  while (more && ncom < bud) {
+    const int srs = __builtin_amdgcn_readlane(rs, cur);
+    if (srs != XS_ROW_OK) {
+      sst = srs;
+      break;
+    }
+    const int t = __builtin_amdgcn_readlane(s, cur);
+    if (lane == ncom) {
+      path = cur;
+      com = t;
+    }
+    ncom++;
+    const uint64_t child = __ballot(lane > 0 && lane < n && par == cur && tok == t);
+    more = child != 0;
+    if (!more) break;
+    const int next = (int)__builtin_ctzll(child);
+    acc++;
+    more = !(((ended >> cur) | (finished >> next)) & 1ull);
+    cur = next;
+  }
+  if (in) {
+    a.path[r0 + lane] = path;
+    a.committed[r0 + lane] = com;
+  }
+  if (lane == 0) {
+    a.accepted[seq] = acc;
+    a.n_committed[seq] = ncom;
+    a.seq_status[seq] = sst;
+  }
+}
+
 // Zeroes n ints (the arrival tickets of the no-allocation entry point; a
 // kernel rather than hipMemsetAsync, so a captured call records no memset node).
 // Each workgroup's XCD (xcd_placement).
@@ -6241,6 +6307,42 @@ int xs_verify(xs_context* ctx, const xs_verify_args* in) {
   a.rec = ctx->rec;
   // tokens are all it returns: the exact sum, checked (draw_settled)
   return launch(ctx, a, rows, (int)in->span, in->allowed != nullptr, false, false);
+}
+
+int xs_verify_tree(xs_context* ctx, const xs_verify_tree_args* in) {
+  if (!ctx) return XS_ERR_ARG;
+  const xs_host_limits lim = limits_of(ctx);
+  const int rc = xs_host_check_verify_tree(&lim, in);
+  if (rc) return rc;
+  if (in->seqs == 0) return XS_OK;
+  if (hipSetDevice(ctx->device) != hipSuccess) return XS_ERR_HIP;
+  int32_t data_err = XS_ROW_OK;
+  if (in->width < in->enc) data_err = XS_ROW_NARROW;
+  else if (in->allowed && in->allowed_words * 32 < in->enc) data_err = XS_ROW_MASK_SHORT;
+  if (data_err == XS_ROW_OK) {
+    xs_sample_args d;
+    memset(&d, 0, sizeof(d));
+    d.logits = in->logits;
+    d.rows = in->seqs * in->nodes;
+    d.ld = in->ld;
+    d.width = in->width;
+    d.enc = in->enc;
+    d.params = in->params;
+    d.uniforms = in->uniforms;
+    d.allowed = in->allowed;
+    d.allowed_words = in->allowed_words;
+    d.allowed_ld = in->allowed_ld;
+    d.token = in->row_token;
+    d.status = in->row_status;
+    d.controls = in->controls;
+    d.ctl_ids = in->ctl_ids;
+    d.ctl_delta = in->ctl_delta;
+    d.k_max = in->k_max;
+    const int src = sample_impl(ctx, &d, false);
+    if (src != XS_OK) return src;
+  }
+  hipLaunchKernelGGL(xs::tree_walk_kernel, dim3((unsigned)in->seqs), dim3(64), 0, ctx->stream, *in, data_err);
+  return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
 }
 
 int xs_argmax_probs(xs_context* ctx, const xs_argmax_args* in) {

@@ -11,6 +11,7 @@ Names, argument meaning and error behaviour follow the reference:
   Sampler.is_eog / eog_ids /
   encodable                         src/sampler.rs:127-128, :245-253
   verify_batch (accept_drafts)      src/generate.rs:4020-4046
+  verify_tree_batch                 (no counterpart: drafts that branch)
   masks_along_drafts                src/generate.rs:2434-2459
   keep_confident                    src/generate.rs:3898-3905
   select_option                     src/batch.rs:1545-1588
@@ -51,6 +52,7 @@ ROW_STATUS_NAMES = {
                         "ctl_max (XS_CTL_MAX unless the context was created with a larger one)",
     _lib.ROW_INTERNAL: "the row's workgroups did not share one XCD (placement check); not sampled",
     _lib.ROW_ID_OOR: "a scored token id is outside the encodable ids",
+    _lib.ROW_CACHE_FULL: "the cache has no room for the accepted path",
 }
 
 
@@ -452,6 +454,68 @@ def verify_batch(ctx: Context, logits, seqs: int, span: int, params, uniforms, d
     if done_after is not None:
         a.done_after = done_after.data_ptr()
     _lib.check(ctx.lib.xs_verify(ctx.h, C.byref(a)), "xs_verify")
+    return out
+
+
+@dataclass
+class TreeVerdict:
+    """Device outputs of one verify_tree_batch (torch tensors on the GPU)."""
+
+    row_token: object
+    row_status: object
+    accepted: object
+    path: object
+    committed: object
+    n_committed: object
+    seq_status: object
+    eog_ids: object = None
+
+
+def verify_tree_batch(ctx: Context, logits, seqs: int, nodes: int, params, uniforms, tokens, parent, *,
+                      n_nodes=None, budget=None, eog=(), enc: int | None = None, allowed=None,
+                      controls: Controls | None = None, done_after=None,
+                      out: TreeVerdict | None = None, k_max: int = 0) -> TreeVerdict:
+    """One xs_verify_tree call over logits [seqs*nodes, ld], row i of a sequence after
+    its node i; tokens and parent int32 [seqs, nodes], n_nodes int32 [seqs] or None.
+    path and n_committed of the result are what tree.cache_commit takes."""
+    torch = _torch()
+    rows, ld = logits.shape
+    if rows != seqs * nodes:
+        raise ValueError(f"logits has {rows} rows, not {seqs} x {nodes}")
+    for name, t, shape in (("tokens", tokens, (seqs, nodes)), ("parent", parent, (seqs, nodes)),
+                           ("n_nodes", n_nodes, (seqs,)), ("budget", budget, (seqs,))):
+        if t is not None and (tuple(t.shape) != shape or t.dtype != torch.int32 or not t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous int32 tensor of {shape}")
+    if done_after is not None and done_after.numel() != rows:
+        raise ValueError(f"done_after must hold {rows} entries")
+    dev = logits.device
+    if out is None:
+        def new(*shape):
+            return torch.empty(shape, dtype=torch.int32, device=dev)
+        out = TreeVerdict(row_token=new(rows), row_status=new(rows), accepted=new(seqs), path=new(seqs, nodes),
+                          committed=new(seqs, nodes), n_committed=new(seqs), seq_status=new(seqs))
+    a = _lib.VerifyTreeArgs()
+    a.logits, a.seqs, a.nodes, a.ld, a.width = logits.data_ptr(), seqs, nodes, ld, ld
+    a.enc = ld if enc is None else enc
+    a.k_max = int(k_max)
+    a.params, a.uniforms = params.data_ptr(), uniforms.data_ptr()
+    if allowed is not None:
+        a.allowed = allowed.data_ptr()
+        a.allowed_words = a.allowed_ld = allowed.shape[1]
+    a.tokens, a.parent = tokens.data_ptr(), parent.data_ptr()
+    a.n_nodes = None if n_nodes is None else n_nodes.data_ptr()
+    a.budget = None if budget is None else budget.data_ptr()
+    a.n_eog = len(eog)
+    if len(eog):
+        out.eog_ids = ctx.eog_list(eog)
+        a.eog = out.eog_ids.data_ptr()
+    for f in ("row_token", "row_status", "accepted", "path", "committed", "n_committed", "seq_status"):
+        setattr(a, f, getattr(out, f).data_ptr())
+    if controls is not None:
+        a.controls, a.ctl_ids, a.ctl_delta = (t.data_ptr() for t in (controls.rows, controls.ids, controls.delta))
+    if done_after is not None:
+        a.done_after = done_after.data_ptr()
+    _lib.check(ctx.lib.xs_verify_tree(ctx.h, C.byref(a)), "xs_verify_tree")
     return out
 
 
