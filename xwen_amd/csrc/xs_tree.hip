@@ -62,62 +62,478 @@ XS_DEV uint64_t ancestors(const int32_t* parent, int n) {
   return up == -1 ? seen : 0ull;
 }
 
-// One wave per (sequence, node, q head): the keys in blocks of 64, a lane's
-// key each for the scores, a lane's elements of the head each for the values.
-template <typename T>
-__global__ __launch_bounds__(64) void attend_kernel(const xs_tree_attend_args a) {
-  __shared__ float qs[256];
-  const int lane = threadIdx.x, D = a.head_dim;
-  const int h = blockIdx.x % a.q_heads, i = (blockIdx.x / a.q_heads) % a.nodes, b = blockIdx.x / (a.q_heads * a.nodes);
-  const int64_t limit = a.max_len ? a.max_len : a.capacity;
-  const int len = a.len[b], n = a.n_nodes ? a.n_nodes[b] : (int)a.nodes;
-  const bool bad = len < 0 || len > limit || n < 0 || n > a.nodes;
-  if (h == 0 && i == 0 && lane == 0) a.seq_status[b] = bad ? XS_ROW_BAD_PARAM : XS_ROW_OK;
-  if (bad || i >= n) return;
-  const int kh = h / (int)(a.q_heads / a.kv_heads);
-  const uint16_t* q = (const uint16_t*)a.q + b * a.q_seq_stride + i * a.q_node_stride + h * a.q_head_stride;
-  for (int d = lane; d < 256; d += 64) qs[d] = d < D ? T::widen(q[d]) : 0.0f;
-  __syncthreads();
-  const uint64_t seen = __shfl(ancestors(a.parent + b * a.nodes, n), i);
-  float m = NEG_INF, l = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  const int total = seen ? len + n : 0;
-  for (int s0 = 0; s0 < total; s0 += 64) {
-    const int s = s0 + lane;
-    const bool on = s < len || (s < total && ((seen >> (s - len)) & 1ull));
-    float x = NEG_INF;
-    if (on) {
-      const uint16_t* k = s < len ? (const uint16_t*)a.cache.k + b * a.cache.seq_stride + s * a.cache.slot_stride + kh * a.cache.head_stride
-                                  : (const uint16_t*)a.fresh.k + b * a.fresh.seq_stride + (s - len) * a.fresh.slot_stride + kh * a.fresh.head_stride;
-      float dot = 0.0f;
-      for (int d = 0; d < D; d++) dot = __builtin_fmaf(qs[d], T::widen(k[d]), dot);
-      x = dot * a.scale;
-    }
-    float top = x;
-    for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const float mn = fmaxf(m, top);
-    const float shift = mn == NEG_INF ? 0.0f : mn;
-    const float keep = expf(m - shift);
-    const float p = on ? expf(x - shift) : 0.0f;
-    m = mn;
-    float sum = p;
-    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
-    l = l * keep + sum;
-    for (int e = 0; e < 4; e++) acc[e] *= keep;
-    const uint64_t live = __ballot(on);
-    for (int j = 0; j < 64; j++) {
-      if (!((live >> j) & 1ull)) continue;
-      const int t = s0 + j;
-      const float w = __shfl(p, j);
-      const uint16_t* v = t < len ? (const uint16_t*)a.cache.v + b * a.cache.seq_stride + t * a.cache.slot_stride + kh * a.cache.head_stride
-                                  : (const uint16_t*)a.fresh.v + b * a.fresh.seq_stride + (t - len) * a.fresh.slot_stride + kh * a.fresh.head_stride;
-      for (int e = 0; e < 4; e++)
-        if (lane + 64 * e < D) acc[e] = __builtin_fmaf(w, T::widen(v[lane + 64 * e]), acc[e]);
+// ---------------------------------------------------------------------------
+// Attention.
+//
+// The rows of one (sequence, kv head) are its nodes times the group of q heads
+// that share the head: row r = node * group + q head.  A wave takes RT tiles of
+// 16 rows and walks the keys in blocks of 32, with v_mfma_f32_16x16x32 (lane =
+// 16 * g + x; A[m = x][k = 8 g + e], B[k = 8 g + e][n = x], C[m = 4 g + r][n = x]):
+//
+//   S^T = K Q^T   A is K (m a key, k the head's elements), B is Q, so a lane
+//                 holds the scores of one row (n = x) with eight keys of the
+//                 block, and a row's statistics are lane-local up to two swaps
+//                 of lane groups;
+//   O^T = V^T P^T the contraction runs over the keys, in the order in which the
+//                 lane already holds them (position 8 g + e is key 4 g + e for
+//                 e < 4 and key 16 + 4 g + e - 4 above), so the weights go
+//                 from the scores' registers to B without crossing lanes, and
+//                 a row's rescaling is lane-local too.  A lane loads 16 bytes of each of
+//                 its eight keys' values, and byte permutes make the eight
+//                 A fragments of them: fragment j is element 8 x + j of V.
+//
+// Softmax in one pass: x = q.k scale log2(e), weights exp2(x - m) with m a
+// running reference that follows the row's maximum only when it has grown by
+// more than 2^8 since (a rescaling of every accumulator otherwise left out;
+// weights stay below 2^8, and the quotient by their sum is the same).  f16
+// weights carry 2^6 more, so that the small ones of a long row stay above
+// the type's subnormals.  Weights round to the inputs' type once; everything
+// else is f32.
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int KB = 32;     // keys of a block
+constexpr int NW = 4;      // waves of a workgroup
+constexpr float LAZY = 8.0f;
+
+XS_DEV f32x4 mfma(Bf16, u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+XS_DEV f32x4 mfma(F16, u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// Two f32 rounded to the type (nearest even), the first in the low half.
+XS_DEV uint32_t pack2(Bf16, float x, float y) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x, y}, bf16x2)); }
+XS_DEV uint32_t pack2(F16, float x, float y) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){x, y}, f16x2)); }
+// The power of two that weights carry, and the least magnitude that is not finite.
+XS_DEV constexpr float offset_of(Bf16) { return 0.0f; }
+XS_DEV constexpr float offset_of(F16) { return 6.0f; }
+XS_DEV constexpr uint32_t inf_of(Bf16) { return 0x7F80u; }
+XS_DEV constexpr uint32_t inf_of(F16) { return 0x7C00u; }
+
+// Over the four lanes of a row (x, 16 + x, 32 + x, 48 + x).
+XS_DEV float row_max(float v) {
+  const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+XS_DEV float row_sum(float v) {
+  const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// How a call is cut: `groups` (sequence, kv head, split) of `tiles` row tiles
+// each, a split taking `chunk` key blocks of its sequence.
+struct Cut {
+  int32_t G, tiles, nsplit, chunk, groups;
+  float scale;          // times log2(e)
+  float* part;          // [groups * tiles] partial results (nsplit > 1)
+};
+
+// A sequence's sizes, or its error.
+struct Seq {
+  int len, n;
+  bool bad;
+  XS_DEV Seq(const xs_tree_attend_args& a, int b) {
+    const int64_t limit = a.max_len ? a.max_len : a.capacity;
+    len = a.len[b];
+    n = a.n_nodes ? a.n_nodes[b] : (int)a.nodes;
+    bad = len < 0 || len > limit || n < 0 || n > a.nodes;
+  }
+  XS_DEV int blocks() const { return (len + KB - 1) / KB + (n + KB - 1) / KB; }
+};
+
+template <int DP, int RT>
+struct Shape {
+  static constexpr int KC = DP / 32;                 // 32-element chunks of a key
+  static constexpr int VH = DP > 128 ? 2 : 1;        // halves of a value row
+  static constexpr int VE = DP >= 128 ? 8 : 4;       // value elements a lane loads of a half
+  static constexpr int NF = VH * VE;                 // A fragments of V^T
+  static constexpr int PART = RT * (NF * 256 + 32);  // floats of a partial result: fragments, m and l
+};
+
+template <typename T, int DP, int RT>
+struct Wave {
+  using S = Shape<DP, RT>;
+  u32x4 q[RT][S::KC];
+  f32x4 o[RT][S::NF];
+  float m[RT], l[RT];
+
+  XS_DEV void init() {
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+      m[t] = NEG_INF;
+      l[t] = 0.0f;
+#pragma unroll
+      for (int f = 0; f < S::NF; f++) o[t][f] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     }
   }
-  uint16_t* out = (uint16_t*)a.out + b * a.out_seq_stride + i * a.out_node_stride + h * a.out_head_stride;
-  for (int e = 0; e < 4; e++)
-    if (lane + 64 * e < D) out[lane + 64 * e] = T::narrow(l == 0.0f ? 0.0f : acc[e] / l);
-  if (a.lse && lane == 0) a.lse[(b * a.nodes + i) * a.q_heads + h] = l == 0.0f ? NEG_INF : m + logf(l);
+  // the reference as it is subtracted: 0 for a row that has seen nothing
+  XS_DEV static float base(float m) { return (m == NEG_INF ? 0.0f : m) - offset_of(T{}); }
+};
+
+// One block of 32 keys from base pointers (elements of one kv head): `limit`
+// keys of the source exist, `on` is the lane's mask of the block's keys for
+// each row tile (masked blocks only).
+template <typename T, int DP, int RT, bool EXACT, bool MASKED>
+XS_DEV void block(Wave<T, DP, RT>& w, const uint16_t* kp, const uint16_t* vp, int64_t stride, int key0, int limit, int D, float scale,
+                  const uint32_t* on) {
+  using S = Shape<DP, RT>;
+  const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
+  u32x4 k[2][S::KC];
+  const u32x4 zero4 = {0, 0, 0, 0};
+#pragma unroll
+  for (int t = 0; t < 2; t++) {
+    int key = key0 + 16 * t + x;
+    if (MASKED) key = min(key, limit - 1);
+    const uint16_t* p = kp + key * stride;
+#pragma unroll
+    for (int c = 0; c < S::KC; c++) {
+      const int d = 32 * c + 8 * g;
+      if (EXACT) k[t][c] = *(const u32x4*)(p + d);
+      else k[t][c] = d < D ? *(const u32x4*)(p + d) : zero4;
+    }
+  }
+  // the values of the lane's eight keys; elements past the head's are those of
+  // its last 16 bytes (their products are never stored)
+  uint32_t v[8][S::VH][S::VE / 2];
+  int key_of[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    int key = key0 + 4 * g + (e & 3) + 16 * (e >> 2);
+    key_of[e] = key;
+    if (MASKED) key = min(key, limit - 1);
+    const uint16_t* p = vp + key * stride;
+#pragma unroll
+    for (int h = 0; h < S::VH; h++) {
+      int d = 128 * h + S::VE * x;
+      if (!EXACT) d = min(d, D - S::VE);
+      if (S::VE == 8) {
+        const u32x4 r = *(const u32x4*)(p + d);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[e][h][i] = r[i];
+      } else {
+        const u32x2 r = *(const u32x2*)(p + d);
+#pragma unroll
+        for (int i = 0; i < 2; i++) v[e][h][i] = r[i];
+      }
+    }
+  }
+  u32x4 pf[RT];
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    f32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+    for (int c = 0; c < S::KC; c++) {
+      s[0] = mfma(T{}, k[0][c], w.q[t][c], s[0]);
+      s[1] = mfma(T{}, k[1][c], w.q[t][c], s[1]);
+    }
+    float xs[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      xs[e] = s[e >> 2][e & 3] * scale;
+      if (MASKED) xs[e] = ((on[t] >> (4 * g + (e & 3) + 16 * (e >> 2))) & 1u) ? xs[e] : NEG_INF;
+    }
+    float top = fmaxf(fmaxf(fmaxf(xs[0], xs[1]), fmaxf(xs[2], xs[3])), fmaxf(fmaxf(xs[4], xs[5]), fmaxf(xs[6], xs[7])));
+    top = row_max(top);
+    if (__any(top > w.m[t] + LAZY)) {
+      const float mn = fmaxf(w.m[t], top);
+      const float keep = __builtin_amdgcn_exp2f(w.m[t] == NEG_INF ? 0.0f : w.m[t] - mn);
+      w.m[t] = mn;
+      w.l[t] *= keep;
+#pragma unroll
+      for (int f = 0; f < S::NF; f++) w.o[t][f] *= keep;
+    }
+    const float base = Wave<T, DP, RT>::base(w.m[t]);
+    float p[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(xs[e] - base);
+    w.l[t] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+#pragma unroll
+    for (int i = 0; i < 4; i++) pf[t][i] = pack2(T{}, p[2 * i], p[2 * i + 1]);
+  }
+  if (MASKED) {
+    // Values of keys past the source count for nothing, whatever they hold.
+    // Neither does a NaN or an infinity in a row that does not see its key,
+    // which the product would give it (0 times it): those are taken out here,
+    // and added below to the rows that see them.
+    u16x2 most = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+#pragma unroll
+      for (int h = 0; h < S::VH; h++)
+#pragma unroll
+        for (int i = 0; i < S::VE / 2; i++) {
+          if (key_of[e] >= limit) v[e][h][i] = 0;
+          most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, v[e][h][i] & 0x7FFF7FFFu));
+        }
+    if (__any(max(most[0], most[1]) >= inf_of(T{}))) {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+#pragma unroll
+        for (int h = 0; h < S::VH; h++)
+#pragma unroll
+          for (int i = 0; i < S::VE / 2; i++) {
+            if ((v[e][h][i] & 0x7FFFu) >= inf_of(T{})) v[e][h][i] &= 0xFFFF0000u;
+            if (((v[e][h][i] >> 16) & 0x7FFFu) >= inf_of(T{})) v[e][h][i] &= 0xFFFFu;
+          }
+#pragma unroll 1
+      for (int key = key0; key < min(key0 + KB, limit); key++) {
+        const uint16_t* p = vp + key * stride;
+        const int at = key - key0, e = (at & 3) + 4 * (at >> 4), from = x + 16 * ((at >> 2) & 3);
+#pragma unroll
+        for (int t = 0; t < RT; t++) {
+          const uint32_t two = e < 2 ? pf[t][0] : e < 4 ? pf[t][1] : e < 6 ? pf[t][2] : pf[t][3];
+          const float weight = T::widen((uint16_t)(__shfl(two, from) >> (16 * (e & 1))));
+          const bool seen = (on[t] >> at) & 1u;
+#pragma unroll
+          for (int h = 0; h < S::VH; h++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              const int d = 128 * h + S::VE * (4 * g + r);
+              if (seen && d < D) {
+                const u32x2* y = (const u32x2*)(p + d);
+#pragma unroll
+                for (int j = 0; j < S::VE; j++) {
+                  const uint16_t u = (uint16_t)(y[j / 4][(j / 2) & 1] >> (16 * (j & 1)));
+                  if ((u & 0x7FFFu) >= inf_of(T{})) w.o[t][h * S::VE + j][r] += weight * T::widen(u);
+                }
+              }
+              __builtin_amdgcn_sched_barrier(0);  // (one load at a time: the registers are the usual path's)
+            }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < S::VH; h++)
+#pragma unroll
+    for (int j = 0; j < S::VE; j++) {
+      u32x4 a;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        a[i] = __builtin_amdgcn_perm(v[2 * i + 1][h][j / 2], v[2 * i][h][j / 2], (j & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+      for (int t = 0; t < RT; t++) w.o[t][h * S::VE + j] = mfma(T{}, a, pf[t], w.o[t][h * S::VE + j]);
+    }
+}
+
+// A row tile's result: the accumulators (a wave's, or a sum of such) over l.
+// Lane (x, g) holds row x, elements 128 h + VE (4 g + r) + j.
+template <typename T, int DP>
+XS_DEV void store_row(const xs_tree_attend_args& a, const Cut& cut, int b, int kh, int row, int R, const f32x4* o, float m, float l) {
+  using S = Shape<DP, 1>;
+  const int g = (threadIdx.x & 63) >> 4;
+  if (row >= R) return;
+  const int node = row / cut.G, head = kh * cut.G + row % cut.G;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* out = (uint16_t*)a.out + b * a.out_seq_stride + node * a.out_node_stride + head * a.out_head_stride;
+#pragma unroll
+  for (int h = 0; h < S::VH; h++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int d = 128 * h + S::VE * (4 * g + r);
+      uint32_t y[S::VE / 2];
+#pragma unroll
+      for (int i = 0; i < S::VE / 2; i++) y[i] = pack2(T{}, o[h * S::VE + 2 * i][r] * inv, o[h * S::VE + 2 * i + 1][r] * inv);
+      if (d < a.head_dim) {
+        if constexpr (S::VE == 8) *(u32x4*)(out + d) = (u32x4){y[0], y[1], y[2], y[3]};
+        else *(u32x2*)(out + d) = (u32x2){y[0], y[1]};
+      }
+    }
+  if (a.lse && g == 0)
+    a.lse[(b * a.nodes + node) * a.q_heads + head] = l == 0.0f ? NEG_INF : LN2 * (m + __builtin_amdgcn_logf(l));
+}
+
+// grid: groups of eight (sequence, kv head, split), each group's row tiles on
+// one XCD (workgroup index mod 8), which then reads their keys once.
+template <typename T, int DP, int RT, bool EXACT>
+__global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 3 : DP * RT <= 128 ? 2 : 1) void attend_kernel(const xs_tree_attend_args a, const Cut cut) {
+  using S = Shape<DP, RT>;
+  __shared__ float stat[NW][RT][2][16];
+  __shared__ f32x4 sum[NW / 2][RT][S::NF][64];
+  const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = (blockIdx.x >> 3) % cut.tiles;
+  const int group = ((blockIdx.x >> 3) / cut.tiles) * 8 + (blockIdx.x & 7);
+  if (group >= cut.groups) return;
+  const int split = group % cut.nsplit, bh = group / cut.nsplit;
+  const int kh = bh % (int)a.kv_heads, b = bh / (int)a.kv_heads;
+  const Seq sq(a, b);
+  if (split == 0 && tile == 0 && kh == 0 && threadIdx.x == 0) a.seq_status[b] = sq.bad ? XS_ROW_BAD_PARAM : XS_ROW_OK;
+  if (sq.bad) return;
+  const int R = sq.n * cut.G, row0 = tile * RT * 16;
+  const int total = sq.blocks(), cached = (sq.len + KB - 1) / KB;
+  const int first = split * cut.chunk, last = min(first + cut.chunk, total);
+  if (row0 >= R || first >= total) return;
+
+  Wave<T, DP, RT> w;
+  w.init();
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    const int row = row0 + 16 * t + x;
+    const bool in = row < R;
+    const int node = in ? row / cut.G : 0, head = kh * cut.G + (in ? row % cut.G : 0);
+    const uint16_t* p = (const uint16_t*)a.q + b * a.q_seq_stride + node * a.q_node_stride + head * a.q_head_stride;
+#pragma unroll
+    for (int c = 0; c < S::KC; c++) {
+      const int d = 32 * c + 8 * g;
+      w.q[t][c] = in && (EXACT || d < a.head_dim) ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0};
+    }
+  }
+  const uint16_t* ck = (const uint16_t*)a.cache.k + b * a.cache.seq_stride + kh * a.cache.head_stride;
+  const uint16_t* cv = (const uint16_t*)a.cache.v + b * a.cache.seq_stride + kh * a.cache.head_stride;
+  int i = first + wave;
+  // whole blocks of the cache
+  for (; i < last && (i + 1) * KB <= sq.len; i += NW)
+    block<T, DP, RT, EXACT, false>(w, ck, cv, a.cache.slot_stride, i * KB, sq.len, a.head_dim, cut.scale, nullptr);
+  // its last one, and the tree's
+  const uint64_t sees = ancestors(a.parent + b * a.nodes, sq.n);
+  uint64_t mine[RT];  // what the lane's rows see of the tree
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    const int row = row0 + 16 * t + x;
+    mine[t] = __shfl(sees, min(row / cut.G, 63));
+    if (row >= R) mine[t] = 0;
+  }
+#pragma unroll 1
+  for (; i < last; i += NW) {
+    const bool in_tree = i >= cached;
+    const int key0 = (in_tree ? i - cached : i) * KB, limit = in_tree ? sq.n : sq.len;
+    const xs_kv& kv = in_tree ? a.fresh : a.cache;
+    const int64_t at = b * kv.seq_stride + kh * kv.head_stride;
+    uint32_t on[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) on[t] = in_tree ? (uint32_t)(mine[t] >> key0) : (1u << (sq.len - key0)) - 1u;
+    block<T, DP, RT, EXACT, true>(w, (const uint16_t*)kv.k + at, (const uint16_t*)kv.v + at, kv.slot_stride, key0, limit, a.head_dim,
+                                  cut.scale, on);
+  }
+
+  // rows that see nothing of the tree see nothing of the cache either
+  float top[RT], all[RT];
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    w.l[t] = row_sum(w.l[t]);
+    if (mine[t] == 0) w.l[t] = 0.0f;
+    w.m[t] = w.l[t] == 0.0f ? NEG_INF : Wave<T, DP, RT>::base(w.m[t]);
+    if (g == 0) {
+      stat[wave][t][0][x] = w.m[t];
+      stat[wave][t][1][x] = w.l[t];
+    }
+  }
+  __syncthreads();
+  // the waves' sums, brought to one reference
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    top[t] = NEG_INF;
+    all[t] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NW; j++) top[t] = fmaxf(top[t], stat[j][t][0][x]);
+#pragma unroll
+    for (int j = 0; j < NW; j++) {
+      const float mj = stat[j][t][0][x];
+      all[t] += mj == NEG_INF ? 0.0f : stat[j][t][1][x] * __builtin_amdgcn_exp2f(mj - top[t]);
+    }
+    const float f = w.m[t] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(w.m[t] - top[t]);
+#pragma unroll
+    for (int n = 0; n < S::NF; n++) w.o[t][n] = w.m[t] == NEG_INF ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : w.o[t][n] * f;
+  }
+  if (wave >= NW / 2) {
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+      for (int n = 0; n < S::NF; n++) sum[wave - NW / 2][t][n][lane] = w.o[t][n];
+  }
+  __syncthreads();
+  if (wave < NW / 2) {
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+      for (int n = 0; n < S::NF; n++) w.o[t][n] += sum[wave][t][n][lane];
+  }
+  __syncthreads();
+  if (wave == 1) {
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+#pragma unroll
+      for (int n = 0; n < S::NF; n++) sum[0][t][n][lane] = w.o[t][n];
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  const bool whole = first == 0 && last == total;
+  float* part = cut.part + ((int64_t)group * cut.tiles + tile) * S::PART;
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+#pragma unroll
+    for (int n = 0; n < S::NF; n++) w.o[t][n] += sum[0][t][n][lane];
+    if (whole) {
+      store_row<T, DP>(a, cut, b, kh, row0 + 16 * t + x, R, w.o[t], top[t], all[t]);
+    } else {
+#pragma unroll
+      for (int n = 0; n < S::NF; n++) ((f32x4*)part)[(t * S::NF + n) * 64 + lane] = w.o[t][n];
+      if (g == 0) {
+        part[RT * S::NF * 256 + 32 * t + x] = top[t];
+        part[RT * S::NF * 256 + 32 * t + 16 + x] = all[t];
+      }
+    }
+  }
+}
+
+// Joins the splits of a row tile of 16: four waves, each a quarter of the splits.
+template <typename T, int DP, int RT>
+__global__ __launch_bounds__(64 * NW) void join_kernel(const xs_tree_attend_args a, const Cut cut) {
+  using S = Shape<DP, RT>;
+  __shared__ f32x4 sum[NW][S::NF][64];
+  const int lane = threadIdx.x & 63, x = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = blockIdx.x % RT, tile = (blockIdx.x / RT) % cut.tiles, bh = blockIdx.x / (RT * cut.tiles);
+  const int kh = bh % (int)a.kv_heads, b = bh / (int)a.kv_heads;
+  const Seq sq(a, b);
+  const int R = sq.n * cut.G, row0 = (tile * RT + t) * 16;
+  const int n = (sq.blocks() + cut.chunk - 1) / cut.chunk;
+  if (sq.bad || row0 >= R || n <= 1) return;
+  const float* part = cut.part + ((int64_t)bh * cut.nsplit * cut.tiles + tile) * S::PART;
+  const int64_t step = (int64_t)cut.tiles * S::PART;
+  float top = NEG_INF, all = 0.0f;
+  for (int s = 0; s < n; s++) top = fmaxf(top, part[s * step + RT * S::NF * 256 + 32 * t + x]);
+  f32x4 o[S::NF];
+#pragma unroll
+  for (int f = 0; f < S::NF; f++) o[f] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+  for (int s = 0; s < n; s++) {
+    const float* p = part + s * step;
+    const float m = p[RT * S::NF * 256 + 32 * t + x], l = p[RT * S::NF * 256 + 32 * t + 16 + x];
+    const float f = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+    if (m != NEG_INF) all += l * f;
+    if ((s & (NW - 1)) == wave) {
+#pragma unroll
+      for (int i = 0; i < S::NF; i++) {
+        const f32x4 y = ((const f32x4*)p)[(t * S::NF + i) * 64 + lane];
+        if (m != NEG_INF) o[i] += y * f;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < S::NF; i++) sum[wave][i][lane] = o[i];
+  __syncthreads();
+  if (wave != 0) return;
+#pragma unroll
+  for (int i = 0; i < S::NF; i++) {
+    o[i] = sum[0][i][lane];
+#pragma unroll
+    for (int j = 1; j < NW; j++) o[i] += sum[j][i][lane];
+  }
+  store_row<T, DP>(a, cut, b, kh, row0 + x, R, o, top, all);
 }
 
 // A sequence's path in lanes [0, m) of the calling wave, or its error.
@@ -261,7 +677,61 @@ struct xs_cache_context {
   hipStream_t stream;
   xs_cache_dims dims;
   uint8_t* kept;  // [max_seqs, kv_heads, capacity]
+  float* part;    // PART_FLOATS: attention's partial results
 };
+
+namespace {
+
+// Workgroups that a split attention call is cut into, by row tiles of a wave:
+// enough for every CU to hold several, so that sequences of different lengths
+// even out; the workspace holds one partial result for each.
+constexpr int attend_target(int rt) { return 2048 / rt; }
+constexpr int64_t PART_FLOATS = (int64_t)attend_target(1) * xst::Shape<256, 1>::PART;
+
+template <typename T, int DP, int RT, bool EXACT>
+int attend_run(xs_cache_context* c, const xs_tree_attend_args& a) {
+  xst::Cut cut;
+  cut.G = (int32_t)(a.q_heads / a.kv_heads);
+  cut.tiles = (int32_t)((a.nodes * cut.G + 16 * RT - 1) / (16 * RT));
+  cut.scale = a.scale * xst::LOG2E;
+  cut.part = c->part;
+  const int64_t limit = a.max_len ? a.max_len : a.capacity;
+  const int64_t blocks = (limit + xst::KB - 1) / xst::KB + (a.nodes + xst::KB - 1) / xst::KB;
+  const int64_t units = a.seqs * a.kv_heads * cut.tiles;
+  int64_t nsplit = attend_target(RT) / units;
+  if (nsplit < 1) nsplit = 1;
+  cut.chunk = (int32_t)((blocks + nsplit - 1) / nsplit);
+  if (cut.chunk < 2 * xst::NW) cut.chunk = 2 * xst::NW;  // two blocks a wave at least
+  cut.nsplit = (int32_t)((blocks + cut.chunk - 1) / cut.chunk);
+  const int64_t groups = a.seqs * a.kv_heads * cut.nsplit;
+  const int64_t grid = (groups + 7) / 8 * 8 * cut.tiles, join = a.seqs * a.kv_heads * cut.tiles * RT;
+  if (grid > 0x7FFFFFFF || join > 0x7FFFFFFF) return XS_ERR_CAPACITY;
+  cut.groups = (int32_t)groups;
+  hipLaunchKernelGGL((xst::attend_kernel<T, DP, RT, EXACT>), dim3((unsigned)grid), dim3(64 * xst::NW), 0, c->stream, a, cut);
+  if (cut.nsplit > 1)
+    hipLaunchKernelGGL((xst::join_kernel<T, DP, RT>), dim3((unsigned)join), dim3(64 * xst::NW), 0, c->stream, a, cut);
+  return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
+}
+
+template <typename T, int DP>
+int attend_rows(xs_cache_context* c, const xs_tree_attend_args& a) {
+  const int64_t rows = a.nodes * (a.q_heads / a.kv_heads);
+  const bool exact = a.head_dim == DP;
+  if constexpr (DP <= 128) {
+    if (rows > 32) return exact ? attend_run<T, DP, 4, true>(c, a) : attend_run<T, DP, 4, false>(c, a);
+  }
+  if (rows > 16) return exact ? attend_run<T, DP, 2, true>(c, a) : attend_run<T, DP, 2, false>(c, a);
+  return exact ? attend_run<T, DP, 1, true>(c, a) : attend_run<T, DP, 1, false>(c, a);
+}
+
+template <typename T>
+int attend_dim(xs_cache_context* c, const xs_tree_attend_args& a) {
+  if (a.head_dim <= 64) return attend_rows<T, 64>(c, a);
+  if (a.head_dim <= 128) return attend_rows<T, 128>(c, a);
+  return attend_rows<T, 256>(c, a);
+}
+
+}  // namespace
 
 extern "C" {
 
@@ -275,7 +745,8 @@ int xs_cache_create(int device, const xs_cache_dims* dims, xs_cache_context** ou
   if (!c) return XS_ERR_HIP;
   c->device = device;
   c->dims = *dims;
-  if (hipMalloc((void**)&c->kept, dims->max_seqs * dims->kv_heads * dims->capacity) != hipSuccess) {
+  if (hipMalloc((void**)&c->kept, dims->max_seqs * dims->kv_heads * dims->capacity) != hipSuccess ||
+      hipMalloc((void**)&c->part, PART_FLOATS * sizeof(float)) != hipSuccess) {
     xs_cache_destroy(c);
     return XS_ERR_HIP;
   }
@@ -288,6 +759,7 @@ int xs_cache_destroy(xs_cache_context* c) {
   (void)hipSetDevice(c->device);
   if (c->stream) (void)hipStreamSynchronize(c->stream); else (void)hipDeviceSynchronize();
   if (c->kept) (void)hipFree(c->kept);
+  if (c->part) (void)hipFree(c->part);
   free(c);
   return XS_OK;
 }
@@ -303,11 +775,8 @@ int xs_tree_attend(xs_cache_context* c, const xs_tree_attend_args* in) {
   if (rc) return rc;
   if (in->seqs == 0) return XS_OK;
   if (hipSetDevice(c->device) != hipSuccess) return XS_ERR_HIP;
-  const int64_t grid = in->seqs * in->nodes * in->q_heads;
-  if (grid > 0x7FFFFFFF) return XS_ERR_CAPACITY;
-  if (in->dtype == XS_BF16) hipLaunchKernelGGL(xst::attend_kernel<xst::Bf16>, dim3((unsigned)grid), dim3(64), 0, c->stream, *in);
-  else hipLaunchKernelGGL(xst::attend_kernel<xst::F16>, dim3((unsigned)grid), dim3(64), 0, c->stream, *in);
-  return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
+  if (in->dtype == XS_BF16) return attend_dim<xst::Bf16>(c, *in);
+  return attend_dim<xst::F16>(c, *in);
 }
 
 int xs_cache_commit(xs_cache_context* c, const xs_cache_commit_args* in) {
