@@ -6,6 +6,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <math.h>
 #include <stdint.h>
 #include <stdlib.h>
@@ -547,55 +548,173 @@ XS_DEV int read_path(const xs_cache_commit_args& a, int b, int len, int64_t limi
   return (int64_t)len + *m > a.capacity ? XS_ROW_CACHE_FULL : XS_ROW_OK;
 }
 
-// One wave per (sequence, kv head, block of 64 slots), a lane a slot; the last
-// block of a head appends the path instead.
-template <typename T>
-__global__ __launch_bounds__(64) void commit_kernel(const xs_cache_commit_args a, int blocks) {
-  const int lane = threadIdx.x, D = a.head_dim;
-  const int blk = blockIdx.x % blocks, kh = (blockIdx.x / blocks) % a.kv_heads, b = blockIdx.x / (blocks * a.kv_heads);
-  const int64_t limit = a.max_len ? a.max_len : a.capacity;
+// ---------------------------------------------------------------------------
+// Commit.
+//
+// Weights: S = Q K^T with A = Q (m a row, path rank * group + q head) and B = K
+// (n a key), so that a lane holds one key and its sum over the rows is a sum over
+// registers and row tiles, and over lane groups once.  A wave keeps RT row tiles
+// in registers and walks its share of the keys in blocks of 32; more rows than that take further passes
+// over the share, which add to what the same lanes wrote.  Bound by the one
+// read of the keys.  The workgroup after a head's last share weighs the
+// path's own keys (a row sees the ranks up to its own) and appends the path.
+
+template <int DP, int RT>
+struct Rows {
+  u32x4 q[RT][DP / 32];
+  float lse[RT][4];  // of rows 4 g + r, times log2(e)
+  uint32_t on;       // bit 4 t + r: the lane's row 4 g + r of tile t counts
+};
+
+// Rows row0 .. row0 + 16 RT of the path (R in all).
+template <int DP, int RT, bool EXACT>
+XS_DEV void load_rows(const xs_cache_commit_args& a, Rows<DP, RT>& w, int b, int kh, int G, int node, int row0, int R) {
+  const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
+  w.on = 0;
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    if (row0 + 16 * t >= R) break;
+    const int row = row0 + 16 * t + x;
+    const int rank = min(row, R - 1) / G, head = kh * G + min(row, R - 1) % G;
+    const int i = __shfl(node, rank);
+    const uint16_t* p = (const uint16_t*)a.q + b * a.q_seq_stride + i * a.q_node_stride + head * a.q_head_stride;
+#pragma unroll
+    for (int c = 0; c < DP / 32; c++) {
+      const int d = 32 * c + 8 * g;
+      w.q[t][c] = EXACT || d < a.head_dim ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int mine = row0 + 16 * t + 4 * g + r, m = min(mine, R - 1);
+      const int k = __shfl(node, m / G);
+      const float v = a.lse[(b * a.nodes + k) * a.q_heads + kh * G + m % G];
+      if (mine < R && v != NEG_INF) w.on |= 1u << (4 * t + r);
+      w.lse[t][r] = v * LOG2E;
+    }
+  }
+}
+
+// The weight that the rows give to two tiles of 16 keys, in every lane group.
+// TAIL: keys are path ranks, seen from their own rank on.
+template <typename T, int DP, int RT, bool EXACT, bool TAIL>
+XS_DEV void weigh(const Rows<DP, RT>& w, const uint16_t* (&kp)[2], int D, float scale, int row0, int R, int G, int rank0, float (&sum)[2]) {
+  const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
+  u32x4 k[2][DP / 32];
+#pragma unroll
+  for (int u = 0; u < 2; u++)
+#pragma unroll
+    for (int c = 0; c < DP / 32; c++) {
+      const int d = 32 * c + 8 * g;
+      k[u][c] = EXACT || d < D ? *(const u32x4*)(kp[u] + d) : (u32x4){0, 0, 0, 0};
+    }
+  sum[0] = sum[1] = 0.0f;
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    if (row0 + 16 * t >= R) break;
+    f32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+    for (int c = 0; c < DP / 32; c++) {
+      s[0] = mfma(T{}, w.q[t][c], k[0][c], s[0]);
+      s[1] = mfma(T{}, w.q[t][c], k[1][c], s[1]);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const float p = __builtin_amdgcn_exp2f(s[u][r] * scale - w.lse[t][r]);
+        bool on = (w.on >> (4 * t + r)) & 1u;
+        if (TAIL) on = on && (row0 + 16 * t + 4 * g + r) / G >= rank0 + 16 * u + x;
+        sum[u] += on ? p : 0.0f;
+      }
+  }
+  sum[0] = row_sum(sum[0]);
+  sum[1] = row_sum(sum[1]);
+}
+
+template <typename T, int DP, int RT, bool EXACT>
+__global__ __launch_bounds__(64 * NW, DP * RT <= 256 ? 3 : 2) void commit_kernel(const xs_cache_commit_args a, int shares, int share, float scale) {
+  const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int blk = blockIdx.x % shares, kh = (blockIdx.x / shares) % (int)a.kv_heads, b = blockIdx.x / (shares * (int)a.kv_heads);
+  const bool tail = blk == shares - 1;
   const int len = a.len[b], G = (int)(a.q_heads / a.kv_heads);
+  if (!tail && blk * NW * share * KB >= len) return;
   int node, m;
-  const int st = read_path(a, b, len, limit, &node, &m);
-  const bool tail = blk == blocks - 1;
-  if (tail && kh == 0 && lane == 0) {
+  const int st = read_path(a, b, len, a.max_len ? a.max_len : a.capacity, &node, &m);
+  if (tail && kh == 0 && threadIdx.x == 0) {
     a.seq_status[b] = st;
     a.new_len[b] = st == XS_ROW_OK ? len + m : len;
     if (a.pos) a.new_next_pos[b] = a.next_pos[b] + (st == XS_ROW_OK ? m : 0);
   }
   if (st != XS_ROW_OK) return;
   const int64_t slots = (b * a.kv_heads + kh) * a.slot_ld;
-  const int s = tail ? lane : blk * 64 + lane;
-  if (a.q && s < (tail ? m : len)) {
-    const uint16_t* k = tail ? (const uint16_t*)a.fresh.k + b * a.fresh.seq_stride + node * a.fresh.slot_stride + kh * a.fresh.head_stride
-                             : (const uint16_t*)a.cache.k + b * a.cache.seq_stride + s * a.cache.slot_stride + kh * a.cache.head_stride;
-    float sum = 0.0f;
-    for (int r = tail ? s : 0; r < m; r++) {
-      const int64_t i = a.path[b * a.path_ld + r];
-      for (int g = 0; g < G; g++) {
-        const int h = kh * G + g;
-        const uint16_t* q = (const uint16_t*)a.q + b * a.q_seq_stride + i * a.q_node_stride + h * a.q_head_stride;
-        const float lse = a.lse[(b * a.nodes + i) * a.q_heads + h];
-        float dot = 0.0f;
-        for (int d = 0; d < D; d++) dot = __builtin_fmaf(T::widen(q[d]), T::widen(k[d]), dot);
-        if (lse != NEG_INF) sum += expf(dot * a.scale - lse);
+  const int R = m * G;
+  Rows<DP, RT> w;
+  if (!tail) {
+    const uint16_t* ck = (const uint16_t*)a.cache.k + b * a.cache.seq_stride + kh * a.cache.head_stride;
+    const int end = min((blk + 1) * NW * share * KB, len);
+    int row0 = 0;
+    do {
+      load_rows<DP, RT, EXACT>(a, w, b, kh, G, node, row0, R);
+      const float* from = row0 == 0 ? a.mass : a.new_mass;
+      for (int key0 = (blk * NW * share + wave) * KB; key0 < end; key0 += NW * KB) {
+        const uint16_t* kp[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) kp[u] = ck + min(key0 + 16 * u + x, len - 1) * a.cache.slot_stride;
+        const int slot = key0 + 16 * (g & 1) + x;
+        const bool mine = g < 2 && slot < end;
+        const float old = mine ? from[slots + slot] : 0.0f;
+        float sum[2];
+        weigh<T, DP, RT, EXACT, false>(w, kp, a.head_dim, scale, row0, R, G, 0, sum);
+        if (mine) a.new_mass[slots + slot] = old + ((g & 1) ? sum[1] : sum[0]);
       }
-    }
-    if (tail) a.new_mass[slots + len + s] = sum;
-    else a.new_mass[slots + s] = a.mass[slots + s] + sum;
+      row0 += 16 * RT;
+    } while (row0 < R);
+    return;
   }
-  if (!tail) return;
-  if (a.pos && lane < m) a.pos[slots + len + lane] = a.next_pos[b] + lane;
-  for (int r = 0; r < m; r++) {
-    const int64_t i = __builtin_amdgcn_readlane(node, r);
-    const int64_t from = b * a.fresh.seq_stride + i * a.fresh.slot_stride + kh * a.fresh.head_stride;
-    const int64_t to = b * a.cache.seq_stride + (len + r) * a.cache.slot_stride + kh * a.cache.head_stride;
-    for (int d = lane; d < D; d += 64) {
-      ((uint16_t*)a.cache.k)[to + d] = ((const uint16_t*)a.fresh.k)[from + d];
-      ((uint16_t*)a.cache.v)[to + d] = ((const uint16_t*)a.fresh.v)[from + d];
+  if (a.q && wave * KB < m) {  // (two waves for at most 64 ranks)
+    const uint16_t* kp[2];
+    const uint16_t* fk = (const uint16_t*)a.fresh.k + b * a.fresh.seq_stride + kh * a.fresh.head_stride;
+#pragma unroll
+    for (int u = 0; u < 2; u++) kp[u] = fk + __shfl(node, min(wave * KB + 16 * u + x, m - 1)) * a.fresh.slot_stride;
+    float all[2] = {0.0f, 0.0f};
+    for (int row0 = 0; row0 < R; row0 += 16 * RT) {
+      load_rows<DP, RT, EXACT>(a, w, b, kh, G, node, row0, R);
+      float sum[2];
+      weigh<T, DP, RT, EXACT, true>(w, kp, a.head_dim, scale, row0, R, G, wave * KB, sum);
+      all[0] += sum[0];
+      all[1] += sum[1];
     }
+    const int rank = wave * KB + 16 * (g & 1) + x;
+    if (g < 2 && rank < m) a.new_mass[slots + len + rank] = (g & 1) ? all[1] : all[0];
+  }
+  if (a.pos && (int)threadIdx.x < m) a.pos[slots + len + threadIdx.x] = a.next_pos[b] + threadIdx.x;
+  const int parts = a.head_dim / 8;
+  const int64_t from = b * a.fresh.seq_stride + kh * a.fresh.head_stride, to = b * a.cache.seq_stride + kh * a.cache.head_stride;
+  for (int j = threadIdx.x; j - lane < m * parts; j += 64 * NW) {  // (whole waves: the path is in their lanes)
+    const int r = min(j / parts, m - 1), d = j % parts * 8;
+    const int64_t f = from + __shfl(node, r) * a.fresh.slot_stride + d, s = to + (len + r) * a.cache.slot_stride + d;
+    if (j >= m * parts) continue;
+    *(u32x4*)((uint16_t*)a.cache.k + s) = *(const u32x4*)((const uint16_t*)a.fresh.k + f);
+    *(u32x4*)((uint16_t*)a.cache.v + s) = *(const u32x4*)((const uint16_t*)a.fresh.v + f);
   }
 }
+
+// ---------------------------------------------------------------------------
+// Eviction.
+//
+// One workgroup per (sequence, kv head) finds the `keep`-th of the slots' 64-bit
+// ranks (rank_key) by counting digits of 11 bits from the top, each pass over
+// the slots whose digits so far are the chosen ones, until a digit's slots are exactly
+// those still needed: weights that differ in their first 22 bits take two passes,
+// equal weights go on into the positions.  The kept slots go to a bitmap, whose prefix
+// counts pair the i-th free slot below `keep` with the i-th kept one past it.
+// Only these move: `keep` of `keep` + a few slots moves a few rows, where
+// keeping the slots in order would move nearly all.
+
+constexpr int EB = 1024;         // threads
+constexpr int EW = EB / 64;      // waves
+constexpr int DIGIT = 11;
 
 // A slot's place in the order of xs_cache_evict, larger first: the held slots
 // above all others, then the weights (the bits of an f32 put in order; NaN
@@ -606,64 +725,193 @@ XS_DEV uint64_t rank_key(float mass, int pos, bool held) {
   return ((uint64_t)(held ? 0xFFFFFFFFu : w) << 32) | (uint32_t)~((uint32_t)pos ^ 0x80000000u);
 }
 
-// kept[slot] by counting the slots before it.
-__global__ __launch_bounds__(256) void evict_rank_kernel(const xs_cache_evict_args a, uint8_t* kept, int blocks) {
-  const int blk = blockIdx.x % blocks;
-  const int64_t bh = blockIdx.x / blocks;
-  const int b = (int)(bh / a.kv_heads);
-  const int64_t limit = a.max_len ? a.max_len : a.capacity;
-  const int len = a.len[b];
-  const int s = blk * 256 + threadIdx.x;
-  if (len < 0 || len > limit || len <= a.keep || s >= len) return;
-  const float* mass = a.mass + bh * a.slot_ld;
-  const int32_t* pos = a.pos + bh * a.slot_ld;
-  const int64_t next = a.next_pos[b];
-  auto key = [&](int t) { return rank_key(mass[t], pos[t], pos[t] < a.sinks || pos[t] >= next - a.recent); };
-  const uint64_t mine = key(s);
-  int before = 0;
-  for (int t = 0; t < len; t++) {
-    const uint64_t k = key(t);
-    before += k > mine || (k == mine && t < s);
+struct EvictWork {
+  uint64_t* kept;   // [heads, words] bitmap of the kept slots
+  int32_t* free_;   // [heads, pairs] freed slots, ascending
+  int32_t* filler;  // [heads, pairs] the slots that move there, ascending
+  int32_t* moves;   // [heads]
+  int64_t words, pairs;
+};
+
+// Exclusive prefix sum over the workgroup (one packed pair of 32-bit counts).
+XS_DEV uint64_t scan_pairs(uint64_t v, uint64_t* lds, uint64_t* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint64_t run = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint64_t y = __shfl_up(run, o);
+    if (lane >= o) run += y;
   }
-  kept[bh * a.capacity + s] = before < a.keep;
+  if (lane == 63) lds[wave] = run;
+  __syncthreads();
+  uint64_t before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < EW; i++) {
+    if (i < wave) before += lds[i];
+    all += lds[i];
+  }
+  __syncthreads();
+  *total = all;
+  return before + run - v;
 }
 
-// One wave per (sequence, kv head): pairs each free slot with its filler.
-__global__ __launch_bounds__(64) void evict_move_kernel(const xs_cache_evict_args a, const uint8_t* kept) {
+// Copies row `from` to row `to` of one kv head's k and v, 16 bytes a lane.
+XS_DEV void move_part(const xs_cache_evict_args& a, int64_t head, int from, int to, int d) {
+  const int64_t f = head + from * a.cache.slot_stride + d, t = head + to * a.cache.slot_stride + d;
+  *(u32x4*)((uint16_t*)a.cache.k + t) = *(const u32x4*)((const uint16_t*)a.cache.k + f);
+  *(u32x4*)((uint16_t*)a.cache.v + t) = *(const u32x4*)((const uint16_t*)a.cache.v + f);
+}
+
+// rows: the rows of k and v are moved here too (few of them), else by evict_rows_kernel.
+__global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, const EvictWork w, int rows) {
+  __shared__ uint32_t hist[1 << DIGIT];
+  __shared__ uint64_t lds[EW];
+  __shared__ uint64_t base[EB];
+  __shared__ int found[3];  // the digit, the slots still needed of it, whether that is all of it
   const int64_t bh = blockIdx.x;
-  const int b = (int)(bh / a.kv_heads), kh = (int)(bh % a.kv_heads), lane = threadIdx.x;
+  const int b = (int)(bh / a.kv_heads), kh = (int)(bh % a.kv_heads), tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t limit = a.max_len ? a.max_len : a.capacity;
   const int len = a.len[b];
   const bool bad = len < 0 || len > limit;
   const int keep = (int)min((int64_t)len, a.keep);
-  if (kh == 0 && lane == 0) {
-    a.seq_status[b] = bad ? XS_ROW_BAD_PARAM : XS_ROW_OK;
-    a.new_len[b] = bad ? len : keep;
+  if (tid == 0) {
+    w.moves[bh] = 0;
+    if (kh == 0) {
+      a.seq_status[b] = bad ? XS_ROW_BAD_PARAM : XS_ROW_OK;
+      a.new_len[b] = bad ? len : keep;
+    }
   }
   if (bad) return;
-  const int64_t slots = bh * a.slot_ld;
-  if (a.new_mass != a.mass)
-    for (int s = lane; s < keep; s += 64) {
-      a.new_mass[slots + s] = a.mass[slots + s];
-      a.new_pos[slots + s] = a.pos[slots + s];
+  const float* mass = a.mass + bh * a.slot_ld;
+  const int32_t* pos = a.pos + bh * a.slot_ld;
+  float* new_mass = a.new_mass + bh * a.slot_ld;
+  int32_t* new_pos = a.new_pos + bh * a.slot_ld;
+  if (new_mass != mass)
+    for (int s = tid; s < keep; s += EB) {
+      new_mass[s] = mass[s];
+      new_pos[s] = pos[s];
     }
   if (len <= keep) return;
+  const int64_t next = a.next_pos[b];
+  auto key = [&](int s) {
+    const int p = pos[s];
+    return rank_key(mass[s], p, p < a.sinks || p >= next - a.recent);
+  };
+
+  uint64_t prefix = 0;
+  int shift = 64, need = keep;
+  bool exact = false;
+  while (shift > 0 && !exact) {
+    const int bits = min(DIGIT, shift);
+    const int above = shift;  // bits above are settled
+    shift -= bits;
+    for (int i = tid; i < 1 << DIGIT; i += EB) hist[i] = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int s0 = 0; s0 < len; s0 += EB) {
+      const int s = s0 + tid;
+      bool in = s < len;
+      const uint64_t k = in ? key(s) : 0;
+      if (above < 64) in = in && (k >> above) == prefix;
+      const uint32_t digit = (uint32_t)(k >> shift) & ((1u << bits) - 1u);
+      const uint64_t who = __ballot(in);
+      if (who == 0) continue;
+      // (a wave that holds one digit adds it at once: equal weights)
+      const uint32_t first = __builtin_amdgcn_readlane(digit, (int)__builtin_ctzll(who));
+      if (__ballot(in && digit != first) == 0) {
+        if (lane == 0) atomicAdd(&hist[first], (uint32_t)__popcll(who));
+      } else if (in) {
+        atomicAdd(&hist[digit], 1u);
+      }
+    }
+    __syncthreads();
+    // thread i: the i-th pair of digits from the top
+    const int hi = (1 << DIGIT) - 1 - 2 * tid;
+    const uint32_t c1 = hist[hi], c0 = hist[hi - 1];
+    uint64_t all;
+    const int before = (int)scan_pairs(c1 + c0, lds, &all);
+    if (before < need && need <= before + (int)(c1 + c0)) {
+      const bool one = need <= before + (int)c1;
+      found[0] = one ? hi : hi - 1;
+      found[1] = need - before - (one ? 0 : (int)c1);
+      found[2] = found[1] == (int)(one ? c1 : c0);
+    }
+    __syncthreads();
+    prefix = above < 64 ? (prefix << bits) | (uint32_t)found[0] : (uint64_t)found[0];
+    need = found[1];
+    exact = found[2] != 0;
+    __syncthreads();
+  }
+  // the bitmap; slots equal in weight and position (not exact) come by wave 0
+  uint64_t* kept = w.kept + bh * w.words;
+  const int words = (len + 63) / 64;
+  for (int i = wave; i < words; i += EW) {
+    const int s = i * 64 + lane;
+    const uint64_t k = s < len ? key(s) >> shift : 0;
+    const uint64_t word = __ballot(s < len && (k > prefix || (exact && k == prefix)));
+    if (lane == 0) kept[i] = word;
+  }
   __syncthreads();
-  const uint8_t* mine = kept + bh * a.capacity;
-  int filler = keep;
-  for (int s = 0; s < keep; s++) {
-    if (mine[s]) continue;
-    while (!mine[filler]) filler++;
-    if (lane == 0) {
-      a.new_mass[slots + s] = a.mass[slots + filler];
-      a.new_pos[slots + s] = a.pos[slots + filler];
+  if (!exact && wave == 0) {
+    for (int i = 0; i < words && need > 0; i++) {
+      const int s = i * 64 + lane;
+      uint64_t eq = __ballot(s < len && key(s) == prefix);
+      while (__popcll(eq) > need) eq &= ~(1ull << (63 - __builtin_clzll(eq)));
+      need -= __popcll(eq);
+      if (eq && lane == 0) kept[i] |= eq;
     }
-    const int64_t row = b * a.cache.seq_stride + kh * a.cache.head_stride;
-    for (int d = lane; d < a.head_dim; d += 64) {
-      ((uint16_t*)a.cache.k)[row + s * a.cache.slot_stride + d] = ((const uint16_t*)a.cache.k)[row + filler * a.cache.slot_stride + d];
-      ((uint16_t*)a.cache.v)[row + s * a.cache.slot_stride + d] = ((const uint16_t*)a.cache.v)[row + filler * a.cache.slot_stride + d];
+  }
+  __syncthreads();
+  // freed slots below keep and kept ones past it, by their ranks
+  int32_t* freed = w.free_ + bh * w.pairs;
+  int32_t* filler = w.filler + bh * w.pairs;
+  uint64_t run = 0;  // low: free slots so far, high: fillers
+  auto split = [&](int i, uint64_t word, uint64_t* f, uint64_t* m) {
+    const int in = min(max(keep - i * 64, 0), 64);  // the word's slots below keep
+    const uint64_t low = in == 64 ? ~0ull : (1ull << in) - 1ull;
+    *f = ~word & low;
+    *m = word & ~low;
+  };
+  for (int w0 = 0; w0 < words; w0 += EB) {
+    const int i = w0 + tid;
+    uint64_t f = 0, m = 0;
+    if (i < words) split(i, kept[i], &f, &m);
+    uint64_t total;
+    base[tid] = run + scan_pairs((uint64_t)__popcll(f) | (uint64_t)__popcll(m) << 32, lds, &total);
+    run += total;
+    __syncthreads();
+    for (int j = wave; j < EB && w0 + j < words; j += EW) {
+      split(w0 + j, kept[w0 + j], &f, &m);
+      const uint64_t below = (1ull << lane) - 1ull, at = base[j];
+      if ((f >> lane) & 1ull) freed[(uint32_t)at + __popcll(f & below)] = (w0 + j) * 64 + lane;
+      if ((m >> lane) & 1ull) filler[(uint32_t)(at >> 32) + __popcll(m & below)] = (w0 + j) * 64 + lane;
     }
-    filler++;
+    __syncthreads();
+  }
+  const int moves = (int)(uint32_t)run;
+  if (tid == 0) w.moves[bh] = moves;
+  for (int i = tid; i < moves; i += EB) {
+    const int to = freed[i], from = filler[i];
+    new_mass[to] = mass[from];
+    new_pos[to] = pos[from];
+  }
+  if (!rows) return;
+  const int parts = a.head_dim / 8;
+  const int64_t head = b * a.cache.seq_stride + kh * a.cache.head_stride;
+  for (int j = tid; j < moves * parts; j += EB) move_part(a, head, filler[j / parts], freed[j / parts], j % parts * 8);
+}
+
+// The rows of a head's moves, ROWS of them a workgroup.
+constexpr int ROWS = 64;
+__global__ __launch_bounds__(256) void evict_rows_kernel(const xs_cache_evict_args a, const EvictWork w, int blocks) {
+  const int64_t bh = blockIdx.x / blocks;
+  const int first = (blockIdx.x % blocks) * ROWS, n = min(ROWS, w.moves[bh] - first);
+  const int parts = a.head_dim / 8;
+  const int64_t head = bh / a.kv_heads * a.cache.seq_stride + bh % a.kv_heads * a.cache.head_stride;
+  for (int j = threadIdx.x; j < n * parts; j += 256) {
+    const int64_t at = bh * w.pairs + first + j / parts;
+    move_part(a, head, w.filler[at], w.free_[at], j % parts * 8);
   }
 }
 
@@ -676,7 +924,7 @@ struct xs_cache_context {
   int device;
   hipStream_t stream;
   xs_cache_dims dims;
-  uint8_t* kept;  // [max_seqs, kv_heads, capacity]
+  xst::EvictWork evict;
   float* part;    // PART_FLOATS: attention's partial results
 };
 
@@ -731,6 +979,47 @@ int attend_dim(xs_cache_context* c, const xs_tree_attend_args& a) {
   return attend_rows<T, 256>(c, a);
 }
 
+// Waves that a commit's keys are dealt to, and the most key blocks that a wave
+// takes: enough waves for every SIMD to hold three, each with many more keys
+// than rows to load.
+constexpr int64_t COMMIT_WAVES = 4096;
+constexpr int64_t COMMIT_BLOCKS = 16;
+
+template <typename T, int DP, int RT>
+int commit_run(xs_cache_context* c, const xs_cache_commit_args& a) {
+  const int64_t limit = a.max_len ? a.max_len : a.capacity;
+  const int64_t blocks = (limit + xst::KB - 1) / xst::KB, heads = a.seqs * a.kv_heads;
+  int64_t share = blocks * heads / COMMIT_WAVES;
+  share = std::max<int64_t>(1, std::min(share, COMMIT_BLOCKS));
+  const int64_t shares = (a.q ? (blocks + xst::NW * share - 1) / (xst::NW * share) : 0) + 1;
+  if (heads * shares > 0x7FFFFFFF) return XS_ERR_CAPACITY;
+  const dim3 grid((unsigned)(heads * shares)), block(64 * xst::NW);
+  const float scale = a.scale * xst::LOG2E;
+  if (a.head_dim == DP)
+    hipLaunchKernelGGL((xst::commit_kernel<T, DP, RT, true>), grid, block, 0, c->stream, a, (int)shares, (int)share, scale);
+  else
+    hipLaunchKernelGGL((xst::commit_kernel<T, DP, RT, false>), grid, block, 0, c->stream, a, (int)shares, (int)share, scale);
+  return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
+}
+
+template <typename T, int DP>
+int commit_rows(xs_cache_context* c, const xs_cache_commit_args& a) {
+  const int64_t rows = a.nodes * (a.q_heads / a.kv_heads);
+  if (rows <= 16) return commit_run<T, DP, 1>(c, a);
+  return rows <= 32 ? commit_run<T, DP, 2>(c, a) : commit_run<T, DP, 4>(c, a);
+}
+
+template <typename T>
+int commit_dim(xs_cache_context* c, const xs_cache_commit_args& a) {
+  if (a.head_dim <= 64) return commit_rows<T, 64>(c, a);
+  if (a.head_dim <= 128) return commit_rows<T, 128>(c, a);
+  return commit_rows<T, 256>(c, a);
+}
+
+// The most moves a head's own workgroup makes; more are dealt to a launch of
+// their own.
+constexpr int64_t EVICT_APART = 128;
+
 }  // namespace
 
 extern "C" {
@@ -745,8 +1034,14 @@ int xs_cache_create(int device, const xs_cache_dims* dims, xs_cache_context** ou
   if (!c) return XS_ERR_HIP;
   c->device = device;
   c->dims = *dims;
-  if (hipMalloc((void**)&c->kept, dims->max_seqs * dims->kv_heads * dims->capacity) != hipSuccess ||
-      hipMalloc((void**)&c->part, PART_FLOATS * sizeof(float)) != hipSuccess) {
+  const int64_t heads = dims->max_seqs * dims->kv_heads;
+  c->evict.words = (dims->capacity + 63) / 64;
+  c->evict.pairs = dims->capacity / 2 + 1;
+  if (hipMalloc((void**)&c->part, PART_FLOATS * sizeof(float)) != hipSuccess ||
+      hipMalloc((void**)&c->evict.kept, heads * c->evict.words * sizeof(uint64_t)) != hipSuccess ||
+      hipMalloc((void**)&c->evict.free_, heads * c->evict.pairs * sizeof(int32_t)) != hipSuccess ||
+      hipMalloc((void**)&c->evict.filler, heads * c->evict.pairs * sizeof(int32_t)) != hipSuccess ||
+      hipMalloc((void**)&c->evict.moves, heads * sizeof(int32_t)) != hipSuccess) {
     xs_cache_destroy(c);
     return XS_ERR_HIP;
   }
@@ -758,8 +1053,11 @@ int xs_cache_destroy(xs_cache_context* c) {
   if (!c) return XS_OK;
   (void)hipSetDevice(c->device);
   if (c->stream) (void)hipStreamSynchronize(c->stream); else (void)hipDeviceSynchronize();
-  if (c->kept) (void)hipFree(c->kept);
   if (c->part) (void)hipFree(c->part);
+  if (c->evict.kept) (void)hipFree(c->evict.kept);
+  if (c->evict.free_) (void)hipFree(c->evict.free_);
+  if (c->evict.filler) (void)hipFree(c->evict.filler);
+  if (c->evict.moves) (void)hipFree(c->evict.moves);
   free(c);
   return XS_OK;
 }
@@ -784,13 +1082,8 @@ int xs_cache_commit(xs_cache_context* c, const xs_cache_commit_args* in) {
   if (rc) return rc;
   if (in->seqs == 0) return XS_OK;
   if (hipSetDevice(c->device) != hipSuccess) return XS_ERR_HIP;
-  const int64_t limit = in->max_len ? in->max_len : in->capacity;
-  const int64_t blocks = in->q ? (limit + 63) / 64 + 1 : 1;
-  const int64_t grid = in->seqs * in->kv_heads * blocks;
-  if (grid > 0x7FFFFFFF) return XS_ERR_CAPACITY;
-  if (in->dtype == XS_BF16) hipLaunchKernelGGL(xst::commit_kernel<xst::Bf16>, dim3((unsigned)grid), dim3(64), 0, c->stream, *in, (int)blocks);
-  else hipLaunchKernelGGL(xst::commit_kernel<xst::F16>, dim3((unsigned)grid), dim3(64), 0, c->stream, *in, (int)blocks);
-  return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
+  if (in->dtype == XS_BF16) return commit_dim<xst::Bf16>(c, *in);
+  return commit_dim<xst::F16>(c, *in);
 }
 
 int xs_cache_evict(xs_cache_context* c, const xs_cache_evict_args* in) {
@@ -799,11 +1092,15 @@ int xs_cache_evict(xs_cache_context* c, const xs_cache_evict_args* in) {
   if (in->seqs == 0) return XS_OK;
   if (hipSetDevice(c->device) != hipSuccess) return XS_ERR_HIP;
   const int64_t limit = in->max_len ? in->max_len : in->capacity;
-  const int64_t blocks = (limit + 255) / 256, grid = in->seqs * in->kv_heads * blocks;
-  if (grid > 0x7FFFFFFF) return XS_ERR_CAPACITY;
-  if (limit > in->keep)
-    hipLaunchKernelGGL(xst::evict_rank_kernel, dim3((unsigned)grid), dim3(256), 0, c->stream, *in, c->kept, (int)blocks);
-  hipLaunchKernelGGL(xst::evict_move_kernel, dim3((unsigned)(in->seqs * in->kv_heads)), dim3(64), 0, c->stream, *in, c->kept);
+  const int64_t heads = in->seqs * in->kv_heads;
+  // moves of a head: at most the slots past keep, and the slots of keep
+  const int64_t most = limit > in->keep ? std::min(in->keep, limit - in->keep) : 0;
+  const bool apart = most > EVICT_APART;
+  const int64_t blocks = (most + xst::ROWS - 1) / xst::ROWS;
+  if (heads > 0x7FFFFFFF || (apart && heads * blocks > 0x7FFFFFFF)) return XS_ERR_CAPACITY;
+  hipLaunchKernelGGL(xst::evict_kernel, dim3((unsigned)heads), dim3(xst::EB), 0, c->stream, *in, c->evict, apart ? 0 : 1);
+  if (apart)
+    hipLaunchKernelGGL(xst::evict_rows_kernel, dim3((unsigned)(heads * blocks)), dim3(256), 0, c->stream, *in, c->evict, (int)blocks);
   return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
 }
 
