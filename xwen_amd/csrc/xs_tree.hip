@@ -83,13 +83,14 @@ XS_DEV uint64_t ancestors(const int32_t* parent, int n) {
 //                 its eight keys' values, and byte permutes make the eight
 //                 A fragments of them: fragment j is element 8 x + j of V.
 //
-// Softmax in one pass: x = q.k scale log2(e), weights exp2(x - m) with m a
-// running reference that follows the row's maximum only when it has grown by
-// more than 2^8 since (a rescaling of every accumulator otherwise left out;
-// weights stay below 2^8, and the quotient by their sum is the same).  f16
-// weights carry 2^6 more, so that the small ones of a long row stay above
-// the type's subnormals.  Weights round to the inputs' type once; everything
-// else is f32.
+// Softmax in one pass: weights exp2(x), x = (q.k - m) scale log2(e), with m a
+// running reference that follows the row's maximum only when that has grown by
+// more than 2^8 since (a rescaling of every accumulator is otherwise left out;
+// weights stay below 2^8, and the quotient by their sum is the same).  The
+// products start from -m, which costs nothing and keeps x exact where q.k is
+// huge (a mask of the type's lowest value).  f16 weights carry 2^6 more, so
+// that the small ones of a long row stay above the type's subnormals.  Weights
+// round to the inputs' type once; everything else is f32.
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -169,19 +170,65 @@ struct Wave {
   using S = Shape<DP, RT>;
   u32x4 q[RT][S::KC];
   f32x4 o[RT][S::NF];
-  float m[RT], l[RT];
+  f32x4 c[RT];     // minus the row's reference (of q.k), four times: what the scores' products start from
+  float most[RT];  // the x above which the reference moves: -inf until the row's first score
+  float l[RT];
 
   XS_DEV void init() {
 #pragma unroll
     for (int t = 0; t < RT; t++) {
-      m[t] = NEG_INF;
+      c[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+      most[t] = NEG_INF;
       l[t] = 0.0f;
 #pragma unroll
       for (int f = 0; f < S::NF; f++) o[t][f] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
     }
   }
-  // the reference as it is subtracted: 0 for a row that has seen nothing
-  XS_DEV static float base(float m) { return (m == NEG_INF ? 0.0f : m) - offset_of(T{}); }
+
+  // The weights of a tile's eight scores s (less the reference) to B's registers.
+  // `on` is the lane's mask of the block's keys.
+  template <bool MASKED>
+  XS_DEV u32x4 weights(int t, const f32x4 (&s)[2], float scale, uint32_t on) {
+    constexpr float OFF = offset_of(T{});
+    const int g = (threadIdx.x & 63) >> 4;
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      x[e] = OFF == 0.0f ? s[e >> 2][e & 3] * scale : __builtin_fmaf(s[e >> 2][e & 3], scale, OFF);
+      if (MASKED) x[e] = ((on >> (4 * g + (e & 3) + 16 * (e >> 2))) & 1u) ? x[e] : NEG_INF;
+    }
+    float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    if (__any(top > most[t])) {
+      top = row_max(top);
+      if (top > most[t]) {
+        const float old = c[t][0];
+        const float ref = scale == 0.0f ? old : old - (top - OFF) / scale;
+        const float step = (ref - old) * scale;  // (to a reference as it is held)
+        const float keep = most[t] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(step);
+        c[t] = (f32x4){ref, ref, ref, ref};
+        most[t] = LAZY + OFF;
+        l[t] *= keep;
+#pragma unroll
+        for (int f = 0; f < S::NF; f++) o[t][f] *= keep;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          x[e] += step;
+          // (a reference so large that it cannot move by so little)
+          if (x[e] > LAZY + OFF) x[e] = LAZY + OFF;
+        }
+      }
+    }
+    float p[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(x[e]);
+    l[t] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+    u32x4 b;
+#pragma unroll
+    for (int i = 0; i < 4; i++) b[i] = pack2(T{}, p[2 * i], p[2 * i + 1]);
+    return b;
+  }
+  // The exponent of two that l and o carry.
+  XS_DEV float reference(int t, float scale) const { return -c[t][0] * scale - offset_of(T{}); }
 };
 
 // One block of 32 keys from base pointers (elements of one kv head): `limit`
@@ -234,35 +281,13 @@ XS_DEV void block(Wave<T, DP, RT>& w, const uint16_t* kp, const uint16_t* vp, in
   u32x4 pf[RT];
 #pragma unroll
   for (int t = 0; t < RT; t++) {
-    f32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+    f32x4 s[2] = {w.c[t], w.c[t]};
 #pragma unroll
     for (int c = 0; c < S::KC; c++) {
       s[0] = mfma(T{}, k[0][c], w.q[t][c], s[0]);
       s[1] = mfma(T{}, k[1][c], w.q[t][c], s[1]);
     }
-    float xs[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      xs[e] = s[e >> 2][e & 3] * scale;
-      if (MASKED) xs[e] = ((on[t] >> (4 * g + (e & 3) + 16 * (e >> 2))) & 1u) ? xs[e] : NEG_INF;
-    }
-    float top = fmaxf(fmaxf(fmaxf(xs[0], xs[1]), fmaxf(xs[2], xs[3])), fmaxf(fmaxf(xs[4], xs[5]), fmaxf(xs[6], xs[7])));
-    top = row_max(top);
-    if (__any(top > w.m[t] + LAZY)) {
-      const float mn = fmaxf(w.m[t], top);
-      const float keep = __builtin_amdgcn_exp2f(w.m[t] == NEG_INF ? 0.0f : w.m[t] - mn);
-      w.m[t] = mn;
-      w.l[t] *= keep;
-#pragma unroll
-      for (int f = 0; f < S::NF; f++) w.o[t][f] *= keep;
-    }
-    const float base = Wave<T, DP, RT>::base(w.m[t]);
-    float p[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(xs[e] - base);
-    w.l[t] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-#pragma unroll
-    for (int i = 0; i < 4; i++) pf[t][i] = pack2(T{}, p[2 * i], p[2 * i + 1]);
+    pf[t] = w.template weights<MASKED>(t, s, scale, MASKED ? on[t] : 0u);
   }
   if (MASKED) {
     // Values of keys past the source count for nothing, whatever they hold.
@@ -369,7 +394,8 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 3 : DP * RT <= 128 ? 2 : 1
   const int tile = (blockIdx.x >> 3) % cut.tiles;
   const int group = ((blockIdx.x >> 3) / cut.tiles) * 8 + (blockIdx.x & 7);
   if (group >= cut.groups) return;
-  const int split = group % cut.nsplit, bh = group / cut.nsplit;
+  // (rotated by the head: the short sequences' few splits would otherwise all be on the first XCDs)
+  const int bh = group / cut.nsplit, split = (group + bh) % cut.nsplit;
   const int kh = bh % (int)a.kv_heads, b = bh / (int)a.kv_heads;
   const Seq sq(a, b);
   if (split == 0 && tile == 0 && kh == 0 && threadIdx.x == 0) a.seq_status[b] = sq.bad ? XS_ROW_BAD_PARAM : XS_ROW_OK;
@@ -422,14 +448,14 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 3 : DP * RT <= 128 ? 2 : 1
   }
 
   // rows that see nothing of the tree see nothing of the cache either
-  float top[RT], all[RT];
+  float top[RT], all[RT], ref[RT];
 #pragma unroll
   for (int t = 0; t < RT; t++) {
     w.l[t] = row_sum(w.l[t]);
     if (mine[t] == 0) w.l[t] = 0.0f;
-    w.m[t] = w.l[t] == 0.0f ? NEG_INF : Wave<T, DP, RT>::base(w.m[t]);
+    ref[t] = w.l[t] == 0.0f ? NEG_INF : w.reference(t, cut.scale);
     if (g == 0) {
-      stat[wave][t][0][x] = w.m[t];
+      stat[wave][t][0][x] = ref[t];
       stat[wave][t][1][x] = w.l[t];
     }
   }
@@ -446,9 +472,9 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 3 : DP * RT <= 128 ? 2 : 1
       const float mj = stat[j][t][0][x];
       all[t] += mj == NEG_INF ? 0.0f : stat[j][t][1][x] * __builtin_amdgcn_exp2f(mj - top[t]);
     }
-    const float f = w.m[t] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(w.m[t] - top[t]);
+    const float f = ref[t] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(ref[t] - top[t]);
 #pragma unroll
-    for (int n = 0; n < S::NF; n++) w.o[t][n] = w.m[t] == NEG_INF ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : w.o[t][n] * f;
+    for (int n = 0; n < S::NF; n++) w.o[t][n] = ref[t] == NEG_INF ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : w.o[t][n] * f;
   }
   if (wave >= NW / 2) {
 #pragma unroll
@@ -473,7 +499,7 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 3 : DP * RT <= 128 ? 2 : 1
   __syncthreads();
   if (wave != 0) return;
   const bool whole = first == 0 && last == total;
-  float* part = cut.part + ((int64_t)group * cut.tiles + tile) * S::PART;
+  float* part = cut.part + (((int64_t)bh * cut.nsplit + split) * cut.tiles + tile) * S::PART;
 #pragma unroll
   for (int t = 0; t < RT; t++) {
 #pragma unroll
@@ -491,14 +517,22 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 3 : DP * RT <= 128 ? 2 : 1
   }
 }
 
-// Joins the splits of a row tile of 16: four waves, each a quarter of the splits.
+// Joins the splits of 16 rows and one half of the head, 16 waves: each wave two
+// fragments of a share of the splits, so that all of their loads are in flight
+// at once (a wave that goes through 64 splits one after the other takes 100
+// us).
+constexpr int SPLITS = 256;  // the most splits of a sequence
 template <typename T, int DP, int RT>
-__global__ __launch_bounds__(64 * NW) void join_kernel(const xs_tree_attend_args a, const Cut cut) {
+__global__ __launch_bounds__(1024) void join_kernel(const xs_tree_attend_args a, const Cut cut) {
   using S = Shape<DP, RT>;
-  __shared__ f32x4 sum[NW][S::NF][64];
-  const int lane = threadIdx.x & 63, x = lane & 15;
+  constexpr int PAIRS = S::VE / 2, SHARES = 16 / PAIRS;
+  __shared__ float weight[SPLITS][16];
+  __shared__ float stat[2][16][16];
+  __shared__ f32x4 sum[SHARES][S::VE][64];
+  const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int t = blockIdx.x % RT, tile = (blockIdx.x / RT) % cut.tiles, bh = blockIdx.x / (RT * cut.tiles);
+  const int h = blockIdx.x % S::VH, t = blockIdx.x / S::VH % RT, tile = blockIdx.x / (S::VH * RT) % cut.tiles;
+  const int bh = blockIdx.x / (S::VH * RT * cut.tiles);
   const int kh = bh % (int)a.kv_heads, b = bh / (int)a.kv_heads;
   const Seq sq(a, b);
   const int R = sq.n * cut.G, row0 = (tile * RT + t) * 16;
@@ -506,35 +540,62 @@ __global__ __launch_bounds__(64 * NW) void join_kernel(const xs_tree_attend_args
   if (sq.bad || row0 >= R || n <= 1) return;
   const float* part = cut.part + ((int64_t)bh * cut.nsplit * cut.tiles + tile) * S::PART;
   const int64_t step = (int64_t)cut.tiles * S::PART;
-  float top = NEG_INF, all = 0.0f;
-  for (int s = 0; s < n; s++) top = fmaxf(top, part[s * step + RT * S::NF * 256 + 32 * t + x]);
-  f32x4 o[S::NF];
+  // lane (x, g) of wave w takes splits 4 w + g, + 64, ... of row x
+  float m[SPLITS / 64], l[SPLITS / 64], top = NEG_INF, all = 0.0f;
 #pragma unroll
-  for (int f = 0; f < S::NF; f++) o[f] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s = 0; s < n; s++) {
-    const float* p = part + s * step;
-    const float m = p[RT * S::NF * 256 + 32 * t + x], l = p[RT * S::NF * 256 + 32 * t + 16 + x];
-    const float f = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-    if (m != NEG_INF) all += l * f;
-    if ((s & (NW - 1)) == wave) {
-#pragma unroll
-      for (int i = 0; i < S::NF; i++) {
-        const f32x4 y = ((const f32x4*)p)[(t * S::NF + i) * 64 + lane];
-        if (m != NEG_INF) o[i] += y * f;
-      }
-    }
+  for (int i = 0; i < SPLITS / 64; i++) {
+    const int s = 64 * i + 4 * wave + g;
+    const float* p = part + min(s, n - 1) * step + RT * S::NF * 256 + 32 * t + x;
+    m[i] = s < n ? p[0] : NEG_INF;
+    l[i] = p[16];
+    top = fmaxf(top, m[i]);
   }
-#pragma unroll
-  for (int i = 0; i < S::NF; i++) sum[wave][i][lane] = o[i];
+  top = row_max(top);
+  if (g == 0) stat[0][wave][x] = top;
   __syncthreads();
-  if (wave != 0) return;
 #pragma unroll
-  for (int i = 0; i < S::NF; i++) {
-    o[i] = sum[0][i][lane];
+  for (int j = 0; j < 16; j++) top = fmaxf(top, stat[0][j][x]);
 #pragma unroll
-    for (int j = 1; j < NW; j++) o[i] += sum[j][i][lane];
+  for (int i = 0; i < SPLITS / 64; i++) {
+    const float f = m[i] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m[i] - top);
+    if (m[i] != NEG_INF) all += l[i] * f;
+    weight[64 * i + 4 * wave + g][x] = f;
   }
-  store_row<T, DP>(a, cut, b, kh, row0 + x, R, o, top, all);
+  all = row_sum(all);
+  if (g == 0) stat[1][wave][x] = all;
+  __syncthreads();
+  const int pair = wave % PAIRS, share = wave / PAIRS, f0 = h * S::VE + 2 * pair;
+  f32x4 o[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll 8
+  for (int s = share; s < n; s += SHARES) {
+    const f32x4* p = (const f32x4*)(part + s * step) + (t * S::NF + f0) * 64 + lane;
+    const float f = weight[s][x];
+    o[0] += p[0] * f;
+    o[1] += p[64] * f;
+  }
+  sum[share][2 * pair][lane] = o[0];
+  sum[share][2 * pair + 1][lane] = o[1];
+  __syncthreads();
+  const int row = row0 + x;
+  if (share != 0 || row >= R) return;
+  all = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 16; j++) all += stat[1][j][x];
+#pragma unroll
+  for (int j = 1; j < SHARES; j++) {
+    o[0] += sum[j][2 * pair][lane];
+    o[1] += sum[j][2 * pair + 1][lane];
+  }
+  const int node = row / cut.G, head = kh * cut.G + row % cut.G;
+  const float inv = all == 0.0f ? 0.0f : 1.0f / all;
+  uint16_t* out = (uint16_t*)a.out + b * a.out_seq_stride + node * a.out_node_stride + head * a.out_head_stride;
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    const int d = 128 * h + S::VE * (4 * g + r) + 2 * pair;
+    if (d < a.head_dim) *(uint32_t*)(out + d) = pack2(T{}, o[0][r] * inv, o[1][r] * inv);
+  }
+  if (a.lse && wave == 0 && h == 0 && g == 0)
+    a.lse[(b * a.nodes + node) * a.q_heads + head] = all == 0.0f ? NEG_INF : LN2 * (top + __builtin_amdgcn_logf(all));
 }
 
 // A sequence's path in lanes [0, m) of the calling wave, or its error.
@@ -933,8 +994,15 @@ namespace {
 // Workgroups that a split attention call is cut into, by row tiles of a wave:
 // enough for every CU to hold several, so that sequences of different lengths
 // even out; the workspace holds one partial result for each.
-constexpr int attend_target(int rt) { return 2048 / rt; }
-constexpr int64_t PART_FLOATS = (int64_t)attend_target(1) * xst::Shape<256, 1>::PART;
+#ifndef TGT
+#define TGT 2048
+#endif
+#ifndef TGT4
+#define TGT4 512
+#endif
+constexpr int64_t attend_target(int rt) { return rt == 4 ? TGT4 : TGT / rt; }
+constexpr int64_t PART_FLOATS = std::max({attend_target(1) * xst::Shape<256, 1>::PART, attend_target(2) * xst::Shape<256, 2>::PART,
+                                          attend_target(4) * xst::Shape<128, 4>::PART});
 
 template <typename T, int DP, int RT, bool EXACT>
 int attend_run(xs_cache_context* c, const xs_tree_attend_args& a) {
@@ -946,18 +1014,18 @@ int attend_run(xs_cache_context* c, const xs_tree_attend_args& a) {
   const int64_t limit = a.max_len ? a.max_len : a.capacity;
   const int64_t blocks = (limit + xst::KB - 1) / xst::KB + (a.nodes + xst::KB - 1) / xst::KB;
   const int64_t units = a.seqs * a.kv_heads * cut.tiles;
-  int64_t nsplit = attend_target(RT) / units;
-  if (nsplit < 1) nsplit = 1;
+  const int64_t nsplit = std::max<int64_t>(1, std::min<int64_t>(xst::SPLITS, attend_target(RT) / units));
   cut.chunk = (int32_t)((blocks + nsplit - 1) / nsplit);
   if (cut.chunk < 2 * xst::NW) cut.chunk = 2 * xst::NW;  // two blocks a wave at least
   cut.nsplit = (int32_t)((blocks + cut.chunk - 1) / cut.chunk);
   const int64_t groups = a.seqs * a.kv_heads * cut.nsplit;
-  const int64_t grid = (groups + 7) / 8 * 8 * cut.tiles, join = a.seqs * a.kv_heads * cut.tiles * RT;
+  const int64_t grid = (groups + 7) / 8 * 8 * cut.tiles, join = a.seqs * a.kv_heads * cut.tiles * RT * xst::Shape<DP, RT>::VH;
   if (grid > 0x7FFFFFFF || join > 0x7FFFFFFF) return XS_ERR_CAPACITY;
+  if (cut.nsplit > 1 && groups * cut.tiles * xst::Shape<DP, RT>::PART > PART_FLOATS) return XS_ERR_CAPACITY;  // (never: groups * tiles <= target)
   cut.groups = (int32_t)groups;
   hipLaunchKernelGGL((xst::attend_kernel<T, DP, RT, EXACT>), dim3((unsigned)grid), dim3(64 * xst::NW), 0, c->stream, a, cut);
   if (cut.nsplit > 1)
-    hipLaunchKernelGGL((xst::join_kernel<T, DP, RT>), dim3((unsigned)join), dim3(64 * xst::NW), 0, c->stream, a, cut);
+    hipLaunchKernelGGL((xst::join_kernel<T, DP, RT>), dim3((unsigned)join), dim3(1024), 0, c->stream, a, cut);
   return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
 }
 
