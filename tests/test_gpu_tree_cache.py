@@ -403,3 +403,15 @@ def test_a_speculative_step_over_a_bounded_cache(ctx):
                 assert torch.equal(cache.v[b, :left, h].cpu(), torch.stack([r[1] for r in plain[b][h]]))
         assert cache.length.tolist() == [len(plain[b][0]) for b in range(B)]
     assert max(seen) > keep
+
+
+@pytest.mark.parametrize("n", [4096, 4097, 8193, 32_768, 32_769, 70_001])
+def test_evict_lengths_at_the_kernels_bounds(n):
+    """Where the slots of a head stop fitting the registers of its workgroup."""
+    big = context(max_seqs=2, kv_heads=2, q_heads=2, head_dim=8, capacity=70_016, max_nodes=1)
+    rng = np.random.default_rng(n)
+    check_evict(big, evict_case(rng, [n, n // 2], 2, 8, (n + 7) // 8 * 8), n // 3, sinks=4, recent=64)
+    c = evict_case(rng, [n, n // 2], 2, 8, (n + 7) // 8 * 8, ties=True)
+    c["pos"][0, 0, :n] = 5  # equal in everything but the slot
+    check_evict(big, c, n - 100, in_place=True)
+    big.close()

@@ -12,6 +12,8 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <type_traits>
+
 #include "../../include/xsamp.h"
 #include "xs_host.h"
 
@@ -42,13 +44,12 @@ struct F16 {
 // ancestor of i; 0 where i's chain of parents does not end in -1 by way of
 // ever lower nodes below n.  Each round doubles the distance a lane has gone
 // up, so six rounds reach the root from any of 64 nodes.  One whole wave.
-XS_DEV uint64_t ancestors(const int32_t* parent, int n) {
+// p: the lane's parent.
+XS_DEV int parent_of(const xs_tree_attend_args& a, int b) { return a.parent[b * a.nodes + min((int)threadIdx.x & 63, (int)a.nodes - 1)]; }
+XS_DEV uint64_t ancestors(int p, int n) {
   const int lane = threadIdx.x & 63;
   int up = -2;  // -1: at the root; -2: the chain is broken
-  if (lane < n) {
-    const int p = parent[lane];
-    up = p == -1 ? -1 : (p >= 0 && p < lane ? p : -2);
-  }
+  if (lane < n) up = p == -1 ? -1 : (p >= 0 && p < lane ? p : -2);
   uint64_t seen = lane < n ? 1ull << lane : 0ull;
 #pragma unroll
   for (int r = 0; r < 6; r++) {
@@ -162,7 +163,9 @@ struct Shape {
   static constexpr int VH = DP > 128 ? 2 : 1;        // halves of a value row
   static constexpr int VE = DP >= 128 ? 8 : 4;       // value elements a lane loads of a half
   static constexpr int NF = VH * VE;                 // A fragments of V^T
-  static constexpr int PART = RT * (NF * 256 + 32);  // floats of a partial result: fragments, m and l
+  static constexpr int STAT = RT * NF * 256;         // floats of a partial result: fragments,
+  static constexpr int ODD = STAT + RT * 32;         // then m and l of each row,
+  static constexpr int PART = ODD + 4;               // then whether odd values are left out
 };
 
 template <typename T, int DP, int RT>
@@ -173,8 +176,10 @@ struct Wave {
   f32x4 c[RT];     // minus the row's reference (of q.k), four times: what the scores' products start from
   float most[RT];  // the x above which the reference moves: -inf until the row's first score
   float l[RT];
+  int odd;         // a node's values held a NaN or an infinity
 
   XS_DEV void init() {
+    odd = 0;
 #pragma unroll
     for (int t = 0; t < RT; t++) {
       c[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
@@ -236,7 +241,7 @@ struct Wave {
 // each row tile (masked blocks only).
 template <typename T, int DP, int RT, bool EXACT, bool MASKED>
 XS_DEV void block(Wave<T, DP, RT>& w, const uint16_t* kp, const uint16_t* vp, int64_t stride, int key0, int limit, int D, float scale,
-                  const uint32_t* on) {
+                  const uint32_t* on, bool in_tree) {
   using S = Shape<DP, RT>;
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
   u32x4 k[2][S::KC];
@@ -256,11 +261,9 @@ XS_DEV void block(Wave<T, DP, RT>& w, const uint16_t* kp, const uint16_t* vp, in
   // the values of the lane's eight keys; elements past the head's are those of
   // its last 16 bytes (their products are never stored)
   uint32_t v[8][S::VH][S::VE / 2];
-  int key_of[8];
 #pragma unroll
   for (int e = 0; e < 8; e++) {
     int key = key0 + 4 * g + (e & 3) + 16 * (e >> 2);
-    key_of[e] = key;
     if (MASKED) key = min(key, limit - 1);
     const uint16_t* p = vp + key * stride;
 #pragma unroll
@@ -291,20 +294,21 @@ XS_DEV void block(Wave<T, DP, RT>& w, const uint16_t* kp, const uint16_t* vp, in
   }
   if (MASKED) {
     // Values of keys past the source count for nothing, whatever they hold.
-    // Neither does a NaN or an infinity in a row that does not see its key,
-    // which the product would give it (0 times it): those are taken out here,
-    // and added below to the rows that see them.
-    u16x2 most = {0, 0};
+    // A NaN or an infinity of a node would, through the product (0 times it),
+    // reach the rows that do not see the node: it is taken out here, and
+    // store_pair adds it to the rows that do.
+    u16x2 top = {0, 0};
 #pragma unroll
     for (int e = 0; e < 8; e++)
 #pragma unroll
       for (int h = 0; h < S::VH; h++)
 #pragma unroll
         for (int i = 0; i < S::VE / 2; i++) {
-          if (key_of[e] >= limit) v[e][h][i] = 0;
-          most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, v[e][h][i] & 0x7FFF7FFFu));
+          if (key0 + 4 * g + (e & 3) + 16 * (e >> 2) >= limit) v[e][h][i] = 0;
+          top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v[e][h][i] & 0x7FFF7FFFu));
         }
-    if (__any(max(most[0], most[1]) >= inf_of(T{}))) {
+    if (in_tree && __any(max(top[0], top[1]) >= inf_of(T{}))) {
+      w.odd = 1;
 #pragma unroll
       for (int e = 0; e < 8; e++)
 #pragma unroll
@@ -313,33 +317,8 @@ XS_DEV void block(Wave<T, DP, RT>& w, const uint16_t* kp, const uint16_t* vp, in
           for (int i = 0; i < S::VE / 2; i++) {
             if ((v[e][h][i] & 0x7FFFu) >= inf_of(T{})) v[e][h][i] &= 0xFFFF0000u;
             if (((v[e][h][i] >> 16) & 0x7FFFu) >= inf_of(T{})) v[e][h][i] &= 0xFFFFu;
+            __builtin_amdgcn_sched_barrier(0);
           }
-#pragma unroll 1
-      for (int key = key0; key < min(key0 + KB, limit); key++) {
-        const uint16_t* p = vp + key * stride;
-        const int at = key - key0, e = (at & 3) + 4 * (at >> 4), from = x + 16 * ((at >> 2) & 3);
-#pragma unroll
-        for (int t = 0; t < RT; t++) {
-          const uint32_t two = e < 2 ? pf[t][0] : e < 4 ? pf[t][1] : e < 6 ? pf[t][2] : pf[t][3];
-          const float weight = T::widen((uint16_t)(__shfl(two, from) >> (16 * (e & 1))));
-          const bool seen = (on[t] >> at) & 1u;
-#pragma unroll
-          for (int h = 0; h < S::VH; h++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-              const int d = 128 * h + S::VE * (4 * g + r);
-              if (seen && d < D) {
-                const u32x2* y = (const u32x2*)(p + d);
-#pragma unroll
-                for (int j = 0; j < S::VE; j++) {
-                  const uint16_t u = (uint16_t)(y[j / 4][(j / 2) & 1] >> (16 * (j & 1)));
-                  if ((u & 0x7FFFu) >= inf_of(T{})) w.o[t][h * S::VE + j][r] += weight * T::widen(u);
-                }
-              }
-              __builtin_amdgcn_sched_barrier(0);  // (one load at a time: the registers are the usual path's)
-            }
-        }
-      }
     }
   }
 #pragma unroll
@@ -355,40 +334,49 @@ XS_DEV void block(Wave<T, DP, RT>& w, const uint16_t* kp, const uint16_t* vp, in
     }
 }
 
-// A row tile's result: the accumulators (a wave's, or a sum of such) over l.
-// Lane (x, g) holds row x, elements 128 h + VE (4 g + r) + j.
+// Two fragments (2 pair and 2 pair + 1 of half h) of a row tile's result: the
+// accumulators over l.  Lane (x, g) holds row x, elements 128 h + VE (4 g + r)
+// + 2 pair of each r.
 template <typename T, int DP>
-XS_DEV void store_row(const xs_tree_attend_args& a, const Cut& cut, int b, int kh, int row, int R, const f32x4* o, float m, float l) {
-  using S = Shape<DP, 1>;
+XS_DEV void store_pair(const xs_tree_attend_args& a, int G, int b, int kh, int row, int R, int h, int pair, f32x4 o0, f32x4 o1, float m, float l, int odd,
+                       int n) {
+  constexpr int VE = Shape<DP, 1>::VE;
   const int g = (threadIdx.x & 63) >> 4;
+  const int node = min(row, R - 1) / G, head = kh * G + min(row, R - 1) % G;
+  if (odd) {  // (rare) the NaNs and infinities among the values of the nodes that the row sees
+    const uint64_t sees = __shfl(ancestors(parent_of(a, b), n), node);
+    const uint16_t* v = (const uint16_t*)a.fresh.v + b * a.fresh.seq_stride + kh * a.fresh.head_stride;
+#pragma unroll 1
+    for (int j = 0; j < n; j++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int d = 128 * h + VE * (4 * g + r) + 2 * pair;
+        const uint32_t two = *(const uint32_t*)(v + j * a.fresh.slot_stride + min(d, a.head_dim - 2));
+        const uint16_t lo = (uint16_t)two, hi = (uint16_t)(two >> 16);
+        if (((sees >> j) & 1ull) && (lo & 0x7FFFu) >= inf_of(T{})) o0[r] += T::widen(lo);
+        if (((sees >> j) & 1ull) && (hi & 0x7FFFu) >= inf_of(T{})) o1[r] += T::widen(hi);
+      }
+  }
   if (row >= R) return;
-  const int node = row / cut.G, head = kh * cut.G + row % cut.G;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint16_t* out = (uint16_t*)a.out + b * a.out_seq_stride + node * a.out_node_stride + head * a.out_head_stride;
 #pragma unroll
-  for (int h = 0; h < S::VH; h++)
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int d = 128 * h + S::VE * (4 * g + r);
-      uint32_t y[S::VE / 2];
-#pragma unroll
-      for (int i = 0; i < S::VE / 2; i++) y[i] = pack2(T{}, o[h * S::VE + 2 * i][r] * inv, o[h * S::VE + 2 * i + 1][r] * inv);
-      if (d < a.head_dim) {
-        if constexpr (S::VE == 8) *(u32x4*)(out + d) = (u32x4){y[0], y[1], y[2], y[3]};
-        else *(u32x2*)(out + d) = (u32x2){y[0], y[1]};
-      }
-    }
-  if (a.lse && g == 0)
+  for (int r = 0; r < 4; r++) {
+    const int d = 128 * h + VE * (4 * g + r) + 2 * pair;
+    if (d < a.head_dim) *(uint32_t*)(out + d) = pack2(T{}, o0[r] * inv, o1[r] * inv);
+  }
+  if (a.lse && h == 0 && pair == 0 && g == 0)
     a.lse[(b * a.nodes + node) * a.q_heads + head] = l == 0.0f ? NEG_INF : LN2 * (m + __builtin_amdgcn_logf(l));
 }
 
 // grid: groups of eight (sequence, kv head, split), each group's row tiles on
 // one XCD (workgroup index mod 8), which then reads their keys once.
 template <typename T, int DP, int RT, bool EXACT>
-__global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 3 : DP * RT <= 128 ? 2 : 1) void attend_kernel(const xs_tree_attend_args a, const Cut cut) {
+__global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : DP * RT <= 256 ? 2 : 1) void attend_kernel(const xs_tree_attend_args a, const Cut cut) {
   using S = Shape<DP, RT>;
   __shared__ float stat[NW][RT][2][16];
-  __shared__ f32x4 sum[NW / 2][RT][S::NF][64];
+  __shared__ f32x4 sum[NW][RT][S::NF][64];
+  __shared__ int odds[NW];
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tile = (blockIdx.x >> 3) % cut.tiles;
@@ -397,20 +385,15 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 3 : DP * RT <= 128 ? 2 : 1
   // (rotated by the head: the short sequences' few splits would otherwise all be on the first XCDs)
   const int bh = group / cut.nsplit, split = (group + bh) % cut.nsplit;
   const int kh = bh % (int)a.kv_heads, b = bh / (int)a.kv_heads;
-  const Seq sq(a, b);
-  if (split == 0 && tile == 0 && kh == 0 && threadIdx.x == 0) a.seq_status[b] = sq.bad ? XS_ROW_BAD_PARAM : XS_ROW_OK;
-  if (sq.bad) return;
-  const int R = sq.n * cut.G, row0 = tile * RT * 16;
-  const int total = sq.blocks(), cached = (sq.len + KB - 1) / KB;
-  const int first = split * cut.chunk, last = min(first + cut.chunk, total);
-  if (row0 >= R || first >= total) return;
-
+  // (the rows that the launch is sized for: their loads need not wait for the
+  // sequence's own sizes)
+  const int row0 = tile * RT * 16, parent = parent_of(a, b);
   Wave<T, DP, RT> w;
   w.init();
 #pragma unroll
   for (int t = 0; t < RT; t++) {
     const int row = row0 + 16 * t + x;
-    const bool in = row < R;
+    const bool in = row < (int)a.nodes * cut.G;
     const int node = in ? row / cut.G : 0, head = kh * cut.G + (in ? row % cut.G : 0);
     const uint16_t* p = (const uint16_t*)a.q + b * a.q_seq_stride + node * a.q_node_stride + head * a.q_head_stride;
 #pragma unroll
@@ -419,14 +402,22 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 3 : DP * RT <= 128 ? 2 : 1
       w.q[t][c] = in && (EXACT || d < a.head_dim) ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0};
     }
   }
+  const Seq sq(a, b);
+  if (split == 0 && tile == 0 && kh == 0 && threadIdx.x == 0) a.seq_status[b] = sq.bad ? XS_ROW_BAD_PARAM : XS_ROW_OK;
+  if (sq.bad) return;
+  const int R = sq.n * cut.G;
+  const int total = sq.blocks(), cached = (sq.len + KB - 1) / KB;
+  const int first = split * cut.chunk, last = min(first + cut.chunk, total);
+  if (row0 >= R || first >= total) return;
+
   const uint16_t* ck = (const uint16_t*)a.cache.k + b * a.cache.seq_stride + kh * a.cache.head_stride;
   const uint16_t* cv = (const uint16_t*)a.cache.v + b * a.cache.seq_stride + kh * a.cache.head_stride;
   int i = first + wave;
   // whole blocks of the cache
   for (; i < last && (i + 1) * KB <= sq.len; i += NW)
-    block<T, DP, RT, EXACT, false>(w, ck, cv, a.cache.slot_stride, i * KB, sq.len, a.head_dim, cut.scale, nullptr);
+    block<T, DP, RT, EXACT, false>(w, ck, cv, a.cache.slot_stride, i * KB, sq.len, a.head_dim, cut.scale, nullptr, false);
   // its last one, and the tree's
-  const uint64_t sees = ancestors(a.parent + b * a.nodes, sq.n);
+  const uint64_t sees = ancestors(parent, sq.n);
   uint64_t mine[RT];  // what the lane's rows see of the tree
 #pragma unroll
   for (int t = 0; t < RT; t++) {
@@ -444,11 +435,13 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 3 : DP * RT <= 128 ? 2 : 1
 #pragma unroll
     for (int t = 0; t < RT; t++) on[t] = in_tree ? (uint32_t)(mine[t] >> key0) : (1u << (sq.len - key0)) - 1u;
     block<T, DP, RT, EXACT, true>(w, (const uint16_t*)kv.k + at, (const uint16_t*)kv.v + at, kv.slot_stride, key0, limit, a.head_dim,
-                                  cut.scale, on);
+                                  cut.scale, on, in_tree);
   }
 
-  // rows that see nothing of the tree see nothing of the cache either
-  float top[RT], all[RT], ref[RT];
+  // the waves' sums, brought to one reference; rows that see nothing of the
+  // tree see nothing of the cache either
+  float ref[RT];
+  if (lane == 0) odds[wave] = w.odd;
 #pragma unroll
   for (int t = 0; t < RT; t++) {
     w.l[t] = row_sum(w.l[t]);
@@ -460,58 +453,45 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 3 : DP * RT <= 128 ? 2 : 1
     }
   }
   __syncthreads();
-  // the waves' sums, brought to one reference
 #pragma unroll
   for (int t = 0; t < RT; t++) {
-    top[t] = NEG_INF;
-    all[t] = 0.0f;
+    float top = NEG_INF;
 #pragma unroll
-    for (int j = 0; j < NW; j++) top[t] = fmaxf(top[t], stat[j][t][0][x]);
+    for (int j = 0; j < NW; j++) top = fmaxf(top, stat[j][t][0][x]);
+    const float f = ref[t] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(ref[t] - top);
+#pragma unroll
+    for (int k = 0; k < S::NF; k++) sum[wave][t][k][lane] = ref[t] == NEG_INF ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : w.o[t][k] * f;
+  }
+  __syncthreads();
+  // a wave takes every fourth pair of fragments
+  constexpr int PAIRS = S::VE / 2;
+  const bool whole = first == 0 && last == total;
+  const int odd = odds[0] | odds[1] | odds[2] | odds[3];
+  float* part = cut.part + (((int64_t)bh * cut.nsplit + split) * cut.tiles + tile) * S::PART;
+#pragma unroll 1
+  for (int u = wave; u < RT * S::VH * PAIRS; u += NW) {
+    const int pair = u % PAIRS, h = u / PAIRS % S::VH, t = u / (PAIRS * S::VH), f0 = h * S::VE + 2 * pair;
+    float top = NEG_INF, all = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NW; j++) top = fmaxf(top, stat[j][t][0][x]);
+    f32x4 o[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
     for (int j = 0; j < NW; j++) {
       const float mj = stat[j][t][0][x];
-      all[t] += mj == NEG_INF ? 0.0f : stat[j][t][1][x] * __builtin_amdgcn_exp2f(mj - top[t]);
+      all += mj == NEG_INF ? 0.0f : stat[j][t][1][x] * __builtin_amdgcn_exp2f(mj - top);
+      o[0] += sum[j][t][f0][lane];
+      o[1] += sum[j][t][f0 + 1][lane];
     }
-    const float f = ref[t] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(ref[t] - top[t]);
-#pragma unroll
-    for (int n = 0; n < S::NF; n++) w.o[t][n] = ref[t] == NEG_INF ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : w.o[t][n] * f;
-  }
-  if (wave >= NW / 2) {
-#pragma unroll
-    for (int t = 0; t < RT; t++)
-#pragma unroll
-      for (int n = 0; n < S::NF; n++) sum[wave - NW / 2][t][n][lane] = w.o[t][n];
-  }
-  __syncthreads();
-  if (wave < NW / 2) {
-#pragma unroll
-    for (int t = 0; t < RT; t++)
-#pragma unroll
-      for (int n = 0; n < S::NF; n++) w.o[t][n] += sum[wave][t][n][lane];
-  }
-  __syncthreads();
-  if (wave == 1) {
-#pragma unroll
-    for (int t = 0; t < RT; t++)
-#pragma unroll
-      for (int n = 0; n < S::NF; n++) sum[0][t][n][lane] = w.o[t][n];
-  }
-  __syncthreads();
-  if (wave != 0) return;
-  const bool whole = first == 0 && last == total;
-  float* part = cut.part + (((int64_t)bh * cut.nsplit + split) * cut.tiles + tile) * S::PART;
-#pragma unroll
-  for (int t = 0; t < RT; t++) {
-#pragma unroll
-    for (int n = 0; n < S::NF; n++) w.o[t][n] += sum[0][t][n][lane];
     if (whole) {
-      store_row<T, DP>(a, cut, b, kh, row0 + 16 * t + x, R, w.o[t], top[t], all[t]);
+      store_pair<T, DP>(a, cut.G, b, kh, row0 + 16 * t + x, R, h, pair, o[0], o[1], top, all, odd, sq.n);
     } else {
-#pragma unroll
-      for (int n = 0; n < S::NF; n++) ((f32x4*)part)[(t * S::NF + n) * 64 + lane] = w.o[t][n];
-      if (g == 0) {
-        part[RT * S::NF * 256 + 32 * t + x] = top[t];
-        part[RT * S::NF * 256 + 32 * t + 16 + x] = all[t];
+      f32x4* p = (f32x4*)part + (t * S::NF + f0) * 64 + lane;
+      p[0] = o[0];
+      p[64] = o[1];
+      if (h == 0 && pair == 0 && g == 0) {
+        part[S::STAT + 32 * t + x] = top;
+        part[S::STAT + 32 * t + 16 + x] = all;
+        part[S::ODD] = odd ? 1.0f : 0.0f;
       }
     }
   }
@@ -528,6 +508,7 @@ __global__ __launch_bounds__(1024) void join_kernel(const xs_tree_attend_args a,
   constexpr int PAIRS = S::VE / 2, SHARES = 16 / PAIRS;
   __shared__ float weight[SPLITS][16];
   __shared__ float stat[2][16][16];
+  __shared__ int odd;
   __shared__ f32x4 sum[SHARES][S::VE][64];
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -538,17 +519,30 @@ __global__ __launch_bounds__(1024) void join_kernel(const xs_tree_attend_args a,
   const int R = sq.n * cut.G, row0 = (tile * RT + t) * 16;
   const int n = (sq.blocks() + cut.chunk - 1) / cut.chunk;
   if (sq.bad || row0 >= R || n <= 1) return;
+  if (threadIdx.x == 0) odd = 0;
+  __syncthreads();
   const float* part = cut.part + ((int64_t)bh * cut.nsplit * cut.tiles + tile) * S::PART;
   const int64_t step = (int64_t)cut.tiles * S::PART;
+  // the first fragments, on their way while the weights are formed
+  constexpr int AHEAD = 4;
+  const int pair = wave % PAIRS, share = wave / PAIRS, f0 = h * S::VE + 2 * pair;
+  f32x4 y[AHEAD][2];
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) {
+    const f32x4* p = (const f32x4*)(part + min(share + SHARES * i, n - 1) * step) + (t * S::NF + f0) * 64 + lane;
+    y[i][0] = p[0];
+    y[i][1] = p[64];
+  }
   // lane (x, g) of wave w takes splits 4 w + g, + 64, ... of row x
   float m[SPLITS / 64], l[SPLITS / 64], top = NEG_INF, all = 0.0f;
 #pragma unroll
   for (int i = 0; i < SPLITS / 64; i++) {
     const int s = 64 * i + 4 * wave + g;
-    const float* p = part + min(s, n - 1) * step + RT * S::NF * 256 + 32 * t + x;
+    const float* p = part + min(s, n - 1) * step + S::STAT + 32 * t + x;
     m[i] = s < n ? p[0] : NEG_INF;
     l[i] = p[16];
     top = fmaxf(top, m[i]);
+    if (p[S::ODD - S::STAT - 32 * t - x] != 0.0f) odd = 1;  // (any of them)
   }
   top = row_max(top);
   if (g == 0) stat[0][wave][x] = top;
@@ -564,10 +558,16 @@ __global__ __launch_bounds__(1024) void join_kernel(const xs_tree_attend_args a,
   all = row_sum(all);
   if (g == 0) stat[1][wave][x] = all;
   __syncthreads();
-  const int pair = wave % PAIRS, share = wave / PAIRS, f0 = h * S::VE + 2 * pair;
   f32x4 o[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) {
+    if (share + SHARES * i >= n) break;
+    const float f = weight[share + SHARES * i][x];
+    o[0] += y[i][0] * f;
+    o[1] += y[i][1] * f;
+  }
 #pragma unroll 8
-  for (int s = share; s < n; s += SHARES) {
+  for (int s = share + SHARES * AHEAD; s < n; s += SHARES) {
     const f32x4* p = (const f32x4*)(part + s * step) + (t * S::NF + f0) * 64 + lane;
     const float f = weight[s][x];
     o[0] += p[0] * f;
@@ -576,8 +576,7 @@ __global__ __launch_bounds__(1024) void join_kernel(const xs_tree_attend_args a,
   sum[share][2 * pair][lane] = o[0];
   sum[share][2 * pair + 1][lane] = o[1];
   __syncthreads();
-  const int row = row0 + x;
-  if (share != 0 || row >= R) return;
+  if (share != 0) return;
   all = 0.0f;
 #pragma unroll
   for (int j = 0; j < 16; j++) all += stat[1][j][x];
@@ -586,16 +585,7 @@ __global__ __launch_bounds__(1024) void join_kernel(const xs_tree_attend_args a,
     o[0] += sum[j][2 * pair][lane];
     o[1] += sum[j][2 * pair + 1][lane];
   }
-  const int node = row / cut.G, head = kh * cut.G + row % cut.G;
-  const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-  uint16_t* out = (uint16_t*)a.out + b * a.out_seq_stride + node * a.out_node_stride + head * a.out_head_stride;
-#pragma unroll
-  for (int r = 0; r < 4; r++) {
-    const int d = 128 * h + S::VE * (4 * g + r) + 2 * pair;
-    if (d < a.head_dim) *(uint32_t*)(out + d) = pack2(T{}, o[0][r] * inv, o[1][r] * inv);
-  }
-  if (a.lse && wave == 0 && h == 0 && g == 0)
-    a.lse[(b * a.nodes + node) * a.q_heads + head] = all == 0.0f ? NEG_INF : LN2 * (top + __builtin_amdgcn_logf(all));
+  store_pair<T, DP>(a, cut.G, b, kh, row0 + x, R, h, pair, o[0], o[1], top, all, odd, sq.n);
 }
 
 // A sequence's path in lanes [0, m) of the calling wave, or its error.
@@ -794,22 +784,42 @@ struct EvictWork {
   int64_t words, pairs;
 };
 
-// Exclusive prefix sum over the workgroup (one packed pair of 32-bit counts).
-XS_DEV uint64_t scan_pairs(uint64_t v, uint64_t* lds, uint64_t* total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint64_t run = v;
+// Inclusive prefix sums over a wave.
+XS_DEV uint32_t wave_scan(uint32_t v) {
+  // within rows of 16 lanes, then each row's last to the rows after it
+#define XS_STEP(ctrl, rows) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, false)
+  XS_STEP(0x111, 0xF);
+  XS_STEP(0x112, 0xF);
+  XS_STEP(0x114, 0xF);
+  XS_STEP(0x118, 0xF);
+  XS_STEP(0x142, 0xA);
+  XS_STEP(0x143, 0xC);
+#undef XS_STEP
+  return v;
+}
+XS_DEV uint64_t wave_scan(uint64_t v) {
+  const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const uint64_t y = __shfl_up(run, o);
-    if (lane >= o) run += y;
+    const uint64_t y = __shfl_up(v, o);
+    if (lane >= o) v += y;
   }
+  return v;
+}
+
+// Exclusive prefix sums over the workgroup, and the total.  Two barriers.
+template <typename U>
+XS_DEV U block_scan(U v, U* lds, U* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const U run = wave_scan(v);
   if (lane == 63) lds[wave] = run;
   __syncthreads();
-  uint64_t before = 0, all = 0;
+  U before = 0, all = 0;
 #pragma unroll
   for (int i = 0; i < EW; i++) {
-    if (i < wave) before += lds[i];
-    all += lds[i];
+    const U y = lds[i];
+    if (i < wave) before += y;
+    all += y;
   }
   __syncthreads();
   *total = all;
@@ -823,11 +833,21 @@ XS_DEV void move_part(const xs_cache_evict_args& a, int64_t head, int from, int 
   *(u32x4*)((uint16_t*)a.cache.v + t) = *(const u32x4*)((const uint16_t*)a.cache.v + f);
 }
 
-// rows: the rows of k and v are moved here too (few of them), else by evict_rows_kernel.
-__global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, const EvictWork w, int rows) {
+// E: slots of a thread, kept in registers (len <= E * EB); 0: any length, read
+// again by every pass.  apart: the rows of k and v are left to
+// evict_rows_kernel (many moves); else there are at most NEAR, made here.
+constexpr int NEAR = 128;
+template <int E>
+__global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, const EvictWork w, int apart) {
+  constexpr int WORDS = E > 0 ? E * EW : 1;
+  typedef typename std::conditional<(E > 0), uint32_t, uint64_t>::type Pair;  // two counts: up to 32,768 each, or any
+  constexpr int HALF = 4 * sizeof(Pair);
   __shared__ uint32_t hist[1 << DIGIT];
-  __shared__ uint64_t lds[EW];
-  __shared__ uint64_t base[EB];
+  __shared__ uint32_t lds32[EW];
+  __shared__ Pair lds[EW];
+  __shared__ Pair base[EB];
+  __shared__ uint64_t word[WORDS];
+  __shared__ int near_free[NEAR], near_filler[NEAR];
   __shared__ int found[3];  // the digit, the slots still needed of it, whether that is all of it
   const int64_t bh = blockIdx.x;
   const int b = (int)(bh / a.kv_heads), kh = (int)(bh % a.kv_heads), tid = threadIdx.x, lane = tid & 63;
@@ -848,16 +868,54 @@ __global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, 
   const int32_t* pos = a.pos + bh * a.slot_ld;
   float* new_mass = a.new_mass + bh * a.slot_ld;
   int32_t* new_pos = a.new_pos + bh * a.slot_ld;
-  if (new_mass != mass)
+  if (len <= keep) {
+    if (new_mass != mass)
+      for (int s = tid; s < keep; s += EB) {
+        new_mass[s] = mass[s];
+        new_pos[s] = pos[s];
+      }
+    return;
+  }
+  const int64_t next = a.next_pos[b];
+  auto key_at = [&](int s) {
+    const int p = pos[s];
+    return rank_key(mass[s], p, p < a.sinks || p >= next - a.recent);
+  };
+  uint64_t mine[E > 0 ? E : 1];
+  if constexpr (E > 0) {
+    float m[E];
+    int p[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const int s = min(e * EB + tid, len - 1);
+      m[e] = mass[s];
+      p[e] = pos[s];
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+      const int s = e * EB + tid;
+      mine[e] = rank_key(m[e], p[e], p[e] < a.sinks || p[e] >= next - a.recent);
+      if (new_mass != mass && s < keep) {
+        new_mass[s] = m[e];
+        new_pos[s] = p[e];
+      }
+    }
+  } else if (new_mass != mass) {
     for (int s = tid; s < keep; s += EB) {
       new_mass[s] = mass[s];
       new_pos[s] = pos[s];
     }
-  if (len <= keep) return;
-  const int64_t next = a.next_pos[b];
-  auto key = [&](int s) {
-    const int p = pos[s];
-    return rank_key(mass[s], p, p < a.sinks || p >= next - a.recent);
+  }
+  // f(first slot of the wave's 64, slot, key) for every slot of the workgroup's waves in turn
+  auto each = [&](auto f) {
+    if constexpr (E > 0) {
+#pragma unroll
+      for (int e = 0; e < E; e++)
+        if (e * EB + wave * 64 < len) f(e * EB + wave * 64, e * EB + tid, mine[e]);
+    } else {
+#pragma unroll 4
+      for (int s0 = wave * 64; s0 < len; s0 += EB) f(s0, s0 + lane, key_at(min(s0 + lane, len - 1)));
+    }
   };
 
   uint64_t prefix = 0;
@@ -867,17 +925,14 @@ __global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, 
     const int bits = min(DIGIT, shift);
     const int above = shift;  // bits above are settled
     shift -= bits;
-    for (int i = tid; i < 1 << DIGIT; i += EB) hist[i] = 0;
+    hist[tid] = 0;
+    hist[tid + EB] = 0;
     __syncthreads();
-#pragma unroll 4
-    for (int s0 = 0; s0 < len; s0 += EB) {
-      const int s = s0 + tid;
-      bool in = s < len;
-      const uint64_t k = in ? key(s) : 0;
-      if (above < 64) in = in && (k >> above) == prefix;
+    each([&](int, int s, uint64_t k) {
+      const bool in = s < len && (above == 64 || (k >> (above & 63)) == prefix);
       const uint32_t digit = (uint32_t)(k >> shift) & ((1u << bits) - 1u);
       const uint64_t who = __ballot(in);
-      if (who == 0) continue;
+      if (who == 0) return;
       // (a wave that holds one digit adds it at once: equal weights)
       const uint32_t first = __builtin_amdgcn_readlane(digit, (int)__builtin_ctzll(who));
       if (__ballot(in && digit != first) == 0) {
@@ -885,13 +940,13 @@ __global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, 
       } else if (in) {
         atomicAdd(&hist[digit], 1u);
       }
-    }
+    });
     __syncthreads();
     // thread i: the i-th pair of digits from the top
     const int hi = (1 << DIGIT) - 1 - 2 * tid;
     const uint32_t c1 = hist[hi], c0 = hist[hi - 1];
-    uint64_t all;
-    const int before = (int)scan_pairs(c1 + c0, lds, &all);
+    uint32_t all;
+    const int before = (int)block_scan(c1 + c0, lds32, &all);
     if (before < need && need <= before + (int)(c1 + c0)) {
       const bool one = need <= before + (int)c1;
       found[0] = one ? hi : hi - 1;
@@ -902,65 +957,66 @@ __global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, 
     prefix = above < 64 ? (prefix << bits) | (uint32_t)found[0] : (uint64_t)found[0];
     need = found[1];
     exact = found[2] != 0;
-    __syncthreads();
   }
   // the bitmap; slots equal in weight and position (not exact) come by wave 0
-  uint64_t* kept = w.kept + bh * w.words;
+  uint64_t* kept = E > 0 ? word : w.kept + bh * w.words;
   const int words = (len + 63) / 64;
-  for (int i = wave; i < words; i += EW) {
-    const int s = i * 64 + lane;
-    const uint64_t k = s < len ? key(s) >> shift : 0;
-    const uint64_t word = __ballot(s < len && (k > prefix || (exact && k == prefix)));
-    if (lane == 0) kept[i] = word;
-  }
+  each([&](int s0, int s, uint64_t k) {
+    k >>= shift;
+    const uint64_t bit = __ballot(s < len && (k > prefix || (exact && k == prefix)));
+    if (lane == 0) kept[s0 / 64] = bit;
+  });
   __syncthreads();
-  if (!exact && wave == 0) {
-    for (int i = 0; i < words && need > 0; i++) {
-      const int s = i * 64 + lane;
-      uint64_t eq = __ballot(s < len && key(s) == prefix);
-      while (__popcll(eq) > need) eq &= ~(1ull << (63 - __builtin_clzll(eq)));
-      need -= __popcll(eq);
-      if (eq && lane == 0) kept[i] |= eq;
-    }
+  if (!exact) {
+    if (wave == 0)
+      for (int i = 0; i < words && need > 0; i++) {
+        const int s = i * 64 + lane;
+        uint64_t eq = __ballot(s < len && key_at(min(s, len - 1)) == prefix);
+        while (__popcll(eq) > need) eq &= ~(1ull << (63 - __builtin_clzll(eq)));
+        need -= __popcll(eq);
+        if (eq && lane == 0) kept[i] |= eq;
+      }
+    __syncthreads();
   }
-  __syncthreads();
   // freed slots below keep and kept ones past it, by their ranks
-  int32_t* freed = w.free_ + bh * w.pairs;
-  int32_t* filler = w.filler + bh * w.pairs;
-  uint64_t run = 0;  // low: free slots so far, high: fillers
-  auto split = [&](int i, uint64_t word, uint64_t* f, uint64_t* m) {
+  int32_t* freed = apart ? w.free_ + bh * w.pairs : near_free;
+  int32_t* filler = apart ? w.filler + bh * w.pairs : near_filler;
+  Pair run = 0;  // low half: free slots so far, high: fillers
+  auto split = [&](int i, uint64_t bits, uint64_t* f, uint64_t* m) {
     const int in = min(max(keep - i * 64, 0), 64);  // the word's slots below keep
     const uint64_t low = in == 64 ? ~0ull : (1ull << in) - 1ull;
-    *f = ~word & low;
-    *m = word & ~low;
+    *f = ~bits & low;
+    *m = bits & ~low;
   };
   for (int w0 = 0; w0 < words; w0 += EB) {
     const int i = w0 + tid;
     uint64_t f = 0, m = 0;
     if (i < words) split(i, kept[i], &f, &m);
-    uint64_t total;
-    base[tid] = run + scan_pairs((uint64_t)__popcll(f) | (uint64_t)__popcll(m) << 32, lds, &total);
+    Pair total;
+    base[tid] = run + block_scan((Pair)__popcll(f) | (Pair)__popcll(m) << HALF, lds, &total);
     run += total;
     __syncthreads();
     for (int j = wave; j < EB && w0 + j < words; j += EW) {
       split(w0 + j, kept[w0 + j], &f, &m);
-      const uint64_t below = (1ull << lane) - 1ull, at = base[j];
-      if ((f >> lane) & 1ull) freed[(uint32_t)at + __popcll(f & below)] = (w0 + j) * 64 + lane;
-      if ((m >> lane) & 1ull) filler[(uint32_t)(at >> 32) + __popcll(m & below)] = (w0 + j) * 64 + lane;
+      const uint64_t below = (1ull << lane) - 1ull;
+      const Pair at = base[j];
+      const int slot = (w0 + j) * 64 + lane;
+      if ((f >> lane) & 1ull) freed[(int)(at & (((Pair)1 << HALF) - 1)) + __popcll(f & below)] = slot;
+      if ((m >> lane) & 1ull) filler[(int)(at >> HALF) + __popcll(m & below)] = slot;
     }
     __syncthreads();
   }
-  const int moves = (int)(uint32_t)run;
+  const int moves = (int)(run >> HALF);
   if (tid == 0) w.moves[bh] = moves;
   for (int i = tid; i < moves; i += EB) {
     const int to = freed[i], from = filler[i];
     new_mass[to] = mass[from];
     new_pos[to] = pos[from];
   }
-  if (!rows) return;
+  if (apart) return;
   const int parts = a.head_dim / 8;
   const int64_t head = b * a.cache.seq_stride + kh * a.cache.head_stride;
-  for (int j = tid; j < moves * parts; j += EB) move_part(a, head, filler[j / parts], freed[j / parts], j % parts * 8);
+  for (int j = tid; j < moves * parts; j += EB) move_part(a, head, near_filler[j / parts], near_free[j / parts], j % parts * 8);
 }
 
 // The rows of a head's moves, ROWS of them a workgroup.
@@ -986,23 +1042,21 @@ struct xs_cache_context {
   hipStream_t stream;
   xs_cache_dims dims;
   xst::EvictWork evict;
-  float* part;    // PART_FLOATS: attention's partial results
+  int n_cu;
+  float* part;    // attention's partial results, one for each workgroup of a split call
+  int64_t part_floats;
 };
 
 namespace {
 
-// Workgroups that a split attention call is cut into, by row tiles of a wave:
-// enough for every CU to hold several, so that sequences of different lengths
-// even out; the workspace holds one partial result for each.
-#ifndef TGT
-#define TGT 2048
-#endif
-#ifndef TGT4
-#define TGT4 512
-#endif
-constexpr int64_t attend_target(int rt) { return rt == 4 ? TGT4 : TGT / rt; }
-constexpr int64_t PART_FLOATS = std::max({attend_target(1) * xst::Shape<256, 1>::PART, attend_target(2) * xst::Shape<256, 2>::PART,
-                                          attend_target(4) * xst::Shape<128, 4>::PART});
+// Workgroups of attend_kernel that a CU holds at once (by its registers; its
+// launch bound asks for as many), by the head's size and the row tiles.
+constexpr int64_t per_cu(int dp, int rt) { return dp * rt <= 64 ? 4 : dp * rt <= 128 ? 3 : dp * rt <= 256 ? 2 : 1; }
+// How many times over a split call fills the device: once where all sequences
+// end together (one of them: 8 heads over 131,072 slots 145 -> 113 us against four times), more
+// often where some end early (32 sequences of 327 to 8,192 slots 151 -> 134 us
+// against twice, while 32 of 8,192 take 222 instead of 214).
+constexpr int64_t rounds(int64_t seqs) { return seqs > 1 ? 4 : 1; }
 
 template <typename T, int DP, int RT, bool EXACT>
 int attend_run(xs_cache_context* c, const xs_tree_attend_args& a) {
@@ -1014,19 +1068,43 @@ int attend_run(xs_cache_context* c, const xs_tree_attend_args& a) {
   const int64_t limit = a.max_len ? a.max_len : a.capacity;
   const int64_t blocks = (limit + xst::KB - 1) / xst::KB + (a.nodes + xst::KB - 1) / xst::KB;
   const int64_t units = a.seqs * a.kv_heads * cut.tiles;
-  const int64_t nsplit = std::max<int64_t>(1, std::min<int64_t>(xst::SPLITS, attend_target(RT) / units));
+  const int64_t most = c->n_cu * per_cu(DP, RT) * rounds(a.seqs);
+  const int64_t nsplit = std::max<int64_t>(1, std::min<int64_t>(xst::SPLITS, most / units));
   cut.chunk = (int32_t)((blocks + nsplit - 1) / nsplit);
-  if (cut.chunk < 2 * xst::NW) cut.chunk = 2 * xst::NW;  // two blocks a wave at least
+  // Two blocks a wave at least, and no split for its own sake: a join costs
+  // 5 us (300 slots: 9.8 us whole, 15 split; 1,777 slots: 14.9 split, 15.8 in
+  // halves).
+  if (cut.chunk < 2 * xst::NW) cut.chunk = 2 * xst::NW;
+  if (blocks <= 4 * xst::NW) cut.chunk = (int32_t)blocks;
   cut.nsplit = (int32_t)((blocks + cut.chunk - 1) / cut.chunk);
   const int64_t groups = a.seqs * a.kv_heads * cut.nsplit;
   const int64_t grid = (groups + 7) / 8 * 8 * cut.tiles, join = a.seqs * a.kv_heads * cut.tiles * RT * xst::Shape<DP, RT>::VH;
   if (grid > 0x7FFFFFFF || join > 0x7FFFFFFF) return XS_ERR_CAPACITY;
-  if (cut.nsplit > 1 && groups * cut.tiles * xst::Shape<DP, RT>::PART > PART_FLOATS) return XS_ERR_CAPACITY;  // (never: groups * tiles <= target)
+  if (cut.nsplit > 1 && groups * cut.tiles * xst::Shape<DP, RT>::PART > c->part_floats) return XS_ERR_CAPACITY;  // (never: groups * tiles <= most)
   cut.groups = (int32_t)groups;
   hipLaunchKernelGGL((xst::attend_kernel<T, DP, RT, EXACT>), dim3((unsigned)grid), dim3(64 * xst::NW), 0, c->stream, a, cut);
   if (cut.nsplit > 1)
     hipLaunchKernelGGL((xst::join_kernel<T, DP, RT>), dim3((unsigned)join), dim3(1024), 0, c->stream, a, cut);
   return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
+}
+
+// The partial results of the largest split call within `dims`.
+int64_t attend_floats(const xs_cache_dims& dims, int n_cu) {
+  int64_t most = 0;
+  auto add = [&](int dp, int rt, int64_t part) { most = std::max(most, n_cu * per_cu(dp, rt) * rounds(dims.max_seqs) * part); };
+  add(64, 1, xst::Shape<64, 1>::PART);
+  add(64, 2, xst::Shape<64, 2>::PART);
+  add(64, 4, xst::Shape<64, 4>::PART);
+  if (dims.head_dim > 64) {
+    add(128, 1, xst::Shape<128, 1>::PART);
+    add(128, 2, xst::Shape<128, 2>::PART);
+    add(128, 4, xst::Shape<128, 4>::PART);
+  }
+  if (dims.head_dim > 128) {
+    add(256, 1, xst::Shape<256, 1>::PART);
+    add(256, 2, xst::Shape<256, 2>::PART);
+  }
+  return most;
 }
 
 template <typename T, int DP>
@@ -1084,9 +1162,10 @@ int commit_dim(xs_cache_context* c, const xs_cache_commit_args& a) {
   return commit_rows<T, 256>(c, a);
 }
 
-// The most moves a head's own workgroup makes; more are dealt to a launch of
-// their own.
-constexpr int64_t EVICT_APART = 128;
+template <int E>
+void evict_run(xs_cache_context* c, const xs_cache_evict_args& a, bool apart) {
+  hipLaunchKernelGGL((xst::evict_kernel<E>), dim3((unsigned)(a.seqs * a.kv_heads)), dim3(xst::EB), 0, c->stream, a, c->evict, apart ? 1 : 0);
+}
 
 }  // namespace
 
@@ -1102,10 +1181,13 @@ int xs_cache_create(int device, const xs_cache_dims* dims, xs_cache_context** ou
   if (!c) return XS_ERR_HIP;
   c->device = device;
   c->dims = *dims;
+  if (hipDeviceGetAttribute(&c->n_cu, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || c->n_cu < 1)
+    c->n_cu = 256;
+  c->part_floats = attend_floats(*dims, c->n_cu);
   const int64_t heads = dims->max_seqs * dims->kv_heads;
   c->evict.words = (dims->capacity + 63) / 64;
   c->evict.pairs = dims->capacity / 2 + 1;
-  if (hipMalloc((void**)&c->part, PART_FLOATS * sizeof(float)) != hipSuccess ||
+  if (hipMalloc((void**)&c->part, c->part_floats * sizeof(float)) != hipSuccess ||
       hipMalloc((void**)&c->evict.kept, heads * c->evict.words * sizeof(uint64_t)) != hipSuccess ||
       hipMalloc((void**)&c->evict.free_, heads * c->evict.pairs * sizeof(int32_t)) != hipSuccess ||
       hipMalloc((void**)&c->evict.filler, heads * c->evict.pairs * sizeof(int32_t)) != hipSuccess ||
@@ -1163,10 +1245,13 @@ int xs_cache_evict(xs_cache_context* c, const xs_cache_evict_args* in) {
   const int64_t heads = in->seqs * in->kv_heads;
   // moves of a head: at most the slots past keep, and the slots of keep
   const int64_t most = limit > in->keep ? std::min(in->keep, limit - in->keep) : 0;
-  const bool apart = most > EVICT_APART;
+  const bool apart = most > xst::NEAR;  // (a head's own workgroup makes a few moves, a launch of its own many)
   const int64_t blocks = (most + xst::ROWS - 1) / xst::ROWS;
   if (heads > 0x7FFFFFFF || (apart && heads * blocks > 0x7FFFFFFF)) return XS_ERR_CAPACITY;
-  hipLaunchKernelGGL(xst::evict_kernel, dim3((unsigned)heads), dim3(xst::EB), 0, c->stream, *in, c->evict, apart ? 0 : 1);
+  if (limit <= 4 * xst::EB) evict_run<4>(c, *in, apart);
+  else if (limit <= 8 * xst::EB) evict_run<8>(c, *in, apart);
+  else if (limit <= 32 * xst::EB) evict_run<32>(c, *in, apart);
+  else evict_run<0>(c, *in, apart);
   if (apart)
     hipLaunchKernelGGL(xst::evict_rows_kernel, dim3((unsigned)(heads * blocks)), dim3(256), 0, c->stream, *in, c->evict, (int)blocks);
   return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
