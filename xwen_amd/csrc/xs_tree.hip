@@ -754,11 +754,11 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 256 ? 3 : 2) void commit_kernel
 // ---------------------------------------------------------------------------
 // Eviction.
 //
-// One workgroup per (sequence, kv head) finds the `keep`-th of the slots' 64-bit
-// ranks (rank_key) by counting digits of 11 bits from the top, each pass over
-// the slots whose digits so far are the chosen ones, until a digit's slots are exactly
-// those still needed: weights that differ in their first 22 bits take two passes,
-// equal weights go on into the positions.  The kept slots go to a bitmap, whose prefix
+// One workgroup per (sequence, kv head) finds the `keep`-th of the slots'
+// weights (weight_word) by counting digits of 11 bits from the top, each pass
+// over the slots whose digits so far are the chosen ones, until a digit's
+// slots are exactly those still needed; where equal weights remain, their positions
+// are counted in the same way.  The kept slots go to a bitmap, whose prefix
 // counts pair the i-th free slot below `keep` with the i-th kept one past it.
 // Only these move: `keep` of `keep` + a few slots moves a few rows, where
 // keeping the slots in order would move nearly all.
@@ -767,14 +767,15 @@ constexpr int EB = 1024;         // threads
 constexpr int EW = EB / 64;      // waves
 constexpr int DIGIT = 11;
 
-// A slot's place in the order of xs_cache_evict, larger first: the held slots
-// above all others, then the weights (the bits of an f32 put in order; NaN
-// below -inf), ties to the lower position.
-XS_DEV uint64_t rank_key(float mass, int pos, bool held) {
+// A slot's place in the order of xs_cache_evict, larger first, in two words:
+// the held slots above all others, then the weights (the bits of an f32 put in
+// order; NaN below -inf), and among equal ones the lower position first.
+XS_DEV uint32_t weight_word(float mass, bool held) {
   const uint32_t u = __float_as_uint(mass + 0.0f);  // (-0 as 0)
   const uint32_t w = mass != mass ? 0u : (u & 0x80000000u ? ~u : u | 0x80000000u);
-  return ((uint64_t)(held ? 0xFFFFFFFFu : w) << 32) | (uint32_t)~((uint32_t)pos ^ 0x80000000u);
+  return held ? 0xFFFFFFFFu : w;
 }
+XS_DEV uint32_t position_word(int pos) { return ~((uint32_t)pos ^ 0x80000000u); }
 
 struct EvictWork {
   uint64_t* kept;   // [heads, words] bitmap of the kept slots
@@ -877,11 +878,8 @@ __global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, 
     return;
   }
   const int64_t next = a.next_pos[b];
-  auto key_at = [&](int s) {
-    const int p = pos[s];
-    return rank_key(mass[s], p, p < a.sinks || p >= next - a.recent);
-  };
-  uint64_t mine[E > 0 ? E : 1];
+  auto held = [&](int p) { return p < a.sinks || p >= next - a.recent; };
+  uint32_t mine[E > 0 ? E : 1];
   if constexpr (E > 0) {
     float m[E];
     int p[E];
@@ -894,7 +892,7 @@ __global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, 
 #pragma unroll
     for (int e = 0; e < E; e++) {
       const int s = e * EB + tid;
-      mine[e] = rank_key(m[e], p[e], p[e] < a.sinks || p[e] >= next - a.recent);
+      mine[e] = weight_word(m[e], held(p[e]));
       if (new_mass != mass && s < keep) {
         new_mass[s] = m[e];
         new_pos[s] = p[e];
@@ -906,7 +904,7 @@ __global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, 
       new_pos[s] = pos[s];
     }
   }
-  // f(first slot of the wave's 64, slot, key) for every slot of the workgroup's waves in turn
+  // f(first of the wave's 64 slots, the lane's, its weight word) over all slots
   auto each = [&](auto f) {
     if constexpr (E > 0) {
 #pragma unroll
@@ -914,28 +912,28 @@ __global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, 
         if (e * EB + wave * 64 < len) f(e * EB + wave * 64, e * EB + tid, mine[e]);
     } else {
 #pragma unroll 4
-      for (int s0 = wave * 64; s0 < len; s0 += EB) f(s0, s0 + lane, key_at(min(s0 + lane, len - 1)));
+      for (int s0 = wave * 64; s0 < len; s0 += EB) {
+        const int s = min(s0 + lane, len - 1), p = pos[s];
+        f(s0, s0 + lane, weight_word(mass[s], held(p)));
+      }
     }
   };
-
-  uint64_t prefix = 0;
-  int shift = 64, need = keep;
+  int need = keep;
   bool exact = false;
-  while (shift > 0 && !exact) {
-    const int bits = min(DIGIT, shift);
-    const int above = shift;  // bits above are settled
-    shift -= bits;
+  // One digit: `digits(s0, s, word, in, digit)` says which slots are counted.
+  // The digit that holds the need-th is returned; need is what of it is needed.
+  auto count = [&](auto digits) {
     hist[tid] = 0;
     hist[tid + EB] = 0;
     __syncthreads();
-    each([&](int, int s, uint64_t k) {
-      const bool in = s < len && (above == 64 || (k >> (above & 63)) == prefix);
-      const uint32_t digit = (uint32_t)(k >> shift) & ((1u << bits) - 1u);
-      const uint64_t who = __ballot(in);
-      if (who == 0) return;
+    each([&](int, int s, uint32_t k) {
+      bool in;
+      uint32_t digit;
+      digits(s, k, in, digit);
       // (a wave that holds one digit adds it at once: equal weights)
-      const uint32_t first = __builtin_amdgcn_readlane(digit, (int)__builtin_ctzll(who));
-      if (__ballot(in && digit != first) == 0) {
+      const uint32_t first = __builtin_amdgcn_readfirstlane(digit);
+      if (__ballot(digit != first) == 0) {
+        const uint64_t who = __ballot(in);
         if (lane == 0) atomicAdd(&hist[first], (uint32_t)__popcll(who));
       } else if (in) {
         atomicAdd(&hist[digit], 1u);
@@ -954,24 +952,67 @@ __global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, 
       found[2] = found[1] == (int)(one ? c1 : c0);
     }
     __syncthreads();
-    prefix = above < 64 ? (prefix << bits) | (uint32_t)found[0] : (uint64_t)found[0];
     need = found[1];
     exact = found[2] != 0;
+    return (uint32_t)found[0];
+  };
+  // from: the least word that is kept for its weight alone; ties: the word of
+  // which only some are kept, those of at least pfrom by position
+  uint32_t d0 = count([&](int s, uint32_t k, bool& in, uint32_t& d) { in = s < len; d = k >> 21; });
+  uint64_t from = (uint64_t)d0 << 21;
+  uint32_t ties = 0, pfrom = 0;
+  bool tied = false;
+  if (!exact) {
+    const uint32_t d1 = count([&](int s, uint32_t k, bool& in, uint32_t& d) { in = s < len && k >> 21 == d0; d = (k >> 10) & 0x7FFu; });
+    d0 = d0 << 11 | d1;
+    from = (uint64_t)d0 << 10;
   }
-  // the bitmap; slots equal in weight and position (not exact) come by wave 0
+  if (!exact) {
+    const uint32_t d1 = count([&](int s, uint32_t k, bool& in, uint32_t& d) { in = s < len && k >> 10 == d0; d = k & 0x3FFu; });
+    ties = d0 << 10 | d1;
+    from = ties;
+  }
+  if (!exact) {
+    tied = true;
+    from = (uint64_t)ties + 1;
+    auto word_at = [&](int s) { return position_word(pos[min(s, len - 1)]); };
+    uint32_t p0 = count([&](int s, uint32_t k, bool& in, uint32_t& d) { in = s < len && k == ties; d = word_at(s) >> 21; });
+    pfrom = p0 << 21;
+    if (!exact) {
+      p0 = p0 << 11 | count([&](int s, uint32_t k, bool& in, uint32_t& d) {
+        const uint32_t q = word_at(s);
+        in = s < len && k == ties && q >> 21 == p0;
+        d = (q >> 10) & 0x7FFu;
+      });
+      pfrom = p0 << 10;
+    }
+    if (!exact) {
+      p0 = p0 << 10 | count([&](int s, uint32_t k, bool& in, uint32_t& d) {
+        const uint32_t q = word_at(s);
+        in = s < len && k == ties && q >> 10 == p0;
+        d = q & 0x3FFu;
+      });
+      pfrom = p0;
+    }
+  }
+  // the bitmap
   uint64_t* kept = E > 0 ? word : w.kept + bh * w.words;
   const int words = (len + 63) / 64;
-  each([&](int s0, int s, uint64_t k) {
-    k >>= shift;
-    const uint64_t bit = __ballot(s < len && (k > prefix || (exact && k == prefix)));
+  each([&](int s0, int s, uint32_t k) {
+    bool in = k >= from;
+    if (tied && k == ties) {
+      const uint32_t q = position_word(pos[min(s, len - 1)]);
+      in = exact ? q >= pfrom : q > pfrom;
+    }
+    const uint64_t bit = __ballot(s < len && in);
     if (lane == 0) kept[s0 / 64] = bit;
   });
   __syncthreads();
-  if (!exact) {
+  if (!exact) {  // slots equal in weight and position: the lowest of them
     if (wave == 0)
       for (int i = 0; i < words && need > 0; i++) {
-        const int s = i * 64 + lane;
-        uint64_t eq = __ballot(s < len && key_at(min(s, len - 1)) == prefix);
+        const int s = min(i * 64 + lane, len - 1), p = pos[s];
+        uint64_t eq = __ballot(i * 64 + lane < len && position_word(p) == pfrom && weight_word(mass[s], held(p)) == ties);
         while (__popcll(eq) > need) eq &= ~(1ull << (63 - __builtin_clzll(eq)));
         need -= __popcll(eq);
         if (eq && lane == 0) kept[i] |= eq;
