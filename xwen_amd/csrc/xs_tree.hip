@@ -136,6 +136,13 @@ XS_DEV float row_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// The i-th of a unit's n workgroups takes this of its parts.  Workgroups go to
+// the XCDs in turn: with n even, a part would be on the same XCDs for every
+// unit, and the first XCDs would have the short sequences' few parts to
+// themselves (32 sequences of 327 to 8,192 slots: 188 us, turned 151); with n
+// odd the units turn by themselves.
+XS_DEV int turned(int i, int unit, int n) { return n & 1 ? i : (int)((unsigned)(i + unit) % (unsigned)n); }
+
 // How a call is cut: `groups` (sequence, kv head, split) of `tiles` row tiles
 // each, a split taking `chunk` key blocks of its sequence.
 struct Cut {
@@ -382,8 +389,7 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
   const int tile = (blockIdx.x >> 3) % cut.tiles;
   const int group = ((blockIdx.x >> 3) / cut.tiles) * 8 + (blockIdx.x & 7);
   if (group >= cut.groups) return;
-  // (rotated by the head: the short sequences' few splits would otherwise all be on the first XCDs)
-  const int bh = group / cut.nsplit, split = (group + bh) % cut.nsplit;
+  const int bh = group / cut.nsplit, split = turned(group % cut.nsplit, bh, cut.nsplit);
   const int kh = bh % (int)a.kv_heads, b = bh / (int)a.kv_heads;
   // (the rows that the launch is sized for: their loads need not wait for the
   // sequence's own sizes)
@@ -607,8 +613,8 @@ XS_DEV int read_path(const xs_cache_commit_args& a, int b, int len, int64_t limi
 // registers and row tiles, and over lane groups once.  A wave keeps RT row tiles
 // in registers and walks its share of the keys in blocks of 32; more rows than that take further passes
 // over the share, which add to what the same lanes wrote.  Bound by the one
-// read of the keys.  The workgroup after a head's last share weighs the
-// path's own keys (a row sees the ranks up to its own) and appends the path.
+// read of the keys.  A head's first workgroup weighs the path's own keys (a
+// row sees the ranks up to its own), with two waves, and appends the path with the others.
 
 template <int DP, int RT>
 struct Rows {
@@ -686,10 +692,11 @@ template <typename T, int DP, int RT, bool EXACT>
 __global__ __launch_bounds__(64 * NW, DP * RT <= 256 ? 3 : 2) void commit_kernel(const xs_cache_commit_args a, int shares, int share, float scale) {
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int blk = blockIdx.x % shares, kh = (blockIdx.x / shares) % (int)a.kv_heads, b = blockIdx.x / (shares * (int)a.kv_heads);
-  const bool tail = blk == shares - 1;
+  const int bh = blockIdx.x / shares, blk = turned(blockIdx.x % shares, bh, shares);
+  const int kh = bh % (int)a.kv_heads, b = bh / (int)a.kv_heads;
+  const bool tail = blk == 0;
   const int len = a.len[b], G = (int)(a.q_heads / a.kv_heads);
-  if (!tail && blk * NW * share * KB >= len) return;
+  if (!tail && (blk - 1) * NW * share * KB >= len) return;
   int node, m;
   const int st = read_path(a, b, len, a.max_len ? a.max_len : a.capacity, &node, &m);
   if (tail && kh == 0 && threadIdx.x == 0) {
@@ -703,12 +710,12 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 256 ? 3 : 2) void commit_kernel
   Rows<DP, RT> w;
   if (!tail) {
     const uint16_t* ck = (const uint16_t*)a.cache.k + b * a.cache.seq_stride + kh * a.cache.head_stride;
-    const int end = min((blk + 1) * NW * share * KB, len);
+    const int end = min(blk * NW * share * KB, len);
     int row0 = 0;
     do {
       load_rows<DP, RT, EXACT>(a, w, b, kh, G, node, row0, R);
       const float* from = row0 == 0 ? a.mass : a.new_mass;
-      for (int key0 = (blk * NW * share + wave) * KB; key0 < end; key0 += NW * KB) {
+      for (int key0 = ((blk - 1) * NW * share + wave) * KB; key0 < end; key0 += NW * KB) {
         const uint16_t* kp[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) kp[u] = ck + min(key0 + 16 * u + x, len - 1) * a.cache.slot_stride;
@@ -742,7 +749,9 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 256 ? 3 : 2) void commit_kernel
   if (a.pos && (int)threadIdx.x < m) a.pos[slots + len + threadIdx.x] = a.next_pos[b] + threadIdx.x;
   const int parts = a.head_dim / 8;
   const int64_t from = b * a.fresh.seq_stride + kh * a.fresh.head_stride, to = b * a.cache.seq_stride + kh * a.cache.head_stride;
-  for (int j = threadIdx.x; j - lane < m * parts; j += 64 * NW) {  // (whole waves: the path is in their lanes)
+  const int skip = a.q ? 128 : 0;  // (the weighing waves' threads)
+  if ((int)threadIdx.x < skip) return;
+  for (int j = threadIdx.x - skip; j - lane < m * parts; j += 64 * NW - skip) {  // (whole waves: the path is in their lanes)
     const int r = min(j / parts, m - 1), d = j % parts * 8;
     const int64_t f = from + __shfl(node, r) * a.fresh.slot_stride + d, s = to + (len + r) * a.cache.slot_stride + d;
     if (j >= m * parts) continue;
@@ -1166,18 +1175,18 @@ int attend_dim(xs_cache_context* c, const xs_tree_attend_args& a) {
   return attend_rows<T, 256>(c, a);
 }
 
-// Waves that a commit's keys are dealt to, and the most key blocks that a wave
-// takes: enough waves for every SIMD to hold three, each with many more keys
-// than rows to load.
-constexpr int64_t COMMIT_WAVES = 4096;
-constexpr int64_t COMMIT_BLOCKS = 16;
+// Workgroups of commit_kernel that a CU holds at once, as its launch bound asks.
+constexpr int64_t commit_per_cu(int dp, int rt) { return dp * rt <= 256 ? 3 : 2; }
 
 template <typename T, int DP, int RT>
 int commit_run(xs_cache_context* c, const xs_cache_commit_args& a) {
   const int64_t limit = a.max_len ? a.max_len : a.capacity;
   const int64_t blocks = (limit + xst::KB - 1) / xst::KB, heads = a.seqs * a.kv_heads;
-  int64_t share = blocks * heads / COMMIT_WAVES;
-  share = std::max<int64_t>(1, std::min(share, COMMIT_BLOCKS));
+  // Key blocks of a wave: the device filled as often as attention's (rounds),
+  // and at least RT, so that a wave reads twice as many keys as rows (2 heads of 65,536
+  // slots of 256, 8 nodes: 38 us with 4, 63 with 1).
+  const int64_t waves = xst::NW * c->n_cu * commit_per_cu(DP, RT) * rounds(a.seqs);
+  const int64_t share = std::max<int64_t>(RT, (blocks * heads + waves - 1) / waves);
   const int64_t shares = (a.q ? (blocks + xst::NW * share - 1) / (xst::NW * share) : 0) + 1;
   if (heads * shares > 0x7FFFFFFF) return XS_ERR_CAPACITY;
   const dim3 grid((unsigned)(heads * shares)), block(64 * xst::NW);
