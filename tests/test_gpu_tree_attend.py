@@ -202,11 +202,40 @@ def test_extreme_scores(ctx, nodes):
     agree(c, run(ctx, c, scale=0.125, out=blank(c)), scale=0.125)
 
 
+@pytest.mark.parametrize("nodes", [5, 48])
 @pytest.mark.parametrize("scale", [0.0, -0.3, 4.0])
-def test_scales(ctx, scale):
+def test_scales(ctx, scale, nodes):
     rng = np.random.default_rng(9)
-    c = case(rng, [120, 3], 5, 4, 2, 64, HF)
+    c = case(rng, [320, 3], nodes, 4, 2, 64, HF)
     agree(c, run(ctx, c, scale=scale, out=blank(c)), scale=scale)
+
+
+@pytest.mark.parametrize("d", [64, 72, 128, 136])
+@pytest.mark.parametrize("nodes,hq,h", [(33, 2, 1), (64, 4, 2), (64, 4, 1), (64, 5, 1), (20, 16, 1), (64, 16, 1)])
+def test_many_rows(ctx, nodes, hq, h, d):
+    """More rows than a wave holds: tiles of several waves, some of them empty, at lengths
+    about the blocks (32) and stages (64) in which the keys are read."""
+    rng = np.random.default_rng(nodes + d)
+    lens = [0, 31, 32, 63, 64, 65, 96, 127, 128, 129, 190, 257]
+    c = case(rng, lens, nodes, hq, h, d, BF if d % 64 else HF, used=[max(0, nodes - (b % 4) * 7) for b in range(len(lens))])
+    agree(c, run(ctx, c, out=blank(c)))
+
+
+def test_extreme_scores_of_many_rows(ctx):
+    """As test_extreme_scores, where four waves share the keys; the maximum grows late, in steps."""
+    rng = np.random.default_rng(16)
+    c = case(rng, [300, 300, 300, 300, 900], 40, 8, 2, 64, BF)
+    for t in ("q", "k", "fk"):
+        c[t][:, :, :, 0] = 0.0
+    c["q"][:, :, :, 0] = 1.0
+    c["k"][0, :, :, 0] = -math.inf
+    c["fk"][0, :, :, 0] = -math.inf
+    c["k"][1, :, :, 0] = torch.finfo(BF).min
+    c["fk"][1, :, :, 0] = torch.finfo(BF).min
+    c["k"][2, 7, 1, 0] = math.inf
+    c["k"][3, 99, 0, 0] = math.nan
+    c["k"][4, :899, :, 0] = (torch.arange(899, device="cuda") * 0.9)[:, None].to(BF)
+    agree(c, run(ctx, c, scale=0.125, out=blank(c)), scale=0.125)
 
 
 def test_offsets_past_32_bits(ctx):

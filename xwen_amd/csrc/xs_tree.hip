@@ -197,39 +197,43 @@ struct Wave {
     }
   }
 
-  // The weights of a tile's eight scores s (less the reference) to B's registers.
+  // A tile's eight scores s (less the reference) times the scale; the largest.
   // `on` is the lane's mask of the block's keys.
   template <bool MASKED>
-  XS_DEV u32x4 weights(int t, const f32x4 (&s)[2], float scale, uint32_t on) {
+  XS_DEV float scaled(const f32x4 (&s)[2], float scale, uint32_t on, float (&x)[8]) {
     constexpr float OFF = offset_of(T{});
     const int g = (threadIdx.x & 63) >> 4;
-    float x[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
       x[e] = OFF == 0.0f ? s[e >> 2][e & 3] * scale : __builtin_fmaf(s[e >> 2][e & 3], scale, OFF);
       if (MASKED) x[e] = ((on >> (4 * g + (e & 3) + 16 * (e >> 2))) & 1u) ? x[e] : NEG_INF;
     }
-    float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    if (__any(top > most[t])) {
-      top = row_max(top);
-      if (top > most[t]) {
-        const float old = c[t][0];
-        const float ref = scale == 0.0f ? old : old - (top - OFF) / scale;
-        const float step = (ref - old) * scale;  // (to a reference as it is held)
-        const float keep = most[t] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(step);
-        c[t] = (f32x4){ref, ref, ref, ref};
-        most[t] = LAZY + OFF;
-        l[t] *= keep;
+    return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+  }
+  // Moves the tile's reference to rows' maxima past `most` (rare).
+  XS_DEV void rebase(int t, float top, float scale, float (&x)[8]) {
+    constexpr float OFF = offset_of(T{});
+    top = row_max(top);
+    if (top > most[t]) {
+      const float old = c[t][0];
+      const float ref = scale == 0.0f ? old : old - (top - OFF) / scale;
+      const float step = (ref - old) * scale;  // (to a reference as it is held)
+      const float keep = most[t] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(step);
+      c[t] = (f32x4){ref, ref, ref, ref};
+      most[t] = LAZY + OFF;
+      l[t] *= keep;
 #pragma unroll
-        for (int f = 0; f < S::NF; f++) o[t][f] *= keep;
+      for (int f = 0; f < S::NF; f++) o[t][f] *= keep;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          x[e] += step;
-          // (a reference so large that it cannot move by so little)
-          if (x[e] > LAZY + OFF) x[e] = LAZY + OFF;
-        }
+      for (int e = 0; e < 8; e++) {
+        x[e] += step;
+        // (a reference so large that it cannot move by so little)
+        if (x[e] > LAZY + OFF) x[e] = LAZY + OFF;
       }
     }
+  }
+  // The weights, rounded, in B's order.
+  XS_DEV u32x4 weights(int t, const float (&x)[8]) {
     float p[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(x[e]);
@@ -242,6 +246,24 @@ struct Wave {
   // The exponent of two that l and o carry.
   XS_DEV float reference(int t, float scale) const { return -c[t][0] * scale - offset_of(T{}); }
 };
+
+// O^T += V^T P^T over a block: v holds 16 bytes of each of the lane's eight
+// keys, pf the weights.
+template <typename T, int DP, int RT>
+XS_DEV void accumulate(Wave<T, DP, RT>& w, const uint32_t (&v)[8][Shape<DP, RT>::VH][Shape<DP, RT>::VE / 2], const u32x4 (&pf)[RT]) {
+  using S = Shape<DP, RT>;
+#pragma unroll
+  for (int h = 0; h < S::VH; h++)
+#pragma unroll
+    for (int j = 0; j < S::VE; j++) {
+      u32x4 a;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        a[i] = __builtin_amdgcn_perm(v[2 * i + 1][h][j / 2], v[2 * i][h][j / 2], (j & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+      for (int t = 0; t < RT; t++) w.o[t][h * S::VE + j] = mfma(T{}, a, pf[t], w.o[t][h * S::VE + j]);
+    }
+}
 
 // One block of 32 keys from base pointers (elements of one kv head): `limit`
 // keys of the source exist, `on` is the lane's mask of the block's keys for
@@ -297,7 +319,10 @@ XS_DEV void block(Wave<T, DP, RT>& w, const uint16_t* kp, const uint16_t* vp, in
       s[0] = mfma(T{}, k[0][c], w.q[t][c], s[0]);
       s[1] = mfma(T{}, k[1][c], w.q[t][c], s[1]);
     }
-    pf[t] = w.template weights<MASKED>(t, s, scale, MASKED ? on[t] : 0u);
+    float xs[8];
+    const float top = w.template scaled<MASKED>(s, scale, MASKED ? on[t] : 0u, xs);
+    if (__any(top > w.most[t])) w.rebase(t, top, scale, xs);
+    pf[t] = w.weights(t, xs);
   }
   if (MASKED) {
     // Values of keys past the source count for nothing, whatever they hold.
@@ -328,17 +353,7 @@ XS_DEV void block(Wave<T, DP, RT>& w, const uint16_t* kp, const uint16_t* vp, in
           }
     }
   }
-#pragma unroll
-  for (int h = 0; h < S::VH; h++)
-#pragma unroll
-    for (int j = 0; j < S::VE; j++) {
-      u32x4 a;
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        a[i] = __builtin_amdgcn_perm(v[2 * i + 1][h][j / 2], v[2 * i][h][j / 2], (j & 1) ? 0x07060302u : 0x05040100u);
-#pragma unroll
-      for (int t = 0; t < RT; t++) w.o[t][h * S::VE + j] = mfma(T{}, a, pf[t], w.o[t][h * S::VE + j]);
-    }
+  accumulate(w, v, pf);
 }
 
 // Two fragments (2 pair and 2 pair + 1 of half h) of a row tile's result: the
@@ -498,6 +513,221 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
         part[S::STAT + 32 * t + x] = top;
         part[S::STAT + 32 * t + 16 + x] = all;
         part[S::ODD] = odd ? 1.0f : 0.0f;
+      }
+    }
+  }
+}
+
+// Many rows (more than one wave's): the four waves of a workgroup take RT row
+// tiles each and share the keys, which come through LDS in stages of SK, three
+// buffers deep: while one is read, the next is complete and the one after it on its way from memory
+// in registers.  Per block of 32 keys a wave does RT * (2 DP/32 + DP/16)
+// matrix instructions of 16 cycles and about as many cycles of vector work (8
+// exponentials a tile of 16 cycles each, then scaling, maxima, sums, packing,
+// the byte permutes), so the two are laid side by side: the next block's
+// scores beside this block's exponentials, this block's products beside the next
+// block's maxima.  Reading the keys from L2 in every wave instead, 64 bytes a
+// cycle and CU, takes as long as the matrix instructions, and not beside them:
+// 8 sequences of 64 nodes over 32,768 slots XWIDE.
+template <int DP>
+struct Stage {
+  static constexpr int SK = DP > 128 ? 32 : 64;
+  static constexpr int CH = DP / 8;                    // 16-byte chunks of a row
+  static constexpr int PER = SK * CH / (64 * NW);      // chunks a thread moves, of k and of v
+  static constexpr int TURN = CH < 16 ? CH - 1 : 15;   // k's chunks are turned by the row, so that 16 rows' reads meet 16 banks
+};
+
+template <typename T, int DP, int RT, bool EXACT>
+__global__ __launch_bounds__(64 * NW, 1) void attend_wide_kernel(const xs_tree_attend_args a, const Cut cut) {
+  using S = Shape<DP, RT>;
+  using G = Stage<DP>;
+  __shared__ u32x4 lk[3][G::SK * G::CH];
+  __shared__ u32x4 lv[3][G::SK * G::CH];
+  const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wgs = cut.tiles / NW;  // workgroups of a split: NW tiles each
+  const int wg = (blockIdx.x >> 3) % wgs, tile = wg * NW + wave;
+  const int group = ((blockIdx.x >> 3) / wgs) * 8 + (blockIdx.x & 7);
+  if (group >= cut.groups) return;
+  const int bh = group / cut.nsplit, split = turned(group % cut.nsplit, bh, cut.nsplit);
+  const int kh = bh % (int)a.kv_heads, b = bh / (int)a.kv_heads;
+  const int row0 = tile * RT * 16, parent = parent_of(a, b);
+  const Seq sq(a, b);
+  if (split == 0 && wg == 0 && kh == 0 && threadIdx.x == 0) a.seq_status[b] = sq.bad ? XS_ROW_BAD_PARAM : XS_ROW_OK;
+  if (sq.bad) return;
+  const int R = sq.n * cut.G;
+  const int total = sq.blocks(), cached = (sq.len + KB - 1) / KB;
+  const int first = split * cut.chunk, last = min(first + cut.chunk, total);
+  if (wg * NW * RT * 16 >= R || first >= total) return;
+
+  Wave<T, DP, RT> w;
+  w.init();
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    const int row = row0 + 16 * t + x;
+    const bool in = row < R;
+    const int node = in ? row / cut.G : 0, head = kh * cut.G + (in ? row % cut.G : 0);
+    const uint16_t* p = (const uint16_t*)a.q + b * a.q_seq_stride + node * a.q_node_stride + head * a.q_head_stride;
+#pragma unroll
+    for (int c = 0; c < S::KC; c++) {
+      const int d = 32 * c + 8 * g;
+      w.q[t][c] = in && (EXACT || d < a.head_dim) ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0};
+    }
+  }
+
+  // whole stages of the cache
+  constexpr int SB = G::SK / KB;
+  const int stages = max(0, min(last, sq.len / KB) - first) / SB;
+  const int64_t c0 = b * a.cache.seq_stride + kh * a.cache.head_stride;
+  u32x4 rk[G::PER], rv[G::PER];
+  auto fetch = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < G::PER; i++) {
+      const int q = i * 64 * NW + threadIdx.x, row = q / G::CH, ch = q % G::CH;
+      const int64_t at = c0 + (int64_t)(first * KB + s * G::SK + row) * a.cache.slot_stride + ch * 8;
+      const bool in = EXACT || ch * 8 < a.head_dim;
+      rk[i] = in ? *(const u32x4*)((const uint16_t*)a.cache.k + at) : (u32x4){0, 0, 0, 0};
+      rv[i] = in ? *(const u32x4*)((const uint16_t*)a.cache.v + at) : (u32x4){0, 0, 0, 0};
+    }
+  };
+  auto put = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < G::PER; i++) {
+      const int q = i * 64 * NW + threadIdx.x, row = q / G::CH, ch = q % G::CH;
+      lk[s % 3][row * G::CH + (ch ^ (row & G::TURN))] = rk[i];
+      lv[s % 3][q] = rv[i];
+    }
+  };
+  // the scores of block j, counted in blocks from `first`
+  auto scores = [&](int j, f32x4 (&s)[RT][2]) {
+    const u32x4* k = lk[(j / SB) % 3];
+#pragma unroll
+    for (int t = 0; t < RT; t++) s[t][0] = s[t][1] = w.c[t];
+#pragma unroll
+    for (int c = 0; c < S::KC; c++) {
+      u32x4 f[2];
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const int row = (j % SB) * KB + 16 * u + x;
+        f[u] = k[row * G::CH + ((4 * c + g) ^ (row & G::TURN))];
+      }
+#pragma unroll
+      for (int t = 0; t < RT; t++) {
+        s[t][0] = mfma(T{}, f[0], w.q[t][c], s[t][0]);
+        s[t][1] = mfma(T{}, f[1], w.q[t][c], s[t][1]);
+      }
+    }
+  };
+  if (stages > 0) {
+    fetch(0);
+    put(0);
+    __syncthreads();
+    if (stages > 1) fetch(1);
+    float xs[RT][8];
+    auto prepare = [&](const f32x4 (&s)[RT][2]) {
+      float top[RT];
+      bool move = false;
+#pragma unroll
+      for (int t = 0; t < RT; t++) {
+        top[t] = w.template scaled<false>(s[t], cut.scale, 0u, xs[t]);
+        move = move || top[t] > w.most[t];
+      }
+      return move;
+    };
+    auto settle = [&]() {
+#pragma unroll
+      for (int t = 0; t < RT; t++) {
+        const float top = fmaxf(fmaxf(fmaxf(xs[t][0], xs[t][1]), fmaxf(xs[t][2], xs[t][3])), fmaxf(fmaxf(xs[t][4], xs[t][5]), fmaxf(xs[t][6], xs[t][7])));
+        w.rebase(t, top, cut.scale, xs[t]);
+      }
+    };
+    {
+      f32x4 s[RT][2];
+      scores(0, s);
+      if (__any(prepare(s))) settle();
+    }
+    const int blocks = stages * SB;
+#pragma unroll 1
+    for (int st = 0; st < stages; st++) {
+#pragma unroll
+      for (int sub = 0; sub < SB; sub++) {
+        const int j = st * SB + sub;
+        if (sub == SB - 1 && st + 1 < stages) {
+          put(st + 1);
+          __syncthreads();
+          if (st + 2 < stages) fetch(st + 2);
+        }
+        const bool more = j + 1 < blocks;
+        f32x4 s[RT][2];
+        u32x4 pf[RT];
+        scores(more ? j + 1 : j, s);
+#pragma unroll
+        for (int t = 0; t < RT; t++) pf[t] = w.weights(t, xs[t]);
+        uint32_t v[8][S::VH][S::VE / 2];
+        const uint32_t* base = (const uint32_t*)lv[st % 3];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int row = sub * KB + 4 * g + (e & 3) + 16 * (e >> 2);
+#pragma unroll
+          for (int h = 0; h < S::VH; h++)
+#pragma unroll
+            for (int i = 0; i < S::VE / 2; i++) v[e][h][i] = base[row * G::CH * 4 + 64 * h + S::VE / 2 * x + i];
+        }
+        accumulate(w, v, pf);
+        const bool move = prepare(s);
+        if (more && __any(move)) settle();
+      }
+    }
+  }
+
+  // the rest: part of a stage, the last block of the cache, the tree
+  const uint64_t sees = ancestors(parent, sq.n);
+  uint64_t mine[RT];  // what the lane's rows see of the tree
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    const int row = row0 + 16 * t + x;
+    mine[t] = __shfl(sees, min(row / cut.G, 63));
+    if (row >= R) mine[t] = 0;
+  }
+  if (row0 >= R) return;
+#pragma unroll 1
+  for (int i = first + stages * SB; i < last; i++) {
+    const bool in_tree = i >= cached;
+    const int key0 = (in_tree ? i - cached : i) * KB, limit = in_tree ? sq.n : sq.len;
+    const xs_kv& kv = in_tree ? a.fresh : a.cache;
+    const int64_t at = b * kv.seq_stride + kh * kv.head_stride;
+    uint32_t on[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+      on[t] = in_tree ? (uint32_t)(mine[t] >> key0) : sq.len - key0 >= KB ? ~0u : (1u << (sq.len - key0)) - 1u;
+    block<T, DP, RT, EXACT, true>(w, (const uint16_t*)kv.k + at, (const uint16_t*)kv.v + at, kv.slot_stride, key0, limit, a.head_dim,
+                                  cut.scale, on, in_tree);
+  }
+  constexpr int PAIRS = S::VE / 2;
+  const bool whole = first == 0 && last == total;
+  float* part = cut.part + (((int64_t)bh * cut.nsplit + split) * cut.tiles + tile) * S::PART;
+#pragma unroll
+  for (int t = 0; t < RT; t++) {
+    float l = row_sum(w.l[t]);
+    if (mine[t] == 0) l = 0.0f;
+    const float ref = l == 0.0f ? NEG_INF : w.reference(t, cut.scale);
+#pragma unroll
+    for (int f = 0; f < S::NF; f++)
+      if (l == 0.0f) w.o[t][f] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+    if (whole) {
+#pragma unroll
+      for (int h = 0; h < S::VH; h++)
+#pragma unroll
+        for (int pair = 0; pair < PAIRS; pair++)
+          store_pair<T, DP>(a, cut.G, b, kh, row0 + 16 * t + x, R, h, pair, w.o[t][h * S::VE + 2 * pair], w.o[t][h * S::VE + 2 * pair + 1], ref,
+                            l, w.odd, sq.n);
+    } else {
+#pragma unroll
+      for (int f = 0; f < S::NF; f++) ((f32x4*)part)[(t * S::NF + f) * 64 + lane] = w.o[t][f];
+      if (g == 0) {
+        part[S::STAT + 32 * t + x] = ref;
+        part[S::STAT + 32 * t + 16 + x] = l;
+        part[S::ODD] = w.odd ? 1.0f : 0.0f;
       }
     }
   }
@@ -1108,17 +1338,19 @@ constexpr int64_t per_cu(int dp, int rt) { return dp * rt <= 64 ? 4 : dp * rt <=
 // against twice, while 32 of 8,192 take 222 instead of 214).
 constexpr int64_t rounds(int64_t seqs) { return seqs > 1 ? 4 : 1; }
 
-template <typename T, int DP, int RT, bool EXACT>
+template <typename T, int DP, int RT, bool EXACT, bool WIDE>
 int attend_run(xs_cache_context* c, const xs_tree_attend_args& a) {
   xst::Cut cut;
   cut.G = (int32_t)(a.q_heads / a.kv_heads);
-  cut.tiles = (int32_t)((a.nodes * cut.G + 16 * RT - 1) / (16 * RT));
+  constexpr int WAVES = WIDE ? xst::NW : 1;  // of a workgroup, with rows of their own
+  const int64_t wgs = (a.nodes * cut.G + 16 * RT * WAVES - 1) / (16 * RT * WAVES);
+  cut.tiles = (int32_t)(wgs * WAVES);
   cut.scale = a.scale * xst::LOG2E;
   cut.part = c->part;
   const int64_t limit = a.max_len ? a.max_len : a.capacity;
   const int64_t blocks = (limit + xst::KB - 1) / xst::KB + (a.nodes + xst::KB - 1) / xst::KB;
-  const int64_t units = a.seqs * a.kv_heads * cut.tiles;
-  const int64_t most = c->n_cu * per_cu(DP, RT) * rounds(a.seqs);
+  const int64_t units = a.seqs * a.kv_heads * wgs;
+  const int64_t most = c->n_cu * (WIDE ? 1 : per_cu(DP, RT)) * rounds(a.seqs);
   const int64_t nsplit = std::max<int64_t>(1, std::min<int64_t>(xst::SPLITS, most / units));
   cut.chunk = (int32_t)((blocks + nsplit - 1) / nsplit);
   // Two blocks a wave at least, and no split for its own sake: a join costs
@@ -1128,11 +1360,14 @@ int attend_run(xs_cache_context* c, const xs_tree_attend_args& a) {
   if (blocks <= 4 * xst::NW) cut.chunk = (int32_t)blocks;
   cut.nsplit = (int32_t)((blocks + cut.chunk - 1) / cut.chunk);
   const int64_t groups = a.seqs * a.kv_heads * cut.nsplit;
-  const int64_t grid = (groups + 7) / 8 * 8 * cut.tiles, join = a.seqs * a.kv_heads * cut.tiles * RT * xst::Shape<DP, RT>::VH;
+  const int64_t grid = (groups + 7) / 8 * 8 * wgs, join = a.seqs * a.kv_heads * cut.tiles * RT * xst::Shape<DP, RT>::VH;
   if (grid > 0x7FFFFFFF || join > 0x7FFFFFFF) return XS_ERR_CAPACITY;
   if (cut.nsplit > 1 && groups * cut.tiles * xst::Shape<DP, RT>::PART > c->part_floats) return XS_ERR_CAPACITY;  // (never: groups * tiles <= most)
   cut.groups = (int32_t)groups;
-  hipLaunchKernelGGL((xst::attend_kernel<T, DP, RT, EXACT>), dim3((unsigned)grid), dim3(64 * xst::NW), 0, c->stream, a, cut);
+  if constexpr (WIDE)
+    hipLaunchKernelGGL((xst::attend_wide_kernel<T, DP, RT, EXACT>), dim3((unsigned)grid), dim3(64 * xst::NW), 0, c->stream, a, cut);
+  else
+    hipLaunchKernelGGL((xst::attend_kernel<T, DP, RT, EXACT>), dim3((unsigned)grid), dim3(64 * xst::NW), 0, c->stream, a, cut);
   if (cut.nsplit > 1)
     hipLaunchKernelGGL((xst::join_kernel<T, DP, RT>), dim3((unsigned)join), dim3(1024), 0, c->stream, a, cut);
   return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
@@ -1141,31 +1376,45 @@ int attend_run(xs_cache_context* c, const xs_tree_attend_args& a) {
 // The partial results of the largest split call within `dims`.
 int64_t attend_floats(const xs_cache_dims& dims, int n_cu) {
   int64_t most = 0;
-  auto add = [&](int dp, int rt, int64_t part) { most = std::max(most, n_cu * per_cu(dp, rt) * rounds(dims.max_seqs) * part); };
-  add(64, 1, xst::Shape<64, 1>::PART);
-  add(64, 2, xst::Shape<64, 2>::PART);
-  add(64, 4, xst::Shape<64, 4>::PART);
+  auto add = [&](int64_t wgs, int64_t part) { most = std::max(most, n_cu * wgs * rounds(dims.max_seqs) * part); };
+  add(per_cu(64, 1), xst::Shape<64, 1>::PART);
+  add(per_cu(64, 2), xst::Shape<64, 2>::PART);
+  add(per_cu(64, 4), xst::Shape<64, 4>::PART);
+  add(1, xst::NW * xst::Shape<64, 4>::PART);
   if (dims.head_dim > 64) {
-    add(128, 1, xst::Shape<128, 1>::PART);
-    add(128, 2, xst::Shape<128, 2>::PART);
-    add(128, 4, xst::Shape<128, 4>::PART);
+    add(per_cu(128, 1), xst::Shape<128, 1>::PART);
+    add(per_cu(128, 2), xst::Shape<128, 2>::PART);
+    add(per_cu(128, 4), xst::Shape<128, 4>::PART);
+    add(1, xst::NW * xst::Shape<128, 4>::PART);
   }
   if (dims.head_dim > 128) {
-    add(256, 1, xst::Shape<256, 1>::PART);
-    add(256, 2, xst::Shape<256, 2>::PART);
+    add(per_cu(256, 1), xst::Shape<256, 1>::PART);
+    add(per_cu(256, 2), xst::Shape<256, 2>::PART);
+    add(1, xst::NW * xst::Shape<256, 2>::PART);
   }
   return most;
+}
+
+#ifndef WIDE_ROWS
+#define WIDE_ROWS 64
+#endif
+template <typename T, int DP, int RT, bool WIDE>
+int attend_exact(xs_cache_context* c, const xs_tree_attend_args& a) {
+  return a.head_dim == DP ? attend_run<T, DP, RT, true, WIDE>(c, a) : attend_run<T, DP, RT, false, WIDE>(c, a);
 }
 
 template <typename T, int DP>
 int attend_rows(xs_cache_context* c, const xs_tree_attend_args& a) {
   const int64_t rows = a.nodes * (a.q_heads / a.kv_heads);
-  const bool exact = a.head_dim == DP;
+  if (rows <= 16) return attend_exact<T, DP, 1, false>(c, a);
+  if (rows <= 32) return attend_exact<T, DP, 2, false>(c, a);
   if constexpr (DP <= 128) {
-    if (rows > 32) return exact ? attend_run<T, DP, 4, true>(c, a) : attend_run<T, DP, 4, false>(c, a);
+    if (rows <= WIDE_ROWS) return attend_exact<T, DP, 4, false>(c, a);
+    if (rows <= 128) return attend_exact<T, DP, 2, true>(c, a);
+    return attend_exact<T, DP, 4, true>(c, a);
+  } else {
+    return attend_exact<T, DP, 2, true>(c, a);
   }
-  if (rows > 16) return exact ? attend_run<T, DP, 2, true>(c, a) : attend_run<T, DP, 2, false>(c, a);
-  return exact ? attend_run<T, DP, 1, true>(c, a) : attend_run<T, DP, 1, false>(c, a);
 }
 
 template <typename T>
