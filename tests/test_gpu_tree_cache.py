@@ -405,6 +405,16 @@ def test_a_speculative_step_over_a_bounded_cache(ctx):
     assert max(seen) > keep
 
 
+@pytest.mark.parametrize("cap", [301, 302, 303, 304])
+def test_evict_slots_off_the_16_byte_grid(ctx, cap):
+    """Per-slot arrays whose rows start anywhere."""
+    rng = np.random.default_rng(cap)
+    c = evict_case(rng, [cap, cap - 7, 150], 3, 64, cap)
+    check_evict(ctx, c, 140, sinks=3, recent=11, in_place=cap % 2 == 0)
+    c = evict_case(rng, [cap, cap - 7, 150], 3, 64, cap, ties=True)
+    check_evict(ctx, c, cap - 9, sinks=3, recent=11)
+
+
 @pytest.mark.parametrize("n", [4096, 4097, 8193, 32_768, 32_769, 70_001])
 def test_evict_lengths_at_the_kernels_bounds(n):
     """Where the slots of a head stop fitting the registers of its workgroup."""

@@ -733,17 +733,25 @@ __global__ __launch_bounds__(64 * NW, 1) void attend_wide_kernel(const xs_tree_a
   }
 }
 
-// Joins the splits of 16 rows and one half of the head, 16 waves: each wave two
-// fragments of a share of the splits, so that all of their loads are in flight
-// at once (a wave that goes through 64 splits one after the other takes 100
-// us).
-constexpr int SPLITS = 256;  // the most splits of a sequence
-template <typename T, int DP, int RT>
-__global__ __launch_bounds__(1024) void join_kernel(const xs_tree_attend_args a, const Cut cut) {
+// Joins the splits of 16 rows and one half of the head: each wave two
+// fragments of one of SHARES shares of the splits, so that the loads of many
+// splits are in flight at once (a wave that goes through 64 splits one after
+// the other takes 100 us), while a few splits take one wave's loads (256 units of four
+// tiles in four splits would start 65,536 waves otherwise).
+constexpr int SPLITS = 256;     // the most splits of a sequence
+constexpr int FEW = 8;          // splits that one share goes through
+template <int DP>
+constexpr int join_shares(bool few) { return few ? 1 : 16 / (Shape<DP, 1>::VE / 2); }
+template <int DP>
+constexpr int join_threads(bool few) { return 64 * (Shape<DP, 1>::VE / 2) * join_shares<DP>(few); }
+
+template <typename T, int DP, int RT, bool FEWER>
+__global__ __launch_bounds__(join_threads<DP>(FEWER)) void join_kernel(const xs_tree_attend_args a, const Cut cut) {
   using S = Shape<DP, RT>;
-  constexpr int PAIRS = S::VE / 2, SHARES = 16 / PAIRS;
-  __shared__ float weight[SPLITS][16];
-  __shared__ float stat[2][16][16];
+  constexpr int PAIRS = S::VE / 2, SHARES = join_shares<DP>(FEWER), WAVES = PAIRS * SHARES;
+  constexpr int MOST = FEWER ? FEW : SPLITS, TURNS = (MOST + 4 * WAVES - 1) / (4 * WAVES);
+  __shared__ float weight[TURNS * 4 * WAVES][16];
+  __shared__ float stat[2][WAVES][16];
   __shared__ int odd;
   __shared__ f32x4 sum[SHARES][S::VE][64];
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
@@ -760,7 +768,7 @@ __global__ __launch_bounds__(1024) void join_kernel(const xs_tree_attend_args a,
   const float* part = cut.part + ((int64_t)bh * cut.nsplit * cut.tiles + tile) * S::PART;
   const int64_t step = (int64_t)cut.tiles * S::PART;
   // the first fragments, on their way while the weights are formed
-  constexpr int AHEAD = 4;
+  constexpr int AHEAD = FEWER ? FEW : 4;
   const int pair = wave % PAIRS, share = wave / PAIRS, f0 = h * S::VE + 2 * pair;
   f32x4 y[AHEAD][2];
 #pragma unroll
@@ -769,11 +777,11 @@ __global__ __launch_bounds__(1024) void join_kernel(const xs_tree_attend_args a,
     y[i][0] = p[0];
     y[i][1] = p[64];
   }
-  // lane (x, g) of wave w takes splits 4 w + g, + 64, ... of row x
-  float m[SPLITS / 64], l[SPLITS / 64], top = NEG_INF, all = 0.0f;
+  // lane (x, g) of wave w takes splits 4 w + g, + 4 WAVES, ... of row x
+  float m[TURNS], l[TURNS], top = NEG_INF, all = 0.0f;
 #pragma unroll
-  for (int i = 0; i < SPLITS / 64; i++) {
-    const int s = 64 * i + 4 * wave + g;
+  for (int i = 0; i < TURNS; i++) {
+    const int s = 4 * (WAVES * i + wave) + g;
     const float* p = part + min(s, n - 1) * step + S::STAT + 32 * t + x;
     m[i] = s < n ? p[0] : NEG_INF;
     l[i] = p[16];
@@ -784,12 +792,12 @@ __global__ __launch_bounds__(1024) void join_kernel(const xs_tree_attend_args a,
   if (g == 0) stat[0][wave][x] = top;
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < 16; j++) top = fmaxf(top, stat[0][j][x]);
+  for (int j = 0; j < WAVES; j++) top = fmaxf(top, stat[0][j][x]);
 #pragma unroll
-  for (int i = 0; i < SPLITS / 64; i++) {
+  for (int i = 0; i < TURNS; i++) {
     const float f = m[i] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m[i] - top);
     if (m[i] != NEG_INF) all += l[i] * f;
-    weight[64 * i + 4 * wave + g][x] = f;
+    weight[4 * (WAVES * i + wave) + g][x] = f;
   }
   all = row_sum(all);
   if (g == 0) stat[1][wave][x] = all;
@@ -809,17 +817,19 @@ __global__ __launch_bounds__(1024) void join_kernel(const xs_tree_attend_args a,
     o[0] += p[0] * f;
     o[1] += p[64] * f;
   }
-  sum[share][2 * pair][lane] = o[0];
-  sum[share][2 * pair + 1][lane] = o[1];
-  __syncthreads();
-  if (share != 0) return;
   all = 0.0f;
 #pragma unroll
-  for (int j = 0; j < 16; j++) all += stat[1][j][x];
+  for (int j = 0; j < WAVES; j++) all += stat[1][j][x];
+  if constexpr (SHARES > 1) {
+    sum[share][2 * pair][lane] = o[0];
+    sum[share][2 * pair + 1][lane] = o[1];
+    __syncthreads();
+    if (share != 0) return;
 #pragma unroll
-  for (int j = 1; j < SHARES; j++) {
-    o[0] += sum[j][2 * pair][lane];
-    o[1] += sum[j][2 * pair + 1][lane];
+    for (int j = 1; j < SHARES; j++) {
+      o[0] += sum[j][2 * pair][lane];
+      o[1] += sum[j][2 * pair + 1][lane];
+    }
   }
   store_pair<T, DP>(a, cut.G, b, kh, row0 + x, R, h, pair, o[0], o[1], top, all, odd, sq.n);
 }
@@ -1073,195 +1083,338 @@ XS_DEV void move_part(const xs_cache_evict_args& a, int64_t head, int from, int 
   *(u32x4*)((uint16_t*)a.cache.v + t) = *(const u32x4*)((const uint16_t*)a.cache.v + f);
 }
 
-// E: slots of a thread, kept in registers (len <= E * EB); 0: any length, read
-// again by every pass.  apart: the rows of k and v are left to
-// evict_rows_kernel (many moves); else there are at most NEAR, made here.
-constexpr int NEAR = 128;
-template <int E>
-__global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, const EvictWork w, int apart) {
-  constexpr int WORDS = E > 0 ? E * EW : 1;
-  typedef typename std::conditional<(E > 0), uint32_t, uint64_t>::type Pair;  // two counts: up to 32,768 each, or any
-  constexpr int HALF = 4 * sizeof(Pair);
-  __shared__ uint32_t hist[1 << DIGIT];
-  __shared__ uint32_t lds32[EW];
-  __shared__ Pair lds[EW];
-  __shared__ Pair base[EB];
-  __shared__ uint64_t word[WORDS];
-  __shared__ int near_free[NEAR], near_filler[NEAR];
-  __shared__ int found[3];  // the digit, the slots still needed of it, whether that is all of it
-  const int64_t bh = blockIdx.x;
-  const int b = (int)(bh / a.kv_heads), kh = (int)(bh % a.kv_heads), tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t limit = a.max_len ? a.max_len : a.capacity;
-  const int len = a.len[b];
-  const bool bad = len < 0 || len > limit;
-  const int keep = (int)min((int64_t)len, a.keep);
-  if (tid == 0) {
-    w.moves[bh] = 0;
-    if (kh == 0) {
-      a.seq_status[b] = bad ? XS_ROW_BAD_PARAM : XS_ROW_OK;
-      a.new_len[b] = bad ? len : keep;
-    }
-  }
-  if (bad) return;
-  const float* mass = a.mass + bh * a.slot_ld;
-  const int32_t* pos = a.pos + bh * a.slot_ld;
-  float* new_mass = a.new_mass + bh * a.slot_ld;
-  int32_t* new_pos = a.new_pos + bh * a.slot_ld;
-  if (len <= keep) {
-    if (new_mass != mass)
-      for (int s = tid; s < keep; s += EB) {
-        new_mass[s] = mass[s];
-        new_pos[s] = pos[s];
-      }
-    return;
-  }
-  const int64_t next = a.next_pos[b];
-  auto held = [&](int p) { return p < a.sinks || p >= next - a.recent; };
-  uint32_t mine[E > 0 ? E : 1];
-  if constexpr (E > 0) {
-    float m[E];
-    int p[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      const int s = min(e * EB + tid, len - 1);
-      m[e] = mass[s];
-      p[e] = pos[s];
-    }
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-      const int s = e * EB + tid;
-      mine[e] = weight_word(m[e], held(p[e]));
-      if (new_mass != mass && s < keep) {
-        new_mass[s] = m[e];
-        new_pos[s] = p[e];
-      }
-    }
-  } else if (new_mass != mass) {
-    for (int s = tid; s < keep; s += EB) {
-      new_mass[s] = mass[s];
-      new_pos[s] = pos[s];
-    }
-  }
-  // f(first of the wave's 64 slots, the lane's, its weight word) over all slots
-  auto each = [&](auto f) {
-    if constexpr (E > 0) {
-#pragma unroll
-      for (int e = 0; e < E; e++)
-        if (e * EB + wave * 64 < len) f(e * EB + wave * 64, e * EB + tid, mine[e]);
-    } else {
-#pragma unroll 4
-      for (int s0 = wave * 64; s0 < len; s0 += EB) {
-        const int s = min(s0 + lane, len - 1), p = pos[s];
-        f(s0, s0 + lane, weight_word(mass[s], held(p)));
-      }
-    }
-  };
-  int need = keep;
+constexpr int REP = 4;     // copies of the counts, by the lane: weights crowd into few digits
+constexpr int NEAR = 128;  // moves that a head's own workgroup makes; more are left to evict_rows_kernel
+
+// What is kept: words above `above`, and of the words equal to `ties` (if tied)
+// those with position words above pabove; and where even positions are alike
+// (need > 0), the first `need` slots of position word ptie.
+struct Cutoff {
+  uint32_t above, ties, pabove, ptie;
+  int need;
+  bool tied;
+};
+
+struct SelectLds {
+  uint32_t hist[REP << DIGIT];
+  uint32_t scan[EW];
+  int found[3];  // the digit, the slots still needed of it, whether that is all of it
+};
+
+// The cutoff of `need` slots.  each(f) calls f(slot, weight word, q) for every
+// slot, whole waves at a time (slots past len among them); q() is its position
+// word, read after positions() has been called.
+template <typename Each, typename Positions>
+XS_DEV Cutoff find_cutoff(SelectLds& lds, int len, int need, Each each, Positions positions) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   bool exact = false;
-  // One digit: `digits(s0, s, word, in, digit)` says which slots are counted.
+  u32x4* const own = (u32x4*)lds.hist + 2 * ((1 << (DIGIT - 1)) - 1 - tid);  // thread i: the i-th pair of digits from the top
+  static_assert(REP == 4, "the copies of a count fill a vector");
+  own[0] = own[1] = (u32x4){0, 0, 0, 0};
+  __syncthreads();
+  // One digit: `digits(s, word, q, in, digit)` says which slots are counted.
   // The digit that holds the need-th is returned; need is what of it is needed.
   auto count = [&](auto digits) {
-    hist[tid] = 0;
-    hist[tid + EB] = 0;
-    __syncthreads();
-    each([&](int, int s, uint32_t k) {
+    each([&](int s, uint32_t k, auto q) {
       bool in;
       uint32_t digit;
-      digits(s, k, in, digit);
+      digits(s, k, q, in, digit);
       // (a wave that holds one digit adds it at once: equal weights)
       const uint32_t first = __builtin_amdgcn_readfirstlane(digit);
       if (__ballot(digit != first) == 0) {
         const uint64_t who = __ballot(in);
-        if (lane == 0) atomicAdd(&hist[first], (uint32_t)__popcll(who));
+        if (lane == 0) atomicAdd(&lds.hist[first * REP], (uint32_t)__popcll(who));
       } else if (in) {
-        atomicAdd(&hist[digit], 1u);
+        atomicAdd(&lds.hist[digit * REP + (lane & (REP - 1))], 1u);
       }
     });
     __syncthreads();
-    // thread i: the i-th pair of digits from the top
-    const int hi = (1 << DIGIT) - 1 - 2 * tid;
-    const uint32_t c1 = hist[hi], c0 = hist[hi - 1];
-    uint32_t all;
-    const int before = (int)block_scan(c1 + c0, lds32, &all);
-    if (before < need && need <= before + (int)(c1 + c0)) {
-      const bool one = need <= before + (int)c1;
-      found[0] = one ? hi : hi - 1;
-      found[1] = need - before - (one ? 0 : (int)c1);
-      found[2] = found[1] == (int)(one ? c1 : c0);
+    const u32x4 h0 = own[0], h1 = own[1];
+    own[0] = own[1] = (u32x4){0, 0, 0, 0};  // (for the next digit)
+    const int c1 = (int)((h1[0] + h1[1]) + (h1[2] + h1[3])), c0 = (int)((h0[0] + h0[1]) + (h0[2] + h0[3]));
+    const uint32_t run = wave_scan((uint32_t)(c1 + c0));
+    if (lane == 63) lds.scan[wave] = run;
+    __syncthreads();
+    int before = (int)run - c1 - c0;
+#pragma unroll
+    for (int i = 0; i < EW; i++) before += i < wave ? (int)lds.scan[i] : 0;
+    if (before < need && need <= before + c1 + c0) {
+      const bool one = need <= before + c1;
+      lds.found[0] = 2 * ((1 << (DIGIT - 1)) - 1 - tid) + (one ? 1 : 0);
+      lds.found[1] = need - before - (one ? 0 : c1);
+      lds.found[2] = lds.found[1] == (one ? c1 : c0);
     }
     __syncthreads();
-    need = found[1];
-    exact = found[2] != 0;
-    return (uint32_t)found[0];
+    need = lds.found[1];
+    exact = lds.found[2] != 0;
+    return (uint32_t)lds.found[0];
   };
-  // from: the least word that is kept for its weight alone; ties: the word of
-  // which only some are kept, those of at least pfrom by position
-  uint32_t d0 = count([&](int s, uint32_t k, bool& in, uint32_t& d) { in = s < len; d = k >> 21; });
-  uint64_t from = (uint64_t)d0 << 21;
-  uint32_t ties = 0, pfrom = 0;
-  bool tied = false;
-  if (!exact) {
-    const uint32_t d1 = count([&](int s, uint32_t k, bool& in, uint32_t& d) { in = s < len && k >> 21 == d0; d = (k >> 10) & 0x7FFu; });
-    d0 = d0 << 11 | d1;
-    from = (uint64_t)d0 << 10;
-  }
-  if (!exact) {
-    const uint32_t d1 = count([&](int s, uint32_t k, bool& in, uint32_t& d) { in = s < len && k >> 10 == d0; d = k & 0x3FFu; });
-    ties = d0 << 10 | d1;
-    from = ties;
-  }
-  if (!exact) {
-    tied = true;
-    from = (uint64_t)ties + 1;
-    auto word_at = [&](int s) { return position_word(pos[min(s, len - 1)]); };
-    uint32_t p0 = count([&](int s, uint32_t k, bool& in, uint32_t& d) { in = s < len && k == ties; d = word_at(s) >> 21; });
-    pfrom = p0 << 21;
-    if (!exact) {
-      p0 = p0 << 11 | count([&](int s, uint32_t k, bool& in, uint32_t& d) {
-        const uint32_t q = word_at(s);
-        in = s < len && k == ties && q >> 21 == p0;
-        d = (q >> 10) & 0x7FFu;
-      });
-      pfrom = p0 << 10;
+  // (a digit that is kept whole lies above a slot that is not, so its lowest
+  // word is at least 1)
+  Cutoff c = {0, 0, 0, 0, 0, false};
+  uint32_t d = count([&](int s, uint32_t k, auto p, bool& in, uint32_t& digit) { in = s < len; digit = k >> 21; });
+  c.above = (d << 21) - 1;
+  if (exact) return c;
+  uint32_t low = count([&](int s, uint32_t k, auto p, bool& in, uint32_t& digit) { in = s < len && k >> 21 == d; digit = (k >> 10) & 0x7FFu; });
+  d = d << 11 | low;
+  c.above = (d << 10) - 1;
+  if (exact) return c;
+  low = count([&](int s, uint32_t k, auto p, bool& in, uint32_t& digit) { in = s < len && k >> 10 == d; digit = k & 0x3FFu; });
+  d = d << 10 | low;
+  c.above = d - 1;
+  if (exact) return c;
+  c.tied = true;
+  c.above = c.ties = d;
+  positions();
+  uint32_t q = count([&](int s, uint32_t k, auto p, bool& in, uint32_t& digit) { in = s < len && k == c.ties; digit = p() >> 21; });
+  c.pabove = (q << 21) - 1;
+  if (exact) return c;
+  low = count([&](int s, uint32_t k, auto p, bool& in, uint32_t& digit) {
+    const uint32_t w = p();
+    in = s < len && k == c.ties && w >> 21 == q;
+    digit = (w >> 10) & 0x7FFu;
+  });
+  q = q << 11 | low;
+  c.pabove = (q << 10) - 1;
+  if (exact) return c;
+  low = count([&](int s, uint32_t k, auto p, bool& in, uint32_t& digit) {
+    const uint32_t w = p();
+    in = s < len && k == c.ties && w >> 10 == q;
+    digit = w & 0x3FFu;
+  });
+  q = q << 10 | low;
+  c.pabove = q - 1;
+  if (exact) return c;
+  c.pabove = c.ptie = q;
+  c.need = need;
+  return c;
+}
+
+// A head's sizes, and the sequence's outputs; false where there is nothing to
+// cut (the slots are then copied, if need be).
+struct Head {
+  int64_t bh;
+  int b, kh, len, keep;
+  const float* mass;
+  const int32_t* pos;
+  float* new_mass;
+  int32_t* new_pos;
+  int64_t next, sinks, recent;
+  bool cut;
+  XS_DEV Head(const xs_cache_evict_args& a, const EvictWork& w) {
+    bh = blockIdx.x;
+    b = (int)(bh / a.kv_heads);
+    kh = (int)(bh % a.kv_heads);
+    len = a.len[b];
+    const int64_t limit = a.max_len ? a.max_len : a.capacity;
+    const bool bad = len < 0 || len > limit;
+    keep = (int)min((int64_t)len, a.keep);
+    if (threadIdx.x == 0) {
+      w.moves[bh] = 0;
+      if (kh == 0) {
+        a.seq_status[b] = bad ? XS_ROW_BAD_PARAM : XS_ROW_OK;
+        a.new_len[b] = bad ? len : keep;
+      }
     }
-    if (!exact) {
-      p0 = p0 << 10 | count([&](int s, uint32_t k, bool& in, uint32_t& d) {
-        const uint32_t q = word_at(s);
-        in = s < len && k == ties && q >> 10 == p0;
-        d = q & 0x3FFu;
-      });
-      pfrom = p0;
+    mass = a.mass + bh * a.slot_ld;
+    pos = a.pos + bh * a.slot_ld;
+    new_mass = a.new_mass + bh * a.slot_ld;
+    new_pos = a.new_pos + bh * a.slot_ld;
+    next = a.next_pos[b];
+    sinks = a.sinks;
+    recent = a.recent;
+    cut = !bad && len > keep;
+    if (!bad && !cut) copy(keep);
+  }
+  XS_DEV void copy(int n) const {
+    if (new_mass == mass) return;
+    for (int s = threadIdx.x; s < n; s += EB) {
+      new_mass[s] = mass[s];
+      new_pos[s] = pos[s];
     }
   }
-  // the bitmap
-  uint64_t* kept = E > 0 ? word : w.kept + bh * w.words;
+  XS_DEV bool held(int p) const { return p < sinks || p >= next - recent; }
+};
+
+// Slots in registers: V times four consecutive ones a thread (len <= 4 V EB;
+// 16-byte aligned arrays of a slot_ld that is a multiple of 4).  apart: the rows of
+// k and v are left to evict_rows_kernel; else there are at most NEAR moves,
+// made here.  4,128 slots to 4,096, 128 heads: 15 us with 4-byte loads and a
+// bitmap, EV1; 32 heads of up to 32,768 to 2,048: 41 us so, EV2.
+template <int V>
+__global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, const EvictWork w, int apart) {
+  __shared__ SelectLds lds;
+  __shared__ uint32_t base[EB];
+  __shared__ int near_free[NEAR], near_filler[NEAR];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Head h(a, w);
+  if (!h.cut) return;
+  const int len = h.len, keep = h.keep;
+  uint32_t word[V][4];
+  {
+    f32x4 m[V];
+    u32x4 p[V];
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+      const int s = (e * EB + tid) * 4, at = s < len ? s : 0;
+      m[e] = *(const f32x4*)(h.mass + at);
+      p[e] = *(const u32x4*)(h.pos + at);
+    }
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+      const int s = (e * EB + tid) * 4;
+#pragma unroll
+      for (int j = 0; j < 4; j++) word[e][j] = weight_word(m[e][j], h.held((int)p[e][j]));
+      if (h.new_mass != h.mass && s < keep) {
+        if (s + 4 <= keep) {
+          *(f32x4*)(h.new_mass + s) = m[e];
+          *(u32x4*)(h.new_pos + s) = p[e];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 3; j++)
+            if (s + j < keep) {
+              h.new_mass[s + j] = m[e][j];
+              h.new_pos[s + j] = (int)p[e][j];
+            }
+        }
+      }
+    }
+  }
+  uint32_t place[V][4];  // the slots' position words, where weights alone do not settle it
+  const Cutoff c = find_cutoff(
+      lds, len, keep,
+      [&](auto f) {
+#pragma unroll
+        for (int e = 0; e < V; e++)
+          if ((e * EB + wave * 64) * 4 < len)
+#pragma unroll
+            for (int j = 0; j < 4; j++) f((e * EB + tid) * 4 + j, word[e][j], [&]() { return place[e][j]; });
+      },
+      [&]() {
+        u32x4 p[V];
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+          const int s = (e * EB + tid) * 4;
+          p[e] = *(const u32x4*)(h.pos + (s < len ? s : 0));
+        }
+#pragma unroll
+        for (int e = 0; e < V; e++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) place[e][j] = position_word((int)p[e][j]);
+      });
+  // bit 4 e + j: the slot is kept
+  uint32_t kept = 0;
+#pragma unroll
+  for (int e = 0; e < V; e++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int s = (e * EB + tid) * 4 + j;
+      bool in = word[e][j] > c.above;
+      if (c.tied && word[e][j] == c.ties) in = place[e][j] > c.pabove;
+      if (in && s < len) kept |= 1u << (4 * e + j);
+    }
+  // use(slot, e, j, n) for every flagged slot, n of which lie before it; the
+  // number of all of them.
+  auto ranks = [&](auto flag, auto use) {
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+      uint32_t n = 0;
+#pragma unroll
+      for (int j = 0; j < 4; j++) n += (uint32_t)__popcll(__ballot(flag((e * EB + tid) * 4 + j, e, j)));
+      if (lane == 0) base[e * EW + wave] = n;
+    }
+    __syncthreads();
+    uint32_t total;
+    const uint32_t mine = block_scan(tid < V * EW ? base[tid] : 0u, lds.scan, &total);
+    if (tid < V * EW) base[tid] = mine;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+      uint32_t n = base[e * EW + wave];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const uint64_t who = __ballot(flag((e * EB + tid) * 4 + j, e, j));
+        n = __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, n));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (flag((e * EB + tid) * 4 + j, e, j)) use((e * EB + tid) * 4 + j, e, j, (int)n++, (int)total);
+    }
+    __syncthreads();
+    return (int)total;
+  };
+  if (c.need > 0)  // (slots alike in weight and position: the first of them)
+    ranks([&](int s, int e, int j) { return s < len && word[e][j] == c.ties && place[e][j] == c.ptie; },
+          [&](int, int e, int j, int n, int) {
+            if (n < c.need) kept |= 1u << (4 * e + j);
+          });
+  // Freed slots below keep, then the kept ones past it, as many: the second
+  // half of the flagged slots.
+  int32_t* freed = apart ? w.free_ + h.bh * w.pairs : near_free;
+  int32_t* filler = apart ? w.filler + h.bh * w.pairs : near_filler;
+  const uint32_t is_kept = kept;
+  const int moves = ranks([&](int s, int e, int j) { return ((is_kept >> (4 * e + j)) & 1u) != (s < keep ? 1u : 0u); },
+                          [&](int s, int, int, int n, int all) { (s < keep ? freed[n] : filler[n - all / 2]) = s; }) / 2;
+  if (tid == 0) w.moves[h.bh] = moves;
+  for (int i = tid; i < moves; i += EB) {
+    const int to = freed[i], from = filler[i];
+    h.new_mass[to] = h.mass[from];
+    h.new_pos[to] = h.pos[from];
+  }
+  if (apart) return;
+  const int parts = a.head_dim / 8;
+  const int64_t head = h.b * a.cache.seq_stride + h.kh * a.cache.head_stride;
+  for (int j = tid; j < moves * parts; j += EB) move_part(a, head, near_filler[j / parts], near_free[j / parts], j % parts * 8);
+}
+
+// The same for any length and alignment: every pass reads the slots again, the
+// kept ones go to a bitmap, and all rows are left to evict_rows_kernel.
+__global__ __launch_bounds__(EB) void evict_long_kernel(const xs_cache_evict_args a, const EvictWork w) {
+  __shared__ SelectLds lds;
+  __shared__ uint64_t scan[EW];
+  __shared__ uint64_t base[EB];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const Head h(a, w);
+  if (!h.cut) return;
+  const int len = h.len, keep = h.keep;
+  h.copy(keep);
+  auto position = [&](int s) { return position_word(h.pos[min(s, len - 1)]); };
+  auto each = [&](auto f) {
+#pragma unroll 4
+    for (int s0 = wave * 64; s0 < len; s0 += EB) {
+      const int s = min(s0 + lane, len - 1);
+      f(s0 + lane, weight_word(h.mass[s], h.held(h.pos[s])), [&]() { return position(s); });
+    }
+  };
+  const Cutoff c = find_cutoff(lds, len, keep, each, []() {});
+  uint64_t* kept = w.kept + h.bh * w.words;
   const int words = (len + 63) / 64;
-  each([&](int s0, int s, uint32_t k) {
-    bool in = k >= from;
-    if (tied && k == ties) {
-      const uint32_t q = position_word(pos[min(s, len - 1)]);
-      in = exact ? q >= pfrom : q > pfrom;
-    }
+  each([&](int s, uint32_t k, auto) {
+    bool in = k > c.above;
+    if (c.tied && k == c.ties) in = position(s) > c.pabove;
     const uint64_t bit = __ballot(s < len && in);
-    if (lane == 0) kept[s0 / 64] = bit;
+    if (lane == 0) kept[s / 64] = bit;
   });
   __syncthreads();
-  if (!exact) {  // slots equal in weight and position: the lowest of them
-    if (wave == 0)
+  if (c.need > 0) {  // (slots alike in weight and position: the first of them)
+    if (wave == 0) {
+      int need = c.need;
       for (int i = 0; i < words && need > 0; i++) {
-        const int s = min(i * 64 + lane, len - 1), p = pos[s];
-        uint64_t eq = __ballot(i * 64 + lane < len && position_word(p) == pfrom && weight_word(mass[s], held(p)) == ties);
+        const int s = min(i * 64 + lane, len - 1);
+        uint64_t eq = __ballot(i * 64 + lane < len && position(s) == c.ptie && weight_word(h.mass[s], h.held(h.pos[s])) == c.ties);
         while (__popcll(eq) > need) eq &= ~(1ull << (63 - __builtin_clzll(eq)));
         need -= __popcll(eq);
         if (eq && lane == 0) kept[i] |= eq;
       }
+    }
     __syncthreads();
   }
   // freed slots below keep and kept ones past it, by their ranks
-  int32_t* freed = apart ? w.free_ + bh * w.pairs : near_free;
-  int32_t* filler = apart ? w.filler + bh * w.pairs : near_filler;
-  Pair run = 0;  // low half: free slots so far, high: fillers
+  int32_t* freed = w.free_ + h.bh * w.pairs;
+  int32_t* filler = w.filler + h.bh * w.pairs;
+  uint64_t run = 0;  // low half: free slots so far, high: fillers
   auto split = [&](int i, uint64_t bits, uint64_t* f, uint64_t* m) {
     const int in = min(max(keep - i * 64, 0), 64);  // the word's slots below keep
     const uint64_t low = in == 64 ? ~0ull : (1ull << in) - 1ull;
@@ -1272,31 +1425,26 @@ __global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, 
     const int i = w0 + tid;
     uint64_t f = 0, m = 0;
     if (i < words) split(i, kept[i], &f, &m);
-    Pair total;
-    base[tid] = run + block_scan((Pair)__popcll(f) | (Pair)__popcll(m) << HALF, lds, &total);
+    uint64_t total;
+    base[tid] = run + block_scan((uint64_t)__popcll(f) | (uint64_t)__popcll(m) << 32, scan, &total);
     run += total;
     __syncthreads();
     for (int j = wave; j < EB && w0 + j < words; j += EW) {
       split(w0 + j, kept[w0 + j], &f, &m);
-      const uint64_t below = (1ull << lane) - 1ull;
-      const Pair at = base[j];
+      const uint64_t below = (1ull << lane) - 1ull, at = base[j];
       const int slot = (w0 + j) * 64 + lane;
-      if ((f >> lane) & 1ull) freed[(int)(at & (((Pair)1 << HALF) - 1)) + __popcll(f & below)] = slot;
-      if ((m >> lane) & 1ull) filler[(int)(at >> HALF) + __popcll(m & below)] = slot;
+      if ((f >> lane) & 1ull) freed[(uint32_t)at + __popcll(f & below)] = slot;
+      if ((m >> lane) & 1ull) filler[(uint32_t)(at >> 32) + __popcll(m & below)] = slot;
     }
     __syncthreads();
   }
-  const int moves = (int)(run >> HALF);
-  if (tid == 0) w.moves[bh] = moves;
+  const int moves = (int)(run >> 32);
+  if (tid == 0) w.moves[h.bh] = moves;
   for (int i = tid; i < moves; i += EB) {
     const int to = freed[i], from = filler[i];
-    new_mass[to] = mass[from];
-    new_pos[to] = pos[from];
+    h.new_mass[to] = h.mass[from];
+    h.new_pos[to] = h.pos[from];
   }
-  if (apart) return;
-  const int parts = a.head_dim / 8;
-  const int64_t head = b * a.cache.seq_stride + kh * a.cache.head_stride;
-  for (int j = tid; j < moves * parts; j += EB) move_part(a, head, near_filler[j / parts], near_free[j / parts], j % parts * 8);
 }
 
 // The rows of a head's moves, ROWS of them a workgroup.
@@ -1350,7 +1498,8 @@ int attend_run(xs_cache_context* c, const xs_tree_attend_args& a) {
   const int64_t limit = a.max_len ? a.max_len : a.capacity;
   const int64_t blocks = (limit + xst::KB - 1) / xst::KB + (a.nodes + xst::KB - 1) / xst::KB;
   const int64_t units = a.seqs * a.kv_heads * wgs;
-  const int64_t most = c->n_cu * (WIDE ? 1 : per_cu(DP, RT)) * rounds(a.seqs);
+  // (rows of several waves: once, their partial results cost as much as 8 blocks each)
+  const int64_t most = c->n_cu * (WIDE ? 1 : per_cu(DP, RT) * rounds(a.seqs));
   const int64_t nsplit = std::max<int64_t>(1, std::min<int64_t>(xst::SPLITS, most / units));
   cut.chunk = (int32_t)((blocks + nsplit - 1) / nsplit);
   // Two blocks a wave at least, and no split for its own sake: a join costs
@@ -1368,8 +1517,10 @@ int attend_run(xs_cache_context* c, const xs_tree_attend_args& a) {
     hipLaunchKernelGGL((xst::attend_wide_kernel<T, DP, RT, EXACT>), dim3((unsigned)grid), dim3(64 * xst::NW), 0, c->stream, a, cut);
   else
     hipLaunchKernelGGL((xst::attend_kernel<T, DP, RT, EXACT>), dim3((unsigned)grid), dim3(64 * xst::NW), 0, c->stream, a, cut);
-  if (cut.nsplit > 1)
-    hipLaunchKernelGGL((xst::join_kernel<T, DP, RT>), dim3((unsigned)join), dim3(1024), 0, c->stream, a, cut);
+  if (cut.nsplit > xst::FEW)
+    hipLaunchKernelGGL((xst::join_kernel<T, DP, RT, false>), dim3((unsigned)join), dim3(xst::join_threads<DP>(false)), 0, c->stream, a, cut);
+  else if (cut.nsplit > 1)
+    hipLaunchKernelGGL((xst::join_kernel<T, DP, RT, true>), dim3((unsigned)join), dim3(xst::join_threads<DP>(true)), 0, c->stream, a, cut);
   return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
 }
 
@@ -1461,10 +1612,12 @@ int commit_dim(xs_cache_context* c, const xs_cache_commit_args& a) {
   return commit_rows<T, 256>(c, a);
 }
 
-template <int E>
+template <int V>
 void evict_run(xs_cache_context* c, const xs_cache_evict_args& a, bool apart) {
-  hipLaunchKernelGGL((xst::evict_kernel<E>), dim3((unsigned)(a.seqs * a.kv_heads)), dim3(xst::EB), 0, c->stream, a, c->evict, apart ? 1 : 0);
+  hipLaunchKernelGGL((xst::evict_kernel<V>), dim3((unsigned)(a.seqs * a.kv_heads)), dim3(xst::EB), 0, c->stream, a, c->evict, apart ? 1 : 0);
 }
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 }  // namespace
 
@@ -1544,13 +1697,15 @@ int xs_cache_evict(xs_cache_context* c, const xs_cache_evict_args* in) {
   const int64_t heads = in->seqs * in->kv_heads;
   // moves of a head: at most the slots past keep, and the slots of keep
   const int64_t most = limit > in->keep ? std::min(in->keep, limit - in->keep) : 0;
-  const bool apart = most > xst::NEAR;  // (a head's own workgroup makes a few moves, a launch of its own many)
+  const bool fits = limit <= 32 * xst::EB && aligned16(in->mass) && aligned16(in->pos) && aligned16(in->new_mass) &&
+                    aligned16(in->new_pos) && in->slot_ld % 4 == 0;
+  const bool apart = most > xst::NEAR || (!fits && most > 0);
   const int64_t blocks = (most + xst::ROWS - 1) / xst::ROWS;
   if (heads > 0x7FFFFFFF || (apart && heads * blocks > 0x7FFFFFFF)) return XS_ERR_CAPACITY;
-  if (limit <= 4 * xst::EB) evict_run<4>(c, *in, apart);
-  else if (limit <= 8 * xst::EB) evict_run<8>(c, *in, apart);
-  else if (limit <= 32 * xst::EB) evict_run<32>(c, *in, apart);
-  else evict_run<0>(c, *in, apart);
+  if (!fits) hipLaunchKernelGGL(xst::evict_long_kernel, dim3((unsigned)heads), dim3(xst::EB), 0, c->stream, *in, c->evict);
+  else if (limit <= 4 * xst::EB) evict_run<1>(c, *in, apart);
+  else if (limit <= 8 * xst::EB) evict_run<2>(c, *in, apart);
+  else evict_run<8>(c, *in, apart);
   if (apart)
     hipLaunchKernelGGL(xst::evict_rows_kernel, dim3((unsigned)(heads * blocks)), dim3(256), 0, c->stream, *in, c->evict, (int)blocks);
   return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
