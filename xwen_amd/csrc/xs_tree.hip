@@ -1006,8 +1006,8 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 256 ? 3 : 2) void commit_kernel
 // One workgroup per (sequence, kv head) finds the `keep`-th of the slots'
 // weights (weight_word) by counting digits of 11 bits from the top, each pass
 // over the slots whose digits so far are the chosen ones, until a digit's
-// slots are exactly those still needed; where equal weights remain, their positions
-// are counted in the same way.  The kept slots go to a bitmap, whose prefix
+// slots are exactly those still needed, or few enough (LIST) to compare each
+// with each; equal weights go on into their positions, and those into the slots.  Prefix
 // counts pair the i-th free slot below `keep` with the i-th kept one past it.
 // Only these move: `keep` of `keep` + a few slots moves a few rows, where
 // keeping the slots in order would move nearly all.
@@ -1084,110 +1084,161 @@ XS_DEV void move_part(const xs_cache_evict_args& a, int64_t head, int from, int 
 }
 
 constexpr int REP = 4;     // copies of the counts, by the lane: weights crowd into few digits
+constexpr int LIST = 256;  // slots that are ranked by comparing each with each
 constexpr int NEAR = 128;  // moves that a head's own workgroup makes; more are left to evict_rows_kernel
 
-// What is kept: words above `above`, and of the words equal to `ties` (if tied)
-// those with position words above pabove; and where even positions are alike
-// (need > 0), the first `need` slots of position word ptie.
+// A slot's place: weight word, position word, and the slot itself, the first
+// two larger first.  Kept is what lies at or before the cutoff (whole: what
+// lies before its weight word).
 struct Cutoff {
-  uint32_t above, ties, pabove, ptie;
-  int need;
-  bool tied;
+  uint32_t weight, position;
+  int slot;
+  bool whole;
+  XS_DEV bool keeps(uint32_t w, int s, const int32_t* pos) const {
+    if (whole || w != weight) return w > weight;
+    const uint32_t p = position_word(pos[s]);  // (few slots)
+    return p != position ? p > position : s <= slot;
+  }
 };
 
 struct SelectLds {
   uint32_t hist[REP << DIGIT];
   uint32_t scan[EW];
-  int found[3];  // the digit, the slots still needed of it, whether that is all of it
+  uint64_t place[LIST];  // weight and position words
+  int slot[LIST];
+  int listed;
+  int found[4];  // the digit, the slots still needed of it, whether that is all of it, how many it has
+  Cutoff cutoff;
 };
 
-// The cutoff of `need` slots.  each(f) calls f(slot, weight word, q) for every
-// slot, whole waves at a time (slots past len among them); q() is its position
-// word, read after positions() has been called.
-template <typename Each, typename Positions>
-XS_DEV Cutoff find_cutoff(SelectLds& lds, int len, int need, Each each, Positions positions) {
+// The cutoff that keeps `need` of len slots (need < len).  each(f) calls
+// f(slot, weight word) for every slot, whole waves at a time (slots past len
+// among them).  bits, if not null: a bitmap over the slots, empty, where the
+// slots that are kept beside those of the cutoff are set.
+template <typename Each>
+XS_DEV Cutoff find_cutoff(SelectLds& lds, int len, int need, const int32_t* pos, uint32_t* bits, Each each) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  bool exact = false;
   u32x4* const own = (u32x4*)lds.hist + 2 * ((1 << (DIGIT - 1)) - 1 - tid);  // thread i: the i-th pair of digits from the top
   static_assert(REP == 4, "the copies of a count fill a vector");
   own[0] = own[1] = (u32x4){0, 0, 0, 0};
+  if (tid == 0) lds.listed = 0;
   __syncthreads();
-  // One digit: `digits(s, word, q, in, digit)` says which slots are counted.
-  // The digit that holds the need-th is returned; need is what of it is needed.
-  auto count = [&](auto digits) {
-    each([&](int s, uint32_t k, auto q) {
-      bool in;
-      uint32_t digit;
-      digits(s, k, q, in, digit);
-      // (a wave that holds one digit adds it at once: equal weights)
-      const uint32_t first = __builtin_amdgcn_readfirstlane(digit);
-      if (__ballot(digit != first) == 0) {
-        const uint64_t who = __ballot(in);
-        if (lane == 0) atomicAdd(&lds.hist[first * REP], (uint32_t)__popcll(who));
-      } else if (in) {
-        atomicAdd(&lds.hist[digit * REP + (lane & (REP - 1))], 1u);
+  // The words of a slot's place, from the weight's (L = 0) to the slot's (2).
+  // The words before L are `known`, and of that one the bits from `shift` on
+  // are `prefix`.
+  uint32_t known[2] = {0, 0}, prefix = 0;
+  int shift = 32;
+  auto word = [&](auto L, int s, uint32_t k) {
+    if constexpr (L == 0) return k;
+    else if constexpr (L == 1) return position_word(pos[s]);
+    else return ~(uint32_t)s;
+  };
+  auto among = [&](auto L, int s, uint32_t k) {
+    if (s >= len || (L >= 1 && k != known[0])) return false;
+    if constexpr (L == 2)
+      if (position_word(pos[s]) != known[1]) return false;
+    return shift == 32 || word(L, s, k) >> (shift & 31) == prefix;
+  };
+  // Counts one word's digits until the cutoff is known, few slots are left, or
+  // the word is at its end.
+  enum { END, DONE, FEWER };
+  auto settle = [&](auto L) {
+    prefix = 0;
+    for (shift = 32; shift > 0;) {
+      const int bits = min(DIGIT, shift), next = shift - bits;
+      each([&](int s, uint32_t k) {
+        const bool in = among(L, s, k);
+        uint32_t digit = 0;
+        if (L == 0 || in) digit = (word(L, s, k) >> next) & ((1u << bits) - 1u);
+        // (a wave that holds one digit adds it at once: equal weights)
+        const uint32_t first = __builtin_amdgcn_readfirstlane(digit);
+        if (__ballot(digit != first) == 0) {
+          const uint64_t who = __ballot(in);
+          if (lane == 0) atomicAdd(&lds.hist[first * REP], (uint32_t)__popcll(who));
+        } else if (in) {
+          atomicAdd(&lds.hist[digit * REP + (lane & (REP - 1))], 1u);
+        }
+      });
+      __syncthreads();
+      const u32x4 h0 = own[0], h1 = own[1];
+      own[0] = own[1] = (u32x4){0, 0, 0, 0};  // (for the next digit)
+      const int c1 = (int)((h1[0] + h1[1]) + (h1[2] + h1[3])), c0 = (int)((h0[0] + h0[1]) + (h0[2] + h0[3]));
+      const uint32_t run = wave_scan((uint32_t)(c1 + c0));
+      if (lane == 63) lds.scan[wave] = run;
+      __syncthreads();
+      int before = (int)run - c1 - c0;
+#pragma unroll
+      for (int i = 0; i < EW; i++) before += i < wave ? (int)lds.scan[i] : 0;
+      if (before < need && need <= before + c1 + c0) {
+        const bool one = need <= before + c1;
+        lds.found[0] = 2 * ((1 << (DIGIT - 1)) - 1 - tid) + (one ? 1 : 0);
+        lds.found[1] = need - before - (one ? 0 : c1);
+        lds.found[2] = lds.found[1] == (one ? c1 : c0);
+        lds.found[3] = one ? c1 : c0;
       }
+      __syncthreads();
+      need = lds.found[1];
+      prefix = shift == 32 ? (uint32_t)lds.found[0] : prefix << bits | (uint32_t)lds.found[0];
+      shift = next;
+      if (lds.found[2]) return DONE;
+      if (lds.found[3] <= LIST) return FEWER;
+    }
+    return END;
+  };
+  auto list = [&](auto L) {
+    each([&](int s, uint32_t k) {
+      if (!among(L, s, k)) return;
+      const int i = atomicAdd(&lds.listed, 1);
+      lds.place[i] = (uint64_t)k << 32;
+      lds.slot[i] = s;
     });
     __syncthreads();
-    const u32x4 h0 = own[0], h1 = own[1];
-    own[0] = own[1] = (u32x4){0, 0, 0, 0};  // (for the next digit)
-    const int c1 = (int)((h1[0] + h1[1]) + (h1[2] + h1[3])), c0 = (int)((h0[0] + h0[1]) + (h0[2] + h0[3]));
-    const uint32_t run = wave_scan((uint32_t)(c1 + c0));
-    if (lane == 63) lds.scan[wave] = run;
-    __syncthreads();
-    int before = (int)run - c1 - c0;
-#pragma unroll
-    for (int i = 0; i < EW; i++) before += i < wave ? (int)lds.scan[i] : 0;
-    if (before < need && need <= before + c1 + c0) {
-      const bool one = need <= before + c1;
-      lds.found[0] = 2 * ((1 << (DIGIT - 1)) - 1 - tid) + (one ? 1 : 0);
-      lds.found[1] = need - before - (one ? 0 : c1);
-      lds.found[2] = lds.found[1] == (one ? c1 : c0);
-    }
-    __syncthreads();
-    need = lds.found[1];
-    exact = lds.found[2] != 0;
-    return (uint32_t)lds.found[0];
+    if (tid < lds.listed) lds.place[tid] |= position_word(pos[lds.slot[tid]]);
   };
-  // (a digit that is kept whole lies above a slot that is not, so its lowest
-  // word is at least 1)
-  Cutoff c = {0, 0, 0, 0, 0, false};
-  uint32_t d = count([&](int s, uint32_t k, auto p, bool& in, uint32_t& digit) { in = s < len; digit = k >> 21; });
-  c.above = (d << 21) - 1;
-  if (exact) return c;
-  uint32_t low = count([&](int s, uint32_t k, auto p, bool& in, uint32_t& digit) { in = s < len && k >> 21 == d; digit = (k >> 10) & 0x7FFu; });
-  d = d << 11 | low;
-  c.above = (d << 10) - 1;
-  if (exact) return c;
-  low = count([&](int s, uint32_t k, auto p, bool& in, uint32_t& digit) { in = s < len && k >> 10 == d; digit = k & 0x3FFu; });
-  d = d << 10 | low;
-  c.above = d - 1;
-  if (exact) return c;
-  c.tied = true;
-  c.above = c.ties = d;
-  positions();
-  uint32_t q = count([&](int s, uint32_t k, auto p, bool& in, uint32_t& digit) { in = s < len && k == c.ties; digit = p() >> 21; });
-  c.pabove = (q << 21) - 1;
-  if (exact) return c;
-  low = count([&](int s, uint32_t k, auto p, bool& in, uint32_t& digit) {
-    const uint32_t w = p();
-    in = s < len && k == c.ties && w >> 21 == q;
-    digit = (w >> 10) & 0x7FFu;
-  });
-  q = q << 11 | low;
-  c.pabove = (q << 10) - 1;
-  if (exact) return c;
-  low = count([&](int s, uint32_t k, auto p, bool& in, uint32_t& digit) {
-    const uint32_t w = p();
-    in = s < len && k == c.ties && w >> 10 == q;
-    digit = w & 0x3FFu;
-  });
-  q = q << 10 | low;
-  c.pabove = q - 1;
-  if (exact) return c;
-  c.pabove = c.ptie = q;
-  c.need = need;
-  return c;
+  const std::integral_constant<int, 0> W;
+  const std::integral_constant<int, 1> P;
+  const std::integral_constant<int, 2> S;
+  // (all of a digit's slots kept: the cutoff lies just before its lowest word)
+  int how = settle(W);
+  if (how == DONE) return Cutoff{(prefix << shift) - 1, 0, 0, true};
+  const bool mark = how == FEWER && bits != nullptr;
+  const uint32_t above = prefix << shift | ((1u << shift) - 1u);  // (the listed weights' largest)
+  if (how == FEWER) list(W);
+  if (how == END) {
+    known[0] = prefix;
+    how = settle(P);
+    if (how == DONE) return Cutoff{known[0], (prefix << shift) - 1, -1, false};
+    if (how == FEWER) list(P);
+  }
+  if (how == END) {
+    known[1] = prefix;
+    how = settle(S);
+    if (how == DONE) return Cutoff{known[0], known[1], (int)~(prefix << shift), false};
+    list(S);
+  }
+  // few are left: each counts those before it
+  static_assert(EB / LIST == 4, "the threads of a slot");
+  __syncthreads();
+  const int n = lds.listed, i = tid / (EB / LIST);  // (four threads a slot)
+  if (i < n) {
+    const uint64_t mine = lds.place[i];
+    const int s = lds.slot[i];
+    int before = 0;
+#pragma unroll 8
+    for (int j = tid % (EB / LIST); j < n; j += EB / LIST) {
+      const uint64_t p = lds.place[j];
+      const int o = lds.slot[j];
+      before += (int)(p > mine) | ((int)(p == mine) & (int)(o < s));
+    }
+    before += __shfl_xor(before, 1);
+    before += __shfl_xor(before, 2);
+    if (tid % (EB / LIST) == 0) {
+      if (before == need - 1) lds.cutoff = Cutoff{(uint32_t)(mine >> 32), (uint32_t)mine, s, false};
+      if (mark && before < need) atomicOr(&bits[s >> 5], 1u << (s & 31));
+    }
+  }
+  __syncthreads();
+  return mark ? Cutoff{above, 0, 0, true} : lds.cutoff;
 }
 
 // A head's sizes, and the sequence's outputs; false where there is nothing to
@@ -1244,7 +1295,8 @@ struct Head {
 template <int V>
 __global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, const EvictWork w, int apart) {
   __shared__ SelectLds lds;
-  __shared__ uint32_t base[EB];
+  __shared__ uint32_t base[V * EW];
+  __shared__ uint32_t bits[V * EB / 8];
   __shared__ int near_free[NEAR], near_filler[NEAR];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1281,81 +1333,60 @@ __global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, 
       }
     }
   }
-  uint32_t place[V][4];  // the slots' position words, where weights alone do not settle it
-  const Cutoff c = find_cutoff(
-      lds, len, keep,
-      [&](auto f) {
+  if (tid < V * EB / 8) bits[tid] = 0;  // (find_cutoff's barriers order it)
+  const Cutoff c = find_cutoff(lds, len, keep, h.pos, bits, [&](auto f) {
 #pragma unroll
-        for (int e = 0; e < V; e++)
-          if ((e * EB + wave * 64) * 4 < len)
+    for (int e = 0; e < V; e++)
+      if ((e * EB + wave * 64) * 4 < len)
 #pragma unroll
-            for (int j = 0; j < 4; j++) f((e * EB + tid) * 4 + j, word[e][j], [&]() { return place[e][j]; });
-      },
-      [&]() {
-        u32x4 p[V];
-#pragma unroll
-        for (int e = 0; e < V; e++) {
-          const int s = (e * EB + tid) * 4;
-          p[e] = *(const u32x4*)(h.pos + (s < len ? s : 0));
-        }
-#pragma unroll
-        for (int e = 0; e < V; e++)
-#pragma unroll
-          for (int j = 0; j < 4; j++) place[e][j] = position_word((int)p[e][j]);
-      });
+        for (int j = 0; j < 4; j++) f((e * EB + tid) * 4 + j, word[e][j]);
+  });
   // bit 4 e + j: the slot is kept
   uint32_t kept = 0;
+#pragma unroll
+  for (int e = 0; e < V; e++) kept |= (bits[(e * EB + tid) >> 3] >> (4 * (tid & 7)) & 15u) << (4 * e);
 #pragma unroll
   for (int e = 0; e < V; e++)
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const int s = (e * EB + tid) * 4 + j;
-      bool in = word[e][j] > c.above;
-      if (c.tied && word[e][j] == c.ties) in = place[e][j] > c.pabove;
-      if (in && s < len) kept |= 1u << (4 * e + j);
+      if (s < len && c.keeps(word[e][j], s, h.pos)) kept |= 1u << (4 * e + j);
     }
-  // use(slot, e, j, n) for every flagged slot, n of which lie before it; the
-  // number of all of them.
-  auto ranks = [&](auto flag, auto use) {
-#pragma unroll
-    for (int e = 0; e < V; e++) {
-      uint32_t n = 0;
-#pragma unroll
-      for (int j = 0; j < 4; j++) n += (uint32_t)__popcll(__ballot(flag((e * EB + tid) * 4 + j, e, j)));
-      if (lane == 0) base[e * EW + wave] = n;
-    }
-    __syncthreads();
-    uint32_t total;
-    const uint32_t mine = block_scan(tid < V * EW ? base[tid] : 0u, lds.scan, &total);
-    if (tid < V * EW) base[tid] = mine;
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < V; e++) {
-      uint32_t n = base[e * EW + wave];
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const uint64_t who = __ballot(flag((e * EB + tid) * 4 + j, e, j));
-        n = __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, n));
-      }
-#pragma unroll
-      for (int j = 0; j < 4; j++)
-        if (flag((e * EB + tid) * 4 + j, e, j)) use((e * EB + tid) * 4 + j, e, j, (int)n++, (int)total);
-    }
-    __syncthreads();
-    return (int)total;
-  };
-  if (c.need > 0)  // (slots alike in weight and position: the first of them)
-    ranks([&](int s, int e, int j) { return s < len && word[e][j] == c.ties && place[e][j] == c.ptie; },
-          [&](int, int e, int j, int n, int) {
-            if (n < c.need) kept |= 1u << (4 * e + j);
-          });
-  // Freed slots below keep, then the kept ones past it, as many: the second
-  // half of the flagged slots.
+  // Freed slots below keep, then the kept ones past it, as many: in their
+  // order, the flagged slots' two halves.
   int32_t* freed = apart ? w.free_ + h.bh * w.pairs : near_free;
   int32_t* filler = apart ? w.filler + h.bh * w.pairs : near_filler;
-  const uint32_t is_kept = kept;
-  const int moves = ranks([&](int s, int e, int j) { return ((is_kept >> (4 * e + j)) & 1u) != (s < keep ? 1u : 0u); },
-                          [&](int s, int, int, int n, int all) { (s < keep ? freed[n] : filler[n - all / 2]) = s; }) / 2;
+  auto flag = [&](int e, int j) { return ((kept >> (4 * e + j)) & 1u) != ((e * EB + tid) * 4 + j < keep ? 1u : 0u); };
+#pragma unroll
+  for (int e = 0; e < V; e++) {
+    uint32_t n = 0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) n += (uint32_t)__popcll(__ballot(flag(e, j)));
+    if (lane == 0) base[e * EW + wave] = n;
+  }
+  __syncthreads();
+  uint32_t total;
+  const uint32_t mine = block_scan(tid < V * EW ? base[tid] : 0u, lds.scan, &total);
+  if (tid < V * EW) base[tid] = mine;
+  __syncthreads();
+  const int moves = (int)total / 2;
+#pragma unroll
+  for (int e = 0; e < V; e++) {
+    uint32_t n = base[e * EW + wave];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const uint64_t who = __ballot(flag(e, j));
+      n = __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, n));
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (flag(e, j)) {
+        const int s = (e * EB + tid) * 4 + j, i = (int)n++;
+        if (s < keep) freed[i] = s;
+        else filler[i - moves] = s;
+      }
+  }
+  __syncthreads();
   if (tid == 0) w.moves[h.bh] = moves;
   for (int i = tid; i < moves; i += EB) {
     const int to = freed[i], from = filler[i];
@@ -1380,37 +1411,21 @@ __global__ __launch_bounds__(EB) void evict_long_kernel(const xs_cache_evict_arg
   if (!h.cut) return;
   const int len = h.len, keep = h.keep;
   h.copy(keep);
-  auto position = [&](int s) { return position_word(h.pos[min(s, len - 1)]); };
   auto each = [&](auto f) {
 #pragma unroll 4
     for (int s0 = wave * 64; s0 < len; s0 += EB) {
       const int s = min(s0 + lane, len - 1);
-      f(s0 + lane, weight_word(h.mass[s], h.held(h.pos[s])), [&]() { return position(s); });
+      f(s0 + lane, weight_word(h.mass[s], h.held(h.pos[s])));
     }
   };
-  const Cutoff c = find_cutoff(lds, len, keep, each, []() {});
+  const Cutoff c = find_cutoff(lds, len, keep, h.pos, nullptr, each);
   uint64_t* kept = w.kept + h.bh * w.words;
   const int words = (len + 63) / 64;
-  each([&](int s, uint32_t k, auto) {
-    bool in = k > c.above;
-    if (c.tied && k == c.ties) in = position(s) > c.pabove;
-    const uint64_t bit = __ballot(s < len && in);
+  each([&](int s, uint32_t k) {
+    const uint64_t bit = __ballot(s < len && c.keeps(k, s, h.pos));
     if (lane == 0) kept[s / 64] = bit;
   });
   __syncthreads();
-  if (c.need > 0) {  // (slots alike in weight and position: the first of them)
-    if (wave == 0) {
-      int need = c.need;
-      for (int i = 0; i < words && need > 0; i++) {
-        const int s = min(i * 64 + lane, len - 1);
-        uint64_t eq = __ballot(i * 64 + lane < len && position(s) == c.ptie && weight_word(h.mass[s], h.held(h.pos[s])) == c.ties);
-        while (__popcll(eq) > need) eq &= ~(1ull << (63 - __builtin_clzll(eq)));
-        need -= __popcll(eq);
-        if (eq && lane == 0) kept[i] |= eq;
-      }
-    }
-    __syncthreads();
-  }
   // freed slots below keep and kept ones past it, by their ranks
   int32_t* freed = w.free_ + h.bh * w.pairs;
   int32_t* filler = w.filler + h.bh * w.pairs;
