@@ -1115,8 +1115,9 @@ struct SelectLds {
 // f(slot, weight word) for every slot, whole waves at a time (slots past len
 // among them).  bits, if not null: a bitmap over the slots, empty, where the
 // slots that are kept beside those of the cutoff are set.
-template <typename Each>
-XS_DEV Cutoff find_cutoff(SelectLds& lds, int len, int need, const int32_t* pos, uint32_t* bits, Each each) {
+// again(f) does the same from memory, for the words after the weight's.
+template <typename Each, typename Again>
+XS_DEV Cutoff find_cutoff(SelectLds& lds, int len, int need, const int32_t* pos, uint32_t* bits, Each each, Again again) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   u32x4* const own = (u32x4*)lds.hist + 2 * ((1 << (DIGIT - 1)) - 1 - tid);  // thread i: the i-th pair of digits from the top
   static_assert(REP == 4, "the copies of a count fill a vector");
@@ -1139,6 +1140,10 @@ XS_DEV Cutoff find_cutoff(SelectLds& lds, int len, int need, const int32_t* pos,
       if (position_word(pos[s]) != known[1]) return false;
     return shift == 32 || word(L, s, k) >> (shift & 31) == prefix;
   };
+  auto over = [&](auto L, auto f) {
+    if constexpr (L == 0) each(f);
+    else again(f);
+  };
   // Counts one word's digits until the cutoff is known, few slots are left, or
   // the word is at its end.
   enum { END, DONE, FEWER };
@@ -1146,7 +1151,7 @@ XS_DEV Cutoff find_cutoff(SelectLds& lds, int len, int need, const int32_t* pos,
     prefix = 0;
     for (shift = 32; shift > 0;) {
       const int bits = min(DIGIT, shift), next = shift - bits;
-      each([&](int s, uint32_t k) {
+      over(L, [&](int s, uint32_t k) {
         const bool in = among(L, s, k);
         uint32_t digit = 0;
         if (L == 0 || in) digit = (word(L, s, k) >> next) & ((1u << bits) - 1u);
@@ -1186,7 +1191,7 @@ XS_DEV Cutoff find_cutoff(SelectLds& lds, int len, int need, const int32_t* pos,
     return END;
   };
   auto list = [&](auto L) {
-    each([&](int s, uint32_t k) {
+    over(L, [&](int s, uint32_t k) {
       if (!among(L, s, k)) return;
       const int i = atomicAdd(&lds.listed, 1);
       lds.place[i] = (uint64_t)k << 32;
@@ -1287,6 +1292,17 @@ struct Head {
   XS_DEV bool held(int p) const { return p < sinks || p >= next - recent; }
 };
 
+// f(slot, weight word) for every slot, from memory.
+template <typename F>
+XS_DEV void each_slot(const Head& h, F f) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll 4
+  for (int s0 = threadIdx.x - lane; s0 < h.len; s0 += EB) {
+    const int s = min(s0 + lane, h.len - 1);
+    f(s0 + lane, weight_word(h.mass[s], h.held(h.pos[s])));
+  }
+}
+
 // Slots in registers: V times four consecutive ones a thread (len <= 4 V EB;
 // 16-byte aligned arrays of a slot_ld that is a multiple of 4).  apart: the rows of
 // k and v are left to evict_rows_kernel; else there are at most NEAR moves,
@@ -1340,7 +1356,7 @@ __global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, 
       if ((e * EB + wave * 64) * 4 < len)
 #pragma unroll
         for (int j = 0; j < 4; j++) f((e * EB + tid) * 4 + j, word[e][j]);
-  });
+  }, [&](auto f) { each_slot(h, f); });
   // bit 4 e + j: the slot is kept
   uint32_t kept = 0;
 #pragma unroll
@@ -1411,14 +1427,8 @@ __global__ __launch_bounds__(EB) void evict_long_kernel(const xs_cache_evict_arg
   if (!h.cut) return;
   const int len = h.len, keep = h.keep;
   h.copy(keep);
-  auto each = [&](auto f) {
-#pragma unroll 4
-    for (int s0 = wave * 64; s0 < len; s0 += EB) {
-      const int s = min(s0 + lane, len - 1);
-      f(s0 + lane, weight_word(h.mass[s], h.held(h.pos[s])));
-    }
-  };
-  const Cutoff c = find_cutoff(lds, len, keep, h.pos, nullptr, each);
+  auto each = [&](auto f) { each_slot(h, f); };
+  const Cutoff c = find_cutoff(lds, len, keep, h.pos, nullptr, each, each);
   uint64_t* kept = w.kept + h.bh * w.words;
   const int words = (len + 63) / 64;
   each([&](int s, uint32_t k) {
