@@ -312,6 +312,37 @@ def test_streams_and_graph_replays(ctx):
         assert torch.equal(out.out, eager.out) and torch.equal(out.lse, eager.lse)
 
 
+def test_streams_in_turn_share_the_workspace(ctx):
+    """One context's calls from two streams, one after the other without a wait of the caller's."""
+    rng = np.random.default_rng(17)
+    cs = [case(rng, [6000, 900], 8, 8, 2, 128, BF), case(rng, [7000, 1200], 8, 8, 2, 128, BF)]
+    want = [run(ctx, c, out=blank(c)) for c in cs]
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(6):
+        for j in range(2):
+            with torch.cuda.stream(streams[j]):
+                outs[j].append(run(ctx, cs[j], out=blank(cs[j])))
+    torch.cuda.synchronize()
+    for j in range(2):
+        for got in outs[j]:
+            assert torch.equal(got.out, want[j].out) and torch.equal(got.lse, want[j].lse)
+
+
+def test_strides_of_single_entries_do_not_matter(ctx):
+    """One kv head, one node, one sequence, their strides any number."""
+    rng = np.random.default_rng(18)
+    c = case(rng, [50], 1, 4, 1, 64, BF)
+    want = run(ctx, c, out=blank(c))
+    for t in ("k", "v"):
+        c[t] = c[t].as_strided(c[t].shape, (3, 64, 5, 1))
+    for t in ("fk", "fv"):
+        c[t] = c[t].as_strided(c[t].shape, (1, 7, 9, 1))
+    c["q"] = c["q"].as_strided(c["q"].shape, (11, 13, 64, 1))
+    got = run(ctx, c, out=blank(c))
+    assert torch.equal(got.out, want.out) and torch.equal(got.lse, want.lse)
+
+
 def test_two_contexts_at_once(ctx):
     rng = np.random.default_rng(15)
     other = context()

@@ -121,6 +121,7 @@ def test_commit_checks(host):
     for f in p:
         assert chk(**{**p, f: None}) == E, f
     assert chk(new_len=DEV) == E and chk(**{**p, "new_next_pos": DEV}) == E
+    assert chk(new_len=DEV + 12) == E and chk(new_len=DEV + 16) == OK and chk(new_len=DEV - 12) == E  # [4] int32 each
     assert chk(path_ld=15) == E and chk(slot_ld=4095) == E and chk(slot_ld=1 << 60) == E and chk(path_ld=1 << 40) == E
     assert chk(cache=kv(0)) == E and chk(cache=kv(64)) == E and chk(fresh=kv(0)) == OK
     assert chk(**{**w, "q": DEV + 2}) == E and chk(**{**w, "q_head_stride": 4}) == E

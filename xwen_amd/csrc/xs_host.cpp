@@ -65,6 +65,12 @@ bool kv_ok(const xs_kv& kv, int64_t seqs, int64_t slots, int64_t kv_heads, int64
          strides_ok(seqs, kv.seq_stride, slots, kv.slot_stride, kv_heads, kv.head_stride, head_dim, written);
 }
 
+// Two per-sequence arrays share no entry.
+bool apart(const int32_t* p, const int32_t* q, int64_t seqs) {
+  const uintptr_t x = (uintptr_t)p, y = (uintptr_t)q, n = (uintptr_t)seqs * sizeof(int32_t);
+  return x + n <= y || y + n <= x;
+}
+
 // Per-slot arrays [seqs, kv_heads, slot_ld] lie within a 64-bit offset.
 bool slots_fit(int64_t seqs, int64_t kv_heads, int64_t slot_ld) {
   return slot_ld <= (INT64_MAX >> 4) / kv_heads / (seqs > 0 ? seqs : 1);
@@ -188,11 +194,11 @@ int xs_host_check_commit(const xs_cache_dims* dims, const xs_cache_commit_args* 
   int rc = check_sizes(dims, in->dtype, in->head_dim, in->seqs, in->kv_heads, in->capacity, in->max_len);
   if (rc == XS_OK) rc = check_queries(dims, in->nodes, in->q_heads, in->kv_heads);
   if (rc != XS_OK || in->seqs == 0) return rc;
-  if (!in->len || !in->path || !in->n_path || !in->new_len || !in->seq_status || in->new_len == in->len) return XS_ERR_ARG;
+  if (!in->len || !in->path || !in->n_path || !in->new_len || !in->seq_status || !apart(in->len, in->new_len, in->seqs)) return XS_ERR_ARG;
   if (in->path_ld < in->nodes || in->slot_ld < in->capacity) return XS_ERR_ARG;
   if (!slots_fit(in->seqs, in->kv_heads, in->slot_ld) || in->path_ld > INT32_MAX) return XS_ERR_ARG;
   const int positions = (in->next_pos != nullptr) + (in->pos != nullptr) + (in->new_next_pos != nullptr);
-  if ((positions != 0 && positions != 3) || (positions == 3 && in->new_next_pos == in->next_pos)) return XS_ERR_ARG;
+  if ((positions != 0 && positions != 3) || (positions == 3 && !apart(in->next_pos, in->new_next_pos, in->seqs))) return XS_ERR_ARG;
   const int weights = (in->q != nullptr) + (in->lse != nullptr) + (in->mass != nullptr) + (in->new_mass != nullptr);
   if (weights != 0 && weights != 4) return XS_ERR_ARG;
   if (!kv_ok(in->cache, in->seqs, in->capacity, in->kv_heads, in->head_dim, true) ||
@@ -209,7 +215,7 @@ int xs_host_check_evict(const xs_cache_dims* dims, const xs_cache_evict_args* in
   const int rc = check_sizes(dims, in->dtype, in->head_dim, in->seqs, in->kv_heads, in->capacity, in->max_len);
   if (rc != XS_OK || in->seqs == 0) return rc;
   if (!in->len || !in->mass || !in->new_mass || !in->pos || !in->new_pos || !in->next_pos || !in->new_len ||
-      !in->seq_status || in->new_len == in->len)
+      !in->seq_status || !apart(in->len, in->new_len, in->seqs))
     return XS_ERR_ARG;
   if ((in->new_mass == in->mass) != (in->new_pos == in->pos)) return XS_ERR_ARG;
   if (in->keep < 1 || in->sinks < 0 || in->recent < 0 || in->sinks > in->keep || in->recent > in->keep - in->sinks)

@@ -7,12 +7,10 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 #include <math.h>
 #include <stdint.h>
 #include <stdlib.h>
-#include <string.h>
-
-#include <type_traits>
 
 #include "../../include/xsamp.h"
 #include "xs_host.h"
@@ -28,24 +26,16 @@ constexpr float NEG_INF = -__builtin_huge_valf();
 // Elements of the two types as f32.
 struct Bf16 {
   XS_DEV static float widen(uint16_t u) { return __uint_as_float((uint32_t)u << 16); }
-  // round to nearest even; NaN stays NaN
-  XS_DEV static uint16_t narrow(float f) {
-    const uint32_t u = __float_as_uint(f);
-    if (f != f) return (uint16_t)((u >> 16) | 0x40u);
-    return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
-  }
 };
 struct F16 {
   XS_DEV static float widen(uint16_t u) { return (float)__builtin_bit_cast(_Float16, u); }
-  XS_DEV static uint16_t narrow(float f) { return __builtin_bit_cast(uint16_t, (_Float16)f); }
 };
 
 // The nodes a node sees: bit j of lane i's result is set when j is i or an
 // ancestor of i; 0 where i's chain of parents does not end in -1 by way of
 // ever lower nodes below n.  Each round doubles the distance a lane has gone
-// up, so six rounds reach the root from any of 64 nodes.  One whole wave.
-// p: the lane's parent.
-XS_DEV int parent_of(const xs_tree_attend_args& a, int b) { return a.parent[b * a.nodes + min((int)threadIdx.x & 63, (int)a.nodes - 1)]; }
+// up, so six rounds reach the root from any of 64 nodes.  One whole wave; p is
+// the lane's parent (parent_of).
 XS_DEV uint64_t ancestors(int p, int n) {
   const int lane = threadIdx.x & 63;
   int up = -2;  // -1: at the root; -2: the chain is broken
@@ -63,6 +53,7 @@ XS_DEV uint64_t ancestors(int p, int n) {
   }
   return up == -1 ? seen : 0ull;
 }
+XS_DEV int parent_of(const xs_tree_attend_args& a, int b) { return a.parent[b * a.nodes + min((int)threadIdx.x & 63, (int)a.nodes - 1)]; }
 
 // ---------------------------------------------------------------------------
 // Attention.
@@ -528,7 +519,8 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
 // scores beside this block's exponentials, this block's products beside the next
 // block's maxima.  Reading the keys from L2 in every wave instead, 64 bytes a
 // cycle and CU, takes as long as the matrix instructions, and not beside them:
-// 8 sequences of 64 nodes over 32,768 slots XWIDE.
+// 8 sequences of 64 nodes over 32,768 slots (256 rows of 8 kv heads) 520 us,
+// so 363 (757 TFLOP/s of the 1,290 of a large library product).
 template <int DP>
 struct Stage {
   static constexpr int SK = DP > 128 ? 32 : 64;
@@ -1306,8 +1298,9 @@ XS_DEV void each_slot(const Head& h, F f) {
 // Slots in registers: V times four consecutive ones a thread (len <= 4 V EB;
 // 16-byte aligned arrays of a slot_ld that is a multiple of 4).  apart: the rows of
 // k and v are left to evict_rows_kernel; else there are at most NEAR moves,
-// made here.  4,128 slots to 4,096, 128 heads: 15 us with 4-byte loads and a
-// bitmap, EV1; 32 heads of up to 32,768 to 2,048: 41 us so, EV2.
+// made here.  Bound by latency and by one CU's share: 128 heads of 4,128 slots
+// cut to 4,096 take 12.8 us (26.6 when every pass read its slots again), 32
+// heads of 1,311 to 32,768 cut to 2,048 take 28 us here (54) and 9 for the rows.
 template <int V>
 __global__ __launch_bounds__(EB) void evict_kernel(const xs_cache_evict_args a, const EvictWork w, int apart) {
   __shared__ SelectLds lds;
@@ -1571,9 +1564,6 @@ int64_t attend_floats(const xs_cache_dims& dims, int n_cu) {
   return most;
 }
 
-#ifndef WIDE_ROWS
-#define WIDE_ROWS 64
-#endif
 template <typename T, int DP, int RT, bool WIDE>
 int attend_exact(xs_cache_context* c, const xs_tree_attend_args& a) {
   return a.head_dim == DP ? attend_run<T, DP, RT, true, WIDE>(c, a) : attend_run<T, DP, RT, false, WIDE>(c, a);
@@ -1585,7 +1575,9 @@ int attend_rows(xs_cache_context* c, const xs_tree_attend_args& a) {
   if (rows <= 16) return attend_exact<T, DP, 1, false>(c, a);
   if (rows <= 32) return attend_exact<T, DP, 2, false>(c, a);
   if constexpr (DP <= 128) {
-    if (rows <= WIDE_ROWS) return attend_exact<T, DP, 4, false>(c, a);
+    // (128 rows as two row tiles of four waves: 261 us for 8 x 32 nodes over
+    // 32,768 slots; as two workgroups of 64 rows each, reading the keys twice, 317)
+    if (rows <= 64) return attend_exact<T, DP, 4, false>(c, a);
     if (rows <= 128) return attend_exact<T, DP, 2, true>(c, a);
     return attend_exact<T, DP, 4, true>(c, a);
   } else {
@@ -1646,6 +1638,20 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 }  // namespace
 
+namespace {
+// The calls run on the context's device and leave the thread's current one as
+// it was.
+struct OnDevice {
+  int before = -1;
+  bool ok;
+  explicit OnDevice(int device) { ok = hipGetDevice(&before) == hipSuccess && (before == device || hipSetDevice(device) == hipSuccess); }
+  ~OnDevice() {
+    int now = -1;
+    if (before >= 0 && hipGetDevice(&now) == hipSuccess && now != before) (void)hipSetDevice(before);
+  }
+};
+}  // namespace
+
 extern "C" {
 
 int xs_cache_create(int device, const xs_cache_dims* dims, xs_cache_context** out) {
@@ -1653,7 +1659,8 @@ int xs_cache_create(int device, const xs_cache_dims* dims, xs_cache_context** ou
   *out = nullptr;
   const int rc = xs_host_check_dims(dims);
   if (rc) return rc;
-  if (hipSetDevice(device) != hipSuccess) return XS_ERR_HIP;
+  const OnDevice on(device);
+  if (!on.ok) return XS_ERR_HIP;
   xs_cache_context* c = (xs_cache_context*)calloc(1, sizeof(xs_cache_context));
   if (!c) return XS_ERR_HIP;
   c->device = device;
@@ -1678,7 +1685,7 @@ int xs_cache_create(int device, const xs_cache_dims* dims, xs_cache_context** ou
 
 int xs_cache_destroy(xs_cache_context* c) {
   if (!c) return XS_OK;
-  (void)hipSetDevice(c->device);
+  const OnDevice on(c->device);
   if (c->stream) (void)hipStreamSynchronize(c->stream); else (void)hipDeviceSynchronize();
   if (c->part) (void)hipFree(c->part);
   if (c->evict.kept) (void)hipFree(c->evict.kept);
@@ -1699,7 +1706,8 @@ int xs_tree_attend(xs_cache_context* c, const xs_tree_attend_args* in) {
   const int rc = xs_host_check_attend(c ? &c->dims : nullptr, in);
   if (rc) return rc;
   if (in->seqs == 0) return XS_OK;
-  if (hipSetDevice(c->device) != hipSuccess) return XS_ERR_HIP;
+  const OnDevice on(c->device);
+  if (!on.ok) return XS_ERR_HIP;
   if (in->dtype == XS_BF16) return attend_dim<xst::Bf16>(c, *in);
   return attend_dim<xst::F16>(c, *in);
 }
@@ -1708,7 +1716,8 @@ int xs_cache_commit(xs_cache_context* c, const xs_cache_commit_args* in) {
   const int rc = xs_host_check_commit(c ? &c->dims : nullptr, in);
   if (rc) return rc;
   if (in->seqs == 0) return XS_OK;
-  if (hipSetDevice(c->device) != hipSuccess) return XS_ERR_HIP;
+  const OnDevice on(c->device);
+  if (!on.ok) return XS_ERR_HIP;
   if (in->dtype == XS_BF16) return commit_dim<xst::Bf16>(c, *in);
   return commit_dim<xst::F16>(c, *in);
 }
@@ -1717,7 +1726,8 @@ int xs_cache_evict(xs_cache_context* c, const xs_cache_evict_args* in) {
   const int rc = xs_host_check_evict(c ? &c->dims : nullptr, in);
   if (rc) return rc;
   if (in->seqs == 0) return XS_OK;
-  if (hipSetDevice(c->device) != hipSuccess) return XS_ERR_HIP;
+  const OnDevice on(c->device);
+  if (!on.ok) return XS_ERR_HIP;
   const int64_t limit = in->max_len ? in->max_len : in->capacity;
   const int64_t heads = in->seqs * in->kv_heads;
   // moves of a head: at most the slots past keep, and the slots of keep

@@ -42,9 +42,16 @@ class CacheContext:
         self._stream = None
 
     def bind_stream(self, stream):
-        if stream.cuda_stream != self._stream:
-            _lib.check(self.lib.xs_cache_set_stream(self.h, C.c_void_p(stream.cuda_stream)), "xs_cache_set_stream")
-            self._stream = stream.cuda_stream
+        """The stream of the calls from here on.  Their workspace is the context's: the new
+        stream waits for the old one's calls (but a stream under capture, which cannot wait
+        for work outside its graph; torch.cuda.graph has the device run dry first)."""
+        old = self._stream
+        if old is not None and stream.cuda_stream == old.cuda_stream:
+            return
+        if old is not None and not _torch().cuda.is_current_stream_capturing():
+            stream.wait_stream(old)
+        _lib.check(self.lib.xs_cache_set_stream(self.h, C.c_void_p(stream.cuda_stream)), "xs_cache_set_stream")
+        self._stream = stream
 
     def bind_current_stream(self):
         self.bind_stream(_torch().cuda.current_stream(self.device))
@@ -92,13 +99,18 @@ def _dtype(t):
 def _kv(ctx, kv, k, v, shape, name):
     kv.k = _tensor(ctx, k, name + "_k", shape, k.dtype, contiguous=False)
     kv.v = _tensor(ctx, v, name + "_v", shape, k.dtype, contiguous=False)
-    _need(k.stride() == v.stride(), f"{name}_k and {name}_v have different strides")
-    kv.seq_stride, kv.slot_stride, kv.head_stride = k.stride()[:3]
+    _need(_strides(k) == _strides(v), f"{name}_k and {name}_v have different strides")
+    kv.seq_stride, kv.slot_stride, kv.head_stride = _strides(k)
+
+
+def _strides(t):
+    """The first three strides; that of a dimension of one entry says nothing."""
+    return [s if n > 1 else 0 for n, s in zip(t.shape[:3], t.stride()[:3])]
 
 
 def _queries(ctx, a, q, shape, dtype):
     a.q = _tensor(ctx, q, "q", shape, dtype, contiguous=False)
-    a.q_seq_stride, a.q_node_stride, a.q_head_stride = q.stride()[:3]
+    a.q_seq_stride, a.q_node_stride, a.q_head_stride = _strides(q)
 
 
 @dataclass
@@ -135,7 +147,7 @@ def tree_attend(ctx: CacheContext, q, cache_k, cache_v, length, fresh_k, fresh_v
                        lse=torch.empty((B, N, HQ), dtype=torch.float32, device=q.device),
                        seq_status=torch.empty(B, dtype=torch.int32, device=q.device))
     a.out = _tensor(ctx, out.out, "out", (B, N, HQ, D), q.dtype, contiguous=False)
-    a.out_seq_stride, a.out_node_stride, a.out_head_stride = out.out.stride()[:3]
+    a.out_seq_stride, a.out_node_stride, a.out_head_stride = _strides(out.out)
     a.lse = None if out.lse is None else _tensor(ctx, out.lse, "lse", (B, N, HQ), torch.float32)
     a.seq_status = _tensor(ctx, out.seq_status, "seq_status", (B,), torch.int32)
     ctx.bind_current_stream()
