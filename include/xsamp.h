@@ -61,7 +61,9 @@ extern "C" {
  *   XS_ROW_BAD_PARAM   min(top_k, enc) larger than the context's k_max, or a
  *                      control list past the context's ctl_max (XS_CTL_MAX by
  *                      default, xs_create_ex) entries (no reference
- *                      counterpart: the reference has no such limits)
+ *                      counterpart: the reference has no such limits); of the
+ *                      tree and cache calls, a sequence whose length, tree or
+ *                      path is out of bounds
  *   XS_ROW_INTERNAL    the row's workgroups did not all run on one XCD, as
  *                      the grid's placement expects (no reference
  *                      counterpart); the row was not sampled, its token is -1.

@@ -329,6 +329,24 @@ def test_streams_in_turn_share_the_workspace(ctx):
             assert torch.equal(got.out, want[j].out) and torch.equal(got.lse, want[j].lse)
 
 
+@pytest.mark.parametrize("nodes", [1, 20])
+def test_many_sequences(nodes):
+    """2,000 sequences over one cache (their stride 0): every one the first one's result."""
+    from xwen_amd import tree
+    rng = np.random.default_rng(19)
+    big = context(max_seqs=2000, max_nodes=nodes, q_heads=8, kv_heads=2, head_dim=64, capacity=128)
+    c = case(rng, [100], nodes, 8, 2, 64, BF)
+    want = run(big, c, out=blank(c))
+    agree(c, want)
+    n = 2000
+    many = {t: c[t].expand(n, *c[t].shape[1:]) for t in ("q", "k", "v", "fk", "fv")}
+    got = tree.tree_attend(big, many["q"], many["k"], many["v"], torch.full((n,), 100, dtype=torch.int32, device="cuda"),
+                           many["fk"], many["fv"], c["parent"].cuda().expand(n, nodes).contiguous())
+    assert bool((got.seq_status == 0).all())
+    assert torch.equal(got.out, want.out.expand_as(got.out)) and torch.equal(got.lse, want.lse.expand_as(got.lse))
+    big.close()
+
+
 def test_strides_of_single_entries_do_not_matter(ctx):
     """One kv head, one node, one sequence, their strides any number."""
     rng = np.random.default_rng(18)

@@ -110,6 +110,23 @@ def test_commit_path_lengths(ctx, nodes):
     check_commit(ctx, c)
 
 
+def test_commit_many_rows_in_place(ctx):
+    """More rows than a wave holds: further passes add to what the first wrote, here into mass itself."""
+    rng = np.random.default_rng(9)
+    c = commit_case(rng, [300, 1000], 64, 16, 2, 128, BF)
+    c["parent"] = torch.tensor([list(range(-1, 63))] * 2, dtype=torch.int32)
+    c["path"], c["m"] = [list(range(64))] * 2, [64, 41]
+    check_commit(ctx, c, in_place=True)
+
+
+def test_commit_a_node_twice(ctx):
+    """A path may name a node again (nothing forbids it): it is appended and counted again."""
+    rng = np.random.default_rng(10)
+    c = commit_case(rng, [70, 5], 6, 4, 2, 64, BF)
+    c["path"], c["m"] = [[0, 0, 2, 0, -1, -1], [3, 3, 3, 3, 3, 3]], [4, 6]
+    check_commit(ctx, c)
+
+
 @pytest.mark.parametrize("nodes,hq,h,d,dtype", [(1, 8, 2, 128, BF), (30, 16, 2, 256, HF), (64, 32, 8, 64, BF)])
 def test_commit_long(ctx, nodes, hq, h, d, dtype):
     rng = np.random.default_rng(nodes)

@@ -2,7 +2,9 @@
 the device is touched, and the Python mirror's refusals."""
 import ctypes as C
 import os
+import shutil
 import subprocess
+import sys
 
 import pytest
 
@@ -169,6 +171,26 @@ def test_verify_tree_checks(host):
     assert chk(n_eog=1) == E and chk(n_eog=-1) == E and chk(n_eog=1, eog=DEV) == OK and chk(k_max=-1) == E
     assert chk(ld=248_322) == E and chk(logits=DEV + 4) == E
     assert host.xs_host_check_verify_tree(None, None) == E
+
+
+def test_the_checks_under_asan_and_ubsan():
+    """The checks above against the sanitized host build, in a child process."""
+    if os.environ.get("XS_HOST_LIB"):
+        pytest.skip("this is the child")
+    rt = subprocess.run(["gcc", "-print-file-name=libasan.so"], capture_output=True, text=True).stdout.strip() if shutil.which("gcc") else ""
+    if not os.path.isabs(rt) or not os.path.exists(rt) or not shutil.which("make"):
+        pytest.skip("gcc's AddressSanitizer runtime is not installed")
+    oracle = os.path.join(_lib.ROOT, "oracle")
+    subprocess.run(["make", "-s", "-C", oracle, "asan"], check=True)
+    env = dict(os.environ, LD_PRELOAD=rt, ASAN_OPTIONS="detect_leaks=0:halt_on_error=1:abort_on_error=1",
+               UBSAN_OPTIONS="halt_on_error=1:print_stacktrace=1",
+               XS_ORACLE_LIB=os.path.join(oracle, "_build", "asan", "libxs_oracle.so"),
+               XS_HOST_LIB=os.path.join(oracle, "_build", "asan", "libxs_host.so"))
+    r = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-p", "no:cacheprovider", "-k", "checks and not asan or sizes",
+                        os.path.abspath(__file__)], cwd=_lib.ROOT, env=env, capture_output=True, text=True, timeout=600)
+    tail = (r.stdout + r.stderr)[-4000:]
+    assert r.returncode == 0 and " passed" in r.stdout, tail
+    assert "AddressSanitizer" not in r.stderr and "runtime error:" not in r.stderr, tail
 
 
 def test_calls_without_a_context():

@@ -511,8 +511,8 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
 
 // Many rows (more than one wave's): the four waves of a workgroup take RT row
 // tiles each and share the keys, which come through LDS in stages of SK, three
-// buffers deep: while one is read, the next is complete and the one after it on its way from memory
-// in registers.  Per block of 32 keys a wave does RT * (2 DP/32 + DP/16)
+// buffers deep: while one is read, the next is complete and the one after it
+// on its way from memory in registers.  Per block of 32 keys a wave does RT * (2 DP/32 + DP/16)
 // matrix instructions of 16 cycles and about as many cycles of vector work (8
 // exponentials a tile of 16 cycles each, then scaling, maxima, sums, packing,
 // the byte permutes), so the two are laid side by side: the next block's
@@ -520,7 +520,7 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
 // block's maxima.  Reading the keys from L2 in every wave instead, 64 bytes a
 // cycle and CU, takes as long as the matrix instructions, and not beside them:
 // 8 sequences of 64 nodes over 32,768 slots (256 rows of 8 kv heads) 520 us,
-// so 363 (757 TFLOP/s of the 1,290 of a large library product).
+// so 375 (733 TFLOP/s, of the 1,291 of a large library product).
 template <int DP>
 struct Stage {
   static constexpr int SK = DP > 128 ? 32 : 64;

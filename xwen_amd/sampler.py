@@ -49,7 +49,8 @@ ROW_STATUS_NAMES = {
     _lib.ROW_NARROW: "logit row is narrower than the encodable ids the sampler draws over",
     _lib.ROW_BAD_PARAM: "top_k exceeds the sampler context's k_max (create the context with a "
                         "larger k_max), or a control list holds more entries than the context's "
-                        "ctl_max (XS_CTL_MAX unless the context was created with a larger one)",
+                        "ctl_max (XS_CTL_MAX unless the context was created with a larger one); of a "
+                        "tree or cache call: the sequence's length, tree or path is out of bounds",
     _lib.ROW_INTERNAL: "the row's workgroups did not share one XCD (placement check); not sampled",
     _lib.ROW_ID_OOR: "a scored token id is outside the encodable ids",
     _lib.ROW_CACHE_FULL: "the cache has no room for the accepted path",
