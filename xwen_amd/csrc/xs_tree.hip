@@ -883,12 +883,10 @@ XS_DEV void load_rows(const xs_cache_commit_args& a, Rows<DP, RT>& w, int b, int
   }
 }
 
-// The weight that the rows give to two tiles of 16 keys, in every lane group.
-// TAIL: keys are path ranks, seen from their own rank on.
-template <typename T, int DP, int RT, bool EXACT, bool TAIL>
-XS_DEV void weigh(const Rows<DP, RT>& w, const uint16_t* (&kp)[2], int D, float scale, int row0, int R, int G, int rank0, float (&sum)[2]) {
-  const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
-  u32x4 k[2][DP / 32];
+// Two tiles of 16 keys.
+template <int DP, bool EXACT>
+XS_DEV void load_keys(const uint16_t* const (&kp)[2], int D, u32x4 (&k)[2][DP / 32]) {
+  const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
   for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -896,6 +894,13 @@ XS_DEV void weigh(const Rows<DP, RT>& w, const uint16_t* (&kp)[2], int D, float 
       const int d = 32 * c + 8 * g;
       k[u][c] = EXACT || d < D ? *(const u32x4*)(kp[u] + d) : (u32x4){0, 0, 0, 0};
     }
+}
+
+// The weight that the rows give to two tiles of keys, in every lane group.
+// TAIL: keys are path ranks, seen from their own rank on.
+template <typename T, int DP, int RT, bool TAIL>
+XS_DEV void weigh(const Rows<DP, RT>& w, const u32x4 (&k)[2][DP / 32], float scale, int row0, int R, int G, int rank0, float (&sum)[2]) {
+  const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
   sum[0] = sum[1] = 0.0f;
 #pragma unroll
   for (int t = 0; t < RT; t++) {
@@ -947,16 +952,26 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 256 ? 3 : 2) void commit_kernel
     do {
       load_rows<DP, RT, EXACT>(a, w, b, kh, G, node, row0, R);
       const float* from = row0 == 0 ? a.mass : a.new_mass;
-      for (int key0 = ((blk - 1) * NW * share + wave) * KB; key0 < end; key0 += NW * KB) {
+      auto load = [&](int key0, u32x4 (&k)[2][DP / 32], float& old) {
         const uint16_t* kp[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) kp[u] = ck + min(key0 + 16 * u + x, len - 1) * a.cache.slot_stride;
+        load_keys<DP, EXACT>(kp, a.head_dim, k);
         const int slot = key0 + 16 * (g & 1) + x;
-        const bool mine = g < 2 && slot < end;
-        const float old = mine ? from[slots + slot] : 0.0f;
+        old = g < 2 && slot < end ? from[slots + slot] : 0.0f;
+      };
+      int key0 = ((blk - 1) * NW * share + wave) * KB;
+      u32x4 k[2][DP / 32];
+      float old;
+      if (key0 < end) load(key0, k, old);
+      while (key0 < end) {
+        const int next = key0 + NW * KB;
         float sum[2];
-        weigh<T, DP, RT, EXACT, false>(w, kp, a.head_dim, scale, row0, R, G, 0, sum);
-        if (mine) a.new_mass[slots + slot] = old + ((g & 1) ? sum[1] : sum[0]);
+        weigh<T, DP, RT, false>(w, k, scale, row0, R, G, 0, sum);
+        const int slot = key0 + 16 * (g & 1) + x;
+        if (g < 2 && slot < end) a.new_mass[slots + slot] = old + ((g & 1) ? sum[1] : sum[0]);
+        if (next < end) load(next, k, old);
+        key0 = next;
       }
       row0 += 16 * RT;
     } while (row0 < R);
@@ -967,11 +982,13 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 256 ? 3 : 2) void commit_kernel
     const uint16_t* fk = (const uint16_t*)a.fresh.k + b * a.fresh.seq_stride + kh * a.fresh.head_stride;
 #pragma unroll
     for (int u = 0; u < 2; u++) kp[u] = fk + __shfl(node, min(wave * KB + 16 * u + x, m - 1)) * a.fresh.slot_stride;
+    u32x4 k[2][DP / 32];
+    load_keys<DP, EXACT>(kp, a.head_dim, k);
     float all[2] = {0.0f, 0.0f};
     for (int row0 = 0; row0 < R; row0 += 16 * RT) {
       load_rows<DP, RT, EXACT>(a, w, b, kh, G, node, row0, R);
       float sum[2];
-      weigh<T, DP, RT, EXACT, true>(w, kp, a.head_dim, scale, row0, R, G, wave * KB, sum);
+      weigh<T, DP, RT, true>(w, k, scale, row0, R, G, wave * KB, sum);
       all[0] += sum[0];
       all[1] += sum[1];
     }
@@ -1499,9 +1516,9 @@ namespace {
 // launch bound asks for as many), by the head's size and the row tiles.
 constexpr int64_t per_cu(int dp, int rt) { return dp * rt <= 64 ? 4 : dp * rt <= 128 ? 3 : dp * rt <= 256 ? 2 : 1; }
 // How many times over a split call fills the device: once where all sequences
-// end together (one of them: 8 heads over 131,072 slots 145 -> 113 us against four times), more
-// often where some end early (32 sequences of 327 to 8,192 slots 151 -> 134 us
-// against twice, while 32 of 8,192 take 222 instead of 214).
+// end together (one of them: 8 heads over 131,072 slots 113 us, filled four
+// times 145), more often where some end early (32 sequences of 327 to 8,192
+// slots: 134 us, filled twice 151; but 32 of 8,192 take 222 instead of 214).
 constexpr int64_t rounds(int64_t seqs) { return seqs > 1 ? 4 : 1; }
 
 template <typename T, int DP, int RT, bool EXACT, bool WIDE>
@@ -1599,10 +1616,11 @@ template <typename T, int DP, int RT>
 int commit_run(xs_cache_context* c, const xs_cache_commit_args& a) {
   const int64_t limit = a.max_len ? a.max_len : a.capacity;
   const int64_t blocks = (limit + xst::KB - 1) / xst::KB, heads = a.seqs * a.kv_heads;
-  // Key blocks of a wave: the device filled as often as attention's (rounds),
-  // and at least RT, so that a wave reads twice as many keys as rows (2 heads of 65,536
-  // slots of 256, 8 nodes: 38 us with 4, 63 with 1).
-  const int64_t waves = xst::NW * c->n_cu * commit_per_cu(DP, RT) * rounds(a.seqs);
+  // Key blocks of a wave: the device filled once, or, where sequences may end
+  // early, five times (64 sequences of 327 to 8,192 slots: 170 us with four,
+  // 146 so), and at least RT, so that a wave reads twice as many keys as rows (2
+  // sequences of 65,536 slots of 256, 8 nodes: 34 us with 4, 63 with 1).
+  const int64_t waves = xst::NW * c->n_cu * commit_per_cu(DP, RT) * (a.seqs > 1 ? 5 : 1);
   const int64_t share = std::max<int64_t>(RT, (blocks * heads + waves - 1) / waves);
   const int64_t shares = (a.q ? (blocks + xst::NW * share - 1) / (xst::NW * share) : 0) + 1;
   if (heads * shares > 0x7FFFFFFF) return XS_ERR_CAPACITY;
