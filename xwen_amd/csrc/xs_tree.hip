@@ -382,6 +382,31 @@ XS_DEV void store_pair(const xs_tree_attend_args& a, int G, int b, int kh, int r
     a.lse[(b * a.nodes + node) * a.q_heads + head] = l == 0.0f ? NEG_INF : LN2 * (m + __builtin_amdgcn_logf(l));
 }
 
+// All fragments of half h, VE elements of each r at a time (pairs of 4 bytes
+// instead: 19 us of a workgroup's 58 where 32 sequences of 500 slots have 256 rows each).
+template <typename T, int DP, int RT>
+XS_DEV void store_half(const xs_tree_attend_args& a, int G, int b, int kh, int row, int R, int h, const f32x4 (&o)[Shape<DP, RT>::NF], float m,
+                       float l) {
+  constexpr int VE = Shape<DP, 1>::VE;
+  const int g = (threadIdx.x & 63) >> 4;
+  if (row >= R) return;
+  const int node = row / G, head = kh * G + row % G;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* out = (uint16_t*)a.out + b * a.out_seq_stride + node * a.out_node_stride + head * a.out_head_stride;
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    const int d = 128 * h + VE * (4 * g + r);
+    uint32_t y[VE / 2];
+#pragma unroll
+    for (int i = 0; i < VE / 2; i++) y[i] = pack2(T{}, o[h * VE + 2 * i][r] * inv, o[h * VE + 2 * i + 1][r] * inv);
+    if (d < a.head_dim) {
+      if constexpr (VE == 8) *(u32x4*)(out + d) = (u32x4){y[0], y[1], y[2], y[3]};
+      else *(u32x2*)(out + d) = (u32x2){y[0], y[1]};
+    }
+  }
+  if (a.lse && h == 0 && g == 0) a.lse[(b * a.nodes + node) * a.q_heads + head] = l == 0.0f ? NEG_INF : LN2 * (m + __builtin_amdgcn_logf(l));
+}
+
 // grid: groups of eight (sequence, kv head, split), each group's row tiles on
 // one XCD (workgroup index mod 8), which then reads their keys once.
 template <typename T, int DP, int RT, bool EXACT>
@@ -520,7 +545,7 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
 // block's maxima.  Reading the keys from L2 in every wave instead, 64 bytes a
 // cycle and CU, takes as long as the matrix instructions, and not beside them:
 // 8 sequences of 64 nodes over 32,768 slots (256 rows of 8 kv heads) 520 us,
-// so 375 (733 TFLOP/s, of the 1,291 of a large library product).
+// so 352 (781 TFLOP/s, of the 1,291 of a large library product).
 template <int DP>
 struct Stage {
   static constexpr int SK = DP > 128 ? 32 : 64;
@@ -622,7 +647,7 @@ __global__ __launch_bounds__(64 * NW, 1) void attend_wide_kernel(const xs_tree_a
 #pragma unroll
       for (int t = 0; t < RT; t++) {
         top[t] = w.template scaled<false>(s[t], cut.scale, 0u, xs[t]);
-        move = move || top[t] > w.most[t];
+        move = move | (top[t] > w.most[t]);
       }
       return move;
     };
@@ -706,7 +731,10 @@ __global__ __launch_bounds__(64 * NW, 1) void attend_wide_kernel(const xs_tree_a
 #pragma unroll
     for (int f = 0; f < S::NF; f++)
       if (l == 0.0f) w.o[t][f] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    if (whole) {
+    if (whole && !w.odd) {
+#pragma unroll
+      for (int h = 0; h < S::VH; h++) store_half<T, DP, RT>(a, cut.G, b, kh, row0 + 16 * t + x, R, h, w.o[t], ref, l);
+    } else if (whole) {
 #pragma unroll
       for (int h = 0; h < S::VH; h++)
 #pragma unroll
