@@ -439,7 +439,10 @@ typedef struct {
  * parent[i] is -1 (node i follows the cache) or a node below i; any other
  * value makes i and what follows it see nothing: out 0, lse -inf, as for a
  * row whose every score is -inf.  A score of NaN or +inf makes its row NaN;
- * what a node does not see never reaches it, whatever it holds.  Rows past
+ * what a node does not see never reaches it, whatever it holds.  q.k is an f32
+ * sum; as long as that is finite, keys may be masked by a finite value of any
+ * size, beside others or all of a row's (where scale q.k itself passes f32,
+ * out is right and lse infinite).  Rows past
  * n_nodes are left as they were, and a sequence whose len is outside
  * [0, max_len] or n_nodes outside [0, nodes] gets XS_ROW_BAD_PARAM and nothing
  * else. */

@@ -76,13 +76,19 @@ XS_DEV int parent_of(const xs_tree_attend_args& a, int b) { return a.parent[b * 
 //                 A fragments of them: fragment j is element 8 x + j of V.
 //
 // Softmax in one pass: weights exp2(x), x = (q.k - m) scale log2(e), with m a
-// running reference that follows the row's maximum only when that has grown by
-// more than 2^8 since (a rescaling of every accumulator is otherwise left out;
-// weights stay below 2^8, and the quotient by their sum is the same).  The
-// products start from -m, which costs nothing and keeps x exact where q.k is
-// huge (a mask of the type's lowest value).  f16 weights carry 2^6 more, so
-// that the small ones of a long row stay above the type's subnormals.  Weights
-// round to the inputs' type once; everything else is f32.
+// running reference, one of the row's own q.k, that follows the best of them
+// only when that has grown by more than 2^8 since (a rescaling of every
+// accumulator is otherwise left out; weights stay below 2^8, and the quotient
+// by their sum is the same).  The products start from -m, which costs nothing
+// and leaves no large term to cancel where every q.k is huge (a mask of the
+// type's lowest value).  A block whose scores lie far above m would be lost in
+// its rounding (masked keys before others): when the reference moves, the
+// block's products are formed again from 0.  Nothing divides by the scale, and
+// references are compared before they are scaled: equal scores have equal
+// weights, and a q.k that is finite may overflow once it is scaled.  f16
+// weights carry 2^6 more, so that the small ones of a long row stay above the
+// type's subnormals.  Weights round to the inputs' type once; everything else
+// is f32.
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -172,7 +178,7 @@ struct Wave {
   u32x4 q[RT][S::KC];
   f32x4 o[RT][S::NF];
   f32x4 c[RT];     // minus the row's reference (of q.k), four times: what the scores' products start from
-  float most[RT];  // the x above which the reference moves: -inf until the row's first score
+  float most[RT];  // the x above which the reference moves: NaN until the row's first score
   float l[RT];
   int odd;         // a node's values held a NaN or an infinity
 
@@ -181,7 +187,7 @@ struct Wave {
 #pragma unroll
     for (int t = 0; t < RT; t++) {
       c[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-      most[t] = NEG_INF;
+      most[t] = __builtin_nanf("");
       l[t] = 0.0f;
 #pragma unroll
       for (int f = 0; f < S::NF; f++) o[t][f] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
@@ -201,25 +207,37 @@ struct Wave {
     }
     return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
   }
-  // Moves the tile's reference to rows' maxima past `most` (rare).
-  XS_DEV void rebase(int t, float top, float scale, float (&x)[8]) {
+  // Whether the lane's row has a score past its reference's reach, or its first
+  // one (-inf too, which then changes nothing).
+  XS_DEV bool passes(int t, float top) const { return !(top <= most[t]); }
+  // Moves the references of the tile's rows to their best score (rare).  s: the
+  // scores from 0, of all rows or of those whose reference is 0.
+  template <bool MASKED>
+  XS_DEV void rebase(int t, const f32x4 (&s)[2], bool all, float scale, uint32_t on, float (&x)[8]) {
     constexpr float OFF = offset_of(T{});
-    top = row_max(top);
-    if (top > most[t]) {
-      const float old = c[t][0];
-      const float ref = scale == 0.0f ? old : old - (top - OFF) / scale;
-      const float step = (ref - old) * scale;  // (to a reference as it is held)
-      const float keep = most[t] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(step);
-      c[t] = (f32x4){ref, ref, ref, ref};
+    const int g = (threadIdx.x & 63) >> 4;
+    const float sign = scale < 0.0f ? -1.0f : 1.0f, old = -c[t][0];
+    const bool unset = most[t] != most[t];
+    // never below the old one (a product that starts elsewhere rounds elsewhere)
+    float best = unset ? NEG_INF : old * sign;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const float y = s[e >> 2][e & 3] * sign;
+      best = fmaxf(best, !MASKED || ((on >> (4 * g + (e & 3) + 16 * (e >> 2))) & 1u) ? y : NEG_INF);
+    }
+    best = row_max(best);
+    if ((all || old == 0.0f) && best > NEG_INF) {
+      const float ref = scale == 0.0f ? 0.0f : best * sign;
+      const float keep = unset ? 0.0f : __builtin_amdgcn_exp2f((old - ref) * scale);
+      c[t] = (f32x4){-ref, -ref, -ref, -ref};
       most[t] = LAZY + OFF;
       l[t] *= keep;
 #pragma unroll
       for (int f = 0; f < S::NF; f++) o[t][f] *= keep;
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        x[e] += step;
-        // (a reference so large that it cannot move by so little)
-        if (x[e] > LAZY + OFF) x[e] = LAZY + OFF;
+        x[e] = (s[e >> 2][e & 3] - ref) * scale + OFF;
+        if (MASKED) x[e] = ((on >> (4 * g + (e & 3) + 16 * (e >> 2))) & 1u) ? x[e] : NEG_INF;
       }
     }
   }
@@ -234,8 +252,9 @@ struct Wave {
     for (int i = 0; i < 4; i++) b[i] = pack2(T{}, p[2 * i], p[2 * i + 1]);
     return b;
   }
-  // The exponent of two that l and o carry.
-  XS_DEV float reference(int t, float scale) const { return -c[t][0] * scale - offset_of(T{}); }
+  // The reference, so that the larger one is the better: l and o carry 2 to the
+  // minus reference |scale|, and offset_of more.
+  XS_DEV float reference(int t, float scale) const { return scale < 0.0f ? c[t][0] : -c[t][0]; }
 };
 
 // O^T += V^T P^T over a block: v holds 16 bytes of each of the lane's eight
@@ -312,7 +331,26 @@ XS_DEV void block(Wave<T, DP, RT>& w, const uint16_t* kp, const uint16_t* vp, in
     }
     float xs[8];
     const float top = w.template scaled<MASKED>(s, scale, MASKED ? on[t] : 0u, xs);
-    if (__any(top > w.most[t])) w.rebase(t, top, scale, xs);
+    if (__any(w.passes(t, top))) {
+      const bool far = __any(w.passes(t, top) && w.c[t][0] != 0.0f);
+      if (far) {
+        s[0] = s[1] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          int key = key0 + 16 * u + x;
+          if (MASKED) key = min(key, limit - 1);
+          const uint16_t* p = kp + key * stride;
+          asm("" : "+v"(p));  // (read again: kept instead, the keys' registers would spill)
+#pragma unroll
+          for (int c = 0; c < S::KC; c++) {
+            const int d = 32 * c + 8 * g;
+            s[u] = mfma(T{}, EXACT || d < D ? *(const u32x4*)(p + d) : zero4, w.q[t][c], s[u]);
+            __builtin_amdgcn_sched_barrier(0);  // (one chunk in registers at a time)
+          }
+        }
+      }
+      w.template rebase<MASKED>(t, s, far, scale, MASKED ? on[t] : 0u, xs);
+    }
     pf[t] = w.weights(t, xs);
   }
   if (MASKED) {
@@ -347,11 +385,17 @@ XS_DEV void block(Wave<T, DP, RT>& w, const uint16_t* kp, const uint16_t* vp, in
   accumulate(w, v, pf);
 }
 
+// ln of a row's sum of weights, from its reference and l.
+template <typename T>
+XS_DEV float lse_of(const xs_tree_attend_args& a, float ref, float l) {
+  return l == 0.0f ? NEG_INF : __builtin_fmaf(ref, fabsf(a.scale), LN2 * (__builtin_amdgcn_logf(l) - offset_of(T{})));
+}
+
 // Two fragments (2 pair and 2 pair + 1 of half h) of a row tile's result: the
 // accumulators over l.  Lane (x, g) holds row x, elements 128 h + VE (4 g + r)
 // + 2 pair of each r.
 template <typename T, int DP>
-XS_DEV void store_pair(const xs_tree_attend_args& a, int G, int b, int kh, int row, int R, int h, int pair, f32x4 o0, f32x4 o1, float m, float l, int odd,
+XS_DEV void store_pair(const xs_tree_attend_args& a, int G, int b, int kh, int row, int R, int h, int pair, f32x4 o0, f32x4 o1, float ref, float l, int odd,
                        int n) {
   constexpr int VE = Shape<DP, 1>::VE;
   const int g = (threadIdx.x & 63) >> 4;
@@ -379,13 +423,13 @@ XS_DEV void store_pair(const xs_tree_attend_args& a, int G, int b, int kh, int r
     if (d < a.head_dim) *(uint32_t*)(out + d) = pack2(T{}, o0[r] * inv, o1[r] * inv);
   }
   if (a.lse && h == 0 && pair == 0 && g == 0)
-    a.lse[(b * a.nodes + node) * a.q_heads + head] = l == 0.0f ? NEG_INF : LN2 * (m + __builtin_amdgcn_logf(l));
+    a.lse[(b * a.nodes + node) * a.q_heads + head] = lse_of<T>(a, ref, l);
 }
 
 // All fragments of half h, VE elements of each r at a time (pairs of 4 bytes
 // instead: 19 us of a workgroup's 58 where 32 sequences of 500 slots have 256 rows each).
 template <typename T, int DP, int RT>
-XS_DEV void store_half(const xs_tree_attend_args& a, int G, int b, int kh, int row, int R, int h, const f32x4 (&o)[Shape<DP, RT>::NF], float m,
+XS_DEV void store_half(const xs_tree_attend_args& a, int G, int b, int kh, int row, int R, int h, const f32x4 (&o)[Shape<DP, RT>::NF], float ref,
                        float l) {
   constexpr int VE = Shape<DP, 1>::VE;
   const int g = (threadIdx.x & 63) >> 4;
@@ -404,7 +448,7 @@ XS_DEV void store_half(const xs_tree_attend_args& a, int G, int b, int kh, int r
       else *(u32x2*)(out + d) = (u32x2){y[0], y[1]};
     }
   }
-  if (a.lse && h == 0 && g == 0) a.lse[(b * a.nodes + node) * a.q_heads + head] = l == 0.0f ? NEG_INF : LN2 * (m + __builtin_amdgcn_logf(l));
+  if (a.lse && h == 0 && g == 0) a.lse[(b * a.nodes + node) * a.q_heads + head] = lse_of<T>(a, ref, l);
 }
 
 // grid: groups of eight (sequence, kv head, split), each group's row tiles on
@@ -490,12 +534,13 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
     }
   }
   __syncthreads();
+  const float mag = fabsf(cut.scale);
 #pragma unroll
   for (int t = 0; t < RT; t++) {
     float top = NEG_INF;
 #pragma unroll
     for (int j = 0; j < NW; j++) top = fmaxf(top, stat[j][t][0][x]);
-    const float f = ref[t] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(ref[t] - top);
+    const float f = ref[t] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((ref[t] - top) * mag);
 #pragma unroll
     for (int k = 0; k < S::NF; k++) sum[wave][t][k][lane] = ref[t] == NEG_INF ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : w.o[t][k] * f;
   }
@@ -515,7 +560,7 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
 #pragma unroll
     for (int j = 0; j < NW; j++) {
       const float mj = stat[j][t][0][x];
-      all += mj == NEG_INF ? 0.0f : stat[j][t][1][x] * __builtin_amdgcn_exp2f(mj - top);
+      all += mj == NEG_INF ? 0.0f : stat[j][t][1][x] * __builtin_amdgcn_exp2f((mj - top) * mag);
       o[0] += sum[j][t][f0][lane];
       o[1] += sum[j][t][f0 + 1][lane];
     }
@@ -615,19 +660,18 @@ __global__ __launch_bounds__(64 * NW, 1) void attend_wide_kernel(const xs_tree_a
       lv[s % 3][q] = rv[i];
     }
   };
-  // the scores of block j, counted in blocks from `first`
+  // 16 keys' chunk c of block j, counted in blocks from `first`
+  auto key = [&](int j, int u, int c) {
+    const int row = (j % SB) * KB + 16 * u + x;
+    return lk[(j / SB) % 3][row * G::CH + ((4 * c + g) ^ (row & G::TURN))];
+  };
+  // the scores of block j
   auto scores = [&](int j, f32x4 (&s)[RT][2]) {
-    const u32x4* k = lk[(j / SB) % 3];
 #pragma unroll
     for (int t = 0; t < RT; t++) s[t][0] = s[t][1] = w.c[t];
 #pragma unroll
     for (int c = 0; c < S::KC; c++) {
-      u32x4 f[2];
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const int row = (j % SB) * KB + 16 * u + x;
-        f[u] = k[row * G::CH + ((4 * c + g) ^ (row & G::TURN))];
-      }
+      const u32x4 f[2] = {key(j, 0, c), key(j, 1, c)};
 #pragma unroll
       for (int t = 0; t < RT; t++) {
         s[t][0] = mfma(T{}, f[0], w.q[t][c], s[t][0]);
@@ -647,21 +691,29 @@ __global__ __launch_bounds__(64 * NW, 1) void attend_wide_kernel(const xs_tree_a
 #pragma unroll
       for (int t = 0; t < RT; t++) {
         top[t] = w.template scaled<false>(s[t], cut.scale, 0u, xs[t]);
-        move = move | (top[t] > w.most[t]);
+        move = move | w.passes(t, top[t]);
       }
       return move;
     };
-    auto settle = [&]() {
+    auto settle = [&](int j) {
 #pragma unroll
       for (int t = 0; t < RT; t++) {
-        const float top = fmaxf(fmaxf(fmaxf(xs[t][0], xs[t][1]), fmaxf(xs[t][2], xs[t][3])), fmaxf(fmaxf(xs[t][4], xs[t][5]), fmaxf(xs[t][6], xs[t][7])));
-        w.rebase(t, top, cut.scale, xs[t]);
+        f32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+        for (int c = 0; c < S::KC; c++) {
+          s[0] = mfma(T{}, key(j, 0, c), w.q[t][c], s[0]);
+          s[1] = mfma(T{}, key(j, 1, c), w.q[t][c], s[1]);
+        }
+        w.template rebase<false>(t, s, true, cut.scale, 0u, xs[t]);
+        // (one tile in registers at a time: else the loop spills, 457 us for 365
+        // where 8 sequences of 64 nodes see 32,768 slots)
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
     {
       f32x4 s[RT][2];
       scores(0, s);
-      if (__any(prepare(s))) settle();
+      if (__any(prepare(s))) settle(0);
     }
     const int blocks = stages * SB;
 #pragma unroll 1
@@ -692,7 +744,7 @@ __global__ __launch_bounds__(64 * NW, 1) void attend_wide_kernel(const xs_tree_a
         }
         accumulate(w, v, pf);
         const bool move = prepare(s);
-        if (more && __any(move)) settle();
+        if (more && __any(move)) settle(j + 1);
       }
     }
   }
@@ -815,7 +867,7 @@ __global__ __launch_bounds__(join_threads<DP>(FEWER)) void join_kernel(const xs_
   for (int j = 0; j < WAVES; j++) top = fmaxf(top, stat[0][j][x]);
 #pragma unroll
   for (int i = 0; i < TURNS; i++) {
-    const float f = m[i] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m[i] - top);
+    const float f = m[i] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((m[i] - top) * fabsf(cut.scale));
     if (m[i] != NEG_INF) all += l[i] * f;
     weight[4 * (WAVES * i + wave) + g][x] = f;
   }
