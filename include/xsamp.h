@@ -438,7 +438,8 @@ typedef struct {
  * multiply the values, and out once at the end.  nodes = 1 is plain decoding.
  * parent[i] is -1 (node i follows the cache) or a node below i; any other
  * value makes i and what follows it see nothing: out 0, lse -inf, as for a
- * row whose every score is -inf.  A score of NaN or +inf makes its row NaN;
+ * row whose every score is -inf, whatever the values.  A score of NaN or +inf
+ * makes its row NaN, a value that is not finite the rows that give it weight;
  * what a node does not see never reaches it, whatever it holds.  q.k is an f32
  * sum; as long as that is finite, keys may be masked by a finite value of any
  * size, beside others or all of a row's (where scale q.k itself passes f32,

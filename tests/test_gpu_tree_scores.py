@@ -160,3 +160,17 @@ def test_scores_past_the_base_2_range(ctx, nodes, scale):
     c["q"][:] = 0.0
     one_column(c, LOWEST)
     agree_with_the_mean(c, run(ctx, c, scale=scale, out=blank(c)), LOWEST, scale=scale)
+
+
+@pytest.mark.parametrize("lens", [[50, 0, 300], [6000]])
+@pytest.mark.parametrize("nodes", [5, 40])
+def test_empty_rows_that_see_odd_values(ctx, nodes, lens):
+    """Every score is -inf: out is 0 and lse -inf, also where the values seen are NaN or infinite."""
+    rng = np.random.default_rng(26)
+    c = case(rng, lens, nodes, 8, 2, 64, BF)
+    one_column(c, -math.inf)
+    c["fv"][:, 0, :, 3] = math.nan
+    c["fv"][:, 2, :, 7] = math.inf
+    c["v"][:, 7, :, 5] = math.nan
+    got = run(ctx, c, out=blank(c))
+    assert bool((got.out == 0.0).all()) and bool((got.lse == -math.inf).all())

@@ -400,7 +400,7 @@ XS_DEV void store_pair(const xs_tree_attend_args& a, int G, int b, int kh, int r
   constexpr int VE = Shape<DP, 1>::VE;
   const int g = (threadIdx.x & 63) >> 4;
   const int node = min(row, R - 1) / G, head = kh * G + min(row, R - 1) % G;
-  if (odd) {  // (rare) the NaNs and infinities among the values of the nodes that the row sees
+  if (odd) {  // (rare) the NaNs and infinities among the values of the nodes that the row sees, but of an empty row's
     const uint64_t sees = __shfl(ancestors(parent_of(a, b), n), node);
     const uint16_t* v = (const uint16_t*)a.fresh.v + b * a.fresh.seq_stride + kh * a.fresh.head_stride;
 #pragma unroll 1
@@ -410,8 +410,8 @@ XS_DEV void store_pair(const xs_tree_attend_args& a, int G, int b, int kh, int r
         const int d = 128 * h + VE * (4 * g + r) + 2 * pair;
         const uint32_t two = *(const uint32_t*)(v + j * a.fresh.slot_stride + min(d, a.head_dim - 2));
         const uint16_t lo = (uint16_t)two, hi = (uint16_t)(two >> 16);
-        if (((sees >> j) & 1ull) && (lo & 0x7FFFu) >= inf_of(T{})) o0[r] += T::widen(lo);
-        if (((sees >> j) & 1ull) && (hi & 0x7FFFu) >= inf_of(T{})) o1[r] += T::widen(hi);
+        if (((sees >> j) & 1ull) && l != 0.0f && (lo & 0x7FFFu) >= inf_of(T{})) o0[r] += T::widen(lo);
+        if (((sees >> j) & 1ull) && l != 0.0f && (hi & 0x7FFFu) >= inf_of(T{})) o1[r] += T::widen(hi);
       }
   }
   if (row >= R) return;
