@@ -931,7 +931,7 @@ XS_DEV int read_path(const xs_cache_commit_args& a, int b, int len, int64_t limi
 template <int DP, int RT>
 struct Rows {
   u32x4 q[RT][DP / 32];
-  float lse[RT][4];  // of rows 4 g + r, times log2(e)
+  float lse[RT][4];  // of rows 4 g + r
   uint32_t on;       // bit 4 t + r: the lane's row 4 g + r of tile t counts
 };
 
@@ -958,7 +958,7 @@ XS_DEV void load_rows(const xs_cache_commit_args& a, Rows<DP, RT>& w, int b, int
       const int k = __shfl(node, m / G);
       const float v = a.lse[(b * a.nodes + k) * a.q_heads + kh * G + m % G];
       if (mine < R && v != NEG_INF) w.on |= 1u << (4 * t + r);
-      w.lse[t][r] = v * LOG2E;
+      w.lse[t][r] = v;
     }
   }
 }
@@ -995,7 +995,8 @@ XS_DEV void weigh(const Rows<DP, RT>& w, const u32x4 (&k)[2][DP / 32], float sca
     for (int r = 0; r < 4; r++)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        const float p = __builtin_amdgcn_exp2f(s[u][r] * scale - w.lse[t][r]);
+        // (the difference of two large terms, rounded once; then to base 2)
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], scale, -w.lse[t][r]) * LOG2E);
         bool on = (w.on >> (4 * t + r)) & 1u;
         if (TAIL) on = on && (row0 + 16 * t + 4 * g + r) / G >= rank0 + 16 * u + x;
         sum[u] += on ? p : 0.0f;
@@ -1006,7 +1007,7 @@ XS_DEV void weigh(const Rows<DP, RT>& w, const u32x4 (&k)[2][DP / 32], float sca
 }
 
 template <typename T, int DP, int RT, bool EXACT>
-__global__ __launch_bounds__(64 * NW, DP * RT <= 256 ? 3 : 2) void commit_kernel(const xs_cache_commit_args a, int shares, int share, float scale) {
+__global__ __launch_bounds__(64 * NW, DP * RT <= 256 ? 3 : 2) void commit_kernel(const xs_cache_commit_args a, int shares, int share) {
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int bh = blockIdx.x / shares, blk = turned(blockIdx.x % shares, bh, shares);
@@ -1047,7 +1048,7 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 256 ? 3 : 2) void commit_kernel
       while (key0 < end) {
         const int next = key0 + NW * KB;
         float sum[2];
-        weigh<T, DP, RT, false>(w, k, scale, row0, R, G, 0, sum);
+        weigh<T, DP, RT, false>(w, k, a.scale, row0, R, G, 0, sum);
         const int slot = key0 + 16 * (g & 1) + x;
         if (g < 2 && slot < end) a.new_mass[slots + slot] = old + ((g & 1) ? sum[1] : sum[0]);
         if (next < end) load(next, k, old);
@@ -1068,7 +1069,7 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 256 ? 3 : 2) void commit_kernel
     for (int row0 = 0; row0 < R; row0 += 16 * RT) {
       load_rows<DP, RT, EXACT>(a, w, b, kh, G, node, row0, R);
       float sum[2];
-      weigh<T, DP, RT, true>(w, k, scale, row0, R, G, wave * KB, sum);
+      weigh<T, DP, RT, true>(w, k, a.scale, row0, R, G, wave * KB, sum);
       all[0] += sum[0];
       all[1] += sum[1];
     }
@@ -1705,11 +1706,10 @@ int commit_run(xs_cache_context* c, const xs_cache_commit_args& a) {
   const int64_t shares = (a.q ? (blocks + xst::NW * share - 1) / (xst::NW * share) : 0) + 1;
   if (heads * shares > 0x7FFFFFFF) return XS_ERR_CAPACITY;
   const dim3 grid((unsigned)(heads * shares)), block(64 * xst::NW);
-  const float scale = a.scale * xst::LOG2E;
   if (a.head_dim == DP)
-    hipLaunchKernelGGL((xst::commit_kernel<T, DP, RT, true>), grid, block, 0, c->stream, a, (int)shares, (int)share, scale);
+    hipLaunchKernelGGL((xst::commit_kernel<T, DP, RT, true>), grid, block, 0, c->stream, a, (int)shares, (int)share);
   else
-    hipLaunchKernelGGL((xst::commit_kernel<T, DP, RT, false>), grid, block, 0, c->stream, a, (int)shares, (int)share, scale);
+    hipLaunchKernelGGL((xst::commit_kernel<T, DP, RT, false>), grid, block, 0, c->stream, a, (int)shares, (int)share);
   return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
 }
 
