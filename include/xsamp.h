@@ -480,7 +480,8 @@ int xs_tree_attend(xs_cache_context* ctx, const xs_tree_attend_args* args);
  *              the same without mass for the appended slots (which a node sees
  *              from its own rank on).  q, lse and scale are xs_tree_attend's.
  * Per-slot arrays are [seqs, kv_heads, slot_ld].  new_mass may be mass.  The
- * sums are f32, in an order fixed by the sizes.  A sequence whose len is
+ * sums are f32, in an order fixed by the sizes.  An exponent is off by the
+ * rounding of lse, 2^-24 of it; a slot of the cache gains at most 1 a row.  A sequence whose len is
  * outside [0, max_len], whose n_path is outside [0, nodes] or whose path holds
  * a node outside [0, nodes) gets XS_ROW_BAD_PARAM, one without room
  * XS_ROW_CACHE_FULL; its new_len and new_next_pos are len and next_pos, and

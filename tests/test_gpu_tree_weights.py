@@ -65,3 +65,39 @@ def test_large_scores_lose_nothing(ctx, nodes, m, hq, h, d, dtype):
         tol = (term * (2 * y.abs() + 2 + m * G) * F32 * 1.01 + 2.0**-126).sum((2, 3)).T
         off = (got[x, :, :n + m] - want).abs()
         assert bool((off <= tol).all()), float((off / tol).max())
+
+
+@pytest.mark.parametrize("value", [-1e6, -1e7, -1e8, -1e9, LOWEST, 1e9])
+@pytest.mark.parametrize("nodes,hq,h,d", [(1, 4, 2, 128), (7, 4, 2, 72), (40, 8, 2, 80)])
+def test_one_huge_score_for_all_stays_in_bounds(ctx, nodes, hq, h, d, value):
+    """lse as an f32 says nothing about such a row's weights (each 1 / n), but that none is above 1:
+    whatever the rounding of the two huge terms leaves, no slot gains more than one a row."""
+    rng = np.random.default_rng(d)
+    m = max(1, nodes - 2)
+    c = chain_case(rng, [300, 33, 0], nodes, m, hq, h, d, BF)
+    c["q"][..., 0] = 1.0
+    c["k"][..., 0] = c["fk"][..., 0] = value
+    lse = run(ctx, c, out=blank(c)).lse
+    mass = torch.rand((3, h, c["k"].shape[1]), device="cuda")
+    got = committed(ctx, c, lse, mass).double().cpu()
+    rows, old = m * hq // h, mass.double().cpu()
+    for b, n in enumerate(c["lens"]):
+        top = old[b, :, :n] + rows
+        assert bool((got[b, :, :n] >= old[b, :, :n]).all()) and bool((got[b, :, :n] <= top * (1 + (rows + 2) * F32)).all())
+        fresh = got[b, :, n:n + m]
+        assert bool((fresh >= 0).all()) and bool((fresh <= rows * (1 + (rows + 2) * F32)).all())
+
+
+def test_a_path_that_is_no_chain_keeps_its_weights(ctx):
+    """A node that the row's lse does not count may weigh more than 1: exp(scale q.k - lse) as it is."""
+    rng = np.random.default_rng(3)
+    c = chain_case(rng, [40], 4, 4, 2, 1, 64, BF)
+    c["parent"] = torch.tensor([[-1, 0, 0, 0]], dtype=torch.int32)
+    c["q"][..., 0] = 1.0
+    c["k"][..., 0] = 0.0
+    c["fk"][..., 0] = torch.tensor([0.0, 64.0, 0.0, 0.0], device="cuda")[None, :, None]
+    lse = run(ctx, c, scale=0.25, out=blank(c)).lse
+    got = committed(ctx, c, lse, torch.zeros((1, 1, c["k"].shape[1]), device="cuda"), scale=0.25)
+    ln = lse.double().cpu()[0]
+    want = sum(float((16.0 - ln[i]).exp().sum()) for i in (1, 2, 3))  # nodes 2 and 3 do not see node 1
+    assert want > 1e5 and abs(float(got[0, 0, 41]) - want) <= 60 * F32 * want

@@ -995,8 +995,14 @@ XS_DEV void weigh(const Rows<DP, RT>& w, const u32x4 (&k)[2][DP / 32], float sca
     for (int r = 0; r < 4; r++)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        // (the difference of two large terms, rounded once; then to base 2)
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], scale, -w.lse[t][r]) * LOG2E);
+        // The difference of two large terms, rounded once; then to base 2.  No
+        // slot of the cache weighs more than 1; where the two are huge, lse's
+        // own rounding may leave more, and exp of that an infinity.  A row of
+        // a path that is no chain may weigh a fresh key more: there only what
+        // rounding leaves (some steps of lse, 2^-24 of it each) is cut.
+        float y = __builtin_fmaf(s[u][r], scale, -w.lse[t][r]);
+        if (y > 0.0f && (!TAIL || y <= fabsf(w.lse[t][r]) * 0x1p-20f)) y = 0.0f;
+        const float p = __builtin_amdgcn_exp2f(y * LOG2E);
         bool on = (w.on >> (4 * t + r)) & 1u;
         if (TAIL) on = on && (row0 + 16 * t + 4 * g + r) / G >= rank0 + 16 * u + x;
         sum[u] += on ? p : 0.0f;
