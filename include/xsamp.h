@@ -405,8 +405,12 @@ int xs_verify_tree(xs_context* ctx, const xs_verify_tree_args* args);
 
 /* The workspace of the cache calls, sized for the largest call.  Allocates
  * once; calls allocate nothing afterwards and may be captured.  Owned by one
- * thread at a time, its calls serialised on its stream, like an xs_context;
- * graphs captured from one context are not to run at the same time. */
+ * thread at a time, its calls serialised on its stream, like an xs_context.
+ * No two of its calls may run at the same time, for they share the workspace:
+ * xs_cache_set_stream orders nothing, so the caller has the new stream wait
+ * for the old one's calls (in a capture too, where streams of one graph fork),
+ * and keeps replays of the context's graphs apart from each other and from its
+ * other calls. */
 typedef struct xs_cache_context xs_cache_context;
 typedef struct {
   int64_t max_seqs;

@@ -39,19 +39,23 @@ class CacheContext:
         h = C.c_void_p()
         _lib.check(self.lib.xs_cache_create(device, C.byref(dims), C.byref(h)), "xs_cache_create")
         self.h = h
-        self._stream = None
+        self._bound = None  # the stream's handle, and whether it recorded into a graph
+        self._last = {False: None, True: None}  # the stream of the last call outside a graph, and in one
 
     def bind_stream(self, stream):
         """The stream of the calls from here on.  Their workspace is the context's: the new
-        stream waits for the old one's calls (but a stream under capture, which cannot wait
-        for work outside its graph; torch.cuda.graph has the device run dry first)."""
-        old = self._stream
-        if old is not None and stream.cuda_stream == old.cuda_stream:
+        stream waits for the last call's, also where both are forks of one stream under capture.
+        A capture does not wait for work outside it (torch.cuda.graph has the device run dry
+        first), nor does that for a capture; replays, and calls beside them, are the caller's to
+        keep apart."""
+        inside = _capturing(stream)
+        if self._bound == (stream.cuda_stream, inside):
             return
-        if old is not None and not _torch().cuda.is_current_stream_capturing():
-            stream.wait_stream(old)
+        last = self._last[inside]
+        if last is not None and last.cuda_stream != stream.cuda_stream and (not inside or _capturing(last)):
+            stream.wait_stream(last)
         _lib.check(self.lib.xs_cache_set_stream(self.h, C.c_void_p(stream.cuda_stream)), "xs_cache_set_stream")
-        self._stream = stream
+        self._bound, self._last[inside] = (stream.cuda_stream, inside), stream
 
     def bind_current_stream(self):
         self.bind_stream(_torch().cuda.current_stream(self.device))
@@ -66,6 +70,17 @@ class CacheContext:
             self.close()
         except Exception:
             pass
+
+
+def _capturing(stream) -> bool:
+    """Whether the stream records into a graph (the null stream never does)."""
+    cuda = _torch().cuda
+    if stream.cuda_stream == 0:
+        return False
+    if stream == cuda.current_stream():
+        return cuda.is_current_stream_capturing()
+    with cuda.stream(stream):
+        return cuda.is_current_stream_capturing()
 
 
 def check(seq_status) -> None:
