@@ -417,6 +417,9 @@ typedef struct {
   int64_t max_nodes;     /* 1..XS_TREE_MAX */
   int64_t q_heads, kv_heads, head_dim, capacity;  /* the largest of each */
 } xs_cache_dims;
+/* (A call one of whose launches would pass 2^32 work-items is XS_ERR_CAPACITY:
+ * from 2^22 (sequence, kv head) pairs to evict, some 2^24 to attend to or to
+ * commit.) */
 int xs_cache_create(int device, const xs_cache_dims* dims, xs_cache_context** out);
 int xs_cache_destroy(xs_cache_context* ctx);
 int xs_cache_set_stream(xs_cache_context* ctx, void* hip_stream);

@@ -169,7 +169,7 @@ int xs_host_check_dims(const xs_cache_dims* d) {
   if (!d || d->max_seqs < 1 || d->max_nodes < 1 || d->max_nodes > XS_TREE_MAX || d->q_heads < 1 || d->kv_heads < 1 ||
       d->head_dim < 8 || d->head_dim > 256 || d->capacity < 1)
     return XS_ERR_ARG;
-  // slots and rows are counted in 32 bits, and so are the workgroups of a launch
+  // slots and rows are counted in 32 bits
   if (d->max_seqs > 65536 || d->q_heads > 4096 || d->kv_heads > d->q_heads || d->capacity > (1 << 28)) return XS_ERR_CAPACITY;
   return XS_OK;
 }
@@ -222,6 +222,10 @@ int xs_host_check_evict(const xs_cache_dims* dims, const xs_cache_evict_args* in
     return XS_ERR_ARG;
   if (in->slot_ld < in->capacity || !slots_fit(in->seqs, in->kv_heads, in->slot_ld)) return XS_ERR_ARG;
   return kv_ok(in->cache, in->seqs, in->capacity, in->kv_heads, in->head_dim, true) ? XS_OK : XS_ERR_ARG;
+}
+
+bool xs_host_launch_fits(int64_t workgroups, int64_t threads) {
+  return workgroups <= INT32_MAX && workgroups * threads <= (int64_t)UINT32_MAX;
 }
 
 int xs_host_check_argmax(const xs_host_limits* lim, const xs_argmax_args* in) {

@@ -32,6 +32,9 @@ int xs_host_check_dims(const xs_cache_dims* dims);
 int xs_host_check_attend(const xs_cache_dims* dims, const xs_tree_attend_args* in);
 int xs_host_check_commit(const xs_cache_dims* dims, const xs_cache_commit_args* in);
 int xs_host_check_evict(const xs_cache_dims* dims, const xs_cache_evict_args* in);
+// Whether one launch takes so many workgroups: their number and that of their
+// work-items are 32 bits wide.
+bool xs_host_launch_fits(int64_t workgroups, int64_t threads);
 // Whether a sample call needs the rows' held_row lse (any held_row or scoring
 // output), and whether it asks for the scoring reads that score_kernel writes.
 bool xs_host_wants_lse(const xs_sample_args* in);

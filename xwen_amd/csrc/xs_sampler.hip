@@ -6315,6 +6315,7 @@ int xs_verify_tree(xs_context* ctx, const xs_verify_tree_args* in) {
   const int rc = xs_host_check_verify_tree(&lim, in);
   if (rc) return rc;
   if (in->seqs == 0) return XS_OK;
+  if (!xs_host_launch_fits(in->seqs, 64)) return XS_ERR_CAPACITY;  // (the walk)
   if (hipSetDevice(ctx->device) != hipSuccess) return XS_ERR_HIP;
   int32_t data_err = XS_ROW_OK;
   if (in->width < in->enc) data_err = XS_ROW_NARROW;

@@ -1632,7 +1632,8 @@ int attend_run(xs_cache_context* c, const xs_tree_attend_args& a) {
   cut.nsplit = (int32_t)((blocks + cut.chunk - 1) / cut.chunk);
   const int64_t groups = a.seqs * a.kv_heads * cut.nsplit;
   const int64_t grid = (groups + 7) / 8 * 8 * wgs, join = a.seqs * a.kv_heads * cut.tiles * RT * xst::Shape<DP, RT>::VH;
-  if (grid > 0x7FFFFFFF || join > 0x7FFFFFFF) return XS_ERR_CAPACITY;
+  const int64_t joiners = xst::join_threads<DP>(cut.nsplit <= xst::FEW);
+  if (!xs_host_launch_fits(grid, 64 * xst::NW) || (cut.nsplit > 1 && !xs_host_launch_fits(join, joiners))) return XS_ERR_CAPACITY;
   if (cut.nsplit > 1 && groups * cut.tiles * xst::Shape<DP, RT>::PART > c->part_floats) return XS_ERR_CAPACITY;  // (never: groups * tiles <= most)
   cut.groups = (int32_t)groups;
   if constexpr (WIDE)
@@ -1710,7 +1711,7 @@ int commit_run(xs_cache_context* c, const xs_cache_commit_args& a) {
   const int64_t waves = xst::NW * c->n_cu * commit_per_cu(DP, RT) * (a.seqs > 1 ? 5 : 1);
   const int64_t share = std::max<int64_t>(RT, (blocks * heads + waves - 1) / waves);
   const int64_t shares = (a.q ? (blocks + xst::NW * share - 1) / (xst::NW * share) : 0) + 1;
-  if (heads * shares > 0x7FFFFFFF) return XS_ERR_CAPACITY;
+  if (!xs_host_launch_fits(heads * shares, 64 * xst::NW)) return XS_ERR_CAPACITY;
   const dim3 grid((unsigned)(heads * shares)), block(64 * xst::NW);
   if (a.head_dim == DP)
     hipLaunchKernelGGL((xst::commit_kernel<T, DP, RT, true>), grid, block, 0, c->stream, a, (int)shares, (int)share);
@@ -1840,7 +1841,7 @@ int xs_cache_evict(xs_cache_context* c, const xs_cache_evict_args* in) {
                     aligned16(in->new_pos) && in->slot_ld % 4 == 0;
   const bool apart = most > xst::NEAR || (!fits && most > 0);
   const int64_t blocks = (most + xst::ROWS - 1) / xst::ROWS;
-  if (heads > 0x7FFFFFFF || (apart && heads * blocks > 0x7FFFFFFF)) return XS_ERR_CAPACITY;
+  if (!xs_host_launch_fits(heads, xst::EB) || (apart && !xs_host_launch_fits(heads * blocks, 256))) return XS_ERR_CAPACITY;
   if (!fits) hipLaunchKernelGGL(xst::evict_long_kernel, dim3((unsigned)heads), dim3(xst::EB), 0, c->stream, *in, c->evict);
   else if (limit <= 4 * xst::EB) evict_run<1>(c, *in, apart);
   else if (limit <= 8 * xst::EB) evict_run<2>(c, *in, apart);
