@@ -1,0 +1,83 @@
+"""The host side of the tree and cache calls against a stand-in HIP runtime (tests/fakehip.c):
+what they leave behind of the thread's current device.  Each test runs in a child process that
+preloads it; nothing is computed."""
+import os
+import shutil
+import subprocess
+import sys
+
+import pytest
+
+from xwen_amd import _lib
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+COMMON = """
+import ctypes as C
+from xwen_amd import _lib
+lib, rt = _lib.load(), C.CDLL(None)
+for f in ("fake_used", "fake_launches", "fake_work_items"):
+    getattr(rt, f).restype = C.c_int64
+rt.fake_room.argtypes = [C.c_int64]
+P = 0x7f0000001000
+
+def device():
+    d = C.c_int(-1)
+    rt.hipGetDevice(C.byref(d))
+    return d.value
+
+def kv():
+    return _lib.Kv(P, P, 64 * 512, 512, 64)
+
+def cache(dims=(4, 16, 16, 8, 64, 64), on=0):
+    h = C.c_void_p()
+    return lib.xs_cache_create(on, C.byref(_lib.CacheDims(*dims)), C.byref(h)), h
+
+def calls(cache_ctx, ctx):
+    a = _lib.TreeAttendArgs(dtype=_lib.BF16, head_dim=64, seqs=4, nodes=16, q_heads=16, kv_heads=8, q=P, q_seq_stride=16 * 1024,
+                            q_node_stride=1024, q_head_stride=64, cache=kv(), capacity=64, len=P, fresh=kv(), parent=P, scale=0.1,
+                            out=P + 4096, out_seq_stride=16 * 1024, out_node_stride=1024, out_head_stride=64, seq_status=P)
+    c = _lib.CacheCommitArgs(dtype=_lib.BF16, head_dim=64, seqs=4, nodes=16, q_heads=8, kv_heads=8, cache=kv(), capacity=64, len=P,
+                             fresh=kv(), path=P, path_ld=16, n_path=P, new_len=P + 64, slot_ld=64, seq_status=P)
+    e = _lib.CacheEvictArgs(dtype=_lib.BF16, head_dim=64, seqs=4, kv_heads=8, cache=kv(), capacity=64, len=P, mass=P, new_mass=P, pos=P,
+                            new_pos=P, slot_ld=64, next_pos=P, keep=40, sinks=4, recent=8, new_len=P + 64, seq_status=P)
+    v = _lib.VerifyTreeArgs(logits=P, seqs=4, nodes=16, ld=1000, width=1000, enc=1000, params=P, uniforms=P, tokens=P, parent=P,
+                            row_token=P, row_status=P, accepted=P, path=P, committed=P, n_committed=P, seq_status=P)
+    return [(lib.xs_tree_attend, cache_ctx, a), (lib.xs_cache_commit, cache_ctx, c), (lib.xs_cache_evict, cache_ctx, e),
+            (lib.xs_verify_tree, ctx, v)]
+"""
+
+
+@pytest.fixture(scope="module")
+def runtime(tmp_path_factory):
+    if not shutil.which("gcc"):
+        pytest.skip("gcc is not installed")
+    so = str(tmp_path_factory.mktemp("fakehip") / "libfakehip.so")
+    subprocess.run(["gcc", "-O1", "-Wall", "-Wextra", "-shared", "-fPIC", os.path.join(HERE, "fakehip.c"), "-o", so], check=True)
+    return so
+
+
+def child(runtime, body):
+    env = dict(os.environ, LD_PRELOAD=runtime, PYTHONPATH=_lib.ROOT)
+    r = subprocess.run([sys.executable, "-c", COMMON + body], cwd=_lib.ROOT, env=env, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout.strip().endswith("done"), r.stdout + r.stderr
+    return r.stdout
+
+
+def test_calls_leave_the_current_device(runtime):
+    child(runtime, """
+rc, h = cache()
+ctx = C.c_void_p()
+assert rc == 0 and lib.xs_create(0, 64, 1000, 0, C.byref(ctx)) == 0
+for now in (0, 1):
+    rt.hipSetDevice(now)
+    for call, c, args in calls(h, ctx):
+        before = rt.fake_launches()
+        assert call(c, C.byref(args)) == 0 and rt.fake_launches() > before, call
+        assert device() == now, (call.__name__, now, device())
+rt.hipSetDevice(1)
+rc, other = cache()
+assert rc == 0 and device() == 1
+assert lib.xs_cache_destroy(other) == 0 and lib.xs_cache_destroy(h) == 0 and device() == 1
+print("done")
+""")

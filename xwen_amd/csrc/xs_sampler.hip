@@ -61,6 +61,7 @@
 
 #include "../../include/xsamp.h"
 #include "xs_exp_table.h"
+#include "xs_device.h"
 #include "xs_host.h"
 
 #define XS_DEV __device__ __forceinline__
@@ -6316,7 +6317,8 @@ int xs_verify_tree(xs_context* ctx, const xs_verify_tree_args* in) {
   if (rc) return rc;
   if (in->seqs == 0) return XS_OK;
   if (!xs_host_launch_fits(in->seqs, 64)) return XS_ERR_CAPACITY;  // (the walk)
-  if (hipSetDevice(ctx->device) != hipSuccess) return XS_ERR_HIP;
+  const xs_host::OnDevice on(ctx->device);
+  if (!on.ok) return XS_ERR_HIP;
   int32_t data_err = XS_ROW_OK;
   if (in->width < in->enc) data_err = XS_ROW_NARROW;
   else if (in->allowed && in->allowed_words * 32 < in->enc) data_err = XS_ROW_MASK_SHORT;

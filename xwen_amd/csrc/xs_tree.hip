@@ -13,6 +13,7 @@
 #include <stdlib.h>
 
 #include "../../include/xsamp.h"
+#include "xs_device.h"
 #include "xs_host.h"
 
 #define XS_DEV __device__ __forceinline__
@@ -1741,20 +1742,8 @@ void evict_run(xs_cache_context* c, const xs_cache_evict_args& a, bool apart) {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
-}  // namespace
+using xs_host::OnDevice;
 
-namespace {
-// The calls run on the context's device and leave the thread's current one as
-// it was.
-struct OnDevice {
-  int before = -1;
-  bool ok;
-  explicit OnDevice(int device) { ok = hipGetDevice(&before) == hipSuccess && (before == device || hipSetDevice(device) == hipSuccess); }
-  ~OnDevice() {
-    int now = -1;
-    if (before >= 0 && hipGetDevice(&now) == hipSuccess && now != before) (void)hipSetDevice(before);
-  }
-};
 }  // namespace
 
 extern "C" {
