@@ -52,3 +52,19 @@ def test_evict_up_to_the_largest_launch():
     assert torch.equal(k[:-1, :4], start[:-1, source]) and torch.equal(k[-1], start[-1])
     assert bool((pos[:-1, :, :4] == torch.tensor(source, dtype=torch.int32, device="cuda")).all())
     ctx.close()
+
+
+def test_a_context_that_cannot_be_made_leaves_no_error():
+    """Sizes that no memory holds and a device that is not there: refused, and what follows runs."""
+    from xwen_amd import tree
+    for bad in (dict(max_seqs=65_536, q_heads=4096, kv_heads=4096, capacity=1 << 28), dict(device=torch.cuda.device_count())):
+        with pytest.raises(_lib.XsError, match="XS_ERR_HIP"):
+            tree.CacheContext(**{**dict(max_seqs=1, max_nodes=1, q_heads=1, kv_heads=1, head_dim=64, capacity=64), **bad})
+        assert float(torch.ones(5, device="cuda").sum()) == 5.0
+        ctx = tree.CacheContext(max_seqs=1, max_nodes=1, q_heads=1, kv_heads=1, head_dim=64, capacity=64)
+        t = torch.ones((1, 64, 1, 64), device="cuda", dtype=BF)
+        n = torch.ones(1, dtype=torch.int32, device="cuda")
+        got = tree.tree_attend(ctx, t[:, :1], t, t, n, t[:, :1], t[:, :1], -n.view(1, 1))
+        tree.check(got.seq_status)
+        assert bool((got.out == 1.0).all())
+        ctx.close()

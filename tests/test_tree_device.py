@@ -81,3 +81,27 @@ assert rc == 0 and device() == 1
 assert lib.xs_cache_destroy(other) == 0 and lib.xs_cache_destroy(h) == 0 and device() == 1
 print("done")
 """)
+
+
+def test_a_context_that_cannot_be_made_leaves_nothing_behind(runtime):
+    """Too little memory at every allocation in turn, sizes that no memory holds, a device that is
+    not there: XS_ERR_HIP, no memory kept, the current device as it was, and no error that the
+    thread's next HIP call would report."""
+    child(runtime, """
+rc, h = cache()
+assert rc == 0
+whole = rt.fake_used()
+assert lib.xs_cache_destroy(h) == 0 and rt.fake_used() == 0
+rt.hipSetDevice(1)
+for room in sorted({0, 1, whole // 2, whole - 1, *range(0, whole, max(1, whole // 64))}):
+    rt.fake_room(room)
+    rc, h = cache()
+    assert rc == _lib.XS_ERR_HIP and not h.value and rt.fake_used() == 0 and device() == 1, room
+    assert rt.fake_last_error() == 0, (room, rt.fake_last_error())
+rt.fake_room(1 << 40)
+rc, h = cache((65536, 64, 4096, 4096, 256, 1 << 28))
+assert rc == _lib.XS_ERR_HIP and not h.value and rt.fake_used() == 0 and rt.fake_last_error() == 0
+rc, h = cache(on=7)
+assert rc == _lib.XS_ERR_HIP and not h.value and device() == 1 and rt.fake_last_error() == 0
+print("done")
+""")

@@ -1744,6 +1744,13 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 
 using xs_host::OnDevice;
 
+// The failure is the call's to report: left in the thread, it would fail the
+// next launch that asks for the last error.
+int create_failed() {
+  (void)hipGetLastError();
+  return XS_ERR_HIP;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1754,7 +1761,7 @@ int xs_cache_create(int device, const xs_cache_dims* dims, xs_cache_context** ou
   const int rc = xs_host_check_dims(dims);
   if (rc) return rc;
   const OnDevice on(device);
-  if (!on.ok) return XS_ERR_HIP;
+  if (!on.ok) return create_failed();
   xs_cache_context* c = (xs_cache_context*)calloc(1, sizeof(xs_cache_context));
   if (!c) return XS_ERR_HIP;
   c->device = device;
@@ -1771,7 +1778,7 @@ int xs_cache_create(int device, const xs_cache_dims* dims, xs_cache_context** ou
       hipMalloc((void**)&c->evict.filler, heads * c->evict.pairs * sizeof(int32_t)) != hipSuccess ||
       hipMalloc((void**)&c->evict.moves, heads * sizeof(int32_t)) != hipSuccess) {
     xs_cache_destroy(c);
-    return XS_ERR_HIP;
+    return create_failed();
   }
   *out = c;
   return XS_OK;
