@@ -105,3 +105,53 @@ rc, h = cache(on=7)
 assert rc == _lib.XS_ERR_HIP and not h.value and device() == 1 and rt.fake_last_error() == 0
 print("done")
 """)
+
+
+def test_a_context_holds_what_its_calls_can_use(runtime):
+    """The partial results of split attention: for single tokens no tree's, none where no call is
+    split; and every call within a context's sizes has room for its own."""
+    out = child(runtime, """
+import random
+def size(*dims):
+    rc, h = cache(dims)
+    assert rc == 0
+    n = rt.fake_used()
+    lib.xs_cache_destroy(h)
+    return n
+def evict(seqs, kv, cap):  # the lists of moves and the bitmap
+    return seqs * kv * ((cap + 63) // 64 * 8 + (cap // 2 + 1) * 8 + 4)
+cases = {"decode": (16, 1, 32, 8, 128, 8192), "tree": (16, 64, 32, 8, 128, 8192), "one": (1, 64, 32, 8, 128, 131072),
+         "short": (16, 64, 32, 8, 128, 448)}
+for name, d in cases.items():
+    print(name, size(*d) - evict(d[0], d[3], d[5]))
+rng = random.Random(1)
+for _ in range(1500):
+    kv = rng.choice([1, 2, 3, 8, 16])
+    dims = dict(seqs=rng.choice([1, 2, 7, 64, 900]), nodes=rng.choice([1, 2, 5, 16, 33, 64]), g=rng.choice([1, 2, 4, 7, 16]),
+                dim=rng.choice([8, 64, 72, 128, 136, 256]), cap=rng.choice([1, 64, 300, 480, 512, 700, 2000, 9000, 70000, 1 << 20]))
+    rc, h = cache((dims["seqs"], dims["nodes"], kv * dims["g"], kv, dims["dim"], dims["cap"]))
+    assert rc == 0
+    for _ in range(12):
+        k = rng.randint(1, kv)
+        q = k * rng.randint(1, kv * dims["g"] // k)
+        seqs, nodes, cap = rng.randint(1, dims["seqs"]), rng.randint(1, dims["nodes"]), rng.randint(1, dims["cap"])
+        dim = 8 * rng.randint(1, dims["dim"] // 8)
+        if rng.random() < 0.5:
+            k, q, seqs, nodes, cap, dim = kv, kv * dims["g"], dims["seqs"], dims["nodes"], dims["cap"], dims["dim"]
+        stride = _lib.Kv(P, P, cap * k * 256, k * 256, 256)
+        a = _lib.TreeAttendArgs(dtype=rng.randint(0, 1), head_dim=dim, seqs=seqs, nodes=nodes, q_heads=q, kv_heads=k, q=P,
+                                q_seq_stride=nodes * q * 256, q_node_stride=q * 256, q_head_stride=256, cache=stride, capacity=cap, len=P,
+                                fresh=stride, parent=P, scale=0.1, out=P + 4096, out_seq_stride=nodes * q * 256, out_node_stride=q * 256,
+                                out_head_stride=256, seq_status=P)
+        assert lib.xs_tree_attend(h, C.byref(a)) == 0, (dims, kv, seqs, nodes, q, k, dim, cap)
+    lib.xs_cache_destroy(h)
+print("done")
+""")
+    got = {k: int(v) for k, v in (line.split() for line in out.splitlines()[:-1])}
+    assert got["short"] == 0
+    # 256 CUs of 2 workgroups (32 rows in two tiles; 3 of one tile are less), four times over
+    assert got["decode"] == 256 * 2 * 4 * 4 * (2 * 8 * 256 + 2 * 32 + 4)
+    # one user's many rows: one workgroup of four waves with 64 rows of 128 each; several users': that
+    # is 4 x 8,324 floats a CU, and 64 rows of 64 two a CU, four times over, 8 x 4,228
+    assert got["one"] == 256 * 4 * 4 * (4 * 8 * 256 + 4 * 32 + 4)
+    assert got["tree"] == 256 * 2 * 4 * 4 * (4 * 4 * 256 + 4 * 32 + 4)

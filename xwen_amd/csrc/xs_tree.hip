@@ -1648,24 +1648,30 @@ int attend_run(xs_cache_context* c, const xs_tree_attend_args& a) {
   return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
 }
 
-// The partial results of the largest split call within `dims`.
+// The partial results of the largest split call within `dims`: those that fill
+// the device, by the shapes that attend_rows takes for so many rows a head.
 int64_t attend_floats(const xs_cache_dims& dims, int n_cu) {
+  const int64_t rows = dims.max_nodes * dims.q_heads;  // (of one kv head)
+  if ((dims.capacity + xst::KB - 1) / xst::KB + (dims.max_nodes + xst::KB - 1) / xst::KB <= 4 * xst::NW) return 0;  // (none is split)
   int64_t most = 0;
-  auto add = [&](int64_t wgs, int64_t part) { most = std::max(most, n_cu * wgs * rounds(dims.max_seqs) * part); };
-  add(per_cu(64, 1), xst::Shape<64, 1>::PART);
-  add(per_cu(64, 2), xst::Shape<64, 2>::PART);
-  add(per_cu(64, 4), xst::Shape<64, 4>::PART);
-  add(1, xst::NW * xst::Shape<64, 4>::PART);
+  auto narrow = [&](int64_t per_cu, int64_t part) { most = std::max(most, n_cu * per_cu * rounds(dims.max_seqs) * part); };
+  auto wide = [&](int64_t part) { most = std::max(most, n_cu * xst::NW * part); };
+  narrow(per_cu(64, 1), xst::Shape<64, 1>::PART);
+  if (rows > 16) narrow(per_cu(64, 2), xst::Shape<64, 2>::PART);
+  if (rows > 32) narrow(per_cu(64, 4), xst::Shape<64, 4>::PART);
+  if (rows > 64) wide(xst::Shape<64, 2>::PART);
+  if (rows > 128) wide(xst::Shape<64, 4>::PART);
   if (dims.head_dim > 64) {
-    add(per_cu(128, 1), xst::Shape<128, 1>::PART);
-    add(per_cu(128, 2), xst::Shape<128, 2>::PART);
-    add(per_cu(128, 4), xst::Shape<128, 4>::PART);
-    add(1, xst::NW * xst::Shape<128, 4>::PART);
+    narrow(per_cu(128, 1), xst::Shape<128, 1>::PART);
+    if (rows > 16) narrow(per_cu(128, 2), xst::Shape<128, 2>::PART);
+    if (rows > 32) narrow(per_cu(128, 4), xst::Shape<128, 4>::PART);
+    if (rows > 64) wide(xst::Shape<128, 2>::PART);
+    if (rows > 128) wide(xst::Shape<128, 4>::PART);
   }
   if (dims.head_dim > 128) {
-    add(per_cu(256, 1), xst::Shape<256, 1>::PART);
-    add(per_cu(256, 2), xst::Shape<256, 2>::PART);
-    add(1, xst::NW * xst::Shape<256, 2>::PART);
+    narrow(per_cu(256, 1), xst::Shape<256, 1>::PART);
+    if (rows > 16) narrow(per_cu(256, 2), xst::Shape<256, 2>::PART);
+    if (rows > 32) wide(xst::Shape<256, 2>::PART);
   }
   return most;
 }
