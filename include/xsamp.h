@@ -442,7 +442,8 @@ typedef struct {
  *   out = sum_j softmax_j(scale q.k_j) v_j,  lse = ln sum_j exp(scale q.k_j)
  * with q head h reading kv head h / (q_heads / kv_heads).  Sums and softmax
  * statistics are f32; the weights are rounded to the inputs' type before they
- * multiply the values, and out once at the end.  nodes = 1 is plain decoding.
+ * multiply the values, and out once at the end.  The sums are of weights up to
+ * 2^8 (f16: 2^14) times values, so that values from about 2^100 on may overflow.  nodes = 1 is plain decoding.
  * parent[i] is -1 (node i follows the cache) or a node below i; any other
  * value makes i and what follows it see nothing: out 0, lse -inf, as for a
  * row whose every score is -inf, whatever the values.  A score of NaN or +inf

@@ -174,3 +174,22 @@ def test_empty_rows_that_see_odd_values(ctx, nodes, lens):
     c["v"][:, 7, :, 5] = math.nan
     got = run(ctx, c, out=blank(c))
     assert bool((got.out == 0.0).all()) and bool((got.lse == -math.inf).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("nodes,lens", [(5, [70, 300, 1000]), (40, [70, 300, 1000]), (9, [7000])])
+def test_values_at_the_end_of_the_type(ctx, nodes, lens, dtype):
+    """A mean of finite values is finite: rounded weights over their exact sum may pass the largest
+    value by half a step of the type, which must not become an infinity.  (bf16's largest over 2^20:
+    sums of weights times values are f32, of weights up to 2^8.)"""
+    rng = np.random.default_rng(27)
+    c = case(rng, lens, nodes, 8, 2, 64, dtype, spread=2.0)
+    top = torch.finfo(dtype).max * (1.0 if dtype == HF else 2.0**-20)
+    for t in ("v", "fv"):
+        c[t][..., ::2], c[t][..., 1::2] = top, -top
+    got = run(ctx, c, out=blank(c)).out.double().cpu()
+    want = torch.tensor([top, -top], dtype=torch.float64).repeat(32)
+    for b, n in enumerate(c["lens"]):
+        for i, chain in enumerate(treeref.sees(c["parent"][b].tolist(), c["used"][b])):
+            # a rounded weight and the rounded output, and the sums
+            assert bool(((got[b, i] - want).abs() <= top * (2.02 * half_step(dtype) + (n + 64) * F32)).all())

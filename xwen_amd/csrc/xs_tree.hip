@@ -386,6 +386,12 @@ XS_DEV void block(Wave<T, DP, RT>& w, const uint16_t* kp, const uint16_t* vp, in
   accumulate(w, v, pf);
 }
 
+// A mean is no larger than the largest value, but rounded weights over the sum
+// of exact ones may pass it by half a step, which at f16's end would round to an
+// infinity (bf16's end is f32's, where the sums overflow first).
+XS_DEV float within(Bf16, float x) { return x; }
+XS_DEV float within(F16, float x) { return fabsf(x) < -NEG_INF ? fminf(fmaxf(x, -65504.0f), 65504.0f) : x; }
+
 // ln of a row's sum of weights, from its reference and l.
 template <typename T>
 XS_DEV float lse_of(const xs_tree_attend_args& a, float ref, float l) {
@@ -421,7 +427,7 @@ XS_DEV void store_pair(const xs_tree_attend_args& a, int G, int b, int kh, int r
 #pragma unroll
   for (int r = 0; r < 4; r++) {
     const int d = 128 * h + VE * (4 * g + r) + 2 * pair;
-    if (d < a.head_dim) *(uint32_t*)(out + d) = pack2(T{}, o0[r] * inv, o1[r] * inv);
+    if (d < a.head_dim) *(uint32_t*)(out + d) = pack2(T{}, within(T{}, o0[r] * inv), within(T{}, o1[r] * inv));
   }
   if (a.lse && h == 0 && pair == 0 && g == 0)
     a.lse[(b * a.nodes + node) * a.q_heads + head] = lse_of<T>(a, ref, l);
@@ -443,7 +449,7 @@ XS_DEV void store_half(const xs_tree_attend_args& a, int G, int b, int kh, int r
     const int d = 128 * h + VE * (4 * g + r);
     uint32_t y[VE / 2];
 #pragma unroll
-    for (int i = 0; i < VE / 2; i++) y[i] = pack2(T{}, o[h * VE + 2 * i][r] * inv, o[h * VE + 2 * i + 1][r] * inv);
+    for (int i = 0; i < VE / 2; i++) y[i] = pack2(T{}, within(T{}, o[h * VE + 2 * i][r] * inv), within(T{}, o[h * VE + 2 * i + 1][r] * inv));
     if (d < a.head_dim) {
       if constexpr (VE == 8) *(u32x4*)(out + d) = (u32x4){y[0], y[1], y[2], y[3]};
       else *(u32x2*)(out + d) = (u32x2){y[0], y[1]};
