@@ -178,16 +178,33 @@ struct Wave {
   using S = Shape<DP, RT>;
   u32x4 q[RT][S::KC];
   f32x4 o[RT][S::NF];
-  f32x4 c[RT];     // minus the row's reference (of q.k), four times: what the scores' products start from
+  // Minus the row's reference (of q.k), which the scores' products start from:
+  // four times, as they take it, or once where registers are short (four times,
+  // the wide kernel's loop reads one from scratch memory, behind the loads of the
+  // next stage: 283 us for 225 where 8 sequences of 64 nodes see 8,192 slots of
+  // head size 136).
+  static constexpr bool ONCE = DP > 128;
+  std::conditional_t<ONCE, float, f32x4> c[RT];
   float most[RT];  // the x above which the reference moves: NaN until the row's first score
   float l[RT];
   int odd;         // a node's values held a NaN or an infinity
+
+  XS_DEV float minus(float v) const { return v; }
+  XS_DEV float minus(const f32x4& v) const { return v[0]; }
+  XS_DEV f32x4 start(int t) const {
+    const float v = minus(c[t]);
+    return (f32x4){v, v, v, v};
+  }
+  XS_DEV void refer(int t, float ref) {
+    if constexpr (ONCE) c[t] = -ref;
+    else c[t] = (f32x4){-ref, -ref, -ref, -ref};
+  }
 
   XS_DEV void init() {
     odd = 0;
 #pragma unroll
     for (int t = 0; t < RT; t++) {
-      c[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+      refer(t, -0.0f);
       most[t] = __builtin_nanf("");
       l[t] = 0.0f;
 #pragma unroll
@@ -217,7 +234,8 @@ struct Wave {
   XS_DEV void rebase(int t, const f32x4 (&s)[2], bool all, float scale, uint32_t on, float (&x)[8]) {
     constexpr float OFF = offset_of(T{});
     const int g = (threadIdx.x & 63) >> 4;
-    const float sign = scale < 0.0f ? -1.0f : 1.0f, old = -c[t][0];
+    asm volatile("" : "+s"(scale));  // (nothing of it is kept from block to block)
+    const float sign = scale < 0.0f ? -1.0f : 1.0f, old = -minus(c[t]);
     const bool unset = most[t] != most[t];
     // never below the old one (a product that starts elsewhere rounds elsewhere)
     float best = unset ? NEG_INF : old * sign;
@@ -230,7 +248,7 @@ struct Wave {
     if ((all || old == 0.0f) && best > NEG_INF) {
       const float ref = scale == 0.0f ? 0.0f : best * sign;
       const float keep = unset ? 0.0f : __builtin_amdgcn_exp2f((old - ref) * scale);
-      c[t] = (f32x4){-ref, -ref, -ref, -ref};
+      refer(t, ref);
       most[t] = LAZY + OFF;
       l[t] *= keep;
 #pragma unroll
@@ -255,7 +273,7 @@ struct Wave {
   }
   // The reference, so that the larger one is the better: l and o carry 2 to the
   // minus reference |scale|, and offset_of more.
-  XS_DEV float reference(int t, float scale) const { return scale < 0.0f ? c[t][0] : -c[t][0]; }
+  XS_DEV float reference(int t, float scale) const { return scale < 0.0f ? minus(c[t]) : -minus(c[t]); }
 };
 
 // O^T += V^T P^T over a block: v holds 16 bytes of each of the lane's eight
@@ -324,7 +342,7 @@ XS_DEV void block(Wave<T, DP, RT>& w, const uint16_t* kp, const uint16_t* vp, in
   u32x4 pf[RT];
 #pragma unroll
   for (int t = 0; t < RT; t++) {
-    f32x4 s[2] = {w.c[t], w.c[t]};
+    f32x4 s[2] = {w.start(t), w.start(t)};
 #pragma unroll
     for (int c = 0; c < S::KC; c++) {
       s[0] = mfma(T{}, k[0][c], w.q[t][c], s[0]);
@@ -332,20 +350,20 @@ XS_DEV void block(Wave<T, DP, RT>& w, const uint16_t* kp, const uint16_t* vp, in
     }
     float xs[8];
     const float top = w.template scaled<MASKED>(s, scale, MASKED ? on[t] : 0u, xs);
-    if (__any(w.passes(t, top))) {
-      const bool far = __any(w.passes(t, top) && w.c[t][0] != 0.0f);
-      if (far) {
+    if (__any(w.passes(t, top))) [[unlikely]] {  // (its registers spill before those of the loop)
+      const bool far = __any(w.passes(t, top) && w.minus(w.c[t]) != 0.0f);
+      if (far) [[unlikely]] {
         s[0] = s[1] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-          int key = key0 + 16 * u + x;
+          int at = lane;
+          asm volatile("" : "+v"(at));  // (addressed and read again: kept instead, both would spill)
+          int key = key0 + 16 * u + (at & 15);
           if (MASKED) key = min(key, limit - 1);
-          const uint16_t* p = kp + key * stride;
-          asm("" : "+v"(p));  // (read again: kept instead, the keys' registers would spill)
+          const uint16_t* p = kp + key * stride + 8 * (at >> 4);
 #pragma unroll
           for (int c = 0; c < S::KC; c++) {
-            const int d = 32 * c + 8 * g;
-            s[u] = mfma(T{}, EXACT || d < D ? *(const u32x4*)(p + d) : zero4, w.q[t][c], s[u]);
+            s[u] = mfma(T{}, EXACT || 32 * c + 8 * (at >> 4) < D ? *(const u32x4*)(p + 32 * c) : zero4, w.q[t][c], s[u]);
             __builtin_amdgcn_sched_barrier(0);  // (one chunk in registers at a time)
           }
         }
@@ -597,7 +615,7 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
 // block's maxima.  Reading the keys from L2 in every wave instead, 64 bytes a
 // cycle and CU, takes as long as the matrix instructions, and not beside them:
 // 8 sequences of 64 nodes over 32,768 slots (256 rows of 8 kv heads) 520 us,
-// so 362 (759 TFLOP/s, of the 1,291 of a large library product).
+// so 358 (769 TFLOP/s, of the 1,291 of a large library product).
 template <int DP>
 struct Stage {
   static constexpr int SK = DP > 128 ? 32 : 64;
@@ -675,7 +693,7 @@ __global__ __launch_bounds__(64 * NW, 1) void attend_wide_kernel(const xs_tree_a
   // the scores of block j
   auto scores = [&](int j, f32x4 (&s)[RT][2]) {
 #pragma unroll
-    for (int t = 0; t < RT; t++) s[t][0] = s[t][1] = w.c[t];
+    for (int t = 0; t < RT; t++) s[t][0] = s[t][1] = w.start(t);
 #pragma unroll
     for (int c = 0; c < S::KC; c++) {
       const u32x4 f[2] = {key(j, 0, c), key(j, 1, c)};
@@ -751,7 +769,7 @@ __global__ __launch_bounds__(64 * NW, 1) void attend_wide_kernel(const xs_tree_a
         }
         accumulate(w, v, pf);
         const bool move = prepare(s);
-        if (more && __any(move)) settle(j + 1);
+        if (more && __any(move)) [[unlikely]] settle(j + 1);
       }
     }
   }
