@@ -80,8 +80,10 @@ def agree_with_the_mean(c, got, value, scale=None):
                 assert bool(((lse[b, i] - full).abs() <= 4 * F32 * (1 + abs(full))).all())
 
 
-# rows of a wave (three nodes) and of several waves that share the keys
-SHAPES = [(3, 8, 2, 128, BF), (3, 4, 2, 72, BF), (40, 8, 2, 128, BF), (40, 8, 2, 72, BF), (20, 4, 1, 256, BF)]
+# one, two and four row tiles of a wave, and several waves that share the keys (float16 holds the
+# masks as -inf)
+SHAPES = [(3, 8, 2, 128, BF), (3, 4, 2, 72, BF), (8, 4, 1, 128, BF), (8, 4, 1, 200, BF), (6, 4, 1, 256, BF), (12, 4, 1, 64, BF),
+          (12, 4, 1, 128, HF), (24, 4, 1, 128, BF), (40, 8, 2, 128, BF), (40, 8, 2, 72, BF), (20, 4, 1, 256, BF), (20, 4, 1, 136, HF)]
 
 
 @pytest.mark.parametrize("mask", [-1e6, -1e7, -1e8, -1e9, LOWEST])
