@@ -443,16 +443,16 @@ typedef struct {
  * with q head h reading kv head h / (q_heads / kv_heads).  Sums and softmax
  * statistics are f32; the weights are rounded to the inputs' type before they
  * multiply the values, and out once at the end.  The sums are of weights up to
- * 2^8 (f16: 2^14) times values, so that values from about 2^100 on may overflow.  nodes = 1 is plain decoding.
- * parent[i] is -1 (node i follows the cache) or a node below i; any other
- * value makes i and what follows it see nothing: out 0, lse -inf, as for a
- * row whose every score is -inf, whatever the values.  A score of NaN or +inf
- * makes its row NaN, a value that is not finite the rows that give it weight;
- * what a node does not see never reaches it, whatever it holds.  q.k is an f32
- * sum; as long as that is finite, keys may be masked by a finite value of any
- * size, beside others or all of a row's (where scale q.k itself passes f32,
- * out is right and lse infinite).  Rows past
- * n_nodes are left as they were, and a sequence whose len is outside
+ * 2^8 (f16: 2^14) times values, so that values from about 2^100 on may
+ * overflow.  nodes = 1 is plain decoding.  parent[i] is -1 (node i follows the
+ * cache) or a node below i; any other value makes i and what follows it see
+ * nothing: out 0, lse -inf, as for a row whose every score is -inf, whatever
+ * the values.  A score of NaN or +inf makes its row NaN, a value that is not
+ * finite the rows that give it weight; what a node does not see never reaches
+ * it, whatever it holds.  q.k is an f32 sum; as long as that is finite, keys
+ * may be masked by a finite value of any size, beside others or all of a row's
+ * (where scale q.k itself passes f32, out is right and lse infinite).  Rows
+ * past n_nodes are left as they were, and a sequence whose len is outside
  * [0, max_len] or n_nodes outside [0, nodes] gets XS_ROW_BAD_PARAM and nothing
  * else. */
 typedef struct {
@@ -470,7 +470,7 @@ typedef struct {
   const int32_t* parent; /* [seqs, nodes] */
   const int32_t* n_nodes;  /* [seqs], or NULL for `nodes` */
   float scale;
-  void* out;             /* [seqs, nodes, q_heads, head_dim] by strides like xs_kv's; not q itself */
+  void* out;             /* [seqs, nodes, q_heads, head_dim] by strides like xs_kv's; overlaps no input */
   int64_t out_seq_stride, out_node_stride, out_head_stride;
   float* lse;            /* [seqs, nodes, q_heads] or NULL */
   int32_t* seq_status;   /* [seqs] */
@@ -487,13 +487,13 @@ int xs_tree_attend(xs_cache_context* ctx, const xs_tree_attend_args* args);
  *              the kv head's q heads of exp(scale q.k_s - lse), s < len, and
  *              the same without mass for the appended slots (which a node sees
  *              from its own rank on).  q, lse and scale are xs_tree_attend's.
- * Per-slot arrays are [seqs, kv_heads, slot_ld].  new_mass may be mass.  The
- * sums are f32, in an order fixed by the sizes.  An exponent is off by the
- * rounding of lse, 2^-24 of it; a slot of the cache gains at most 1 a row.  A sequence whose len is
- * outside [0, max_len], whose n_path is outside [0, nodes] or whose path holds
- * a node outside [0, nodes) gets XS_ROW_BAD_PARAM, one without room
- * XS_ROW_CACHE_FULL; its new_len and new_next_pos are len and next_pos, and
- * nothing else of it is written. */
+ * Per-slot arrays are [seqs, kv_heads, slot_ld].  new_mass is mass itself, or
+ * overlaps it nowhere.  The sums are f32, in an order fixed by the sizes.  An
+ * exponent is off by the rounding of lse, 2^-24 of it; a slot of the cache
+ * gains at most 1 a row.  A sequence whose len is outside [0, max_len], whose
+ * n_path is outside [0, nodes] or whose path holds a node outside [0, nodes)
+ * gets XS_ROW_BAD_PARAM, one without room XS_ROW_CACHE_FULL; its new_len and
+ * new_next_pos are len and next_pos, and nothing else of it is written. */
 typedef struct {
   int32_t dtype, head_dim;
   int64_t seqs, nodes, q_heads, kv_heads;
@@ -529,9 +529,10 @@ int xs_cache_commit(xs_cache_context* ctx, const xs_cache_commit_args* args);
  * The kept slots below `keep` stay where they are, and the i-th free one
  * among them takes the keys, values, mass and position of the i-th kept slot
  * at or past `keep` (attention does not depend on the slots' order).  new_len
- * = min(len, keep).  new_mass and new_pos may be mass and pos, both or
- * neither; entries past new_len are left as they were.  A sequence whose len is
- * outside [0, max_len] gets XS_ROW_BAD_PARAM and new_len = len. */
+ * = min(len, keep).  new_mass and new_pos are mass and pos themselves, or
+ * overlap them nowhere; entries past new_len are left as they were.  A
+ * sequence whose len is outside [0, max_len] gets XS_ROW_BAD_PARAM and new_len
+ * = len. */
 typedef struct {
   int32_t dtype, head_dim;
   int64_t seqs, kv_heads;

@@ -615,7 +615,7 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
 // block's maxima.  Reading the keys from L2 in every wave instead, 64 bytes a
 // cycle and CU, takes as long as the matrix instructions, and not beside them:
 // 8 sequences of 64 nodes over 32,768 slots (256 rows of 8 kv heads) 520 us,
-// so 358 (769 TFLOP/s, of the 1,291 of a large library product).
+// so 354 to 366 (751 to 776 TFLOP/s, of the 1,291 of a large library product).
 template <int DP>
 struct Stage {
   static constexpr int SK = DP > 128 ? 32 : 64;
