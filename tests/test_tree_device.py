@@ -58,7 +58,8 @@ def runtime(tmp_path_factory):
 
 
 def child(runtime, body):
-    env = dict(os.environ, LD_PRELOAD=runtime, PYTHONPATH=_lib.ROOT)
+    before = os.environ.get("LD_PRELOAD")
+    env = dict(os.environ, LD_PRELOAD=f"{runtime} {before}" if before else runtime, PYTHONPATH=_lib.ROOT)
     r = subprocess.run([sys.executable, "-c", COMMON + body], cwd=_lib.ROOT, env=env, capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and r.stdout.strip().endswith("done"), r.stdout + r.stderr
     return r.stdout
