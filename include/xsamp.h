@@ -554,6 +554,164 @@ typedef struct {
 int xs_cache_evict(xs_cache_context* ctx, const xs_cache_evict_args* args);
 
 /* ---------------------------------------------------------------------------
+ * From a prompt to a cache held in 8 bits.  One layer's calls are
+ *
+ *   xs_qk_rotate      the projections' queries and keys: normed per head,
+ *                     turned by their positions
+ *   xs_prompt_attend  a prompt's tokens attend to themselves, causally
+ *   xs_cache_append8  the prompt's keys and values, and later those of each
+ *                     step's accepted path, go into the cache
+ *   xs_tree_attend8   a step's tree attends to the cache, as in xs_tree_attend
+ *                     (xs_verify_tree then gives the path to append)
+ *
+ * They run on the stream of an xs_cache_context; only xs_tree_attend8 uses the
+ * context's workspace, and its sizes bound that call and the append. */
+
+/* Norms and positions of queries and keys, each head of each token on its own:
+ *   y = x / sqrt(mean(x^2) + eps) * weight   (weights NULL: y = x)
+ * and of y the first rot_dim elements in pairs (a, b), i < rot_dim / 2:
+ *   (a cos t - b sin t, b cos t + a sin t),  t = pos * inv_freq[i]
+ * with (a, b) elements i and i + rot_dim / 2 (XS_ROT_HALVES) or 2 i and 2 i + 1
+ * (XS_ROT_NEIGHBOURS).  Angles are formed in f64 (any int32 position), the rest
+ * in f32, rounded once.  An output may be its input itself (same strides), and
+ * overlaps no other input or output. */
+#define XS_ROT_HALVES 0
+#define XS_ROT_NEIGHBOURS 1
+typedef struct {
+  int32_t dtype;         /* XS_BF16 or XS_F16: q, k and the outputs */
+  int32_t head_dim;      /* a multiple of 8, 8..256 */
+  int64_t tokens;
+  int64_t q_heads, kv_heads;  /* either may be 0, its pointers then NULL */
+  const void* q;         /* [tokens, q_heads, head_dim]: strides in elements, multiples of 8, pointers 16-byte aligned */
+  int64_t q_token_stride, q_head_stride;
+  const void* k;         /* [tokens, kv_heads, head_dim] */
+  int64_t k_token_stride, k_head_stride;
+  const float* q_weight; /* [head_dim], 16-byte aligned; both weights or none (that of an absent side may be NULL) */
+  const float* k_weight;
+  float eps;
+  int32_t rot_dim;       /* 0..head_dim: a multiple of 16 (halves) or 8 (neighbours) */
+  int32_t pairs;         /* XS_ROT_HALVES or XS_ROT_NEIGHBOURS */
+  const float* inv_freq; /* [rot_dim / 2] */
+  const int32_t* pos;    /* [tokens] (rot_dim 0: not read) */
+  void* q_out;
+  int64_t q_out_token_stride, q_out_head_stride;
+  void* k_out;
+  int64_t k_out_token_stride, k_out_head_stride;
+} xs_qk_rotate_args;
+
+int xs_qk_rotate(xs_cache_context* ctx, const xs_qk_rotate_args* args);
+
+/* Causal attention of whole prompts, packed: sequence b's tokens are rows
+ * [start[b], start[b + 1]) of q, k and v, and token i of it sees its tokens 0..i:
+ *   out = sum_j softmax_j(scale q.k_j) v_j,  lse = ln sum_j exp(scale q.k_j)
+ * with q head h reading kv head h / (q_heads / kv_heads).  What is said of
+ * rounding, masks, infinities and NaN at xs_tree_attend holds here too: a row
+ * whose every score is -inf gets out 0 and lse -inf, a score of NaN or +inf
+ * makes its row NaN, and what a token does not see never reaches it, whatever
+ * it holds.  A sequence may be empty.  One whose start lies below 0 or below an
+ * earlier entry of start, or whose end lies below its start or past `tokens`,
+ * gets XS_ROW_BAD_PARAM and nothing else; rows of no sequence are left as they
+ * were. */
+typedef struct {
+  int32_t dtype;         /* XS_BF16 or XS_F16: q, k, v and out */
+  int32_t head_dim;      /* a multiple of 8, 8..256 */
+  int64_t seqs, tokens;  /* tokens: rows of the tensors */
+  int64_t q_heads, kv_heads;  /* q_heads a multiple of kv_heads */
+  const void* q;         /* [tokens, q_heads, head_dim]: strides in elements, multiples of 8, pointers 16-byte aligned */
+  int64_t q_token_stride, q_head_stride;
+  const void* k;         /* [tokens, kv_heads, head_dim], k and v of the same strides */
+  const void* v;
+  int64_t kv_token_stride, kv_head_stride;
+  const int32_t* start;  /* [seqs + 1] */
+  float scale;
+  void* out;             /* [tokens, q_heads, head_dim]; overlaps no input */
+  int64_t out_token_stride, out_head_stride;
+  float* lse;            /* [tokens, q_heads] or NULL */
+  int32_t* seq_status;   /* [seqs] */
+} xs_prompt_attend_args;
+
+int xs_prompt_attend(xs_cache_context* ctx, const xs_prompt_attend_args* args);
+
+/* Keys and values of one layer in 8 bits (e4m3: sign, 4 bits of exponent, 3 of
+ * fraction, largest 448, no infinities), [seqs, slots, kv_heads, head_dim] like
+ * xs_kv with strides in bytes, multiples of 16.  Every XS_CACHE8_BLOCK slots of
+ * a head share a power of two, for keys and for values: element = byte * 2^e,
+ * with e + 127 held in a byte of k_exp or v_exp [seqs, kv_heads, exp_ld].  The
+ * exponents of blocks that hold no slot in use need no values. */
+#define XS_CACHE8_BLOCK 32
+typedef struct {
+  uint8_t* k;
+  uint8_t* v;
+  int64_t seq_stride, slot_stride, head_stride;
+  uint8_t* k_exp;
+  uint8_t* v_exp;
+  int64_t exp_ld;        /* >= capacity / XS_CACHE8_BLOCK, rounded up */
+} xs_kv8;
+
+/* Appends rows: slot len + r takes the keys and values of row r, r < n, and
+ * new_len = len + n.  The rows of sequence b are
+ *   start NULL  of fresh [seqs, rows, ...]: row r is row path[r] (NULL: r), and
+ *               n = n_path[b] (NULL: rows); path and n_path are xs_verify_tree's
+ *   start       of fresh [tokens, ...] (its seq_stride is not read): row r is
+ *               row start[b] + r, and n = start[b + 1] - start[b]
+ * A block's e is the least with |x| <= 448 * 2^e for all its finite elements,
+ * -100 at least; x is held as x * 2^-e, rounded once to e4m3 (nearest, ties to
+ * even), a NaN or an infinity as NaN.  In a block that held slots already e
+ * grows where the new rows ask for it, never shrinks, and the old slots are
+ * then rounded again at the new e (exact but for what falls below e4m3's normal
+ * numbers).  Results do not depend on how rows are cut into calls but for that
+ * second rounding.  A sequence whose len is outside [0, capacity], whose n is
+ * outside [0, rows] or whose path or start holds a row outside fresh gets
+ * XS_ROW_BAD_PARAM, one without room XS_ROW_CACHE_FULL; its new_len is len, and
+ * nothing else of it is written. */
+typedef struct {
+  int32_t dtype;         /* XS_BF16 or XS_F16: fresh */
+  int32_t head_dim;      /* a multiple of 16, 16..256 */
+  int64_t seqs, rows, kv_heads;  /* rows: the most that a sequence takes */
+  xs_kv8 cache;
+  int64_t capacity;
+  const int32_t* len;    /* [seqs] */
+  xs_kv fresh;
+  int64_t tokens;        /* rows of fresh where start is given */
+  const int32_t* start;  /* [seqs + 1] or NULL */
+  const int32_t* path;   /* [seqs, path_ld] or NULL */
+  int64_t path_ld;       /* >= rows */
+  const int32_t* n_path; /* [seqs] or NULL */
+  int32_t* new_len;      /* [seqs], not len itself */
+  int32_t* seq_status;   /* [seqs] */
+} xs_cache_append8_args;
+
+int xs_cache_append8(xs_cache_context* ctx, const xs_cache_append8_args* args);
+
+/* xs_tree_attend over a cache in 8 bits: all that is said there holds, with the
+ * cache's elements as they stand (byte * 2^e).  The tree's own keys and values
+ * (fresh) are in the inputs' type.  Weights are rounded to bf16 where q is bf16;
+ * where it is f16, to the sum of two bf16 (16 bits), since an element of the
+ * cache may pass f16's range (and a mean of such elements f16's end: an
+ * infinity then). */
+typedef struct {
+  int32_t dtype;         /* XS_BF16 or XS_F16: q, fresh and out */
+  int32_t head_dim;      /* a multiple of 16, 16..256 */
+  int64_t seqs, nodes;   /* nodes 1..XS_TREE_MAX */
+  int64_t q_heads, kv_heads;
+  const void* q;
+  int64_t q_seq_stride, q_node_stride, q_head_stride;
+  xs_kv8 cache;
+  int64_t capacity, max_len;  /* as in xs_tree_attend_args */
+  const int32_t* len;    /* [seqs] */
+  xs_kv fresh;
+  const int32_t* parent; /* [seqs, nodes] */
+  const int32_t* n_nodes;  /* [seqs], or NULL for `nodes` */
+  float scale;
+  void* out;
+  int64_t out_seq_stride, out_node_stride, out_head_stride;
+  float* lse;            /* [seqs, nodes, q_heads] or NULL */
+  int32_t* seq_status;   /* [seqs] */
+} xs_tree_attend8_args;
+
+int xs_tree_attend8(xs_cache_context* ctx, const xs_tree_attend8_args* args);
+
+/* ---------------------------------------------------------------------------
  * Drafter confidence: argmax_probs_device / draft_argmax_probs
  * (generate.rs:4059-4087).  For each row of logits [rows, ld] (all `width`
  * columns: the reference reduces the raw lm_head row, with no encodable bound

@@ -28,6 +28,8 @@ NOALLOC_VOCAB = 262144
 NOALLOC_BYTES = 15030784
 TREE_MAX = 64
 BF16, F16 = 0, 1
+ROT_HALVES, ROT_NEIGHBOURS = 0, 1
+CACHE8_BLOCK = 32
 
 _vp = C.c_void_p
 _i64 = C.c_int64
@@ -140,6 +142,54 @@ class CacheEvictArgs(C.Structure):
     ]
 
 
+class QkRotateArgs(C.Structure):
+    _fields_ = [
+        ("dtype", _i32), ("head_dim", _i32), ("tokens", _i64), ("q_heads", _i64), ("kv_heads", _i64),
+        ("q", _vp), ("q_token_stride", _i64), ("q_head_stride", _i64),
+        ("k", _vp), ("k_token_stride", _i64), ("k_head_stride", _i64),
+        ("q_weight", _vp), ("k_weight", _vp), ("eps", C.c_float), ("rot_dim", _i32), ("pairs", _i32),
+        ("inv_freq", _vp), ("pos", _vp),
+        ("q_out", _vp), ("q_out_token_stride", _i64), ("q_out_head_stride", _i64),
+        ("k_out", _vp), ("k_out_token_stride", _i64), ("k_out_head_stride", _i64),
+    ]
+
+
+class PromptAttendArgs(C.Structure):
+    _fields_ = [
+        ("dtype", _i32), ("head_dim", _i32), ("seqs", _i64), ("tokens", _i64), ("q_heads", _i64), ("kv_heads", _i64),
+        ("q", _vp), ("q_token_stride", _i64), ("q_head_stride", _i64),
+        ("k", _vp), ("v", _vp), ("kv_token_stride", _i64), ("kv_head_stride", _i64),
+        ("start", _vp), ("scale", C.c_float),
+        ("out", _vp), ("out_token_stride", _i64), ("out_head_stride", _i64), ("lse", _vp), ("seq_status", _vp),
+    ]
+
+
+class Kv8(C.Structure):
+    """xs_kv8: keys and values in e4m3, their strides in bytes, and the exponents of their scales."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("seq_stride", _i64), ("slot_stride", _i64), ("head_stride", _i64),
+                ("k_exp", _vp), ("v_exp", _vp), ("exp_ld", _i64)]
+
+
+class CacheAppend8Args(C.Structure):
+    _fields_ = [
+        ("dtype", _i32), ("head_dim", _i32), ("seqs", _i64), ("rows", _i64), ("kv_heads", _i64),
+        ("cache", Kv8), ("capacity", _i64), ("len", _vp), ("fresh", Kv), ("tokens", _i64), ("start", _vp),
+        ("path", _vp), ("path_ld", _i64), ("n_path", _vp), ("new_len", _vp), ("seq_status", _vp),
+    ]
+
+
+class TreeAttend8Args(C.Structure):
+    _fields_ = [
+        ("dtype", _i32), ("head_dim", _i32), ("seqs", _i64), ("nodes", _i64), ("q_heads", _i64), ("kv_heads", _i64),
+        ("q", _vp), ("q_seq_stride", _i64), ("q_node_stride", _i64), ("q_head_stride", _i64),
+        ("cache", Kv8), ("capacity", _i64), ("max_len", _i64), ("len", _vp), ("fresh", Kv),
+        ("parent", _vp), ("n_nodes", _vp), ("scale", C.c_float),
+        ("out", _vp), ("out_seq_stride", _i64), ("out_node_stride", _i64), ("out_head_stride", _i64),
+        ("lse", _vp), ("seq_status", _vp),
+    ]
+
+
 class XsError(RuntimeError):
     pass
 
@@ -183,6 +233,14 @@ def load() -> C.CDLL:
     L.xs_cache_commit.argtypes = [_vp, C.POINTER(CacheCommitArgs)]
     L.xs_cache_evict.restype = C.c_int
     L.xs_cache_evict.argtypes = [_vp, C.POINTER(CacheEvictArgs)]
+    L.xs_qk_rotate.restype = C.c_int
+    L.xs_qk_rotate.argtypes = [_vp, C.POINTER(QkRotateArgs)]
+    L.xs_prompt_attend.restype = C.c_int
+    L.xs_prompt_attend.argtypes = [_vp, C.POINTER(PromptAttendArgs)]
+    L.xs_cache_append8.restype = C.c_int
+    L.xs_cache_append8.argtypes = [_vp, C.POINTER(CacheAppend8Args)]
+    L.xs_tree_attend8.restype = C.c_int
+    L.xs_tree_attend8.argtypes = [_vp, C.POINTER(TreeAttend8Args)]
     L.xs_argmax_probs.restype = C.c_int
     L.xs_argmax_probs.argtypes = [_vp, C.POINTER(ArgmaxArgs)]
     L.xs_select_option.restype = _i32

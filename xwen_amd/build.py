@@ -15,7 +15,7 @@ import tempfile
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SOURCES = [os.path.join(HERE, "csrc", f) for f in ("xs_sampler.hip", "xs_tree.hip")]
+SOURCES = [os.path.join(HERE, "csrc", f) for f in ("xs_sampler.hip", "xs_tree.hip", "xs_prompt.hip", "xs_cache8.hip")]
 HOST_SRC = os.path.join(HERE, "csrc", "xs_host.cpp")  # host-only C ABI (also built alone for ASan)
 OUT = os.path.join(HERE, "libxsamp.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

@@ -65,6 +65,14 @@ bool kv_ok(const xs_kv& kv, int64_t seqs, int64_t slots, int64_t kv_heads, int64
          strides_ok(seqs, kv.seq_stride, slots, kv.slot_stride, kv_heads, kv.head_stride, head_dim, written);
 }
 
+// The same in bytes, of which 16 are a load; and the exponents.
+bool kv8_ok(const xs_kv8& kv, int64_t seqs, int64_t slots, int64_t kv_heads, int64_t head_dim, bool written) {
+  return kv.k && kv.v && kv.k_exp && kv.v_exp && aligned16(kv.k) && aligned16(kv.v) && kv.seq_stride % 16 == 0 &&
+         kv.slot_stride % 16 == 0 && kv.head_stride % 16 == 0 && kv.exp_ld >= (slots + XS_CACHE8_BLOCK - 1) / XS_CACHE8_BLOCK &&
+         kv.exp_ld <= (INT64_MAX >> 4) / kv_heads / (seqs > 0 ? seqs : 1) &&
+         strides_ok(seqs, kv.seq_stride, slots, kv.slot_stride, kv_heads, kv.head_stride, head_dim, written);
+}
+
 // Two per-sequence arrays share no entry.
 bool apart(const int32_t* p, const int32_t* q, int64_t seqs) {
   const uintptr_t x = (uintptr_t)p, y = (uintptr_t)q, n = (uintptr_t)seqs * sizeof(int32_t);
@@ -222,6 +230,86 @@ int xs_host_check_evict(const xs_cache_dims* dims, const xs_cache_evict_args* in
     return XS_ERR_ARG;
   if (in->slot_ld < in->capacity || !slots_fit(in->seqs, in->kv_heads, in->slot_ld)) return XS_ERR_ARG;
   return kv_ok(in->cache, in->seqs, in->capacity, in->kv_heads, in->head_dim, true) ? XS_OK : XS_ERR_ARG;
+}
+
+int xs_host_check_rotate(const xs_qk_rotate_args* in) {
+  if (!in) return XS_ERR_ARG;
+  const int64_t d = in->head_dim, r = in->rot_dim;
+  if (in->dtype != XS_BF16 && in->dtype != XS_F16) return XS_ERR_ARG;
+  if (d < 8 || d > 256 || d % 8 || in->tokens < 0 || in->q_heads < 0 || in->kv_heads < 0) return XS_ERR_ARG;
+  if (in->pairs != XS_ROT_HALVES && in->pairs != XS_ROT_NEIGHBOURS) return XS_ERR_ARG;
+  if (r < 0 || r > d || r % (in->pairs == XS_ROT_HALVES ? 16 : 8)) return XS_ERR_ARG;
+  if (!(in->eps >= 0.0f)) return XS_ERR_ARG;
+  // heads are counted in 32 bits
+  if (in->q_heads > 65536 || in->kv_heads > 65536) return XS_ERR_CAPACITY;
+  if (in->tokens == 0 || in->q_heads + in->kv_heads == 0) return XS_OK;
+  if (r > 0 && (!in->inv_freq || !in->pos)) return XS_ERR_ARG;
+  if (in->q_heads && in->kv_heads && !in->q_weight != !in->k_weight) return XS_ERR_ARG;
+  auto side = [&](int64_t heads, const void* x, int64_t ts, int64_t hs, const float* w, void* y, int64_t yts, int64_t yhs) {
+    if (heads == 0) return true;
+    return x && y && aligned16(x) && aligned16(y) && aligned16(w) && strides_ok(in->tokens, ts, heads, hs, 1, 0, d, false) &&
+           strides_ok(in->tokens, yts, heads, yhs, 1, 0, d, true) && (x != y || ((in->tokens == 1 || ts == yts) && (heads == 1 || hs == yhs)));
+  };
+  if (!side(in->q_heads, in->q, in->q_token_stride, in->q_head_stride, in->q_weight, in->q_out, in->q_out_token_stride, in->q_out_head_stride) ||
+      !side(in->kv_heads, in->k, in->k_token_stride, in->k_head_stride, in->k_weight, in->k_out, in->k_out_token_stride, in->k_out_head_stride))
+    return XS_ERR_ARG;
+  if (in->q_heads && in->kv_heads && (in->q_out == in->k_out || in->q_out == in->k || in->k_out == in->q)) return XS_ERR_ARG;
+  return XS_OK;
+}
+
+int xs_host_check_prompt(const xs_prompt_attend_args* in) {
+  if (!in) return XS_ERR_ARG;
+  if (in->dtype != XS_BF16 && in->dtype != XS_F16) return XS_ERR_ARG;
+  if (in->head_dim < 8 || in->head_dim > 256 || in->head_dim % 8) return XS_ERR_ARG;
+  if (in->seqs < 0 || in->tokens < 0 || in->q_heads < 1 || in->kv_heads < 1 || in->q_heads % in->kv_heads) return XS_ERR_ARG;
+  // a sequence's rows (tokens and q heads of one kv head) are counted in 32 bits
+  if (in->seqs > 65536 || in->q_heads > 4096 || in->tokens > (1 << 30) / (in->q_heads / in->kv_heads)) return XS_ERR_CAPACITY;
+  // and so are the elements that 64 tokens of k span
+  if (in->kv_token_stride > (1 << 24)) return XS_ERR_CAPACITY;
+  if (in->seqs == 0) return XS_OK;
+  if (!in->start || !in->seq_status) return XS_ERR_ARG;
+  if (in->tokens == 0) return XS_OK;
+  if (!in->q || !in->k || !in->v || !in->out || in->out == in->q || in->out == in->k || in->out == in->v) return XS_ERR_ARG;
+  if (!aligned16(in->q) || !aligned16(in->k) || !aligned16(in->v) || !aligned16(in->out) ||
+      !strides_ok(in->tokens, in->q_token_stride, in->q_heads, in->q_head_stride, 1, 0, in->head_dim, false) ||
+      !strides_ok(in->tokens, in->kv_token_stride, in->kv_heads, in->kv_head_stride, 1, 0, in->head_dim, false) ||
+      !strides_ok(in->tokens, in->out_token_stride, in->q_heads, in->out_head_stride, 1, 0, in->head_dim, true))
+    return XS_ERR_ARG;
+  return XS_OK;
+}
+
+int xs_host_check_append8(const xs_cache_dims* dims, const xs_cache_append8_args* in) {
+  if (!dims || !in) return XS_ERR_ARG;
+  const int rc = check_sizes(dims, in->dtype, in->head_dim, in->seqs, in->kv_heads, in->capacity, 0);
+  if (rc != XS_OK) return rc;
+  if (in->head_dim % 16 || in->rows < 0 || in->tokens < 0) return XS_ERR_ARG;
+  if (in->rows > INT32_MAX || in->tokens > INT32_MAX || in->path_ld > INT32_MAX) return XS_ERR_CAPACITY;
+  if (in->seqs == 0) return XS_OK;
+  if (!in->len || !in->new_len || !in->seq_status || !apart(in->len, in->new_len, in->seqs)) return XS_ERR_ARG;
+  if (in->start && (in->path || in->n_path)) return XS_ERR_ARG;
+  if (in->path && in->path_ld < in->rows) return XS_ERR_ARG;
+  if (!kv8_ok(in->cache, in->seqs, in->capacity, in->kv_heads, in->head_dim, true)) return XS_ERR_ARG;
+  const int64_t source = in->start ? in->tokens : in->rows;
+  if (in->rows == 0 || source == 0) return XS_OK;  // (no row to read)
+  xs_kv fresh = in->fresh;
+  if (in->start) fresh.seq_stride = 0;
+  return kv_ok(fresh, in->seqs, source, in->kv_heads, in->head_dim, false) ? XS_OK : XS_ERR_ARG;
+}
+
+int xs_host_check_attend8(const xs_cache_dims* dims, const xs_tree_attend8_args* in) {
+  if (!dims || !in) return XS_ERR_ARG;
+  int rc = check_sizes(dims, in->dtype, in->head_dim, in->seqs, in->kv_heads, in->capacity, in->max_len);
+  if (rc == XS_OK) rc = check_queries(dims, in->nodes, in->q_heads, in->kv_heads);
+  if (rc == XS_OK && in->head_dim % 16) return XS_ERR_ARG;
+  if (rc != XS_OK || in->seqs == 0) return rc;
+  if (!in->len || !in->parent || !in->seq_status || !in->q || !in->out || in->q == in->out) return XS_ERR_ARG;
+  if (!aligned16(in->q) || !aligned16(in->out) ||
+      !kv8_ok(in->cache, in->seqs, in->capacity, in->kv_heads, in->head_dim, false) ||
+      !kv_ok(in->fresh, in->seqs, in->nodes, in->kv_heads, in->head_dim, false) ||
+      !strides_ok(in->seqs, in->q_seq_stride, in->nodes, in->q_node_stride, in->q_heads, in->q_head_stride, in->head_dim, false) ||
+      !strides_ok(in->seqs, in->out_seq_stride, in->nodes, in->out_node_stride, in->q_heads, in->out_head_stride, in->head_dim, true))
+    return XS_ERR_ARG;
+  return XS_OK;
 }
 
 bool xs_host_launch_fits(int64_t workgroups, int64_t threads) {

@@ -32,6 +32,10 @@ int xs_host_check_dims(const xs_cache_dims* dims);
 int xs_host_check_attend(const xs_cache_dims* dims, const xs_tree_attend_args* in);
 int xs_host_check_commit(const xs_cache_dims* dims, const xs_cache_commit_args* in);
 int xs_host_check_evict(const xs_cache_dims* dims, const xs_cache_evict_args* in);
+int xs_host_check_rotate(const xs_qk_rotate_args* in);
+int xs_host_check_prompt(const xs_prompt_attend_args* in);
+int xs_host_check_append8(const xs_cache_dims* dims, const xs_cache_append8_args* in);
+int xs_host_check_attend8(const xs_cache_dims* dims, const xs_tree_attend8_args* in);
 // Whether one launch takes so many workgroups: their number and that of their
 // work-items are 32 bits wide.
 bool xs_host_launch_fits(int64_t workgroups, int64_t threads);

@@ -1,0 +1,623 @@
+// xs_prompt.hip -- a prompt's way to its attention (MI355X, gfx950): norms and
+// positions of queries and keys, and causal attention of packed prompts.
+//
+// Compiled with -ffp-contract=off; fused multiply-adds are written out.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <stdint.h>
+
+#include "../../include/xsamp.h"
+#include "xs_attend.h"
+#include "xs_cache.h"
+#include "xs_device.h"
+#include "xs_host.h"
+
+namespace xsp {
+
+using namespace xst;
+
+// ---------------------------------------------------------------------------
+// Norms and positions.
+//
+// A head of a token is LPH lanes (a power of two, head_dim / 16 at least) of 16
+// elements each: two 16-byte pieces, which for halves are those of a rotated
+// pair, so that no element crosses lanes.  A workgroup takes `span` heads in a
+// row (tokens outermost, a token's q heads before its kv heads); the angles of
+// its tokens are computed once, into LDS.  Bound by the one read and write of
+// the heads.
+
+constexpr int RT = 256;  // threads of a workgroup
+
+template <typename T>
+XS_DEV void widen8(u32x4 r, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    x[2 * i] = T::widen((uint16_t)r[i]);
+    x[2 * i + 1] = T::widen((uint16_t)(r[i] >> 16));
+  }
+}
+
+template <typename T, int LPH, int ITER>
+__global__ __launch_bounds__(RT) void rotate_kernel(const xs_qk_rotate_args a) {
+  extern __shared__ f32x2 turn[];  // [tokens of the workgroup][rot_dim / 2] cos, sin
+  constexpr int PER = RT / LPH;    // heads of a pass
+  const int heads = (int)(a.q_heads + a.kv_heads), D = a.head_dim, half = a.rot_dim / 2;
+  const bool halves = a.pairs == XS_ROT_HALVES;
+  const int p = threadIdx.x % LPH;
+  const int64_t first = (int64_t)blockIdx.x * (PER * ITER), all = a.tokens * heads;
+  const int64_t t0 = first / heads;
+
+  // the lane's two pieces
+  const int rc = halves ? half / 8 : 0, chunks = D / 8;
+  const int c0 = p < rc ? p : 2 * p, c1 = p < rc ? p + rc : 2 * p + 1;
+  const bool in0 = c0 < chunks, in1 = c1 < chunks;
+
+  u32x4 raw[ITER][2];
+#pragma unroll
+  for (int i = 0; i < ITER; i++) {
+    const int64_t at = first + i * PER + threadIdx.x / LPH;
+    raw[i][0] = raw[i][1] = (u32x4){0, 0, 0, 0};
+    if (at < all) {
+      const int64_t t = t0 + (int)(at - t0 * heads) / heads;
+      const int h = (int)(at - t * heads);
+      const uint16_t* x = h < a.q_heads ? (const uint16_t*)a.q + t * a.q_token_stride + h * a.q_head_stride
+                                        : (const uint16_t*)a.k + t * a.k_token_stride + (h - a.q_heads) * a.k_head_stride;
+      if (in0) raw[i][0] = *(const u32x4*)(x + 8 * c0);
+      if (in1) raw[i][1] = *(const u32x4*)(x + 8 * c1);
+    }
+  }
+
+  if (half > 0) {
+    // The angle in turns, from f64 (a position of 2^31 times a frequency of 1
+    // leaves 2^-23 of a turn); cos and sin of its fraction in f32.
+    const int64_t last = min(first + PER * ITER, all) - 1;
+    const int tokens = (int)(last / heads - t0) + 1;
+    for (int i = threadIdx.x; i < tokens * half; i += RT) {
+      const double x = (double)a.pos[t0 + i / half] * (double)a.inv_freq[i % half] * 0.15915494309189533577;
+      float s, c;
+      sincospif((float)(2.0 * (x - rint(x))), &s, &c);
+      turn[i] = (f32x2){c, s};
+    }
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int i = 0; i < ITER; i++) {
+    const int64_t at = first + i * PER + threadIdx.x / LPH;
+    const int64_t t = t0 + (int)(at - t0 * heads) / heads;
+    const int h = (int)(at - t * heads);
+    float x[2][8];
+    widen8<T>(raw[i][0], x[0]);
+    widen8<T>(raw[i][1], x[1]);
+    const float* w = h < a.q_heads ? a.q_weight : a.k_weight;
+    if (w) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; e++) sum = __builtin_fmaf(x[1][e], x[1][e], __builtin_fmaf(x[0][e], x[0][e], sum));
+#pragma unroll
+      for (int m = 1; m < LPH; m *= 2) sum += __shfl_xor(sum, m);
+      const float inv = 1.0f / sqrtf(sum / (float)D + a.eps);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        if (in0) x[0][e] = x[0][e] * inv * w[8 * c0 + e];
+        if (in1) x[1][e] = x[1][e] * inv * w[8 * c1 + e];
+      }
+    }
+    if (at >= all) continue;
+    const f32x2* cs = turn + (int)(t - t0) * half;
+    if (halves) {
+      if (p < rc) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const f32x2 z = cs[8 * p + e];
+          const float u = x[0][e], v = x[1][e];
+          x[0][e] = __builtin_fmaf(u, z[0], -(v * z[1]));
+          x[1][e] = __builtin_fmaf(v, z[0], u * z[1]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+        if (8 * (2 * p + j) < a.rot_dim) {
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const f32x2 z = cs[4 * (2 * p + j) + e / 2];
+            const float u = x[j][e], v = x[j][e + 1];
+            x[j][e] = __builtin_fmaf(u, z[0], -(v * z[1]));
+            x[j][e + 1] = __builtin_fmaf(v, z[0], u * z[1]);
+          }
+        }
+    }
+    uint16_t* y = h < a.q_heads ? (uint16_t*)a.q_out + t * a.q_out_token_stride + h * a.q_out_head_stride
+                                : (uint16_t*)a.k_out + t * a.k_out_token_stride + (h - a.q_heads) * a.k_out_head_stride;
+    u32x4 r;
+    if (in0) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) r[j] = pack2(T{}, x[0][2 * j], x[0][2 * j + 1]);
+      *(u32x4*)(y + 8 * c0) = r;
+    }
+    if (in1) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) r[j] = pack2(T{}, x[1][2 * j], x[1][2 * j + 1]);
+      *(u32x4*)(y + 8 * c1) = r;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Causal attention of packed prompts.
+//
+// The rows of one (sequence, kv head) are its tokens times the group of q heads
+// that share the head: row r = token * group + q head.  A workgroup takes 32 NWV
+// rows, 32 a wave, and walks the keys up to its last row's token in stages of 64,
+// through two LDS buffers that loads fill while the other is read.  With
+// v_mfma_f32_32x32x16 (lane = 32 g + x; A[m = x][k = 8 g + e], B[k = 8 g + e][n = x],
+// C[m = 8 (r / 4) + 4 g + r % 4][n = x]):
+//
+//   S^T = K Q^T   a lane holds scores of one row (n = x), of 16 of every 32 keys
+//   O^T = V^T P^T the contraction runs over the keys in the order in which the
+//                 lane holds them (position 8 g + e of 16 is key 8 (e / 4) + 4 g +
+//                 e % 4), so the weights go to B as they are; V's fragments come
+//                 through transposing LDS reads, four keys of a column each
+//
+// The softmax is that of xs_attend.h: one pass, a running reference which is one
+// of the row's own scores, products that start from it, moved only when the best
+// has grown by 2^8.
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+XS_DEV f32x16 mfma32(Bf16, u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+XS_DEV f32x16 mfma32(F16, u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+XS_DEV f32x16 fill16(float v) { return (f32x16){v, v, v, v, v, v, v, v, v, v, v, v, v, v, v, v}; }
+
+// Over the two lanes of a row.
+XS_DEV float pair_max(float v) {
+  const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+XS_DEV float pair_sum(float v) {
+  const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+constexpr int SK = 64;  // keys of a stage
+
+// A stage in LDS: rows of CH 16-byte chunks.  Chunk c of a row lies at c ^ turn,
+// so that rows read together meet all banks: 16 rows' chunk of K (16 bytes each),
+// four rows' 64 bytes of V.
+template <int DP>
+struct Keys {
+  static constexpr int CH = DP / 8;
+  XS_DEV static int turn_k(int row) { return CH % 16 == 0 ? row & 15 : CH % 8 == 0 ? row >> 1 & 7 : row >> 2 & 3; }
+  XS_DEV static int turn_v(int row) { return CH % 16 == 0 ? (row & 3) << 2 : CH % 8 == 0 ? (row >> 1 & 1) << 2 : 0; }
+};
+// The sequence and the row tile of a workgroup: tiles of the device's valid
+// sequences, those with the most keys first, sequences of more than 64 in order.
+struct Place {
+  int b, tile;  // b < 0: none
+  int first, n;
+};
+
+template <int ROWS>
+XS_DEV Place place(const xs_prompt_attend_args& a, int G, int64_t want, bool report) {
+  const int lane = threadIdx.x & 63;
+  Place p = {-1, 0, 0, 0};
+  int high = 0;         // the largest entry of start so far
+  int64_t before = 0;   // tiles of earlier sequences
+  const bool small = a.seqs <= 64;
+  for (int64_t b0 = 0; b0 < a.seqs; b0 += 64) {
+    const int64_t b = b0 + lane;
+    const bool in = b < a.seqs;
+    const int s = in ? a.start[b] : 0, e = in ? a.start[b + 1] : 0;
+    int top = in ? s : INT32_MIN;  // inclusive prefix maximum
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) {
+      const int y = __shfl_up(top, m);
+      if (lane >= m) top = max(top, y);
+    }
+    top = max(top, high);
+    high = __shfl(top, 63);
+    const bool good = in && s >= top && e >= s && e <= a.tokens;
+    if (report && in) a.seq_status[b] = good ? XS_ROW_OK : XS_ROW_BAD_PARAM;
+    const int tiles = good ? (int)(((int64_t)(e - s) * G + ROWS - 1) / ROWS) : 0;
+    if (p.b >= 0) continue;  // (found; the rest is only reported)
+    int who = -1, tile = 0;
+    if (small) {
+      // above(L): tiles at a level past L, the level of a tile its place in its sequence
+      auto above = [&](int L) {
+        int64_t v = max(0, tiles - L);
+#pragma unroll
+        for (int m = 1; m < 64; m *= 2) v += __shfl_xor(v, m);
+        return v;
+      };
+      int lo = 0, hi = tiles;  // the largest L with above(L) > want
+#pragma unroll
+      for (int m = 1; m < 64; m *= 2) hi = max(hi, __shfl_xor(hi, m));
+      if (above(0) <= want) return p;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (above(mid) > want) lo = mid;
+        else hi = mid;
+      }
+      const int nth = (int)(want - above(lo + 1));
+      uint64_t have = __ballot(tiles > lo);
+      for (int i = 0; i < nth; i++) have &= have - 1;
+      who = __ffsll((unsigned long long)have) - 1;
+      tile = lo;
+    } else {
+      int64_t upto = tiles;
+#pragma unroll
+      for (int m = 1; m < 64; m *= 2) {
+        const int64_t y = __shfl_up(upto, m);
+        if (lane >= m) upto += y;
+      }
+      upto += before;
+      const uint64_t past = __ballot(upto > want);
+      before = __shfl(upto, 63);
+      if (past) {
+        who = __ffsll((unsigned long long)past) - 1;
+        tile = (int)(__shfl(upto, who) - 1 - want);  // the last of a sequence first
+      }
+    }
+    if (who >= 0) {
+      p.b = (int)b0 + who;
+      p.tile = tile;
+      p.first = __shfl(s, who);
+      p.n = __shfl(e, who) - p.first;
+      if (!report) return p;
+    }
+  }
+  return p;
+}
+
+// 16 bytes a lane from global memory to LDS (lane i's at to + 16 i), in flight
+// until vmcnt says otherwise.  In assembly, so that the compiler, which cannot
+// tell the buffers apart, does not wait for it before every read of LDS; what
+// reads the bytes waits first (arrived).
+XS_DEV void load_lds(const uint16_t* base, uint32_t bytes, u32x4* to) {
+  const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)to;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(bytes), "s"(base) : "memory", "m0");
+}
+XS_DEV void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+template <typename T, int DP, int NWV, bool EXACT>
+__global__ __launch_bounds__(64 * NWV, DP <= 128 ? 2 : 1) void prompt_kernel(const xs_prompt_attend_args a, float scale) {
+  using K = Keys<DP>;
+  constexpr int KC = DP / 16, DT = DP / 32, ROWS = 32 * NWV, CH = K::CH;
+  constexpr int STAGE = SK * CH;                      // chunks of a stage, of k and of v
+  constexpr int PER = STAGE / (64 * NWV);             // of a thread
+  static_assert(STAGE % (64 * NWV) == 0, "a stage is whole chunks of every thread");
+  __shared__ u32x4 lds[2][2][STAGE];                  // [buffer][k, v]
+  __shared__ int odds;
+  const int lane = threadIdx.x & 63, x = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = (int)(a.q_heads / a.kv_heads);
+  const int kh = (int)(blockIdx.x % (unsigned)a.kv_heads);
+  const Place at = place<ROWS>(a, G, blockIdx.x / (unsigned)a.kv_heads, blockIdx.x == 0 && wave == 0);
+  const int b = __builtin_amdgcn_readfirstlane(at.b);
+  if (b < 0) return;
+  const int n = __builtin_amdgcn_readfirstlane(at.n), t0 = __builtin_amdgcn_readfirstlane(at.first);
+  const int R = n * G;
+  const int row0 = __builtin_amdgcn_readfirstlane(at.tile) * ROWS, wrow = row0 + 32 * wave;
+  const int row = wrow + x, token = min(row, R - 1) / G, head = kh * G + min(row, R - 1) % G;
+  const int low = min(wrow, R - 1) / G, top_token = min(wrow + 31, R - 1) / G;  // of the wave's rows
+  const int wg_low = row0 / G;                                                 // of the workgroup's
+  const int end = min(row0 + ROWS - 1, R - 1) / G + 1;                         // keys that it needs
+  const int stages = (end + SK - 1) / SK;
+  const bool live = wrow < R;
+
+  u32x4 q[KC];
+  {
+    const uint16_t* p = (const uint16_t*)a.q + (int64_t)(t0 + token) * a.q_token_stride + head * a.q_head_stride;
+#pragma unroll
+    for (int c = 0; c < KC; c++) {
+      const int d = 16 * c + 8 * g;
+      q[c] = row < R && (EXACT || d < a.head_dim) ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0};
+    }
+  }
+  // A stage's chunks, each by the lane whose place in LDS it takes.  Chunks past
+  // the head's end are zero from the start.
+  const uint16_t* kp = (const uint16_t*)a.k + (int64_t)t0 * a.kv_token_stride + kh * a.kv_head_stride;
+  const uint16_t* vp = (const uint16_t*)a.v + (int64_t)t0 * a.kv_token_stride + kh * a.kv_head_stride;
+  if (!EXACT) {
+#pragma unroll
+    for (int i = 0; i < 4 * PER; i++) (&lds[0][0][0])[i * 64 * NWV + threadIdx.x] = (u32x4){0, 0, 0, 0};
+    __syncthreads();
+  }
+  auto fetch = [&](int s) {
+    const int64_t o = (int64_t)s * SK * a.kv_token_stride;
+    const int last = n - 1 - s * SK;
+    const uint32_t stride = 2 * (uint32_t)a.kv_token_stride;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const int u = i * 64 * NWV + threadIdx.x, r = u / CH, ck = u % CH ^ K::turn_k(r), cv = u % CH ^ K::turn_v(r);
+      const uint32_t rows = (uint32_t)min(r, last) * stride;
+      u32x4* to = &lds[s & 1][0][i * 64 * NWV + 64 * wave];
+      if (EXACT || 8 * ck < a.head_dim) load_lds(kp + o, rows + 16u * ck, to);
+      if (EXACT || 8 * cv < a.head_dim) load_lds(vp + o, rows + 16u * cv, to + STAGE);
+    }
+  };
+
+  constexpr float OFF = offset_of(T{});
+  f32x16 o[DT], base = fill16(0.0f);  // base: minus the reference, which the products start from
+#pragma unroll
+  for (int d = 0; d < DT; d++) o[d] = fill16(0.0f);
+  float most = __builtin_nanf(""), l = 0.0f;
+  int odd = 0;
+  if (threadIdx.x == 0) odds = 0;
+
+  // Byte offsets of the lane's reads within a stage: K's chunk 2 c + g of row x
+  // (of 32 u + x: 32 rows on), V's columns 32 d + 16 q4 + 4 (i % 4) of row 4 g + i / 4.
+  const int i16 = lane & 15, vr = 4 * g + (i16 >> 2);
+  auto key = [&](int u, int c, int kb) {
+    int c16;  // 16 (c's chunk ^ the row's turn), kb holding g's and the turn
+    if constexpr (CH % 16 == 0) c16 = (kb ^ (32 * (c % 8))) + 256 * (c / 8);
+    else if constexpr (CH % 8 == 0) c16 = kb ^ (32 * c);
+    else c16 = (kb ^ (32 * (c % 2))) + 64 * (c / 2);
+    return c16 + 32 * u * CH * 16;
+  };
+  // kb's row part has to keep clear of the bits that c turns
+  const int krow = x * CH * 16, kturn = 16 * (g ^ K::turn_k(x));
+  const int vrow = vr * CH * 16 + 8 * (i16 & 1), vcol = 16 * ((2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1)) ^ K::turn_v(vr));
+
+  fetch(0);
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the rows' loads too, which the loop would wait for at every stage
+  for (int s = 0; s < stages; s++) {
+    arrived();
+    __syncthreads();
+    if (s + 1 < stages) fetch(s + 1);
+    const bool masked_wg = s * SK + SK - 1 > wg_low;
+    if (masked_wg) {
+      // A NaN or an infinity of V would, through the product, reach rows that do
+      // not see its token: taken out here, and added at the end to the rows that do.
+      bool found = false;
+#pragma unroll
+      for (int i = 0; i < PER; i++) {
+        const u32x4 v = lds[s & 1][1][i * 64 * NWV + threadIdx.x];
+#pragma unroll
+        for (int j = 0; j < 4; j++) found |= (v[j] & 0x7FFFu) >= inf_of(T{}) || ((v[j] >> 16) & 0x7FFFu) >= inf_of(T{});
+      }
+      if (__any(found) && lane == 0) odds = 1;
+      __syncthreads();
+      if (odds) {  // (rare; uniform)
+        odd = 1;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+          u32x4 v = lds[s & 1][1][i * 64 * NWV + threadIdx.x];
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            if ((v[j] & 0x7FFFu) >= inf_of(T{})) v[j] &= 0xFFFF0000u;
+            if (((v[j] >> 16) & 0x7FFFu) >= inf_of(T{})) v[j] &= 0xFFFFu;
+          }
+          lds[s & 1][1][i * 64 * NWV + threadIdx.x] = v;
+        }
+        __syncthreads();
+      }
+    }
+    if (live && s * SK <= top_token) {
+      const char* ks = (const char*)&lds[s & 1][0][0] + krow;
+      const char* vs = (const char*)&lds[s & 1][1][0] + vrow;
+      int kb = kturn, vb = vcol;
+      asm volatile("" : "+v"(kb), "+v"(vb));  // (its sums with constants are formed where they are used)
+      f32x16 sc[2] = {base, base};
+#pragma unroll
+      for (int c = 0; c < KC; c++)
+#pragma unroll
+        for (int u = 0; u < 2; u++) sc[u] = mfma32(T{}, *(const u32x4*)(ks + key(u, c, kb)), q[c], sc[u]);
+      float xs[2][16], top = NEG_INF;
+      const bool masked = s * SK + SK - 1 > low;
+      const int lim = token - s * SK - 4 * g;  // the lane's key 32 u + 8 (r / 4) + r % 4 counts up to here
+      auto weigh = [&](bool from0, float ref) {
+        top = NEG_INF;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const float v = from0 ? sc[u][r] - ref : sc[u][r];
+            xs[u][r] = OFF == 0.0f ? v * scale : __builtin_fmaf(v, scale, OFF);
+          }
+        if (masked) {
+#pragma unroll
+          for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) xs[u][r] = 32 * u + 8 * (r / 4) + r % 4 <= lim ? xs[u][r] : NEG_INF;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) top = fmaxf(top, xs[u][r]);
+      };
+      weigh(false, 0.0f);
+      if (__any(!(top <= most))) [[unlikely]] {
+        // the references of the rows that have grown move to their best scores
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          sc[u] = fill16(0.0f);
+#pragma unroll
+          for (int c = 0; c < KC; c++) sc[u] = mfma32(T{}, *(const u32x4*)(ks + key(u, c, kb)), q[c], sc[u]);
+        }
+        const float sign = scale < 0.0f ? -1.0f : 1.0f, old = -base[0];
+        const bool unset = most != most;
+        float best = unset ? NEG_INF : old * sign;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) {
+            const float y = sc[u][r] * sign;
+            best = fmaxf(best, !masked || 32 * u + 8 * (r / 4) + r % 4 <= lim ? y : NEG_INF);
+          }
+        best = pair_max(best);
+        float ref = old;
+        if (best > NEG_INF) {
+          ref = scale == 0.0f ? 0.0f : best * sign;
+          const float keep = unset ? 0.0f : __builtin_amdgcn_exp2f((old - ref) * scale);
+          base = fill16(-ref);
+          most = LAZY + OFF;
+          l *= keep;
+#pragma unroll
+          for (int d = 0; d < DT; d++) o[d] *= keep;
+        }
+        weigh(true, ref);
+      }
+      u32x4 pf[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          float p[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(xs[u][8 * c + e]);
+          l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+#pragma unroll
+          for (int e = 0; e < 4; e++) pf[u][c][e] = pack2(T{}, p[2 * e], p[2 * e + 1]);
+        }
+#pragma unroll
+      for (int d = 0; d < DT; d++) {
+        const char* vd = vs + (CH % 16 == 0 ? (vb ^ (64 * (d % 4))) + 256 * (d / 4) : CH % 8 == 0 ? vb ^ (64 * d) : vb + 64 * d);
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            s16x4 v[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+              v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vd + (32 * u + 16 * c + 8 * h) * CH * 16));
+            const u32x2 v0 = __builtin_bit_cast(u32x2, v[0]), v1 = __builtin_bit_cast(u32x2, v[1]);
+            o[d] = mfma32(T{}, (u32x4){v0[0], v0[1], v1[0], v1[1]}, pf[u][c], o[d]);
+          }
+      }
+    }
+  }
+
+  if (row >= R) return;
+  l = pair_sum(l);
+  const float ref = -base[0];
+  if (l == 0.0f) {  // every score -inf
+#pragma unroll
+    for (int d = 0; d < DT; d++) o[d] = fill16(0.0f);
+  }
+  if (odd && l != 0.0f) {  // (rare) the NaNs and infinities that were taken out, of the tokens that the row sees
+#pragma unroll 1
+    for (int j = wg_low / SK * SK; j <= token; j++)
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const int e = 32 * d + 8 * (r / 4) + 4 * g + r % 4;
+          const uint16_t v = e < a.head_dim ? vp[(int64_t)j * a.kv_token_stride + e] : 0;
+          if ((v & 0x7FFFu) >= inf_of(T{})) o[d][r] += T::widen(v);
+        }
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* out = (uint16_t*)a.out + (int64_t)(t0 + token) * a.out_token_stride + head * a.out_head_stride;
+#pragma unroll
+  for (int d = 0; d < DT; d++)
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const int e = 32 * d + 2 * r + 4 * g;
+      if (e < a.head_dim)
+        *(u32x2*)(out + e) = (u32x2){pack2(T{}, within(T{}, o[d][r] * inv), within(T{}, o[d][r + 1] * inv)),
+                                     pack2(T{}, within(T{}, o[d][r + 2] * inv), within(T{}, o[d][r + 3] * inv))};
+    }
+  if (a.lse && g == 0)
+    a.lse[(int64_t)(t0 + token) * a.q_heads + head] =
+        l == 0.0f ? NEG_INF : __builtin_fmaf(ref, a.scale, LN2 * (__builtin_amdgcn_logf(l) - OFF));
+}
+
+// No token: only the sequences' statuses.
+__global__ __launch_bounds__(64) void prompt_status_kernel(const xs_prompt_attend_args a) { place<64>(a, 1, INT64_MAX, true); }
+
+}  // namespace xsp
+
+// ---------------------------------------------------------------------------
+// Host side.
+
+namespace {
+
+using xs_host::OnDevice;
+
+template <typename T, int LPH>
+int rotate_lanes(xs_cache_context* c, const xs_qk_rotate_args& a) {
+  const int64_t heads = a.q_heads + a.kv_heads, all = a.tokens * heads;
+  constexpr int64_t per = xsp::RT / LPH;
+  auto run = [&](auto kernel, int64_t iter) {
+    const int64_t span = per * iter, grid = (all + span - 1) / span;
+    if (!xs_host_launch_fits(grid, xsp::RT)) return XS_ERR_CAPACITY;
+    const int64_t tokens = std::min(a.tokens, (span + heads - 1) / heads + 1);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(xsp::RT), (size_t)(tokens * (a.rot_dim / 2) * 8), c->stream, a);
+    return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
+  };
+  // several passes a workgroup where that still fills the device, and where its
+  // tokens' angles are few
+  if (all >= per * 4 * 4 * c->n_cu && heads * 64 >= per * 4) return run(xsp::rotate_kernel<T, LPH, 4>, 4);
+  return run(xsp::rotate_kernel<T, LPH, 1>, 1);
+}
+
+template <typename T>
+int rotate_dim(xs_cache_context* c, const xs_qk_rotate_args& a) {
+  if (a.head_dim <= 16) return rotate_lanes<T, 1>(c, a);
+  if (a.head_dim <= 32) return rotate_lanes<T, 2>(c, a);
+  if (a.head_dim <= 64) return rotate_lanes<T, 4>(c, a);
+  if (a.head_dim <= 128) return rotate_lanes<T, 8>(c, a);
+  return rotate_lanes<T, 16>(c, a);
+}
+
+template <typename T, int DP, int NWV, bool EXACT>
+int prompt_run(xs_cache_context* c, const xs_prompt_attend_args& a) {
+  const int64_t rows = a.tokens * (a.q_heads / a.kv_heads), tile = 32 * NWV;
+  // no more tiles than this, whatever the sequences' lengths: each leaves less than one
+  const int64_t grid = (rows / tile + std::min(a.seqs, a.tokens)) * a.kv_heads;
+  if (!xs_host_launch_fits(grid, 64 * NWV)) return XS_ERR_CAPACITY;
+  hipLaunchKernelGGL((xsp::prompt_kernel<T, DP, NWV, EXACT>), dim3((unsigned)grid), dim3(64 * NWV), 0, c->stream, a, a.scale * xst::LOG2E);
+  return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
+}
+
+template <typename T, int DP>
+int prompt_exact(xs_cache_context* c, const xs_prompt_attend_args& a) {
+  return a.head_dim == DP ? prompt_run<T, DP, 4, true>(c, a) : prompt_run<T, DP, 4, false>(c, a);
+}
+
+template <typename T>
+int prompt_dim(xs_cache_context* c, const xs_prompt_attend_args& a) {
+  if (a.head_dim <= 64) return prompt_exact<T, 64>(c, a);
+  if (a.head_dim <= 96) return prompt_exact<T, 96>(c, a);
+  if (a.head_dim <= 128) return prompt_exact<T, 128>(c, a);
+  return prompt_exact<T, 256>(c, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int xs_qk_rotate(xs_cache_context* c, const xs_qk_rotate_args* in) {
+  const int rc = c ? xs_host_check_rotate(in) : XS_ERR_ARG;
+  if (rc) return rc;
+  if (in->tokens == 0 || in->q_heads + in->kv_heads == 0) return XS_OK;
+  const OnDevice on(c->device);
+  if (!on.ok) return XS_ERR_HIP;
+  if (in->dtype == XS_BF16) return rotate_dim<xst::Bf16>(c, *in);
+  return rotate_dim<xst::F16>(c, *in);
+}
+
+int xs_prompt_attend(xs_cache_context* c, const xs_prompt_attend_args* in) {
+  const int rc = c ? xs_host_check_prompt(in) : XS_ERR_ARG;
+  if (rc) return rc;
+  if (in->seqs == 0) return XS_OK;
+  const OnDevice on(c->device);
+  if (!on.ok) return XS_ERR_HIP;
+  if (in->tokens == 0) {
+    hipLaunchKernelGGL(xsp::prompt_status_kernel, dim3(1), dim3(64), 0, c->stream, *in);
+    return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
+  }
+  if (in->dtype == XS_BF16) return prompt_dim<xst::Bf16>(c, *in);
+  return prompt_dim<xst::F16>(c, *in);
+}
+
+}  // extern "C"
