@@ -611,7 +611,8 @@ int xs_qk_rotate(xs_cache_context* ctx, const xs_qk_rotate_args* args);
  * it holds.  A sequence may be empty.  One whose start lies below 0 or below an
  * earlier entry of start, or whose end lies below its start or past `tokens`,
  * gets XS_ROW_BAD_PARAM and nothing else; rows of no sequence are left as they
- * were. */
+ * were.  kv_token_stride is at most 2^24, a kv head's rows (tokens times its
+ * q heads) at most 2^30 (XS_ERR_CAPACITY). */
 typedef struct {
   int32_t dtype;         /* XS_BF16 or XS_F16: q, k, v and out */
   int32_t head_dim;      /* a multiple of 8, 8..256 */
@@ -688,7 +689,7 @@ int xs_cache_append8(xs_cache_context* ctx, const xs_cache_append8_args* args);
  * (fresh) are in the inputs' type.  Weights are rounded to bf16 where q is bf16;
  * where it is f16, to the sum of two bf16 (16 bits), since an element of the
  * cache may pass f16's range (and a mean of such elements f16's end: an
- * infinity then). */
+ * infinity then).  slot_stride is at most 2^25 (XS_ERR_CAPACITY). */
 typedef struct {
   int32_t dtype;         /* XS_BF16 or XS_F16: q, fresh and out */
   int32_t head_dim;      /* a multiple of 16, 16..256 */

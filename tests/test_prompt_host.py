@@ -155,6 +155,7 @@ def test_attend8_checks(host):
     assert chk(seqs=0, q=None) == OK and chk(seqs=9) == CAP and chk(q_heads=12) == E and chk(q_heads=48) == CAP and chk(kv_heads=16) == CAP
     assert chk(q=DEV + 8) == E and chk(out=DEV) == E and chk(q_node_stride=1020) == E and chk(out_head_stride=0) == E
     assert chk(cache=kv8(v=None)) == E and chk(cache=kv8(k_exp=None)) == E and chk(cache=kv8(slot_stride=8)) == E and chk(cache=kv8(exp_ld=1)) == E
+    assert chk(cache=kv8(slot_stride=(1 << 25) + 16)) == CAP and chk(cache=kv8(slot_stride=1 << 25)) == OK
     assert chk(cache=kv8(slot_stride=0)) == OK and chk(fresh=kv(v=DEV + 4)) == E and chk(fresh=kv(0)) == OK
 
 

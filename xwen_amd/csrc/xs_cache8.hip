@@ -13,6 +13,7 @@
 #include "xs_cache.h"
 #include "xs_device.h"
 #include "xs_host.h"
+#include "xs_rows32.h"
 
 namespace xs8 {
 
@@ -207,112 +208,168 @@ struct Tile {
   u32x4 q[N][RT][S::KC];
 };
 
-// The scores of 32 keys (parts kn of each), from the reference or from 0.
-template <typename T, int DP, int RT, int KN>
-XS_DEV void scores(const Tile<T, DP, RT>& z, int t, const u32x4 (&k)[KN][2][Shape<DP, RT>::KC], f32x4 start, f32x4 (&s)[2]) {
-  s[0] = s[1] = start;
+// The weights of a row tile from its scores, as parts.
+template <typename T, int DP, int RT>
+XS_DEV void weights8(Tile<T, DP, RT>& z, int t, const float (&x)[8], u32x4 (&pf)[Parts<T>::N][RT]) {
+  if constexpr (Parts<T>::N == 1) {
+    pf[0][t] = z.w.weights(t, x);
+  } else {
+    float p[8];
 #pragma unroll
-  for (int m = 0; m < KN; m++)
+    for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(x[e]);
+    z.w.l[t] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 #pragma unroll
-    for (int n = 0; n < Tile<T, DP, RT>::N; n++)
-#pragma unroll
-      for (int c = 0; c < Shape<DP, RT>::KC; c++) {
-        s[0] = mfma(Bf16{}, k[m][0][c], z.q[n][t][c], s[0]);
-        s[1] = mfma(Bf16{}, k[m][1][c], z.q[n][t][c], s[1]);
-      }
-}
-
-// The softmax and the second product of a block, keys and values as parts.
-template <typename T, int DP, int RT, bool MASKED, int KN>
-XS_DEV void block8(Tile<T, DP, RT>& z, const u32x4 (&k)[KN][2][Shape<DP, RT>::KC], const uint32_t (&v)[KN][8][Shape<DP, RT>::VH][Shape<DP, RT>::VE / 2],
-                   float scale, const uint32_t* on) {
-  constexpr int N = Tile<T, DP, RT>::N;
-  u32x4 pf[N][RT];
-#pragma unroll
-  for (int t = 0; t < RT; t++) {
-    f32x4 s[2];
-    scores<T, DP, RT, KN>(z, t, k, z.w.start(t), s);
-    float x[8];
-    const float top = z.w.template scaled<MASKED>(s, scale, MASKED ? on[t] : 0u, x);
-    if (__any(z.w.passes(t, top))) [[unlikely]] {
-      const bool far = __any(z.w.passes(t, top) && z.w.minus(z.w.c[t]) != 0.0f);
-      if (far) [[unlikely]] scores<T, DP, RT, KN>(z, t, k, (f32x4){0.0f, 0.0f, 0.0f, 0.0f}, s);
-      z.w.template rebase<MASKED>(t, s, far, scale, MASKED ? on[t] : 0u, x);
-    }
-    if constexpr (N == 1) {
-      pf[0][t] = z.w.weights(t, x);
-    } else {
-      float p[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(x[e]);
-      z.w.l[t] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        pf[0][t][i] = pack2(Bf16{}, p[2 * i], p[2 * i + 1]);
-        pf[1][t][i] = pack2(Bf16{}, p[2 * i] - Bf16::widen((uint16_t)pf[0][t][i]), p[2 * i + 1] - Bf16::widen((uint16_t)(pf[0][t][i] >> 16)));
-      }
+    for (int i = 0; i < 4; i++) {
+      pf[0][t][i] = pack2(Bf16{}, p[2 * i], p[2 * i + 1]);
+      pf[1][t][i] = pack2(Bf16{}, p[2 * i] - Bf16::widen((uint16_t)pf[0][t][i]), p[2 * i + 1] - Bf16::widen((uint16_t)(pf[0][t][i] >> 16)));
     }
   }
-#pragma unroll
-  for (int m = 0; m < KN; m++)
-#pragma unroll
-    for (int n = 0; n < N; n++) accumulate(z.w, v[m], pf[n]);
 }
 
-// A block of the cache: 32 slots, `limit` of them in use.
-template <typename T, int DP, int RT, bool EXACT, bool MASKED>
-XS_DEV void cache_block(Tile<T, DP, RT>& z, const uint8_t* kp, const uint8_t* vp, int64_t stride, int ke, int ve, int limit, int D, float scale,
-                        const uint32_t* on) {
+// The weights of 32 keys: keys(u, c, m) is part m of chunk c of 16 of them,
+// again(u, c, m) the same formed anew where references move.
+template <typename T, int DP, int RT, bool MASKED, int KN, typename Keys, typename Again>
+XS_DEV void softmax8(Tile<T, DP, RT>& z, float scale, const uint32_t* on, u32x4 (&pf)[Parts<T>::N][RT], Keys keys, Again again) {
   using S = Shape<DP, RT>;
-  const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
-  const float kscale = pow2(ke - 127), vscale = pow2(ve - 127);
-  u32x4 k8[2][S::KC / 2];
+  f32x4 s[RT][2];
 #pragma unroll
-  for (int t = 0; t < 2; t++) {
-    const int key = MASKED ? min(16 * t + x, limit - 1) : 16 * t + x;
+  for (int t = 0; t < RT; t++) s[t][0] = s[t][1] = z.w.start(t);
 #pragma unroll
-    for (int c = 0; c < S::KC / 2; c++) {
-      const int d = 64 * c + 16 * g;
-      k8[t][c] = EXACT || d < D ? *(const u32x4*)(kp + key * stride + d) : (u32x4){0, 0, 0, 0};
-    }
-  }
-  uint32_t v8[8][S::VH][S::VE / 4];
-#pragma unroll
-  for (int e = 0; e < 8; e++) {
-    const int slot = 4 * g + (e & 3) + 16 * (e >> 2), key = MASKED ? min(slot, limit - 1) : slot;
-#pragma unroll
-    for (int h = 0; h < S::VH; h++) {
-      int d = 128 * h + S::VE * x;
-      if (!EXACT) d = min(d, D - S::VE);  // (products of elements past the head's are never stored)
-      const uint8_t* p = vp + key * stride + d;
-      if constexpr (S::VE == 8) {
-        const u32x2 r = *(const u32x2*)p;
-        v8[e][h][0] = r[0];
-        v8[e][h][1] = r[1];
-      } else {
-        v8[e][h][0] = *(const uint32_t*)p;
-      }
-      if (MASKED && slot >= limit) {
-#pragma unroll
-        for (int i = 0; i < S::VE / 4; i++) v8[e][h][i] = 0;  // count for nothing, whatever they hold
-      }
-    }
-  }
-  u32x4 k[1][2][S::KC];
-#pragma unroll
-  for (int t = 0; t < 2; t++)
+  for (int m = 0; m < KN; m++)
 #pragma unroll
     for (int c = 0; c < S::KC; c++)
 #pragma unroll
-      for (int i = 0; i < 4; i++) k[0][t][c][i] = wide2(k8[t][c / 2][2 * (c % 2) + i / 2], kscale, i % 2);
-  uint32_t v[1][8][S::VH][S::VE / 2];
+      for (int u = 0; u < 2; u++) {
+        const u32x4 k = keys(u, c, m);
 #pragma unroll
-  for (int e = 0; e < 8; e++)
+        for (int t = 0; t < RT; t++)
 #pragma unroll
-    for (int h = 0; h < S::VH; h++)
+          for (int n = 0; n < Parts<T>::N; n++) s[t][u] = mfma(Bf16{}, k, z.q[n][t][c], s[t][u]);
+      }
 #pragma unroll
-      for (int i = 0; i < S::VE / 2; i++) v[0][e][h][i] = wide2(v8[e][h][i / 2], vscale, i % 2);
-  block8<T, DP, RT, MASKED, 1>(z, k, v, scale, on);
+  for (int t = 0; t < RT; t++) {
+    float x[8];
+    const float top = z.w.template scaled<MASKED>(s[t], scale, MASKED ? on[t] : 0u, x);
+    if (__any(z.w.passes(t, top))) [[unlikely]] {
+      const bool far = __any(z.w.passes(t, top) && z.w.minus(z.w.c[t]) != 0.0f);
+      if (far) [[unlikely]] {
+        s[t][0] = s[t][1] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int m = 0; m < KN; m++)
+#pragma unroll
+          for (int c = 0; c < S::KC; c++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+              const u32x4 k = again(u, c, m);
+#pragma unroll
+              for (int n = 0; n < Parts<T>::N; n++) s[t][u] = mfma(Bf16{}, k, z.q[n][t][c], s[t][u]);
+              __builtin_amdgcn_sched_barrier(0);  // (one chunk in registers at a time)
+            }
+      }
+      z.w.template rebase<MASKED>(t, s[t], far, scale, MASKED ? on[t] : 0u, x);
+    }
+    weights8<T, DP, RT>(z, t, x, pf);
+  }
+}
+
+// A block of the cache as it lies there, and the bytes of its exponents.
+template <int DP>
+struct Raw {
+  using S = Shape<DP, 1>;
+  u32x4 k[2][S::KC / 2];
+  uint32_t v[8][S::VH][S::VE / 4];
+  uint32_t ke, ve;
+};
+
+// Load block i; of the last, `limit` slots are in use.  Rows' bases are uniform,
+// so that a lane keeps two 32-bit offsets for all of them.
+template <int DP, bool EXACT, bool MASKED>
+XS_DEV void load_keys8(Raw<DP>& r, const xs_kv8& c8, int64_t at, int64_t eat, int i, int limit, int D) {
+  using S = Shape<DP, 1>;
+  const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
+  const uint32_t stride = (uint32_t)c8.slot_stride, ko = x * stride + 16 * g;
+  const uint8_t* kp = c8.k + at + (int64_t)i * KB * c8.slot_stride;
+  r.ke = c8.k_exp[eat + i];
+#pragma unroll
+  for (int u = 0; u < 2; u++)
+#pragma unroll
+    for (int c = 0; c < S::KC / 2; c++) {
+      const uint32_t off = MASKED ? min(16 * u + x, limit - 1) * stride + 16 * g : ko;
+      const uint8_t* p = kp + (MASKED ? 0 : (int64_t)(16 * u) * stride) + off + 64 * c;
+      r.k[u][c] = EXACT || 64 * c + 16 * g < D ? *(const u32x4*)p : (u32x4){0, 0, 0, 0};
+    }
+}
+template <int DP, bool EXACT, bool MASKED>
+XS_DEV void load_values8(Raw<DP>& r, const xs_kv8& c8, int64_t at, int64_t eat, int i, int limit, int D) {
+  using S = Shape<DP, 1>;
+  const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
+  const uint32_t stride = (uint32_t)c8.slot_stride, vo = 4 * g * stride + S::VE * x;
+  const uint8_t* vp = c8.v + at + (int64_t)i * KB * c8.slot_stride;
+  r.ve = c8.v_exp[eat + i];
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const int slot = 4 * g + (e & 3) + 16 * (e >> 2);
+#pragma unroll
+    for (int h = 0; h < S::VH; h++) {
+      const int d = EXACT ? 128 * h + S::VE * x : min(128 * h + S::VE * x, D - S::VE);  // (products of elements past the head's are never stored)
+      const uint8_t* p;
+      if constexpr (MASKED) p = vp + (uint32_t)(min(slot, limit - 1) * stride + d);
+      else if constexpr (EXACT) p = vp + (int64_t)((e & 3) + 16 * (e >> 2)) * stride + vo + 128 * h;
+      else p = vp + (int64_t)((e & 3) + 16 * (e >> 2)) * stride + (uint32_t)(4 * g * stride + d);
+      if constexpr (S::VE == 8) {
+        const u32x2 y = *(const u32x2*)p;
+        r.v[e][h][0] = y[0];
+        r.v[e][h][1] = y[1];
+      } else {
+        r.v[e][h][0] = *(const uint32_t*)p;
+      }
+      if (MASKED && slot >= limit) {
+#pragma unroll
+        for (int w = 0; w < S::VE / 4; w++) r.v[e][h][w] = 0;  // count for nothing, whatever they hold
+      }
+    }
+  }
+}
+
+// The weights of a block of the cache.
+template <typename T, int DP, int RT, bool MASKED>
+XS_DEV void cache_weights(Tile<T, DP, RT>& z, const Raw<DP>& r, float scale, const uint32_t* on, u32x4 (&pf)[Parts<T>::N][RT]) {
+  const float kscale = pow2((int)r.ke - 127);
+  auto widen = [](uint32_t a, uint32_t b, float s) { return (u32x4){wide2(a, s, false), wide2(a, s, true), wide2(b, s, false), wide2(b, s, true)}; };
+  softmax8<T, DP, RT, MASKED, 1>(
+      z, scale, on, pf, [&](int u, int c, int) { return widen(r.k[u][c / 2][2 * (c % 2)], r.k[u][c / 2][2 * (c % 2) + 1], kscale); },
+      [&](int u, int c, int) {
+        uint32_t a = r.k[u][c / 2][2 * (c % 2)], b = r.k[u][c / 2][2 * (c % 2) + 1];
+        asm volatile("" : "+v"(a), "+v"(b));  // (not the first products' operands, kept)
+        return widen(a, b, kscale);
+      });
+}
+
+// Its second product.
+template <typename T, int DP, int RT>
+XS_DEV void cache_product(Tile<T, DP, RT>& z, const Raw<DP>& r, const u32x4 (&pf)[Parts<T>::N][RT]) {
+  using S = Shape<DP, RT>;
+  const float vscale = pow2((int)r.ve - 127);
+#pragma unroll
+  for (int h = 0; h < S::VH; h++)
+#pragma unroll
+    for (int j = 0; j < S::VE; j += 2) {  // two fragments: element j and j + 1 of the lane's eight keys
+      uint32_t y[8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) y[e] = wide2(r.v[e][h][j / 4], vscale, j / 2 % 2);
+      u32x4 a[2];
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        a[0][i] = __builtin_amdgcn_perm(y[2 * i + 1], y[2 * i], 0x05040100u);
+        a[1][i] = __builtin_amdgcn_perm(y[2 * i + 1], y[2 * i], 0x07060302u);
+      }
+#pragma unroll
+      for (int w = 0; w < 2; w++)
+#pragma unroll
+        for (int t = 0; t < RT; t++)
+#pragma unroll
+          for (int n = 0; n < Parts<T>::N; n++) z.w.o[t][h * S::VE + j + w] = mfma(Bf16{}, a[w], pf[n][t], z.w.o[t][h * S::VE + j + w]);
+    }
 }
 
 // A block of the tree's own keys, in the inputs' type.
@@ -320,21 +377,16 @@ template <typename T, int DP, int RT, bool EXACT>
 XS_DEV void tree_block(Tile<T, DP, RT>& z, const uint16_t* kp, const uint16_t* vp, int64_t stride, int key0, int limit, int D, float scale,
                        const uint32_t* on) {
   using S = Shape<DP, RT>;
-  constexpr int N = Tile<T, DP, RT>::N;
+  constexpr int N = Parts<T>::N;
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
-  u32x4 k[N][2][S::KC];
-#pragma unroll
-  for (int t = 0; t < 2; t++) {
-    const int key = min(key0 + 16 * t + x, limit - 1);
-#pragma unroll
-    for (int c = 0; c < S::KC; c++) {
-      const int d = 64 * (c / 2) + 16 * g + 8 * (c % 2);
-      u32x4 y[N];
-      split8(T{}, EXACT || d < D ? *(const u32x4*)(kp + key * stride + d) : (u32x4){0, 0, 0, 0}, y);
-#pragma unroll
-      for (int n = 0; n < N; n++) k[n][t][c] = y[n];
-    }
-  }
+  u32x4 pf[N][RT];
+  auto keys = [&](int u, int c, int m) {
+    const int key = min(key0 + 16 * u + x, limit - 1), d = 64 * (c / 2) + 16 * g + 8 * (c % 2);
+    u32x4 y[N];
+    split8(T{}, EXACT || d < D ? *(const u32x4*)(kp + key * stride + d) : (u32x4){0, 0, 0, 0}, y);
+    return y[m];
+  };
+  softmax8<T, DP, RT, true, N>(z, scale, on, pf, keys, keys);
   uint32_t v[N][8][S::VH][S::VE / 2];
 #pragma unroll
   for (int e = 0; e < 8; e++) {
@@ -368,7 +420,10 @@ XS_DEV void tree_block(Tile<T, DP, RT>& z, const uint16_t* kp, const uint16_t* v
     }
   }
   z.w.odd = __any(z.w.odd);
-  block8<T, DP, RT, true, N>(z, k, v, scale, on);
+#pragma unroll
+  for (int m = 0; m < N; m++)
+#pragma unroll
+    for (int n = 0; n < N; n++) accumulate(z.w, v[m], pf[n]);
 }
 
 // Up to 16 RT rows a workgroup, whose waves split the keys and add up through
@@ -414,6 +469,26 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
   if (row0 >= R || first >= total) return;
 
   const int64_t at = b * c8.seq_stride + kh * c8.head_stride, eat = (int64_t)bh * c8.exp_ld;
+  int i = first + wave;
+  // whole blocks of the cache: a block's registers take the next one's keys once
+  // its scores are formed, and the next one's values after its second product
+  {
+    const int end = min(last, sq.len / KB);
+    Raw<DP> r;
+    if (i < end) {
+      load_keys8<DP, EXACT, false>(r, c8, at, eat, i, KB, a.head_dim);
+      load_values8<DP, EXACT, false>(r, c8, at, eat, i, KB, a.head_dim);
+    }
+#pragma unroll 1
+    for (; i < end; i += NW) {
+      u32x4 pf[Parts<T>::N][RT];
+      cache_weights<T, DP, RT, false>(z, r, cut.scale, nullptr, pf);
+      if (i + NW < end) load_keys8<DP, EXACT, false>(r, c8, at, eat, i + NW, KB, a.head_dim);
+      cache_product<T, DP, RT>(z, r, pf);
+      if (i + NW < end) load_values8<DP, EXACT, false>(r, c8, at, eat, i + NW, KB, a.head_dim);
+    }
+  }
+  // its last one, and the tree's
   const uint64_t sees = ancestors(parent, sq.n);
   uint64_t mine[RT];  // what the lane's rows see of the tree
 #pragma unroll
@@ -422,19 +497,19 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
     mine[t] = __shfl(sees, min(row / cut.G, 63));
     if (row >= R) mine[t] = 0;
   }
-  int i = first + wave;
-  for (; i < last && (i + 1) * KB <= sq.len; i += NW)
-    cache_block<T, DP, RT, EXACT, false>(z, c8.k + at + (int64_t)i * KB * c8.slot_stride, c8.v + at + (int64_t)i * KB * c8.slot_stride,
-                                         c8.slot_stride, c8.k_exp[eat + i], c8.v_exp[eat + i], KB, a.head_dim, cut.scale, nullptr);
 #pragma unroll 1
   for (; i < last; i += NW) {
     uint32_t on[RT];
     if (i < cached) {
       const int limit = sq.len - i * KB;
 #pragma unroll
-      for (int t = 0; t < RT; t++) on[t] = limit >= KB ? ~0u : (1u << limit) - 1u;
-      cache_block<T, DP, RT, EXACT, true>(z, c8.k + at + (int64_t)i * KB * c8.slot_stride, c8.v + at + (int64_t)i * KB * c8.slot_stride,
-                                          c8.slot_stride, c8.k_exp[eat + i], c8.v_exp[eat + i], limit, a.head_dim, cut.scale, on);
+      for (int t = 0; t < RT; t++) on[t] = (1u << limit) - 1u;
+      Raw<DP> r;
+      load_keys8<DP, EXACT, true>(r, c8, at, eat, i, limit, a.head_dim);
+      load_values8<DP, EXACT, true>(r, c8, at, eat, i, limit, a.head_dim);
+      u32x4 pf[Parts<T>::N][RT];
+      cache_weights<T, DP, RT, true>(z, r, cut.scale, on, pf);
+      cache_product<T, DP, RT>(z, r, pf);
     } else {
       const int key0 = (i - cached) * KB;
 #pragma unroll
@@ -505,6 +580,309 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
   }
 }
 
+// More rows than that: 32 a wave (xs_rows32.h), of keys that the workgroup's
+// threads turn into bf16 on their way to LDS, in stages of 64 through two
+// buffers: while one is read, the next is written from registers and the one
+// after it on its way from memory.  WK waves share 32 rows, each with its half of
+// a stage's keys, and add up at the end; 128 / WK rows a workgroup.
+template <int DP, int WK>
+struct Shape32 {
+  static constexpr int ROWS = 32 * NW / WK, WR = NW / WK;
+  static constexpr int DT = DP / 32, NF = 4 * DT;    // fragments of four elements a lane
+  static constexpr int STAT = WR * NF * 256;         // floats of a partial result: fragments,
+  static constexpr int ODD = STAT + 2 * ROWS;        // then m and l of each row,
+  static constexpr int PART = ODD + 4;               // then whether odd values are left out
+};
+
+struct Cut32 {
+  int32_t G, tiles, nsplit, chunk, groups;  // chunk: stages of a split
+  float scale;
+  float* part;
+};
+XS_DEV int stages_of(const Seq& sq) { return (sq.len + SK - 1) / SK + (sq.n > 0 ? 1 : 0); }
+
+// Fragment f (elements e .. e + 4 of row `row`, e = 8 f + 4 g) of the result.
+template <typename T>
+XS_DEV void store_four(const xs_tree_attend_args& a, int G, int b, int kh, int row, int R, int f, f32x4 o, float ref, float l, int odd, int n) {
+  const int g = (threadIdx.x & 63) >> 5, e = 8 * f + 4 * g;
+  const int node = min(row, R - 1) / G, head = kh * G + min(row, R - 1) % G;
+  if (odd) {  // (rare) the NaNs and infinities among the values of the nodes that the row sees, but of an empty row's
+    const uint64_t sees = __shfl(ancestors(parent_of(a, b), n), node);
+    const uint16_t* v = (const uint16_t*)a.fresh.v + b * a.fresh.seq_stride + kh * a.fresh.head_stride;
+#pragma unroll 1
+    for (int j = 0; j < n; j++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const uint16_t y = v[j * a.fresh.slot_stride + min(e + i, a.head_dim - 1)];
+        if (((sees >> j) & 1ull) && l != 0.0f && (y & 0x7FFFu) >= inf_of(T{})) o[i] += T::widen(y);
+      }
+  }
+  if (row >= R) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* out = (uint16_t*)a.out + b * a.out_seq_stride + node * a.out_node_stride + head * a.out_head_stride;
+  if (e < a.head_dim) *(u32x2*)(out + e) = (u32x2){pack2(T{}, o[0] * inv, o[1] * inv), pack2(T{}, o[2] * inv, o[3] * inv)};
+  if (a.lse && f == 0 && g == 0) a.lse[(b * a.nodes + node) * a.q_heads + head] = lse_of<E4m3>(a, ref, l);
+}
+
+template <typename T, int DP, int WK, bool EXACT>
+__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void attend8_wide_kernel(const xs_tree_attend_args a, const xs_kv8 c8, const Cut32 cut) {
+  using S = Shape32<DP, WK>;
+  using K = Keys<DP>;
+  constexpr int N = Parts<T>::N, CH = K::CH, KC = DP / 16, DT = DP / 32, TH = 64 * NW;
+  constexpr int PER = SK * (DP / 16) / TH;  // 16-byte pieces of the cache that a thread moves, of k and of v
+  __shared__ u32x4 lk[2][K::STAGE];
+  __shared__ u32x4 lv[2][K::STAGE];
+  __shared__ int odds;
+  const int lane = threadIdx.x & 63, x = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / WK, wk = wave % WK;
+  const int tile = (blockIdx.x >> 3) % cut.tiles;
+  const int group = ((blockIdx.x >> 3) / cut.tiles) * 8 + (blockIdx.x & 7);
+  if (group >= cut.groups) return;
+  const int bh = group / cut.nsplit, split = turned(group % cut.nsplit, bh, cut.nsplit);
+  const int kh = bh % (int)a.kv_heads, b = bh / (int)a.kv_heads;
+  const int parent = parent_of(a, b);
+  const Seq sq(a, b);
+  if (split == 0 && tile == 0 && kh == 0 && threadIdx.x == 0) a.seq_status[b] = sq.bad ? XS_ROW_BAD_PARAM : XS_ROW_OK;
+  if (sq.bad) return;
+  const int R = sq.n * cut.G, row = tile * S::ROWS + 32 * wr + x;
+  const int total = stages_of(sq), first = split * cut.chunk, last = min(first + cut.chunk, total);
+  if (tile * S::ROWS >= R || first >= total) return;
+
+  Rows32<Bf16, DP, N> w;
+  w.init();
+  {
+    const int node = min(row, R - 1) / cut.G, head = kh * cut.G + min(row, R - 1) % cut.G;
+    const uint16_t* p = (const uint16_t*)a.q + b * a.q_seq_stride + node * a.q_node_stride + head * a.q_head_stride;
+#pragma unroll
+    for (int c = 0; c < KC; c++) {
+      const int d = 16 * c + 8 * g;
+      u32x4 y[N];
+      split8(T{}, row < R && (EXACT || d < a.head_dim) ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0}, y);
+#pragma unroll
+      for (int n = 0; n < N; n++) w.q[n][c] = y[n];
+    }
+  }
+  const uint64_t seen = ancestors(parent, sq.n);
+  const uint64_t mine = __shfl(seen, min(row / cut.G, 63)) & (row < R ? ~0ull : 0ull);  // what the lane's row sees of the tree
+  const Reads<DP> reads;
+
+  // whole and part stages of the cache
+  const int end = min(last, (sq.len + SK - 1) / SK);
+  const int64_t at = b * c8.seq_stride + kh * c8.head_stride, eat = (int64_t)bh * c8.exp_ld;
+  const uint32_t stride = (uint32_t)c8.slot_stride;
+  u32x4 rk[PER], rv[PER];
+  uint32_t ek[PER], ev[PER];
+  auto fetch = [&](int s) {
+    const int64_t base = at + (int64_t)s * SK * c8.slot_stride;
+    const int most = sq.len - 1 - s * SK;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      const int p = j * TH + threadIdx.x, r = min(p / (DP / 16), most), c = p % (DP / 16);
+      const uint32_t off = (uint32_t)r * stride + 16 * c;
+      const bool in = EXACT || 16 * c < a.head_dim;
+      rk[j] = in ? *(const u32x4*)(c8.k + base + off) : (u32x4){0, 0, 0, 0};
+      rv[j] = in ? *(const u32x4*)(c8.v + base + off) : (u32x4){0, 0, 0, 0};
+      ek[j] = c8.k_exp[eat + s * (SK / KB) + r / KB];
+      ev[j] = c8.v_exp[eat + s * (SK / KB) + r / KB];
+    }
+  };
+  auto put = [&](int s) {
+    const int most = sq.len - 1 - s * SK;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      const int p = j * TH + threadIdx.x, r = p / (DP / 16), c = p % (DP / 16);
+      const float ks = pow2((int)ek[j] - 127), vs = pow2((int)ev[j] - 127);
+      const u32x4 y = r <= most ? rv[j] : (u32x4){0, 0, 0, 0};  // (past the length: nothing, whatever it holds)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        u32x4 k, v;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          k[i] = wide2(rk[j][2 * h + i / 2], ks, i % 2);
+          v[i] = wide2(y[2 * h + i / 2], vs, i % 2);
+        }
+        lk[s & 1][r * CH + ((2 * c + h) ^ K::turn_k(r))] = k;
+        lv[s & 1][r * CH + ((2 * c + h) ^ K::turn_v(r))] = v;
+      }
+    }
+  };
+  auto step = [&](const u32x4* ks, const u32x4* vs, bool masked, uint64_t on) {
+    // (f16: a tile at a time, which the registers hold beside two parts of each row)
+    constexpr int U = N == 1 && WK == 1 ? 2 : 1, STEPS = 2 / (U * WK);
+#pragma unroll
+    for (int i = 0; i < STEPS; i++) {
+      const int u = WK == 1 ? i : wk;
+      const uint64_t bits = on >> (32 * u + 4 * g);
+      w.template step<U, 1>(reads, {ks + 32 * u * CH}, {vs + 32 * u * CH}, cut.scale, masked, Bits{(uint32_t)bits, (uint32_t)(bits >> 32)});
+    }
+  };
+  if (first < end) {
+    fetch(first);
+    put(first);
+    if (first + 1 < end) fetch(first + 1);
+  }
+#pragma unroll 1
+  for (int s = first; s < end; s++) {
+    __syncthreads();
+    if (s + 1 < end) put(s + 1);
+    if (s + 2 < end) fetch(s + 2);
+    const int limit = sq.len - s * SK;
+    step(lk[s & 1], lv[s & 1], limit < SK, limit < SK ? (1ull << limit) - 1ull : ~0ull);
+  }
+  // the tree: parts in a buffer each
+  int odd = 0;
+  if (last == total) {
+    if (threadIdx.x == 0) odds = 0;
+    __syncthreads();
+    const int64_t f = b * a.fresh.seq_stride + kh * a.fresh.head_stride;
+#pragma unroll 1
+    for (int p = threadIdx.x; p < K::STAGE; p += TH) {
+      const int r = p / CH, c = p % CH;
+      u32x4 k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+      if (r < sq.n && (EXACT || 8 * c < a.head_dim)) {
+        k = *(const u32x4*)((const uint16_t*)a.fresh.k + f + r * a.fresh.slot_stride + 8 * c);
+        v = *(const u32x4*)((const uint16_t*)a.fresh.v + f + r * a.fresh.slot_stride + 8 * c);
+      }
+      // What is not finite would, through the product, reach the rows that do not
+      // see the node: taken out here, added by store_four to the rows that do.
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        if ((v[i] & 0x7FFFu) >= inf_of(T{})) v[i] &= 0xFFFF0000u, odds = 1;
+        if (((v[i] >> 16) & 0x7FFFu) >= inf_of(T{})) v[i] &= 0xFFFFu, odds = 1;
+      }
+      u32x4 ks[N], vs[N];
+      split8(T{}, k, ks);
+      split8(T{}, v, vs);
+#pragma unroll
+      for (int n = 0; n < N; n++) {
+        lk[n][r * CH + (c ^ K::turn_k(r))] = ks[n];
+        lv[n][r * CH + (c ^ K::turn_v(r))] = vs[n];
+      }
+    }
+    __syncthreads();
+    odd = odds;
+#pragma unroll 1
+    for (int i = 0; i < 2 / WK; i++) {
+      const int u = WK == 1 ? i : wk;
+      const uint64_t bits = mine >> (32 * u + 4 * g);
+      const Bits on = {(uint32_t)bits, (uint32_t)(bits >> 32)};
+      if (32 * u >= sq.n) continue;
+      if constexpr (N == 1) w.template step<1, 1>(reads, {lk[0] + 32 * u * CH}, {lv[0] + 32 * u * CH}, cut.scale, true, on);
+      else w.template step<1, 2>(reads, {lk[0] + 32 * u * CH, lk[1] + 32 * u * CH}, {lv[0] + 32 * u * CH, lv[1] + 32 * u * CH}, cut.scale, true, on);
+    }
+  }
+
+  // rows that see nothing of the tree see nothing of the cache either
+  float l = mine == 0 ? 0.0f : pair_sum(w.l);
+  float ref = l == 0.0f ? NEG_INF : cut.scale < 0.0f ? -w.reference() : w.reference();
+  if (l == 0.0f) {
+#pragma unroll
+    for (int d = 0; d < DT; d++) w.o[d] = fill16(0.0f);
+  }
+  if constexpr (WK == 2) {
+    __syncthreads();  // (the stages' last readers)
+    f32x4* sum = (f32x4*)&lk[0][0] + wr * S::NF * 64;
+    float* stat = (float*)&lv[0][0] + wr * 64;
+    if (wk == 1) {
+#pragma unroll
+      for (int f = 0; f < S::NF; f++) {
+        const f32x16 o = w.o[f / 4];
+        sum[f * 64 + lane] = (f32x4){o[4 * (f % 4)], o[4 * (f % 4) + 1], o[4 * (f % 4) + 2], o[4 * (f % 4) + 3]};
+      }
+      if (g == 0) {
+        stat[x] = ref;
+        stat[32 + x] = l;
+      }
+    }
+    __syncthreads();
+    if (wk == 1) return;
+    const float ref1 = stat[x], l1 = stat[32 + x], top = fmaxf(ref, ref1), mag = fabsf(cut.scale);
+    const float f0 = ref == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((ref - top) * mag);
+    const float f1 = ref1 == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((ref1 - top) * mag);
+    l = (ref == NEG_INF ? 0.0f : l * f0) + (ref1 == NEG_INF ? 0.0f : l1 * f1);
+    ref = top;
+#pragma unroll
+    for (int f = 0; f < S::NF; f++) {
+      const f32x4 y = sum[f * 64 + lane];
+#pragma unroll
+      for (int i = 0; i < 4; i++) w.o[f / 4][4 * (f % 4) + i] = __builtin_fmaf(w.o[f / 4][4 * (f % 4) + i], f0, y[i] * f1);
+    }
+  }
+  const bool whole = first == 0 && last == total;
+  float* part = cut.part + (((int64_t)bh * cut.nsplit + split) * cut.tiles + tile) * S::PART;
+#pragma unroll
+  for (int f = 0; f < S::NF; f++) {
+    const f32x16 o = w.o[f / 4];
+    const f32x4 y = {o[4 * (f % 4)], o[4 * (f % 4) + 1], o[4 * (f % 4) + 2], o[4 * (f % 4) + 3]};
+    if (whole) store_four<T>(a, cut.G, b, kh, row, R, f, y, ref, l, odd, sq.n);
+    else ((f32x4*)part)[(wr * S::NF + f) * 64 + lane] = y;
+  }
+  if (!whole && g == 0) {
+    part[S::STAT + 32 * wr + x] = ref;
+    part[S::STAT + S::ROWS + 32 * wr + x] = l;
+    if (wr == 0) part[S::ODD] = odd ? 1.0f : 0.0f;
+  }
+}
+
+// Joins the splits of 32 rows, four fragments a workgroup: each wave one of them
+// over one of SHARES shares of the splits.
+constexpr int join32_threads(bool few) { return few ? 256 : 1024; }
+
+template <typename T, int DP, int WK, bool FEWER>
+__global__ __launch_bounds__(join32_threads(FEWER)) void join32_kernel(const xs_tree_attend_args a, const Cut32 cut) {
+  using S = Shape32<DP, WK>;
+  constexpr int SHARES = FEWER ? 1 : 4, WAVES = 4 * SHARES, MOST = FEWER ? FEW : SPLITS;
+  __shared__ float weight[MOST][32];
+  __shared__ float stat[2][2 * WAVES][32];
+  __shared__ int odd;
+  __shared__ f32x4 sum[SHARES][4][64];
+  const int lane = threadIdx.x & 63, x = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), share = wave / 4;
+  const int f = blockIdx.x % S::DT * 4 + wave % 4, wr = blockIdx.x / S::DT % S::WR, tile = blockIdx.x / (S::DT * S::WR) % cut.tiles;
+  const int bh = blockIdx.x / (S::DT * S::WR * cut.tiles), kh = bh % (int)a.kv_heads, b = bh / (int)a.kv_heads;
+  const Seq sq(a, b);
+  const int R = sq.n * cut.G, row = tile * S::ROWS + 32 * wr + x;
+  const int n = (stages_of(sq) + cut.chunk - 1) / cut.chunk;
+  if (sq.bad || tile * S::ROWS + 32 * wr >= R || n <= 1) return;
+  if (threadIdx.x == 0) odd = 0;
+  __syncthreads();
+  const float* part = cut.part + ((int64_t)bh * cut.nsplit * cut.tiles + tile) * S::PART;
+  const int64_t step = (int64_t)cut.tiles * S::PART;
+  // half a wave takes a split's rows
+  float top = NEG_INF, all = 0.0f;
+  for (int s = 2 * wave + g; s < n; s += 2 * WAVES) {
+    const float* p = part + s * step;
+    top = fmaxf(top, p[S::STAT + 32 * wr + x]);
+    if (p[S::ODD] != 0.0f) odd = 1;  // (any of them)
+  }
+  stat[0][2 * wave + g][x] = top;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 2 * WAVES; j++) top = fmaxf(top, stat[0][j][x]);
+  for (int s = 2 * wave + g; s < n; s += 2 * WAVES) {
+    const float* p = part + s * step + S::STAT + 32 * wr + x;
+    const float m = p[0], y = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((m - top) * fabsf(cut.scale));
+    if (m != NEG_INF) all += p[S::ROWS] * y;
+    weight[s][x] = y;
+  }
+  stat[1][2 * wave + g][x] = all;
+  __syncthreads();
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+  for (int s = share; s < n; s += SHARES) o += ((const f32x4*)(part + s * step))[(wr * S::NF + f) * 64 + lane] * weight[s][x];
+  all = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 2 * WAVES; j++) all += stat[1][j][x];
+  if constexpr (SHARES > 1) {
+    sum[share][wave % 4][lane] = o;
+    __syncthreads();
+    if (share != 0) return;
+#pragma unroll
+    for (int j = 1; j < SHARES; j++) o += sum[j][wave % 4][lane];
+  }
+  store_four<T>(a, cut.G, b, kh, row, R, f, o, top, all, odd, sq.n);
+}
+
 }  // namespace xs8
 
 // ---------------------------------------------------------------------------
@@ -546,6 +924,41 @@ int attend8_run(xs_cache_context* c, const xs_tree_attend_args& a, const xs_kv8&
   return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
 }
 
+template <typename T, int DP, int WK, bool EXACT>
+int attend8_wide_run(xs_cache_context* c, const xs_tree_attend_args& a, const xs_kv8& c8) {
+  using S = xs8::Shape32<DP, WK>;
+  xs8::Cut32 cut;
+  cut.G = (int32_t)(a.q_heads / a.kv_heads);
+  cut.tiles = (int32_t)((a.nodes * cut.G + S::ROWS - 1) / S::ROWS);
+  cut.scale = a.scale * xst::LOG2E;
+  cut.part = c->part;
+  const int64_t limit = a.max_len ? a.max_len : a.capacity, stages = (limit + xst::SK - 1) / xst::SK + 1;
+  const int64_t units = a.seqs * a.kv_heads * cut.tiles;
+  // the device filled once, by as many workgroups as its LDS holds, as far as
+  // the context has room for their partial results
+  const int64_t most = std::min<int64_t>(c->n_cu * (DP <= 128 ? 2 : 1), c->part_floats / S::PART);
+  const int64_t nsplit = std::max<int64_t>(1, std::min<int64_t>(xst::SPLITS, most / units));
+  cut.chunk = (int32_t)std::max<int64_t>((stages + nsplit - 1) / nsplit, 4);
+  cut.nsplit = (int32_t)((stages + cut.chunk - 1) / cut.chunk);
+  if (cut.nsplit > most / units) cut.nsplit = 1, cut.chunk = (int32_t)stages;  // (not worth a join, or no room)
+  const int64_t groups = a.seqs * a.kv_heads * cut.nsplit;
+  const int64_t grid = (groups + 7) / 8 * 8 * cut.tiles, join = a.seqs * a.kv_heads * cut.tiles * S::WR * S::DT;
+  const bool few = cut.nsplit <= xst::FEW;
+  if (!xs_host_launch_fits(grid, 64 * xst::NW) || (cut.nsplit > 1 && !xs_host_launch_fits(join, xs8::join32_threads(few)))) return XS_ERR_CAPACITY;
+  cut.groups = (int32_t)groups;
+  hipLaunchKernelGGL((xs8::attend8_wide_kernel<T, DP, WK, EXACT>), dim3((unsigned)grid), dim3(64 * xst::NW), 0, c->stream, a, c8, cut);
+  if (cut.nsplit > 1 && few)
+    hipLaunchKernelGGL((xs8::join32_kernel<T, DP, WK, true>), dim3((unsigned)join), dim3(xs8::join32_threads(true)), 0, c->stream, a, cut);
+  else if (cut.nsplit > 1)
+    hipLaunchKernelGGL((xs8::join32_kernel<T, DP, WK, false>), dim3((unsigned)join), dim3(xs8::join32_threads(false)), 0, c->stream, a, cut);
+  return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
+}
+
+template <typename T, int DP, int WK>
+int attend8_wide(xs_cache_context* c, const xs_tree_attend_args& a, const xs_kv8& c8) {
+  return a.head_dim == DP ? attend8_wide_run<T, DP, WK, true>(c, a, c8) : attend8_wide_run<T, DP, WK, false>(c, a, c8);
+}
+
 template <typename T, int DP, int RT>
 int attend8_exact(xs_cache_context* c, const xs_tree_attend_args& a, const xs_kv8& c8) {
   return a.head_dim == DP ? attend8_run<T, DP, RT, true>(c, a, c8) : attend8_run<T, DP, RT, false>(c, a, c8);
@@ -555,10 +968,9 @@ template <typename T, int DP>
 int attend8_rows(xs_cache_context* c, const xs_tree_attend_args& a, const xs_kv8& c8) {
   const int64_t rows = a.nodes * (a.q_heads / a.kv_heads);
   if (rows <= 16) return attend8_exact<T, DP, 1>(c, a, c8);
-  if constexpr (DP <= 128) {
-    if (rows > 32) return attend8_exact<T, DP, 4>(c, a, c8);
-  }
-  return attend8_exact<T, DP, 2>(c, a, c8);
+  if (rows <= 32) return attend8_exact<T, DP, 2>(c, a, c8);
+  if (rows <= 64) return attend8_wide<T, DP, 2>(c, a, c8);
+  return attend8_wide<T, DP, 1>(c, a, c8);
 }
 
 template <typename T>

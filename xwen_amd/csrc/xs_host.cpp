@@ -302,6 +302,8 @@ int xs_host_check_attend8(const xs_cache_dims* dims, const xs_tree_attend8_args*
   if (rc == XS_OK) rc = check_queries(dims, in->nodes, in->q_heads, in->kv_heads);
   if (rc == XS_OK && in->head_dim % 16) return XS_ERR_ARG;
   if (rc != XS_OK || in->seqs == 0) return rc;
+  // the bytes that 64 slots span are counted in 32 bits
+  if (in->cache.slot_stride > (1 << 25)) return XS_ERR_CAPACITY;
   if (!in->len || !in->parent || !in->seq_status || !in->q || !in->out || in->q == in->out) return XS_ERR_ARG;
   if (!aligned16(in->q) || !aligned16(in->out) ||
       !kv8_ok(in->cache, in->seqs, in->capacity, in->kv_heads, in->head_dim, false) ||

@@ -13,6 +13,7 @@
 #include "xs_cache.h"
 #include "xs_device.h"
 #include "xs_host.h"
+#include "xs_rows32.h"
 
 namespace xsp {
 
@@ -151,53 +152,9 @@ __global__ __launch_bounds__(RT) void rotate_kernel(const xs_qk_rotate_args a) {
 //
 // The rows of one (sequence, kv head) are its tokens times the group of q heads
 // that share the head: row r = token * group + q head.  A workgroup takes 32 NWV
-// rows, 32 a wave, and walks the keys up to its last row's token in stages of 64,
-// through two LDS buffers that loads fill while the other is read.  With
-// v_mfma_f32_32x32x16 (lane = 32 g + x; A[m = x][k = 8 g + e], B[k = 8 g + e][n = x],
-// C[m = 8 (r / 4) + 4 g + r % 4][n = x]):
-//
-//   S^T = K Q^T   a lane holds scores of one row (n = x), of 16 of every 32 keys
-//   O^T = V^T P^T the contraction runs over the keys in the order in which the
-//                 lane holds them (position 8 g + e of 16 is key 8 (e / 4) + 4 g +
-//                 e % 4), so the weights go to B as they are; V's fragments come
-//                 through transposing LDS reads, four keys of a column each
-//
-// The softmax is that of xs_attend.h: one pass, a running reference which is one
-// of the row's own scores, products that start from it, moved only when the best
-// has grown by 2^8.
+// rows, 32 a wave (xs_rows32.h), and walks the keys up to its last row's token in
+// stages of 64, through two LDS buffers that loads fill while the other is read.
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
-XS_DEV f32x16 mfma32(Bf16, u32x4 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-XS_DEV f32x16 mfma32(F16, u32x4 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-XS_DEV f32x16 fill16(float v) { return (f32x16){v, v, v, v, v, v, v, v, v, v, v, v, v, v, v, v}; }
-
-// Over the two lanes of a row.
-XS_DEV float pair_max(float v) {
-  const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
-  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-}
-XS_DEV float pair_sum(float v) {
-  const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
-  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
-}
-
-constexpr int SK = 64;  // keys of a stage
-
-// A stage in LDS: rows of CH 16-byte chunks.  Chunk c of a row lies at c ^ turn,
-// so that rows read together meet all banks: 16 rows' chunk of K (16 bytes each),
-// four rows' 64 bytes of V.
-template <int DP>
-struct Keys {
-  static constexpr int CH = DP / 8;
-  XS_DEV static int turn_k(int row) { return CH % 16 == 0 ? row & 15 : CH % 8 == 0 ? row >> 1 & 7 : row >> 2 & 3; }
-  XS_DEV static int turn_v(int row) { return CH % 16 == 0 ? (row & 3) << 2 : CH % 8 == 0 ? (row >> 1 & 1) << 2 : 0; }
-};
 // The sequence and the row tile of a workgroup: tiles of the device's valid
 // sequences, those with the most keys first, sequences of more than 64 in order.
 struct Place {
@@ -290,8 +247,7 @@ XS_DEV void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 template <typename T, int DP, int NWV, bool EXACT>
 __global__ __launch_bounds__(64 * NWV, DP <= 128 ? 2 : 1) void prompt_kernel(const xs_prompt_attend_args a, float scale) {
   using K = Keys<DP>;
-  constexpr int KC = DP / 16, DT = DP / 32, ROWS = 32 * NWV, CH = K::CH;
-  constexpr int STAGE = SK * CH;                      // chunks of a stage, of k and of v
+  constexpr int KC = DP / 16, DT = DP / 32, ROWS = 32 * NWV, CH = K::CH, STAGE = K::STAGE;
   constexpr int PER = STAGE / (64 * NWV);             // of a thread
   static_assert(STAGE % (64 * NWV) == 0, "a stage is whole chunks of every thread");
   __shared__ u32x4 lds[2][2][STAGE];                  // [buffer][k, v]
@@ -313,13 +269,14 @@ __global__ __launch_bounds__(64 * NWV, DP <= 128 ? 2 : 1) void prompt_kernel(con
   const int stages = (end + SK - 1) / SK;
   const bool live = wrow < R;
 
-  u32x4 q[KC];
+  Rows32<T, DP, 1> w;
+  w.init();
   {
     const uint16_t* p = (const uint16_t*)a.q + (int64_t)(t0 + token) * a.q_token_stride + head * a.q_head_stride;
 #pragma unroll
     for (int c = 0; c < KC; c++) {
       const int d = 16 * c + 8 * g;
-      q[c] = row < R && (EXACT || d < a.head_dim) ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0};
+      w.q[0][c] = row < R && (EXACT || d < a.head_dim) ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0};
     }
   }
   // A stage's chunks, each by the lane whose place in LDS it takes.  Chunks past
@@ -345,27 +302,9 @@ __global__ __launch_bounds__(64 * NWV, DP <= 128 ? 2 : 1) void prompt_kernel(con
     }
   };
 
-  constexpr float OFF = offset_of(T{});
-  f32x16 o[DT], base = fill16(0.0f);  // base: minus the reference, which the products start from
-#pragma unroll
-  for (int d = 0; d < DT; d++) o[d] = fill16(0.0f);
-  float most = __builtin_nanf(""), l = 0.0f;
+  const Reads<DP> reads;
   int odd = 0;
   if (threadIdx.x == 0) odds = 0;
-
-  // Byte offsets of the lane's reads within a stage: K's chunk 2 c + g of row x
-  // (of 32 u + x: 32 rows on), V's columns 32 d + 16 q4 + 4 (i % 4) of row 4 g + i / 4.
-  const int i16 = lane & 15, vr = 4 * g + (i16 >> 2);
-  auto key = [&](int u, int c, int kb) {
-    int c16;  // 16 (c's chunk ^ the row's turn), kb holding g's and the turn
-    if constexpr (CH % 16 == 0) c16 = (kb ^ (32 * (c % 8))) + 256 * (c / 8);
-    else if constexpr (CH % 8 == 0) c16 = kb ^ (32 * c);
-    else c16 = (kb ^ (32 * (c % 2))) + 64 * (c / 2);
-    return c16 + 32 * u * CH * 16;
-  };
-  // kb's row part has to keep clear of the bits that c turns
-  const int krow = x * CH * 16, kturn = 16 * (g ^ K::turn_k(x));
-  const int vrow = vr * CH * 16 + 8 * (i16 & 1), vcol = 16 * ((2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1)) ^ K::turn_v(vr));
 
   fetch(0);
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the rows' loads too, which the loop would wait for at every stage
@@ -402,103 +341,13 @@ __global__ __launch_bounds__(64 * NWV, DP <= 128 ? 2 : 1) void prompt_kernel(con
       }
     }
     if (live && s * SK <= top_token) {
-      const char* ks = (const char*)&lds[s & 1][0][0] + krow;
-      const char* vs = (const char*)&lds[s & 1][1][0] + vrow;
-      int kb = kturn, vb = vcol;
-      asm volatile("" : "+v"(kb), "+v"(vb));  // (its sums with constants are formed where they are used)
-      f32x16 sc[2] = {base, base};
-#pragma unroll
-      for (int c = 0; c < KC; c++)
-#pragma unroll
-        for (int u = 0; u < 2; u++) sc[u] = mfma32(T{}, *(const u32x4*)(ks + key(u, c, kb)), q[c], sc[u]);
-      float xs[2][16], top = NEG_INF;
-      const bool masked = s * SK + SK - 1 > low;
-      const int lim = token - s * SK - 4 * g;  // the lane's key 32 u + 8 (r / 4) + r % 4 counts up to here
-      auto weigh = [&](bool from0, float ref) {
-        top = NEG_INF;
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) {
-            const float v = from0 ? sc[u][r] - ref : sc[u][r];
-            xs[u][r] = OFF == 0.0f ? v * scale : __builtin_fmaf(v, scale, OFF);
-          }
-        if (masked) {
-#pragma unroll
-          for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) xs[u][r] = 32 * u + 8 * (r / 4) + r % 4 <= lim ? xs[u][r] : NEG_INF;
-        }
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) top = fmaxf(top, xs[u][r]);
-      };
-      weigh(false, 0.0f);
-      if (__any(!(top <= most))) [[unlikely]] {
-        // the references of the rows that have grown move to their best scores
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-          sc[u] = fill16(0.0f);
-#pragma unroll
-          for (int c = 0; c < KC; c++) sc[u] = mfma32(T{}, *(const u32x4*)(ks + key(u, c, kb)), q[c], sc[u]);
-        }
-        const float sign = scale < 0.0f ? -1.0f : 1.0f, old = -base[0];
-        const bool unset = most != most;
-        float best = unset ? NEG_INF : old * sign;
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) {
-            const float y = sc[u][r] * sign;
-            best = fmaxf(best, !masked || 32 * u + 8 * (r / 4) + r % 4 <= lim ? y : NEG_INF);
-          }
-        best = pair_max(best);
-        float ref = old;
-        if (best > NEG_INF) {
-          ref = scale == 0.0f ? 0.0f : best * sign;
-          const float keep = unset ? 0.0f : __builtin_amdgcn_exp2f((old - ref) * scale);
-          base = fill16(-ref);
-          most = LAZY + OFF;
-          l *= keep;
-#pragma unroll
-          for (int d = 0; d < DT; d++) o[d] *= keep;
-        }
-        weigh(true, ref);
-      }
-      u32x4 pf[2][2];
-#pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int c = 0; c < 2; c++) {
-          float p[8];
-#pragma unroll
-          for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(xs[u][8 * c + e]);
-          l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-#pragma unroll
-          for (int e = 0; e < 4; e++) pf[u][c][e] = pack2(T{}, p[2 * e], p[2 * e + 1]);
-        }
-#pragma unroll
-      for (int d = 0; d < DT; d++) {
-        const char* vd = vs + (CH % 16 == 0 ? (vb ^ (64 * (d % 4))) + 256 * (d / 4) : CH % 8 == 0 ? vb ^ (64 * d) : vb + 64 * d);
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-          for (int c = 0; c < 2; c++) {
-            s16x4 v[2];
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-              v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(vd + (32 * u + 16 * c + 8 * h) * CH * 16));
-            const u32x2 v0 = __builtin_bit_cast(u32x2, v[0]), v1 = __builtin_bit_cast(u32x2, v[1]);
-            o[d] = mfma32(T{}, (u32x4){v0[0], v0[1], v1[0], v1[1]}, pf[u][c], o[d]);
-          }
-      }
+      w.template step<2, 1>(reads, {lds[s & 1][0]}, {lds[s & 1][1]}, scale, s * SK + SK - 1 > low, Upto{token - s * SK - 4 * g});
     }
   }
 
   if (row >= R) return;
-  l = pair_sum(l);
-  const float ref = -base[0];
+  const float l = pair_sum(w.l);
+  f32x16(&o)[DT] = w.o;
   if (l == 0.0f) {  // every score -inf
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = fill16(0.0f);
@@ -528,7 +377,7 @@ __global__ __launch_bounds__(64 * NWV, DP <= 128 ? 2 : 1) void prompt_kernel(con
     }
   if (a.lse && g == 0)
     a.lse[(int64_t)(t0 + token) * a.q_heads + head] =
-        l == 0.0f ? NEG_INF : __builtin_fmaf(ref, a.scale, LN2 * (__builtin_amdgcn_logf(l) - OFF));
+        l == 0.0f ? NEG_INF : __builtin_fmaf(w.reference(), a.scale, LN2 * (__builtin_amdgcn_logf(l) - offset_of(T{})));
 }
 
 // No token: only the sequences' statuses.
