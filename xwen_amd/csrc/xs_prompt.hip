@@ -24,12 +24,16 @@ using namespace xst;
 //
 // A head of a token is LPH lanes (a power of two, head_dim / 16 at least) of 16
 // elements each: two 16-byte pieces, which for halves are those of a rotated
-// pair, so that no element crosses lanes.  A workgroup takes `span` heads in a
-// row (tokens outermost, a token's q heads before its kv heads); the angles of
-// its tokens are computed once, into LDS.  Bound by the one read and write of
-// the heads.
+// pair, so that no element crosses lanes.  A workgroup takes `passes` passes of
+// RT / LPH heads in a row (tokens outermost, a token's q heads before its kv
+// heads), a pass's pieces on their way while the last one is worked on; the
+// angles of its tokens, and the weights, are in LDS.  Bound by the one read and
+// write of the heads: 16,384 tokens of 40 heads of 128 (336 MB) in 80 us.
+// All passes' pieces in registers at once take 204 of them, which leaves two
+// waves a SIMD: 186 us.
 
 constexpr int RT = 256;  // threads of a workgroup
+constexpr int ROT_PASSES = 8;
 
 template <typename T>
 XS_DEV void widen8(u32x4 r, float (&x)[8]) {
@@ -40,14 +44,15 @@ XS_DEV void widen8(u32x4 r, float (&x)[8]) {
   }
 }
 
-template <typename T, int LPH, int ITER>
-__global__ __launch_bounds__(RT) void rotate_kernel(const xs_qk_rotate_args a) {
-  extern __shared__ f32x2 turn[];  // [tokens of the workgroup][rot_dim / 2] cos, sin
-  constexpr int PER = RT / LPH;    // heads of a pass
+template <typename T, int LPH>
+__global__ __launch_bounds__(RT, 8) void rotate_kernel(const xs_qk_rotate_args a, int passes) {
+  extern __shared__ float shared[];  // [q, k][head_dim] weights; [tokens of the workgroup][rot_dim / 2] cos, sin
+  constexpr int PER = RT / LPH;      // heads of a pass
   const int heads = (int)(a.q_heads + a.kv_heads), D = a.head_dim, half = a.rot_dim / 2;
-  const bool halves = a.pairs == XS_ROT_HALVES;
+  const bool halves = a.pairs == XS_ROT_HALVES, norm = a.q_weight || a.k_weight;
+  f32x2* turn = (f32x2*)(shared + 2 * D);
   const int p = threadIdx.x % LPH;
-  const int64_t first = (int64_t)blockIdx.x * (PER * ITER), all = a.tokens * heads;
+  const int64_t first = (int64_t)blockIdx.x * PER * passes, all = a.tokens * heads;
   const int64_t t0 = first / heads;
 
   // the lane's two pieces
@@ -55,61 +60,76 @@ __global__ __launch_bounds__(RT) void rotate_kernel(const xs_qk_rotate_args a) {
   const int c0 = p < rc ? p : 2 * p, c1 = p < rc ? p + rc : 2 * p + 1;
   const bool in0 = c0 < chunks, in1 = c1 < chunks;
 
-  u32x4 raw[ITER][2];
-#pragma unroll
-  for (int i = 0; i < ITER; i++) {
-    const int64_t at = first + i * PER + threadIdx.x / LPH;
-    raw[i][0] = raw[i][1] = (u32x4){0, 0, 0, 0};
-    if (at < all) {
-      const int64_t t = t0 + (int)(at - t0 * heads) / heads;
-      const int h = (int)(at - t * heads);
-      const uint16_t* x = h < a.q_heads ? (const uint16_t*)a.q + t * a.q_token_stride + h * a.q_head_stride
-                                        : (const uint16_t*)a.k + t * a.k_token_stride + (h - a.q_heads) * a.k_head_stride;
-      if (in0) raw[i][0] = *(const u32x4*)(x + 8 * c0);
-      if (in1) raw[i][1] = *(const u32x4*)(x + 8 * c1);
-    }
-  }
+  // the lane's head of the first pass; a pass on is `over` tokens and `by` heads
+  int64_t at = first + threadIdx.x / LPH;
+  int t = (int)(at - t0 * heads) / heads, h = (int)(at - t0 * heads) - t * heads;  // (t counted from t0)
+  const int over = PER / heads, by = PER % heads;
 
+  auto fetch = [&](u32x4 (&raw)[2]) {
+    raw[0] = raw[1] = (u32x4){0, 0, 0, 0};
+    if (at >= all) return;
+    const uint16_t* x = h < a.q_heads ? (const uint16_t*)a.q + (t0 + t) * a.q_token_stride + h * a.q_head_stride
+                                      : (const uint16_t*)a.k + (t0 + t) * a.k_token_stride + (h - a.q_heads) * a.k_head_stride;
+    if (in0) raw[0] = *(const u32x4*)(x + 8 * c0);
+    if (in1) raw[1] = *(const u32x4*)(x + 8 * c1);
+  };
+  u32x4 raw[2];
+  fetch(raw);
+
+  if (norm)
+    for (int i = threadIdx.x; i < 2 * D; i += RT) {
+      const float* w = i < D ? a.q_weight : a.k_weight;
+      shared[i] = w ? w[i < D ? i : i - D] : 0.0f;
+    }
   if (half > 0) {
     // The angle in turns, from f64 (a position of 2^31 times a frequency of 1
     // leaves 2^-23 of a turn); cos and sin of its fraction in f32.
-    const int64_t last = min(first + PER * ITER, all) - 1;
+    const int64_t last = min(first + (int64_t)PER * passes, all) - 1;
     const int tokens = (int)(last / heads - t0) + 1;
     for (int i = threadIdx.x; i < tokens * half; i += RT) {
-      const double x = (double)a.pos[t0 + i / half] * (double)a.inv_freq[i % half] * 0.15915494309189533577;
-      float s, c;
-      sincospif((float)(2.0 * (x - rint(x))), &s, &c);
-      turn[i] = (f32x2){c, s};
+      const double y = (double)a.pos[t0 + i / half] * (double)a.inv_freq[i % half] * 0.15915494309189533577;
+      float sn, cn;
+      sincospif((float)(2.0 * (y - rint(y))), &sn, &cn);
+      turn[i] = (f32x2){cn, sn};
     }
-    __syncthreads();
   }
+  __syncthreads();
 
-#pragma unroll
-  for (int i = 0; i < ITER; i++) {
-    const int64_t at = first + i * PER + threadIdx.x / LPH;
-    const int64_t t = t0 + (int)(at - t0 * heads) / heads;
-    const int h = (int)(at - t * heads);
+#pragma unroll 1
+  for (int i = 0; i < passes; i++) {
+    const bool live = at < all, key = h >= a.q_heads;
+    const int t1 = t, h1 = h;
     float x[2][8];
-    widen8<T>(raw[i][0], x[0]);
-    widen8<T>(raw[i][1], x[1]);
-    const float* w = h < a.q_heads ? a.q_weight : a.k_weight;
-    if (w) {
+    widen8<T>(raw[0], x[0]);
+    widen8<T>(raw[1], x[1]);
+    at += PER;
+    t += over;
+    h += by;
+    if (h >= heads) {
+      h -= heads;
+      t++;
+    }
+    if (i + 1 < passes) fetch(raw);
+    if (norm) {
       float sum = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; e++) sum = __builtin_fmaf(x[1][e], x[1][e], __builtin_fmaf(x[0][e], x[0][e], sum));
 #pragma unroll
       for (int m = 1; m < LPH; m *= 2) sum += __shfl_xor(sum, m);
-      const float inv = 1.0f / sqrtf(sum / (float)D + a.eps);
+      // (a square root's reciprocal to a step or so; below the normal numbers, of 2^48 times as much)
+      const float mean = sum / (float)D + a.eps;
+      const bool tiny = mean < 0x1p-100f;
+      const float inv = __builtin_amdgcn_rsqf(tiny ? mean * 0x1p48f : mean) * (tiny ? 0x1p24f : 1.0f);
+      const float* w = shared + (key ? D : 0);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         if (in0) x[0][e] = x[0][e] * inv * w[8 * c0 + e];
         if (in1) x[1][e] = x[1][e] * inv * w[8 * c1 + e];
       }
     }
-    if (at >= all) continue;
-    const f32x2* cs = turn + (int)(t - t0) * half;
+    const f32x2* cs = turn + t1 * half;
     if (halves) {
-      if (p < rc) {
+      if (live && p < rc) {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           const f32x2 z = cs[8 * p + e];
@@ -121,7 +141,7 @@ __global__ __launch_bounds__(RT) void rotate_kernel(const xs_qk_rotate_args a) {
     } else {
 #pragma unroll
       for (int j = 0; j < 2; j++)
-        if (8 * (2 * p + j) < a.rot_dim) {
+        if (live && 8 * (2 * p + j) < a.rot_dim) {
 #pragma unroll
           for (int e = 0; e < 8; e += 2) {
             const f32x2 z = cs[4 * (2 * p + j) + e / 2];
@@ -131,8 +151,9 @@ __global__ __launch_bounds__(RT) void rotate_kernel(const xs_qk_rotate_args a) {
           }
         }
     }
-    uint16_t* y = h < a.q_heads ? (uint16_t*)a.q_out + t * a.q_out_token_stride + h * a.q_out_head_stride
-                                : (uint16_t*)a.k_out + t * a.k_out_token_stride + (h - a.q_heads) * a.k_out_head_stride;
+    if (!live) break;
+    uint16_t* y = key ? (uint16_t*)a.k_out + (t0 + t1) * a.k_out_token_stride + (h1 - a.q_heads) * a.k_out_head_stride
+                      : (uint16_t*)a.q_out + (t0 + t1) * a.q_out_token_stride + h1 * a.q_out_head_stride;
     u32x4 r;
     if (in0) {
 #pragma unroll
@@ -396,17 +417,16 @@ template <typename T, int LPH>
 int rotate_lanes(xs_cache_context* c, const xs_qk_rotate_args& a) {
   const int64_t heads = a.q_heads + a.kv_heads, all = a.tokens * heads;
   constexpr int64_t per = xsp::RT / LPH;
-  auto run = [&](auto kernel, int64_t iter) {
-    const int64_t span = per * iter, grid = (all + span - 1) / span;
-    if (!xs_host_launch_fits(grid, xsp::RT)) return XS_ERR_CAPACITY;
-    const int64_t tokens = std::min(a.tokens, (span + heads - 1) / heads + 1);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(xsp::RT), (size_t)(tokens * (a.rot_dim / 2) * 8), c->stream, a);
-    return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
-  };
-  // several passes a workgroup where that still fills the device, and where its
-  // tokens' angles are few
-  if (all >= per * 4 * 4 * c->n_cu && heads * 64 >= per * 4) return run(xsp::rotate_kernel<T, LPH, 4>, 4);
-  return run(xsp::rotate_kernel<T, LPH, 1>, 1);
+  // as many passes as leave every CU eight workgroups, of 16 tokens at most (their
+  // angles fill LDS)
+  const int64_t want = std::min(all / (per * 8 * c->n_cu), 16 * heads / per);
+  const int passes = (int)std::max<int64_t>(1, std::min<int64_t>(xsp::ROT_PASSES, want));
+  const int64_t span = per * passes, grid = (all + span - 1) / span;
+  if (!xs_host_launch_fits(grid, xsp::RT)) return XS_ERR_CAPACITY;
+  const int64_t tokens = std::min(a.tokens, (span + heads - 1) / heads + 1);
+  const size_t lds = 8 * (size_t)(a.head_dim + tokens * (a.rot_dim / 2));
+  hipLaunchKernelGGL((xsp::rotate_kernel<T, LPH>), dim3((unsigned)grid), dim3(xsp::RT), lds, c->stream, a, passes);
+  return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
 }
 
 template <typename T>
