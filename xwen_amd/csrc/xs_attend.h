@@ -30,6 +30,20 @@ struct F16 {
   XS_DEV static float widen(uint16_t u) { return (float)__builtin_bit_cast(_Float16, u); }
 };
 
+// Inclusive prefix sums over a wave.
+XS_DEV uint32_t wave_scan(uint32_t v) {
+  // within rows of 16 lanes, then each row's last to the rows after it
+#define XS_STEP(ctrl, rows) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, false)
+  XS_STEP(0x111, 0xF);
+  XS_STEP(0x112, 0xF);
+  XS_STEP(0x114, 0xF);
+  XS_STEP(0x118, 0xF);
+  XS_STEP(0x142, 0xA);
+  XS_STEP(0x143, 0xC);
+#undef XS_STEP
+  return v;
+}
+
 // The nodes a node sees: bit j of lane i's result is set when j is i or an
 // ancestor of i; 0 where i's chain of parents does not end in -1 by way of
 // ever lower nodes below n.  Each round doubles the distance a lane has gone

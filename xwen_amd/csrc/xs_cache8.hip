@@ -282,20 +282,23 @@ struct Raw {
 };
 
 // Load block i; of the last, `limit` slots are in use.  Rows' bases are uniform,
-// so that a lane keeps two 32-bit offsets for all of them.
+// so that a lane keeps two 32-bit offsets for all of them (made new to the
+// compiler's eyes, else it keeps sixteen sums of 64 bits).
 template <int DP, bool EXACT, bool MASKED>
 XS_DEV void load_keys8(Raw<DP>& r, const xs_kv8& c8, int64_t at, int64_t eat, int i, int limit, int D) {
   using S = Shape<DP, 1>;
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
-  const uint32_t stride = (uint32_t)c8.slot_stride, ko = x * stride + 16 * g;
-  const uint8_t* kp = c8.k + at + (int64_t)i * KB * c8.slot_stride;
+  const uint32_t stride = (uint32_t)c8.slot_stride;
+  uint32_t ko = x * stride + 16 * g;
+  asm volatile("" : "+v"(ko));
+  const uint8_t* kp = c8.k + (at + (int64_t)i * KB * c8.slot_stride);
   r.ke = c8.k_exp[eat + i];
 #pragma unroll
   for (int u = 0; u < 2; u++)
 #pragma unroll
     for (int c = 0; c < S::KC / 2; c++) {
       const uint32_t off = MASKED ? min(16 * u + x, limit - 1) * stride + 16 * g : ko;
-      const uint8_t* p = kp + (MASKED ? 0 : (int64_t)(16 * u) * stride) + off + 64 * c;
+      const uint8_t* p = (kp + (MASKED ? 0 : (int64_t)(16 * u) * stride) + 64 * c) + off;
       r.k[u][c] = EXACT || 64 * c + 16 * g < D ? *(const u32x4*)p : (u32x4){0, 0, 0, 0};
     }
 }
@@ -303,8 +306,10 @@ template <int DP, bool EXACT, bool MASKED>
 XS_DEV void load_values8(Raw<DP>& r, const xs_kv8& c8, int64_t at, int64_t eat, int i, int limit, int D) {
   using S = Shape<DP, 1>;
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
-  const uint32_t stride = (uint32_t)c8.slot_stride, vo = 4 * g * stride + S::VE * x;
-  const uint8_t* vp = c8.v + at + (int64_t)i * KB * c8.slot_stride;
+  const uint32_t stride = (uint32_t)c8.slot_stride;
+  uint32_t vo = 4 * g * stride + S::VE * x;
+  asm volatile("" : "+v"(vo));
+  const uint8_t* vp = c8.v + (at + (int64_t)i * KB * c8.slot_stride);
   r.ve = c8.v_exp[eat + i];
 #pragma unroll
   for (int e = 0; e < 8; e++) {
@@ -314,7 +319,7 @@ XS_DEV void load_values8(Raw<DP>& r, const xs_kv8& c8, int64_t at, int64_t eat, 
       const int d = EXACT ? 128 * h + S::VE * x : min(128 * h + S::VE * x, D - S::VE);  // (products of elements past the head's are never stored)
       const uint8_t* p;
       if constexpr (MASKED) p = vp + (uint32_t)(min(slot, limit - 1) * stride + d);
-      else if constexpr (EXACT) p = vp + (int64_t)((e & 3) + 16 * (e >> 2)) * stride + vo + 128 * h;
+      else if constexpr (EXACT) p = (vp + (int64_t)((e & 3) + 16 * (e >> 2)) * stride + 128 * h) + vo;
       else p = vp + (int64_t)((e & 3) + 16 * (e >> 2)) * stride + (uint32_t)(4 * g * stride + d);
       if constexpr (S::VE == 8) {
         const u32x2 y = *(const u32x2*)p;
@@ -387,6 +392,7 @@ XS_DEV void tree_block(Tile<T, DP, RT>& z, const uint16_t* kp, const uint16_t* v
     return y[m];
   };
   softmax8<T, DP, RT, true, N>(z, scale, on, pf, keys, keys);
+  __builtin_amdgcn_sched_barrier(0);  // (the values' registers not beside the keys')
   uint32_t v[N][8][S::VH][S::VE / 2];
 #pragma unroll
   for (int e = 0; e < 8; e++) {
@@ -426,70 +432,171 @@ XS_DEV void tree_block(Tile<T, DP, RT>& z, const uint16_t* kp, const uint16_t* v
     for (int n = 0; n < N; n++) accumulate(z.w, v[m], pf[n]);
 }
 
+// How a call is cut.  The keys are counted in units (blocks of 32, stages of 64),
+// and a sequence of u units is split in u / share of them, rounded up.  The share
+// is one for all sequences, so that long and short ones' workgroups end together:
+// the smallest that leaves no more splits than the device holds at once, `room`
+// for each head and row tile, so that no workgroup starts when the others end (as
+// many splits for every sequence instead, 32 of 327 to 8,192 slots: @RAG0@ us for
+// @RAG2@).  The lengths are on the device, so every workgroup finds the share and
+// its place among the sequences itself.
+struct Cut8 {
+  int32_t G, tiles, units, room;  // units: (sequence, split) that the launch has; room 0: nothing is split
+  float scale;
+  float* part;                    // [units, kv heads, tiles] partial results
+};
+struct Place8 {
+  int b, split, share, n;  // b < 0: none; n: splits of the sequence
+  int unit;                // place among the units
+  int len, nodes;          // of the sequence; nodes < 0: bad
+};
+
+// UNIT keys a unit, shares of LEAST units at least, sequences of up to WHOLE of
+// them in one piece.
+template <int UNIT>
+XS_DEV int units_of(const Seq& sq) { return sq.bad ? 0 : (sq.len + UNIT - 1) / UNIT + (sq.n + UNIT - 1) / UNIT; }
+
+// The place of unit `want`, or (want < 0) the first of sequence `seq`.
+template <int UNIT, int LEAST, int WHOLE>
+XS_DEV Place8 place8(const xs_tree_attend_args& a, const Cut8& cut, int want, int seq) {
+  const int lane = threadIdx.x & 63, seqs = (int)a.seqs;
+  if (cut.room == 0) {
+    const int b = want < 0 ? seq : want;
+    if (b >= seqs) return {-1, 0, 1, 1, 0, 0, 0};
+    const Seq sq(a, b);
+    return {b, 0, 1, 1, b, sq.len, sq.bad ? -1 : sq.n};
+  }
+  uint32_t u = 0;  // of the lane's sequence (of the last 64)
+  int len = 0, nodes = -1;
+  auto load = [&](int b0) {
+    u = 0;
+    if (b0 + lane >= seqs) return;
+    const Seq sq(a, b0 + lane);
+    u = (uint32_t)units_of<UNIT>(sq);
+    len = sq.len;
+    nodes = sq.bad ? -1 : sq.n;
+  };
+  auto last = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(v), 63); };
+  auto splits = [&](int b0, uint32_t share) { return b0 + lane >= seqs ? 0u : u <= WHOLE ? 1u : (u + share - 1) / share; };
+  uint32_t all = 0;  // (at most 256 sequences of 2^23 units and some)
+  for (int b0 = 0; b0 < seqs; b0 += 64) {
+    load(b0);
+    all += last(u);
+  }
+  const uint32_t room = (uint32_t)cut.room;
+  uint32_t share = max((uint32_t)LEAST, (all + room - 1) / room);
+  if (room > (uint32_t)seqs) {
+    uint32_t high = max(share, (all + room - seqs - 1) / (room - seqs));  // (a share too many for each sequence fits)
+    while (share < high) {
+      const uint32_t mid = (share + high) / 2;
+      uint32_t sum = 0;
+      for (int b0 = 0; b0 < seqs; b0 += 64) {
+        if (seqs > 64) load(b0);
+        sum += last(splits(b0, mid));
+      }
+      if (sum <= room) high = mid;
+      else share = mid + 1;
+    }
+  }
+  uint32_t before = 0;
+  for (int b0 = 0; b0 < seqs; b0 += 64) {
+    if (seqs > 64) load(b0);
+    const uint32_t n = splits(b0, share), upto = wave_scan(n) + before;
+    const uint64_t hit = want >= 0 ? __ballot(b0 + lane < seqs && upto > (uint32_t)want) : seq < b0 + 64 ? 1ull << (seq - b0) : 0ull;
+    before = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    if (!hit) continue;
+    const int who = __ffsll((unsigned long long)hit) - 1, parts = __builtin_amdgcn_readlane((int)n, who);
+    const int first = __builtin_amdgcn_readlane((int)upto, who) - parts;
+    return {b0 + who, want >= 0 ? want - first : 0, (int)share, parts, want >= 0 ? want : first,
+            __builtin_amdgcn_readlane(len, who), __builtin_amdgcn_readlane(nodes, who)};
+  }
+  return {-1, 0, 1, 1, 0, 0, 0};
+}
+
+// Workgroup i's part: groups of eight (kv head, sequence, split), each group's row
+// tiles on one XCD (workgroup index mod 8), which then reads their keys once.  A
+// head's units one after the other: with a unit's heads side by side, where a
+// slot's heads lie side by side too, every XCD reads one head's 128 bytes of every
+// 1,024, and 32 sequences of 4,608 slots take 84 us for 74.
+XS_DEV void deal(const Cut8& cut, int* tile, int* kh, int* unit) {
+  const int i = blockIdx.x >> 3, group = i / cut.tiles * 8 + (blockIdx.x & 7);
+  *tile = i % cut.tiles;
+  *unit = group % cut.units;
+  *kh = group / cut.units;
+}
+
 // Up to 16 RT rows a workgroup, whose waves split the keys and add up through
-// LDS; grid as in attend_kernel.
+// LDS.
 template <typename T, int DP, int RT, bool EXACT>
 __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : DP * RT <= 256 ? 2 : 1) void attend8_kernel(
-    const xs_tree_attend_args a, const xs_kv8 c8, const Cut cut) {
+    const xs_tree_attend_args a, const xs_kv8 c8, const Cut8 cut) {
   using S = Shape<DP, RT>;
   __shared__ float stat[NW][RT][2][16];
   __shared__ f32x4 sum[NW][RT][S::NF][64];
   __shared__ int odds[NW];
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tile = (blockIdx.x >> 3) % cut.tiles;
-  const int group = ((blockIdx.x >> 3) / cut.tiles) * 8 + (blockIdx.x & 7);
-  if (group >= cut.groups) return;
-  const int bh = group / cut.nsplit, split = turned(group % cut.nsplit, bh, cut.nsplit);
-  const int kh = bh % (int)a.kv_heads, b = bh / (int)a.kv_heads;
-  const int row0 = tile * RT * 16, parent = parent_of(a, b);
+  int tile, kh, unit;
+  deal(cut, &tile, &kh, &unit);
+  if (kh >= (int)a.kv_heads) return;
+  const Place8 pl = place8<KB, 2 * NW, 4 * NW>(a, cut, unit, 0);
+  const int b = __builtin_amdgcn_readfirstlane(pl.b), split = __builtin_amdgcn_readfirstlane(pl.split);
+  const int splits = __builtin_amdgcn_readfirstlane(pl.n);
+  if (b < 0) return;
+  const int share = __builtin_amdgcn_readfirstlane(pl.share), bh = b * (int)a.kv_heads + kh;
+  const int len = __builtin_amdgcn_readfirstlane(pl.len), n = __builtin_amdgcn_readfirstlane(pl.nodes);
+  if (split == 0 && tile == 0 && kh == 0 && threadIdx.x == 0) a.seq_status[b] = n < 0 ? XS_ROW_BAD_PARAM : XS_ROW_OK;
+  const int R = n * cut.G, row0 = tile * RT * 16;
+  const int cached = (len + KB - 1) / KB, total = cached + (n + KB - 1) / KB;
+  const int first = split * share, last = splits == 1 ? total : min(first + share, total);  // (one split: share says nothing)
+  if (row0 >= R || first >= total) return;  // (nodes below 0 too)
+
+  // the first keys and values leave before the queries
+  const int64_t at = b * c8.seq_stride + kh * c8.head_stride, eat = (int64_t)bh * c8.exp_ld;
+  int i = first + wave;
+  const int end = min(last, len / KB);
+  Raw<DP> r;
+  if (i < end) {
+    load_keys8<DP, EXACT, false>(r, c8, at, eat, i, KB, a.head_dim);
+    load_values8<DP, EXACT, false>(r, c8, at, eat, i, KB, a.head_dim);
+  }
+  const int parent = parent_of(a, b);
   Tile<T, DP, RT> z;
   z.w.init();
 #pragma unroll
   for (int t = 0; t < RT; t++) {
-    const int row = row0 + 16 * t + x;
-    const bool in = row < (int)a.nodes * cut.G;
-    const int node = in ? row / cut.G : 0, head = kh * cut.G + (in ? row % cut.G : 0);
+    const int row = min(row0 + 16 * t + x, R - 1);  // (rows past the last are not stored)
+    const int node = row / cut.G, head = kh * cut.G + row % cut.G;
     const uint16_t* p = (const uint16_t*)a.q + b * a.q_seq_stride + node * a.q_node_stride + head * a.q_head_stride;
 #pragma unroll
     for (int c = 0; c < S::KC; c++) {
       const int d = 64 * (c / 2) + 16 * g + 8 * (c % 2);
       u32x4 y[Tile<T, DP, RT>::N];
-      split8(T{}, in && (EXACT || d < a.head_dim) ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0}, y);
+      split8(T{}, EXACT || d < a.head_dim ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0}, y);
 #pragma unroll
-      for (int n = 0; n < Tile<T, DP, RT>::N; n++) z.q[n][t][c] = y[n];
+      for (int m = 0; m < Tile<T, DP, RT>::N; m++) z.q[m][t][c] = y[m];
     }
   }
-  const Seq sq(a, b);
-  if (split == 0 && tile == 0 && kh == 0 && threadIdx.x == 0) a.seq_status[b] = sq.bad ? XS_ROW_BAD_PARAM : XS_ROW_OK;
-  if (sq.bad) return;
-  const int R = sq.n * cut.G;
-  const int total = sq.blocks(), cached = (sq.len + KB - 1) / KB;
-  const int first = split * cut.chunk, last = min(first + cut.chunk, total);
-  if (row0 >= R || first >= total) return;
 
-  const int64_t at = b * c8.seq_stride + kh * c8.head_stride, eat = (int64_t)bh * c8.exp_ld;
-  int i = first + wave;
   // whole blocks of the cache: a block's registers take the next one's keys once
-  // its scores are formed, and the next one's values after its second product
-  {
-    const int end = min(last, sq.len / KB);
-    Raw<DP> r;
-    if (i < end) {
-      load_keys8<DP, EXACT, false>(r, c8, at, eat, i, KB, a.head_dim);
-      load_values8<DP, EXACT, false>(r, c8, at, eat, i, KB, a.head_dim);
-    }
+  // its scores are formed, and the next one's values after its second product (a
+  // wave's last one again after it: a branch round the loads would have the
+  // products wait for all of them)
 #pragma unroll 1
-    for (; i < end; i += NW) {
-      u32x4 pf[Parts<T>::N][RT];
-      cache_weights<T, DP, RT, false>(z, r, cut.scale, nullptr, pf);
-      if (i + NW < end) load_keys8<DP, EXACT, false>(r, c8, at, eat, i + NW, KB, a.head_dim);
-      cache_product<T, DP, RT>(z, r, pf);
-      if (i + NW < end) load_values8<DP, EXACT, false>(r, c8, at, eat, i + NW, KB, a.head_dim);
-    }
+  for (; i < end; i += NW) {
+    u32x4 pf[Parts<T>::N][RT];
+    cache_weights<T, DP, RT, false>(z, r, cut.scale, nullptr, pf);
+    const int next = min(i + NW, end - 1);
+    __builtin_amdgcn_sched_barrier(0);  // (the loads leave here, not where the last ones have come)
+    load_keys8<DP, EXACT, false>(r, c8, at, eat, next, KB, a.head_dim);
+    __builtin_amdgcn_sched_barrier(0);
+    cache_product<T, DP, RT>(z, r, pf);
+    __builtin_amdgcn_sched_barrier(0);
+    load_values8<DP, EXACT, false>(r, c8, at, eat, next, KB, a.head_dim);
+    __builtin_amdgcn_sched_barrier(0);
   }
   // its last one, and the tree's
-  const uint64_t sees = ancestors(parent, sq.n);
+  const uint64_t sees = ancestors(parent, n);
   uint64_t mine[RT];  // what the lane's rows see of the tree
 #pragma unroll
   for (int t = 0; t < RT; t++) {
@@ -501,21 +608,22 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
   for (; i < last; i += NW) {
     uint32_t on[RT];
     if (i < cached) {
-      const int limit = sq.len - i * KB;
+      const int limit = len - i * KB;
 #pragma unroll
       for (int t = 0; t < RT; t++) on[t] = (1u << limit) - 1u;
-      Raw<DP> r;
       load_keys8<DP, EXACT, true>(r, c8, at, eat, i, limit, a.head_dim);
-      load_values8<DP, EXACT, true>(r, c8, at, eat, i, limit, a.head_dim);
       u32x4 pf[Parts<T>::N][RT];
+      load_values8<DP, EXACT, true>(r, c8, at, eat, i, limit, a.head_dim);
+      __builtin_amdgcn_sched_barrier(0);
       cache_weights<T, DP, RT, true>(z, r, cut.scale, on, pf);
+      __builtin_amdgcn_sched_barrier(0);
       cache_product<T, DP, RT>(z, r, pf);
     } else {
       const int key0 = (i - cached) * KB;
 #pragma unroll
       for (int t = 0; t < RT; t++) on[t] = (uint32_t)(mine[t] >> key0);
       const int64_t f = b * a.fresh.seq_stride + kh * a.fresh.head_stride;
-      tree_block<T, DP, RT, EXACT>(z, (const uint16_t*)a.fresh.k + f, (const uint16_t*)a.fresh.v + f, a.fresh.slot_stride, key0, sq.n,
+      tree_block<T, DP, RT, EXACT>(z, (const uint16_t*)a.fresh.k + f, (const uint16_t*)a.fresh.v + f, a.fresh.slot_stride, key0, n,
                                    a.head_dim, cut.scale, on);
     }
   }
@@ -550,7 +658,7 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
   constexpr int PAIRS = S::VE / 2;
   const bool whole = first == 0 && last == total;
   const int odd = odds[0] | odds[1] | odds[2] | odds[3];
-  float* part = cut.part + (((int64_t)bh * cut.nsplit + split) * cut.tiles + tile) * S::PART;
+  float* part = cut.part + (((int64_t)unit * a.kv_heads + kh) * cut.tiles + tile) * S::PART;
 #pragma unroll 1
   for (int u = wave; u < RT * S::VH * PAIRS; u += NW) {
     const int pair = u % PAIRS, h = u / PAIRS % S::VH, t = u / (PAIRS * S::VH), f0 = h * S::VE + 2 * pair;
@@ -566,7 +674,7 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
       o[1] += sum[j][t][f0 + 1][lane];
     }
     if (whole) {
-      store_pair<T, DP, E4m3>(a, cut.G, b, kh, row0 + 16 * t + x, R, h, pair, o[0], o[1], top, all, odd, sq.n);
+      store_pair<T, DP, E4m3>(a, cut.G, b, kh, row0 + 16 * t + x, R, h, pair, o[0], o[1], top, all, odd, n);
     } else {
       f32x4* p = (f32x4*)part + (t * S::NF + f0) * 64 + lane;
       p[0] = o[0];
@@ -578,6 +686,73 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
       }
     }
   }
+}
+
+// Joins the splits of 16 rows and one half of the head: a pair of fragments a
+// wave, over one of SHARES shares of the splits.
+template <int DP, int SHARES>
+constexpr int join8_threads() { return 64 * (Shape<DP, 1>::VE / 2) * SHARES; }
+
+template <typename T, int DP, int SHARES>
+__global__ __launch_bounds__((join8_threads<DP, SHARES>())) void join8_kernel(const xs_tree_attend_args a, const Cut8 cut) {
+  using S = Shape<DP, 1>;
+  constexpr int PAIRS = S::VE / 2, WAVES = PAIRS * SHARES;
+  __shared__ float weight[SPLITS][16];
+  __shared__ float stat[2][4 * WAVES][16];
+  __shared__ int odd;
+  __shared__ f32x4 sum[SHARES][S::VE][64];
+  const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pair = wave % PAIRS, share = wave / PAIRS;
+  const int h = blockIdx.x % S::VH, tile = blockIdx.x / S::VH % cut.tiles, bh = blockIdx.x / (S::VH * cut.tiles);
+  const int kh = bh % (int)a.kv_heads, b = bh / (int)a.kv_heads;
+  const Place8 pl = place8<KB, 2 * NW, 4 * NW>(a, cut, -1, b);
+  const int n = __builtin_amdgcn_readfirstlane(pl.n), nodes = __builtin_amdgcn_readfirstlane(pl.nodes), R = nodes * cut.G, row0 = 16 * tile;
+  if (row0 >= R || n <= 1) return;
+  if (threadIdx.x == 0) odd = 0;
+  __syncthreads();
+  const float* part = cut.part + (((int64_t)__builtin_amdgcn_readfirstlane((int)pl.unit) * a.kv_heads + kh) * cut.tiles + tile) * S::PART;
+  const int64_t step = a.kv_heads * cut.tiles * S::PART;
+  // a quarter of a wave takes a split's rows
+  float top = NEG_INF, all = 0.0f;
+  for (int s = 4 * wave + g; s < n; s += 4 * WAVES) {
+    const float* p = part + s * step;
+    top = fmaxf(top, p[S::STAT + x]);
+    if (p[S::ODD] != 0.0f) odd = 1;  // (any of them)
+  }
+  stat[0][4 * wave + g][x] = top;
+  __syncthreads();
+#pragma unroll 8
+  for (int j = 0; j < 4 * WAVES; j++) top = fmaxf(top, stat[0][j][x]);
+  for (int s = 4 * wave + g; s < n; s += 4 * WAVES) {
+    const float* p = part + s * step + S::STAT + x;
+    const float m = p[0], y = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((m - top) * fabsf(cut.scale));
+    if (m != NEG_INF) all += p[16] * y;
+    weight[s][x] = y;
+  }
+  stat[1][4 * wave + g][x] = all;
+  __syncthreads();
+  const int f0 = h * S::VE + 2 * pair;
+  f32x4 o[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll 4
+  for (int s = share; s < n; s += SHARES) {
+    const f32x4* p = (const f32x4*)(part + s * step) + f0 * 64 + lane;
+    const float y = weight[s][x];
+    o[0] += p[0] * y;
+    o[1] += p[64] * y;
+  }
+  sum[share][2 * pair][lane] = o[0];
+  sum[share][2 * pair + 1][lane] = o[1];
+  __syncthreads();
+  if (share != 0) return;
+  all = 0.0f;
+#pragma unroll 8
+  for (int j = 0; j < 4 * WAVES; j++) all += stat[1][j][x];
+#pragma unroll
+  for (int j = 1; j < SHARES; j++) {
+    o[0] += sum[j][2 * pair][lane];
+    o[1] += sum[j][2 * pair + 1][lane];
+  }
+  store_pair<T, DP, E4m3>(a, cut.G, b, kh, row0 + x, R, h, pair, o[0], o[1], top, all, odd, nodes);
 }
 
 // More rows than that: 32 a wave (xs_rows32.h), of keys that the workgroup's
@@ -594,12 +769,8 @@ struct Shape32 {
   static constexpr int PART = ODD + 4;               // then whether odd values are left out
 };
 
-struct Cut32 {
-  int32_t G, tiles, nsplit, chunk, groups;  // chunk: stages of a split
-  float scale;
-  float* part;
-};
-XS_DEV int stages_of(const Seq& sq) { return (sq.len + SK - 1) / SK + (sq.n > 0 ? 1 : 0); }
+// Stages of a sequence: the cache's, and the tree's one.
+constexpr int STAGES_LEAST = 4, STAGES_WHOLE = 8;
 
 // Fragment f (elements e .. e + 4 of row `row`, e = 8 f + 4 g) of the result.
 template <typename T>
@@ -625,7 +796,7 @@ XS_DEV void store_four(const xs_tree_attend_args& a, int G, int b, int kh, int r
 }
 
 template <typename T, int DP, int WK, bool EXACT>
-__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void attend8_wide_kernel(const xs_tree_attend_args a, const xs_kv8 c8, const Cut32 cut) {
+__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void attend8_wide_kernel(const xs_tree_attend_args a, const xs_kv8 c8, const Cut8 cut) {
   using S = Shape32<DP, WK>;
   using K = Keys<DP>;
   constexpr int N = Parts<T>::N, CH = K::CH, KC = DP / 16, DT = DP / 32, TH = 64 * NW;
@@ -635,19 +806,21 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void attend8_wide_kerne
   __shared__ int odds;
   const int lane = threadIdx.x & 63, x = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / WK, wk = wave % WK;
-  const int tile = (blockIdx.x >> 3) % cut.tiles;
-  const int group = ((blockIdx.x >> 3) / cut.tiles) * 8 + (blockIdx.x & 7);
-  if (group >= cut.groups) return;
-  const int bh = group / cut.nsplit, split = turned(group % cut.nsplit, bh, cut.nsplit);
-  const int kh = bh % (int)a.kv_heads, b = bh / (int)a.kv_heads;
-  const int parent = parent_of(a, b);
-  const Seq sq(a, b);
-  if (split == 0 && tile == 0 && kh == 0 && threadIdx.x == 0) a.seq_status[b] = sq.bad ? XS_ROW_BAD_PARAM : XS_ROW_OK;
-  if (sq.bad) return;
-  const int R = sq.n * cut.G, row = tile * S::ROWS + 32 * wr + x;
-  const int total = stages_of(sq), first = split * cut.chunk, last = min(first + cut.chunk, total);
-  if (tile * S::ROWS >= R || first >= total) return;
+  int tile, kh, unit;
+  deal(cut, &tile, &kh, &unit);
+  if (kh >= (int)a.kv_heads) return;
+  const Place8 pl = place8<SK, STAGES_LEAST, STAGES_WHOLE>(a, cut, unit, 0);
+  const int b = __builtin_amdgcn_readfirstlane(pl.b), split = __builtin_amdgcn_readfirstlane(pl.split);
+  const int splits = __builtin_amdgcn_readfirstlane(pl.n);
+  if (b < 0) return;
+  const int share = __builtin_amdgcn_readfirstlane(pl.share), bh = b * (int)a.kv_heads + kh;
+  const int len = __builtin_amdgcn_readfirstlane(pl.len), n = __builtin_amdgcn_readfirstlane(pl.nodes);
+  if (split == 0 && tile == 0 && kh == 0 && threadIdx.x == 0) a.seq_status[b] = n < 0 ? XS_ROW_BAD_PARAM : XS_ROW_OK;
+  const int R = n * cut.G, row = tile * S::ROWS + 32 * wr + x;
+  const int cached = (len + SK - 1) / SK, total = cached + (n > 0 ? 1 : 0), first = split * share, last = splits == 1 ? total : min(first + share, total);
+  if (tile * S::ROWS >= R || first >= total) return;  // (nodes below 0 too)
 
+  const int parent = parent_of(a, b);
   Rows32<Bf16, DP, N> w;
   w.init();
   {
@@ -659,22 +832,22 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void attend8_wide_kerne
       u32x4 y[N];
       split8(T{}, row < R && (EXACT || d < a.head_dim) ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0}, y);
 #pragma unroll
-      for (int n = 0; n < N; n++) w.q[n][c] = y[n];
+      for (int m = 0; m < N; m++) w.q[m][c] = y[m];
     }
   }
-  const uint64_t seen = ancestors(parent, sq.n);
+  const uint64_t seen = ancestors(parent, n);
   const uint64_t mine = __shfl(seen, min(row / cut.G, 63)) & (row < R ? ~0ull : 0ull);  // what the lane's row sees of the tree
   const Reads<DP> reads;
 
   // whole and part stages of the cache
-  const int end = min(last, (sq.len + SK - 1) / SK);
+  const int end = min(last, cached);
   const int64_t at = b * c8.seq_stride + kh * c8.head_stride, eat = (int64_t)bh * c8.exp_ld;
   const uint32_t stride = (uint32_t)c8.slot_stride;
   u32x4 rk[PER], rv[PER];
   uint32_t ek[PER], ev[PER];
   auto fetch = [&](int s) {
     const int64_t base = at + (int64_t)s * SK * c8.slot_stride;
-    const int most = sq.len - 1 - s * SK;
+    const int most = len - 1 - s * SK;
 #pragma unroll
     for (int j = 0; j < PER; j++) {
       const int p = j * TH + threadIdx.x, r = min(p / (DP / 16), most), c = p % (DP / 16);
@@ -687,7 +860,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void attend8_wide_kerne
     }
   };
   auto put = [&](int s) {
-    const int most = sq.len - 1 - s * SK;
+    const int most = len - 1 - s * SK;
 #pragma unroll
     for (int j = 0; j < PER; j++) {
       const int p = j * TH + threadIdx.x, r = p / (DP / 16), c = p % (DP / 16);
@@ -726,7 +899,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void attend8_wide_kerne
     __syncthreads();
     if (s + 1 < end) put(s + 1);
     if (s + 2 < end) fetch(s + 2);
-    const int limit = sq.len - s * SK;
+    const int limit = len - s * SK;
     step(lk[s & 1], lv[s & 1], limit < SK, limit < SK ? (1ull << limit) - 1ull : ~0ull);
   }
   // the tree: parts in a buffer each
@@ -739,7 +912,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void attend8_wide_kerne
     for (int p = threadIdx.x; p < K::STAGE; p += TH) {
       const int r = p / CH, c = p % CH;
       u32x4 k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
-      if (r < sq.n && (EXACT || 8 * c < a.head_dim)) {
+      if (r < n && (EXACT || 8 * c < a.head_dim)) {
         k = *(const u32x4*)((const uint16_t*)a.fresh.k + f + r * a.fresh.slot_stride + 8 * c);
         v = *(const u32x4*)((const uint16_t*)a.fresh.v + f + r * a.fresh.slot_stride + 8 * c);
       }
@@ -754,9 +927,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void attend8_wide_kerne
       split8(T{}, k, ks);
       split8(T{}, v, vs);
 #pragma unroll
-      for (int n = 0; n < N; n++) {
-        lk[n][r * CH + (c ^ K::turn_k(r))] = ks[n];
-        lv[n][r * CH + (c ^ K::turn_v(r))] = vs[n];
+      for (int m = 0; m < N; m++) {
+        lk[m][r * CH + (c ^ K::turn_k(r))] = ks[m];
+        lv[m][r * CH + (c ^ K::turn_v(r))] = vs[m];
       }
     }
     __syncthreads();
@@ -766,7 +939,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void attend8_wide_kerne
       const int u = WK == 1 ? i : wk;
       const uint64_t bits = mine >> (32 * u + 4 * g);
       const Bits on = {(uint32_t)bits, (uint32_t)(bits >> 32)};
-      if (32 * u >= sq.n) continue;
+      if (32 * u >= n) continue;
       if constexpr (N == 1) w.template step<1, 1>(reads, {lk[0] + 32 * u * CH}, {lv[0] + 32 * u * CH}, cut.scale, true, on);
       else w.template step<1, 2>(reads, {lk[0] + 32 * u * CH, lk[1] + 32 * u * CH}, {lv[0] + 32 * u * CH, lv[1] + 32 * u * CH}, cut.scale, true, on);
     }
@@ -809,12 +982,12 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void attend8_wide_kerne
     }
   }
   const bool whole = first == 0 && last == total;
-  float* part = cut.part + (((int64_t)bh * cut.nsplit + split) * cut.tiles + tile) * S::PART;
+  float* part = cut.part + (((int64_t)unit * a.kv_heads + kh) * cut.tiles + tile) * S::PART;
 #pragma unroll
   for (int f = 0; f < S::NF; f++) {
     const f32x16 o = w.o[f / 4];
     const f32x4 y = {o[4 * (f % 4)], o[4 * (f % 4) + 1], o[4 * (f % 4) + 2], o[4 * (f % 4) + 3]};
-    if (whole) store_four<T>(a, cut.G, b, kh, row, R, f, y, ref, l, odd, sq.n);
+    if (whole) store_four<T>(a, cut.G, b, kh, row, R, f, y, ref, l, odd, n);
     else ((f32x4*)part)[(wr * S::NF + f) * 64 + lane] = y;
   }
   if (!whole && g == 0) {
@@ -826,13 +999,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void attend8_wide_kerne
 
 // Joins the splits of 32 rows, four fragments a workgroup: each wave one of them
 // over one of SHARES shares of the splits.
-constexpr int join32_threads(bool few) { return few ? 256 : 1024; }
-
-template <typename T, int DP, int WK, bool FEWER>
-__global__ __launch_bounds__(join32_threads(FEWER)) void join32_kernel(const xs_tree_attend_args a, const Cut32 cut) {
+template <typename T, int DP, int WK, int SHARES>
+__global__ __launch_bounds__(256 * SHARES) void join32_kernel(const xs_tree_attend_args a, const Cut8 cut) {
   using S = Shape32<DP, WK>;
-  constexpr int SHARES = FEWER ? 1 : 4, WAVES = 4 * SHARES, MOST = FEWER ? FEW : SPLITS;
-  __shared__ float weight[MOST][32];
+  constexpr int WAVES = 4 * SHARES;
+  __shared__ float weight[SPLITS][32];
   __shared__ float stat[2][2 * WAVES][32];
   __shared__ int odd;
   __shared__ f32x4 sum[SHARES][4][64];
@@ -840,14 +1011,13 @@ __global__ __launch_bounds__(join32_threads(FEWER)) void join32_kernel(const xs_
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), share = wave / 4;
   const int f = blockIdx.x % S::DT * 4 + wave % 4, wr = blockIdx.x / S::DT % S::WR, tile = blockIdx.x / (S::DT * S::WR) % cut.tiles;
   const int bh = blockIdx.x / (S::DT * S::WR * cut.tiles), kh = bh % (int)a.kv_heads, b = bh / (int)a.kv_heads;
-  const Seq sq(a, b);
-  const int R = sq.n * cut.G, row = tile * S::ROWS + 32 * wr + x;
-  const int n = (stages_of(sq) + cut.chunk - 1) / cut.chunk;
-  if (sq.bad || tile * S::ROWS + 32 * wr >= R || n <= 1) return;
+  const Place8 pl = place8<SK, STAGES_LEAST, STAGES_WHOLE>(a, cut, -1, b);
+  const int n = __builtin_amdgcn_readfirstlane(pl.n), nodes = __builtin_amdgcn_readfirstlane(pl.nodes), R = nodes * cut.G, row = tile * S::ROWS + 32 * wr + x;
+  if (tile * S::ROWS + 32 * wr >= R || n <= 1) return;
   if (threadIdx.x == 0) odd = 0;
   __syncthreads();
-  const float* part = cut.part + ((int64_t)bh * cut.nsplit * cut.tiles + tile) * S::PART;
-  const int64_t step = (int64_t)cut.tiles * S::PART;
+  const float* part = cut.part + (((int64_t)__builtin_amdgcn_readfirstlane((int)pl.unit) * a.kv_heads + kh) * cut.tiles + tile) * S::PART;
+  const int64_t step = a.kv_heads * cut.tiles * S::PART;
   // half a wave takes a split's rows
   float top = NEG_INF, all = 0.0f;
   for (int s = 2 * wave + g; s < n; s += 2 * WAVES) {
@@ -857,7 +1027,7 @@ __global__ __launch_bounds__(join32_threads(FEWER)) void join32_kernel(const xs_
   }
   stat[0][2 * wave + g][x] = top;
   __syncthreads();
-#pragma unroll
+#pragma unroll 8
   for (int j = 0; j < 2 * WAVES; j++) top = fmaxf(top, stat[0][j][x]);
   for (int s = 2 * wave + g; s < n; s += 2 * WAVES) {
     const float* p = part + s * step + S::STAT + 32 * wr + x;
@@ -870,17 +1040,15 @@ __global__ __launch_bounds__(join32_threads(FEWER)) void join32_kernel(const xs_
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
   for (int s = share; s < n; s += SHARES) o += ((const f32x4*)(part + s * step))[(wr * S::NF + f) * 64 + lane] * weight[s][x];
+  sum[share][wave % 4][lane] = o;
+  __syncthreads();
+  if (share != 0) return;
   all = 0.0f;
-#pragma unroll
+#pragma unroll 8
   for (int j = 0; j < 2 * WAVES; j++) all += stat[1][j][x];
-  if constexpr (SHARES > 1) {
-    sum[share][wave % 4][lane] = o;
-    __syncthreads();
-    if (share != 0) return;
 #pragma unroll
-    for (int j = 1; j < SHARES; j++) o += sum[j][wave % 4][lane];
-  }
-  store_four<T>(a, cut.G, b, kh, row, R, f, o, top, all, odd, sq.n);
+  for (int j = 1; j < SHARES; j++) o += sum[j][wave % 4][lane];
+  store_four<T>(a, cut.G, b, kh, row, R, f, o, top, all, odd, nodes);
 }
 
 }  // namespace xs8
@@ -892,92 +1060,80 @@ namespace {
 
 using xs_host::OnDevice;
 using xs_host::per_cu;
-using xs_host::rounds;
 
-template <typename T, int DP, int RT, bool EXACT>
+// The launch's units and room, for shares of up to `slots` workgroups with
+// partial results of `part` floats; false: too many for one launch.
+bool cut8(xs_cache_context* c, const xs_tree_attend_args& a, int rows, int64_t slots, int64_t part, int64_t unit, int64_t least, int64_t whole,
+          xs8::Cut8* cut, int64_t* grid) {
+  cut->G = (int32_t)(a.q_heads / a.kv_heads);
+  cut->tiles = (int32_t)((a.nodes * cut->G + rows - 1) / rows);
+  cut->scale = a.scale * xst::LOG2E;
+  cut->part = c->part;
+  const int64_t limit = a.max_len ? a.max_len : a.capacity, units = (limit + unit - 1) / unit + (a.nodes + unit - 1) / unit;
+  const int64_t heads = a.kv_heads * cut->tiles;
+  const int64_t places = c->part_floats / (heads * part);
+  int64_t room = std::min<int64_t>(std::min(slots / heads, places), xst::SPLITS);
+  // one round of the device, or, of more sequences than that, more by a share each
+  const bool fits = room > a.seqs || places >= room + a.seqs;
+  if (units <= whole || a.seqs > 256 || room < 2 || !fits) room = 0;
+  cut->room = (int32_t)room;
+  cut->units = (int32_t)(!room ? a.seqs : std::min(room > a.seqs ? room : room + a.seqs, a.seqs * ((units + least - 1) / least)));
+  *grid = ((int64_t)cut->units * a.kv_heads + 7) / 8 * 8 * cut->tiles;
+  return xs_host_launch_fits(*grid, 64 * xst::NW);
+}
+
+// Shares of the splits that a join goes through side by side: several where a
+// sequence has many (an average of more than eight).
+bool many8(const xs8::Cut8& cut, const xs_tree_attend_args& a) { return cut.room > 8 * a.seqs; }
+
+template <typename T, int DP, bool EXACT>
 int attend8_run(xs_cache_context* c, const xs_tree_attend_args& a, const xs_kv8& c8) {
-  xst::Cut cut;
-  cut.G = (int32_t)(a.q_heads / a.kv_heads);
-  cut.tiles = (int32_t)((a.nodes * cut.G + 16 * RT - 1) / (16 * RT));
-  cut.scale = a.scale * xst::LOG2E;
-  cut.part = c->part;
-  const int64_t limit = a.max_len ? a.max_len : a.capacity;
-  const int64_t blocks = (limit + xst::KB - 1) / xst::KB + (a.nodes + xst::KB - 1) / xst::KB;
-  const int64_t units = a.seqs * a.kv_heads * cut.tiles;
-  const int64_t most = c->n_cu * per_cu(DP, RT) * rounds(a.seqs);
-  const int64_t nsplit = std::max<int64_t>(1, std::min<int64_t>(xst::SPLITS, most / units));
-  cut.chunk = (int32_t)((blocks + nsplit - 1) / nsplit);
-  if (cut.chunk < 2 * xst::NW) cut.chunk = 2 * xst::NW;
-  if (blocks <= 4 * xst::NW) cut.chunk = (int32_t)blocks;
-  cut.nsplit = (int32_t)((blocks + cut.chunk - 1) / cut.chunk);
-  const int64_t groups = a.seqs * a.kv_heads * cut.nsplit;
-  const int64_t grid = (groups + 7) / 8 * 8 * cut.tiles, join = a.seqs * a.kv_heads * cut.tiles * RT * xst::Shape<DP, RT>::VH;
-  const int64_t joiners = xst::join_threads<DP>(cut.nsplit <= xst::FEW);
-  if (!xs_host_launch_fits(grid, 64 * xst::NW) || (cut.nsplit > 1 && !xs_host_launch_fits(join, joiners))) return XS_ERR_CAPACITY;
-  if (cut.nsplit > 1 && groups * cut.tiles * xst::Shape<DP, RT>::PART > c->part_floats) return XS_ERR_CAPACITY;  // (never: groups * tiles <= most)
-  cut.groups = (int32_t)groups;
-  hipLaunchKernelGGL((xs8::attend8_kernel<T, DP, RT, EXACT>), dim3((unsigned)grid), dim3(64 * xst::NW), 0, c->stream, a, c8, cut);
-  if (cut.nsplit > xst::FEW)
-    hipLaunchKernelGGL((xst::join_kernel<T, DP, RT, false, xs8::E4m3>), dim3((unsigned)join), dim3(xst::join_threads<DP>(false)), 0, c->stream, a, cut);
-  else if (cut.nsplit > 1)
-    hipLaunchKernelGGL((xst::join_kernel<T, DP, RT, true, xs8::E4m3>), dim3((unsigned)join), dim3(xst::join_threads<DP>(true)), 0, c->stream, a, cut);
+  xs8::Cut8 cut;
+  int64_t grid;
+  if (!cut8(c, a, 16, c->n_cu * per_cu(DP, 1), xst::Shape<DP, 1>::PART, xst::KB, 2 * xst::NW, 4 * xst::NW, &cut, &grid)) return XS_ERR_CAPACITY;
+  const int64_t join = a.seqs * a.kv_heads * cut.tiles * xst::Shape<DP, 1>::VH;
+  if (cut.room && !xs_host_launch_fits(join, xs8::join8_threads<DP, 4>())) return XS_ERR_CAPACITY;
+  hipLaunchKernelGGL((xs8::attend8_kernel<T, DP, 1, EXACT>), dim3((unsigned)grid), dim3(64 * xst::NW), 0, c->stream, a, c8, cut);
+  if (cut.room && many8(cut, a))
+    hipLaunchKernelGGL((xs8::join8_kernel<T, DP, 4>), dim3((unsigned)join), dim3(xs8::join8_threads<DP, 4>()), 0, c->stream, a, cut);
+  else if (cut.room)
+    hipLaunchKernelGGL((xs8::join8_kernel<T, DP, 1>), dim3((unsigned)join), dim3(xs8::join8_threads<DP, 1>()), 0, c->stream, a, cut);
   return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
 }
 
 template <typename T, int DP, int WK, bool EXACT>
 int attend8_wide_run(xs_cache_context* c, const xs_tree_attend_args& a, const xs_kv8& c8) {
   using S = xs8::Shape32<DP, WK>;
-  xs8::Cut32 cut;
-  cut.G = (int32_t)(a.q_heads / a.kv_heads);
-  cut.tiles = (int32_t)((a.nodes * cut.G + S::ROWS - 1) / S::ROWS);
-  cut.scale = a.scale * xst::LOG2E;
-  cut.part = c->part;
-  const int64_t limit = a.max_len ? a.max_len : a.capacity, stages = (limit + xst::SK - 1) / xst::SK + 1;
-  const int64_t units = a.seqs * a.kv_heads * cut.tiles;
-  // the device filled once, by as many workgroups as its LDS holds, as far as
-  // the context has room for their partial results
-  const int64_t most = std::min<int64_t>(c->n_cu * (DP <= 128 ? 2 : 1), c->part_floats / S::PART);
-  const int64_t nsplit = std::max<int64_t>(1, std::min<int64_t>(xst::SPLITS, most / units));
-  cut.chunk = (int32_t)std::max<int64_t>((stages + nsplit - 1) / nsplit, 4);
-  cut.nsplit = (int32_t)((stages + cut.chunk - 1) / cut.chunk);
-  if (cut.nsplit > most / units) cut.nsplit = 1, cut.chunk = (int32_t)stages;  // (not worth a join, or no room)
-  const int64_t groups = a.seqs * a.kv_heads * cut.nsplit;
-  const int64_t grid = (groups + 7) / 8 * 8 * cut.tiles, join = a.seqs * a.kv_heads * cut.tiles * S::WR * S::DT;
-  const bool few = cut.nsplit <= xst::FEW;
-  if (!xs_host_launch_fits(grid, 64 * xst::NW) || (cut.nsplit > 1 && !xs_host_launch_fits(join, xs8::join32_threads(few)))) return XS_ERR_CAPACITY;
-  cut.groups = (int32_t)groups;
+  xs8::Cut8 cut;
+  int64_t grid;
+  // (as many workgroups as a CU's LDS holds)
+  if (!cut8(c, a, S::ROWS, c->n_cu * (DP <= 128 ? 2 : 1), S::PART, xst::SK, xs8::STAGES_LEAST, xs8::STAGES_WHOLE, &cut, &grid)) return XS_ERR_CAPACITY;
+  const int64_t join = a.seqs * a.kv_heads * cut.tiles * S::WR * S::DT;
+  if (cut.room && !xs_host_launch_fits(join, 1024)) return XS_ERR_CAPACITY;
   hipLaunchKernelGGL((xs8::attend8_wide_kernel<T, DP, WK, EXACT>), dim3((unsigned)grid), dim3(64 * xst::NW), 0, c->stream, a, c8, cut);
-  if (cut.nsplit > 1 && few)
-    hipLaunchKernelGGL((xs8::join32_kernel<T, DP, WK, true>), dim3((unsigned)join), dim3(xs8::join32_threads(true)), 0, c->stream, a, cut);
-  else if (cut.nsplit > 1)
-    hipLaunchKernelGGL((xs8::join32_kernel<T, DP, WK, false>), dim3((unsigned)join), dim3(xs8::join32_threads(false)), 0, c->stream, a, cut);
+  if (cut.room && many8(cut, a)) hipLaunchKernelGGL((xs8::join32_kernel<T, DP, WK, 4>), dim3((unsigned)join), dim3(1024), 0, c->stream, a, cut);
+  else if (cut.room) hipLaunchKernelGGL((xs8::join32_kernel<T, DP, WK, 1>), dim3((unsigned)join), dim3(256), 0, c->stream, a, cut);
   return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
 }
 
-template <typename T, int DP, int WK>
-int attend8_wide(xs_cache_context* c, const xs_tree_attend_args& a, const xs_kv8& c8) {
-  return a.head_dim == DP ? attend8_wide_run<T, DP, WK, true>(c, a, c8) : attend8_wide_run<T, DP, WK, false>(c, a, c8);
-}
-
-template <typename T, int DP, int RT>
-int attend8_exact(xs_cache_context* c, const xs_tree_attend_args& a, const xs_kv8& c8) {
-  return a.head_dim == DP ? attend8_run<T, DP, RT, true>(c, a, c8) : attend8_run<T, DP, RT, false>(c, a, c8);
+template <typename T, int DP, bool EXACT>
+int attend8_rows(xs_cache_context* c, const xs_tree_attend_args& a, const xs_kv8& c8) {
+  const int64_t rows = a.nodes * (a.q_heads / a.kv_heads);
+  if (rows <= 16) return attend8_run<T, DP, EXACT>(c, a, c8);
+  if (rows <= 64) return attend8_wide_run<T, DP, 2, EXACT>(c, a, c8);
+  return attend8_wide_run<T, DP, 1, EXACT>(c, a, c8);
 }
 
 template <typename T, int DP>
-int attend8_rows(xs_cache_context* c, const xs_tree_attend_args& a, const xs_kv8& c8) {
-  const int64_t rows = a.nodes * (a.q_heads / a.kv_heads);
-  if (rows <= 16) return attend8_exact<T, DP, 1>(c, a, c8);
-  if (rows <= 32) return attend8_exact<T, DP, 2>(c, a, c8);
-  if (rows <= 64) return attend8_wide<T, DP, 2>(c, a, c8);
-  return attend8_wide<T, DP, 1>(c, a, c8);
+int attend8_exact(xs_cache_context* c, const xs_tree_attend_args& a, const xs_kv8& c8) {
+  return a.head_dim == DP ? attend8_rows<T, DP, true>(c, a, c8) : attend8_rows<T, DP, false>(c, a, c8);
 }
 
 template <typename T>
 int attend8_dim(xs_cache_context* c, const xs_tree_attend_args& a, const xs_kv8& c8) {
-  if (a.head_dim <= 64) return attend8_rows<T, 64>(c, a, c8);
-  if (a.head_dim <= 128) return attend8_rows<T, 128>(c, a, c8);
-  return attend8_rows<T, 256>(c, a, c8);
+  if (a.head_dim <= 64) return attend8_exact<T, 64>(c, a, c8);
+  if (a.head_dim <= 128) return attend8_exact<T, 128>(c, a, c8);
+  return attend8_exact<T, 256>(c, a, c8);
 }
 
 }  // namespace

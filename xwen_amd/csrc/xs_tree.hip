@@ -588,19 +588,6 @@ XS_DEV uint32_t weight_word(float mass, bool held) {
 }
 XS_DEV uint32_t position_word(int pos) { return ~((uint32_t)pos ^ 0x80000000u); }
 
-// Inclusive prefix sums over a wave.
-XS_DEV uint32_t wave_scan(uint32_t v) {
-  // within rows of 16 lanes, then each row's last to the rows after it
-#define XS_STEP(ctrl, rows) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, false)
-  XS_STEP(0x111, 0xF);
-  XS_STEP(0x112, 0xF);
-  XS_STEP(0x114, 0xF);
-  XS_STEP(0x118, 0xF);
-  XS_STEP(0x142, 0xA);
-  XS_STEP(0x143, 0xC);
-#undef XS_STEP
-  return v;
-}
 XS_DEV uint64_t wave_scan(uint64_t v) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
