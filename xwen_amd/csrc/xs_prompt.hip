@@ -172,8 +172,9 @@ __global__ __launch_bounds__(RT, 8) void rotate_kernel(const xs_qk_rotate_args a
 // Causal attention of packed prompts.
 //
 // The rows of one (sequence, kv head) are its tokens times the group of q heads
-// that share the head: row r = token * group + q head.  A workgroup takes 32 NWV
-// rows, 32 a wave (xs_rows32.h), and walks the keys up to its last row's token in
+// that share the head: row r = token * group + q head.  A workgroup takes 128 / WK
+// rows, 32 a wave (xs_rows32.h; WK waves share them, each with its half of a stage's
+// keys, and add up at the end), and walks the keys up to its last row's token in
 // stages of 64, through two LDS buffers that loads fill while the other is read.
 
 // The sequence and the row tile of a workgroup: tiles of the device's valid
@@ -187,68 +188,61 @@ template <int ROWS>
 XS_DEV Place place(const xs_prompt_attend_args& a, int G, int64_t want, bool report) {
   const int lane = threadIdx.x & 63;
   Place p = {-1, 0, 0, 0};
-  int high = 0;         // the largest entry of start so far
-  int64_t before = 0;   // tiles of earlier sequences
-  const bool small = a.seqs <= 64;
+  int high = 0;        // the largest entry of start so far
+  uint32_t before = 0; // tiles of earlier sequences (2^30 rows at most)
+  auto last = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(v), 63); };
   for (int64_t b0 = 0; b0 < a.seqs; b0 += 64) {
     const int64_t b = b0 + lane;
     const bool in = b < a.seqs;
-    const int s = in ? a.start[b] : 0, e = in ? a.start[b + 1] : 0;
-    int top = in ? s : INT32_MIN;  // inclusive prefix maximum
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-      const int y = __shfl_up(top, m);
-      if (lane >= m) top = max(top, y);
-    }
-    top = max(top, high);
-    high = __shfl(top, 63);
-    const bool good = in && s >= top && e >= s && e <= a.tokens;
-    if (report && in) a.seq_status[b] = good ? XS_ROW_OK : XS_ROW_BAD_PARAM;
-    const int tiles = good ? (int)(((int64_t)(e - s) * G + ROWS - 1) / ROWS) : 0;
-    if (p.b >= 0) continue;  // (found; the rest is only reported)
-    int who = -1, tile = 0;
-    if (small) {
-      // above(L): tiles at a level past L, the level of a tile its place in its sequence
-      auto above = [&](int L) {
-        int64_t v = max(0, tiles - L);
-#pragma unroll
-        for (int m = 1; m < 64; m *= 2) v += __shfl_xor(v, m);
-        return v;
-      };
-      int lo = 0, hi = tiles;  // the largest L with above(L) > want
-#pragma unroll
-      for (int m = 1; m < 64; m *= 2) hi = max(hi, __shfl_xor(hi, m));
-      if (above(0) <= want) return p;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (above(mid) > want) lo = mid;
-        else hi = mid;
-      }
-      const int nth = (int)(want - above(lo + 1));
-      uint64_t have = __ballot(tiles > lo);
-      for (int i = 0; i < nth; i++) have &= have - 1;
-      who = __ffsll((unsigned long long)have) - 1;
-      tile = lo;
-    } else {
-      int64_t upto = tiles;
+    const int s = in ? a.start[b] : INT32_MIN, e = in ? a.start[b + 1] : 0;
+    int top = s;  // inclusive prefix maximum
+    const int prev = __shfl_up(s, 1);
+    if (__any(in && lane > 0 && prev > s)) {  // (rare)
 #pragma unroll
       for (int m = 1; m < 64; m *= 2) {
-        const int64_t y = __shfl_up(upto, m);
-        if (lane >= m) upto += y;
+        const int y = __shfl_up(top, m);
+        if (lane >= m) top = max(top, y);
       }
-      upto += before;
+    }
+    top = max(top, high);
+    const bool good = in && s >= top && e >= s && e <= a.tokens;
+    if (report && in) a.seq_status[b] = good ? XS_ROW_OK : XS_ROW_BAD_PARAM;
+    if (b0 + 64 < a.seqs) high = __builtin_amdgcn_readlane(top, 63);
+    if (p.b >= 0) continue;  // (found; the rest is only reported)
+    const uint32_t tiles = good ? (uint32_t)(((int64_t)(e - s) * G + ROWS - 1) / ROWS) : 0u;
+    int who = -1, tile = 0;
+    if (a.seqs == 1) {
+      tile = __builtin_amdgcn_readlane((int)tiles, 0) - 1 - (int)want;
+      if (tile >= 0) who = 0;
+    } else if (a.seqs <= 64) {
+      // above(L): tiles at a level past L, the level of a tile its place in its sequence
+      auto above = [&](uint32_t L) { return last(tiles > L ? tiles - L : 0u); };
+      if (above(0) > want) {
+        uint32_t lo = 0, hi = above(0);  // the largest L with above(L) > want
+        while (hi - lo > 1) {
+          const uint32_t mid = (lo + hi) / 2;
+          if (above(mid) > want) lo = mid;
+          else hi = mid;
+        }
+        uint64_t have = __ballot(tiles > lo);
+        for (uint32_t i = above(lo + 1); i < want; i++) have &= have - 1;
+        who = __ffsll((unsigned long long)have) - 1;
+        tile = (int)lo;
+      }
+    } else {
+      const uint32_t upto = wave_scan(tiles) + before;
       const uint64_t past = __ballot(upto > want);
-      before = __shfl(upto, 63);
+      before = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
       if (past) {
         who = __ffsll((unsigned long long)past) - 1;
-        tile = (int)(__shfl(upto, who) - 1 - want);  // the last of a sequence first
+        tile = __builtin_amdgcn_readlane((int)upto, who) - 1 - (int)want;  // the last of a sequence first
       }
     }
     if (who >= 0) {
       p.b = (int)b0 + who;
       p.tile = tile;
-      p.first = __shfl(s, who);
-      p.n = __shfl(e, who) - p.first;
+      p.first = __builtin_amdgcn_readlane(s, who);
+      p.n = __builtin_amdgcn_readlane(e, who) - p.first;
       if (!report) return p;
     }
   }
@@ -265,16 +259,16 @@ XS_DEV void load_lds(const uint16_t* base, uint32_t bytes, u32x4* to) {
 }
 XS_DEV void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-template <typename T, int DP, int NWV, bool EXACT>
-__global__ __launch_bounds__(64 * NWV, DP <= 128 ? 2 : 1) void prompt_kernel(const xs_prompt_attend_args a, float scale) {
+template <typename T, int DP, int WK, bool EXACT>
+__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_kernel(const xs_prompt_attend_args a, float scale) {
   using K = Keys<DP>;
-  constexpr int KC = DP / 16, DT = DP / 32, ROWS = 32 * NWV, CH = K::CH, STAGE = K::STAGE;
-  constexpr int PER = STAGE / (64 * NWV);             // of a thread
-  static_assert(STAGE % (64 * NWV) == 0, "a stage is whole chunks of every thread");
+  constexpr int KC = DP / 16, DT = DP / 32, ROWS = 32 * NW / WK, CH = K::CH, STAGE = K::STAGE;
+  constexpr int PER = STAGE / (64 * NW);             // of a thread
+  static_assert(STAGE % (64 * NW) == 0, "a stage is whole chunks of every thread");
   __shared__ u32x4 lds[2][2][STAGE];                  // [buffer][k, v]
   __shared__ int odds;
   const int lane = threadIdx.x & 63, x = lane & 31, g = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / WK, wk = wave % WK;
   const int G = (int)(a.q_heads / a.kv_heads);
   const int kh = (int)(blockIdx.x % (unsigned)a.kv_heads);
   const Place at = place<ROWS>(a, G, blockIdx.x / (unsigned)a.kv_heads, blockIdx.x == 0 && wave == 0);
@@ -282,13 +276,41 @@ __global__ __launch_bounds__(64 * NWV, DP <= 128 ? 2 : 1) void prompt_kernel(con
   if (b < 0) return;
   const int n = __builtin_amdgcn_readfirstlane(at.n), t0 = __builtin_amdgcn_readfirstlane(at.first);
   const int R = n * G;
-  const int row0 = __builtin_amdgcn_readfirstlane(at.tile) * ROWS, wrow = row0 + 32 * wave;
+  const int row0 = __builtin_amdgcn_readfirstlane(at.tile) * ROWS, wrow = row0 + 32 * wr;
   const int row = wrow + x, token = min(row, R - 1) / G, head = kh * G + min(row, R - 1) % G;
   const int low = min(wrow, R - 1) / G, top_token = min(wrow + 31, R - 1) / G;  // of the wave's rows
   const int wg_low = row0 / G;                                                 // of the workgroup's
   const int end = min(row0 + ROWS - 1, R - 1) / G + 1;                         // keys that it needs
   const int stages = (end + SK - 1) / SK;
   const bool live = wrow < R;
+
+  // A stage's chunks, each by the lane whose place in LDS it takes.  Chunks past
+  // the head's end are zero from the start.
+  const uint16_t* kp = (const uint16_t*)a.k + (int64_t)t0 * a.kv_token_stride + kh * a.kv_head_stride;
+  const uint16_t* vp = (const uint16_t*)a.v + (int64_t)t0 * a.kv_token_stride + kh * a.kv_head_stride;
+  if (!EXACT) {
+#pragma unroll
+    for (int i = 0; i < 4 * PER; i++) (&lds[0][0][0])[i * 64 * NW + threadIdx.x] = (u32x4){0, 0, 0, 0};
+    __syncthreads();
+  }
+  auto fetch = [&](int s) {
+    const int64_t o = (int64_t)s * SK * a.kv_token_stride;
+    const int last = n - 1 - s * SK;
+    const uint32_t stride = 2 * (uint32_t)a.kv_token_stride;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const int u = i * 64 * NW + threadIdx.x, r = u / CH, ck = u % CH ^ K::turn_k(r), cv = u % CH ^ K::turn_v(r);
+      const uint32_t rows = (uint32_t)min(r, last) * stride;
+      u32x4* to = &lds[s & 1][0][i * 64 * NW + 64 * wave];
+      if (EXACT || 8 * ck < a.head_dim) load_lds(kp + o, rows + 16u * ck, to);
+      if (EXACT || 8 * cv < a.head_dim) load_lds(vp + o, rows + 16u * cv, to + STAGE);
+    }
+  };
+
+  fetch(0);
+  const Reads<DP> reads;
+  int odd = 0;
+  if (threadIdx.x == 0) odds = 0;
 
   Rows32<T, DP, 1> w;
   w.init();
@@ -300,34 +322,6 @@ __global__ __launch_bounds__(64 * NWV, DP <= 128 ? 2 : 1) void prompt_kernel(con
       w.q[0][c] = row < R && (EXACT || d < a.head_dim) ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0};
     }
   }
-  // A stage's chunks, each by the lane whose place in LDS it takes.  Chunks past
-  // the head's end are zero from the start.
-  const uint16_t* kp = (const uint16_t*)a.k + (int64_t)t0 * a.kv_token_stride + kh * a.kv_head_stride;
-  const uint16_t* vp = (const uint16_t*)a.v + (int64_t)t0 * a.kv_token_stride + kh * a.kv_head_stride;
-  if (!EXACT) {
-#pragma unroll
-    for (int i = 0; i < 4 * PER; i++) (&lds[0][0][0])[i * 64 * NWV + threadIdx.x] = (u32x4){0, 0, 0, 0};
-    __syncthreads();
-  }
-  auto fetch = [&](int s) {
-    const int64_t o = (int64_t)s * SK * a.kv_token_stride;
-    const int last = n - 1 - s * SK;
-    const uint32_t stride = 2 * (uint32_t)a.kv_token_stride;
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-      const int u = i * 64 * NWV + threadIdx.x, r = u / CH, ck = u % CH ^ K::turn_k(r), cv = u % CH ^ K::turn_v(r);
-      const uint32_t rows = (uint32_t)min(r, last) * stride;
-      u32x4* to = &lds[s & 1][0][i * 64 * NWV + 64 * wave];
-      if (EXACT || 8 * ck < a.head_dim) load_lds(kp + o, rows + 16u * ck, to);
-      if (EXACT || 8 * cv < a.head_dim) load_lds(vp + o, rows + 16u * cv, to + STAGE);
-    }
-  };
-
-  const Reads<DP> reads;
-  int odd = 0;
-  if (threadIdx.x == 0) odds = 0;
-
-  fetch(0);
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the rows' loads too, which the loop would wait for at every stage
   for (int s = 0; s < stages; s++) {
     arrived();
@@ -340,7 +334,7 @@ __global__ __launch_bounds__(64 * NWV, DP <= 128 ? 2 : 1) void prompt_kernel(con
       bool found = false;
 #pragma unroll
       for (int i = 0; i < PER; i++) {
-        const u32x4 v = lds[s & 1][1][i * 64 * NWV + threadIdx.x];
+        const u32x4 v = lds[s & 1][1][i * 64 * NW + threadIdx.x];
 #pragma unroll
         for (int j = 0; j < 4; j++) found |= (v[j] & 0x7FFFu) >= inf_of(T{}) || ((v[j] >> 16) & 0x7FFFu) >= inf_of(T{});
       }
@@ -350,25 +344,59 @@ __global__ __launch_bounds__(64 * NWV, DP <= 128 ? 2 : 1) void prompt_kernel(con
         odd = 1;
 #pragma unroll
         for (int i = 0; i < PER; i++) {
-          u32x4 v = lds[s & 1][1][i * 64 * NWV + threadIdx.x];
+          u32x4 v = lds[s & 1][1][i * 64 * NW + threadIdx.x];
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             if ((v[j] & 0x7FFFu) >= inf_of(T{})) v[j] &= 0xFFFF0000u;
             if (((v[j] >> 16) & 0x7FFFu) >= inf_of(T{})) v[j] &= 0xFFFFu;
           }
-          lds[s & 1][1][i * 64 * NWV + threadIdx.x] = v;
+          lds[s & 1][1][i * 64 * NW + threadIdx.x] = v;
         }
         __syncthreads();
       }
     }
     if (live && s * SK <= top_token) {
-      w.template step<2, 1>(reads, {lds[s & 1][0]}, {lds[s & 1][1]}, scale, s * SK + SK - 1 > low, Upto{token - s * SK - 4 * g});
+      const bool masked = s * SK + SK - 1 > low;
+      if constexpr (WK == 1 && DP <= 128) {
+        w.template step<2, 1>(reads, {lds[s & 1][0]}, {lds[s & 1][1]}, scale, masked, Upto{token - s * SK - 4 * g});
+      } else {
+        // a tile of 32 keys at a time: a wave's own, or what the registers hold
+#pragma unroll
+        for (int i = 0; i < 2 / WK; i++) {
+          const int u = WK == 1 ? i : wk;
+          w.template step<1, 1>(reads, {lds[s & 1][0] + 32 * u * CH}, {lds[s & 1][1] + 32 * u * CH}, scale, masked, Upto{token - s * SK - 32 * u - 4 * g});
+        }
+      }
     }
   }
 
-  if (row >= R) return;
-  const float l = pair_sum(w.l);
+  float l = pair_sum(w.l), ref = l == 0.0f ? NEG_INF : scale < 0.0f ? -w.reference() : w.reference();
   f32x16(&o)[DT] = w.o;
+  if constexpr (WK == 2) {  // the two waves of the rows add up
+    __syncthreads();        // (the last stage's readers)
+    f32x16* sum = (f32x16*)&lds[0][0][0] + wr * DT * 64;
+    float* stat = (float*)&lds[1][0][0] + wr * 128;
+    if (wk == 1) {
+#pragma unroll
+      for (int d = 0; d < DT; d++) sum[d * 64 + lane] = o[d];
+      stat[lane] = ref;
+      stat[64 + lane] = l;
+    }
+    __syncthreads();
+    if (wk == 1) return;
+    const float ref1 = stat[lane], l1 = stat[64 + lane], top = fmaxf(ref, ref1), mag = fabsf(scale);
+    // (a half without weights may hold what its masked products left)
+    const float f0 = ref == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((ref - top) * mag), f1 = ref1 == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((ref1 - top) * mag);
+    l = (ref == NEG_INF ? 0.0f : l * f0) + (ref1 == NEG_INF ? 0.0f : l1 * f1);
+#pragma unroll
+    for (int d = 0; d < DT; d++) {
+      const f32x16 y = sum[d * 64 + lane];
+#pragma unroll
+      for (int i = 0; i < 16; i++) o[d][i] = (ref == NEG_INF ? 0.0f : o[d][i] * f0) + (ref1 == NEG_INF ? 0.0f : y[i] * f1);
+    }
+    ref = top;
+  }
+  if (row >= R) return;
   if (l == 0.0f) {  // every score -inf
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = fill16(0.0f);
@@ -398,7 +426,7 @@ __global__ __launch_bounds__(64 * NWV, DP <= 128 ? 2 : 1) void prompt_kernel(con
     }
   if (a.lse && g == 0)
     a.lse[(int64_t)(t0 + token) * a.q_heads + head] =
-        l == 0.0f ? NEG_INF : __builtin_fmaf(w.reference(), a.scale, LN2 * (__builtin_amdgcn_logf(l) - offset_of(T{})));
+        l == 0.0f ? NEG_INF : __builtin_fmaf(ref, fabsf(a.scale), LN2 * (__builtin_amdgcn_logf(l) - offset_of(T{})));
 }
 
 // No token: only the sequences' statuses.
@@ -438,19 +466,27 @@ int rotate_dim(xs_cache_context* c, const xs_qk_rotate_args& a) {
   return rotate_lanes<T, 16>(c, a);
 }
 
-template <typename T, int DP, int NWV, bool EXACT>
+template <typename T, int DP, int WK, bool EXACT>
 int prompt_run(xs_cache_context* c, const xs_prompt_attend_args& a) {
-  const int64_t rows = a.tokens * (a.q_heads / a.kv_heads), tile = 32 * NWV;
+  const int64_t rows = a.tokens * (a.q_heads / a.kv_heads), tile = 32 * xst::NW / WK;
   // no more tiles than this, whatever the sequences' lengths: each leaves less than one
   const int64_t grid = (rows / tile + std::min(a.seqs, a.tokens)) * a.kv_heads;
-  if (!xs_host_launch_fits(grid, 64 * NWV)) return XS_ERR_CAPACITY;
-  hipLaunchKernelGGL((xsp::prompt_kernel<T, DP, NWV, EXACT>), dim3((unsigned)grid), dim3(64 * NWV), 0, c->stream, a, a.scale * xst::LOG2E);
+  if (!xs_host_launch_fits(grid, 64 * xst::NW)) return XS_ERR_CAPACITY;
+  hipLaunchKernelGGL((xsp::prompt_kernel<T, DP, WK, EXACT>), dim3((unsigned)grid), dim3(64 * xst::NW), 0, c->stream, a, a.scale * xst::LOG2E);
   return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
+}
+
+// Rows of 128 a workgroup, or of 64 where those do not fill the device (@WK@).
+template <typename T, int DP, bool EXACT>
+int prompt_rows(xs_cache_context* c, const xs_prompt_attend_args& a) {
+  const int64_t held = c->n_cu * (DP <= 128 ? 2 : 1);
+  if (a.tokens * a.q_heads < held * 128) return prompt_run<T, DP, 2, EXACT>(c, a);
+  return prompt_run<T, DP, 1, EXACT>(c, a);
 }
 
 template <typename T, int DP>
 int prompt_exact(xs_cache_context* c, const xs_prompt_attend_args& a) {
-  return a.head_dim == DP ? prompt_run<T, DP, 4, true>(c, a) : prompt_run<T, DP, 4, false>(c, a);
+  return a.head_dim == DP ? prompt_rows<T, DP, true>(c, a) : prompt_rows<T, DP, false>(c, a);
 }
 
 template <typename T>
