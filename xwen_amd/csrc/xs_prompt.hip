@@ -185,7 +185,7 @@ struct Place {
 };
 
 template <int ROWS>
-XS_DEV Place place(const xs_prompt_attend_args& a, int G, int64_t want, bool report) {
+XS_DEV Place place(const xs_prompt_attend_args& a, int G, uint32_t want, bool report) {
   const int lane = threadIdx.x & 63;
   Place p = {-1, 0, 0, 0};
   int high = 0;        // the largest entry of start so far
@@ -211,14 +211,15 @@ XS_DEV Place place(const xs_prompt_attend_args& a, int G, int64_t want, bool rep
     if (p.b >= 0) continue;  // (found; the rest is only reported)
     const uint32_t tiles = good ? (uint32_t)(((int64_t)(e - s) * G + ROWS - 1) / ROWS) : 0u;
     int who = -1, tile = 0;
-    if (a.seqs == 1) {
-      tile = __builtin_amdgcn_readlane((int)tiles, 0) - 1 - (int)want;
-      if (tile >= 0) who = 0;
-    } else if (a.seqs <= 64) {
+    if (a.seqs <= 64) {
       // above(L): tiles at a level past L, the level of a tile its place in its sequence
       auto above = [&](uint32_t L) { return last(tiles > L ? tiles - L : 0u); };
-      if (above(0) > want) {
-        uint32_t lo = 0, hi = above(0);  // the largest L with above(L) > want
+      const uint32_t total = above(0);
+      if (a.seqs == 1) {
+        tile = (int)total - 1 - (int)want;
+        if (tile >= 0) who = 0;
+      } else if (total > want) {
+        uint32_t lo = 0, hi = total;  // the largest L with above(L) > want
         while (hi - lo > 1) {
           const uint32_t mid = (lo + hi) / 2;
           if (above(mid) > want) lo = mid;
@@ -260,7 +261,7 @@ XS_DEV void load_lds(const uint16_t* base, uint32_t bytes, u32x4* to) {
 XS_DEV void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 template <typename T, int DP, int WK, bool EXACT>
-__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_kernel(const xs_prompt_attend_args a, float scale) {
+__global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void prompt_kernel(const xs_prompt_attend_args a, float scale) {
   using K = Keys<DP>;
   constexpr int KC = DP / 16, DT = DP / 32, ROWS = 32 * NW / WK, CH = K::CH, STAGE = K::STAGE;
   constexpr int PER = STAGE / (64 * NW);             // of a thread
@@ -430,7 +431,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_kernel(cons
 }
 
 // No token: only the sequences' statuses.
-__global__ __launch_bounds__(64) void prompt_status_kernel(const xs_prompt_attend_args a) { place<64>(a, 1, INT64_MAX, true); }
+__global__ __launch_bounds__(64) void prompt_status_kernel(const xs_prompt_attend_args a) { place<64>(a, 1, UINT32_MAX, true); }
 
 }  // namespace xsp
 
@@ -479,8 +480,9 @@ int prompt_run(xs_cache_context* c, const xs_prompt_attend_args& a) {
 // Rows of 128 a workgroup, or of 64 where those do not fill the device (@WK@).
 template <typename T, int DP, bool EXACT>
 int prompt_rows(xs_cache_context* c, const xs_prompt_attend_args& a) {
-  const int64_t held = c->n_cu * (DP <= 128 ? 2 : 1);
-  if (a.tokens * a.q_heads < held * 128) return prompt_run<T, DP, 2, EXACT>(c, a);
+  if constexpr (DP <= 128) {
+    if (a.tokens * a.q_heads < c->n_cu * 2 * 128) return prompt_run<T, DP, 2, EXACT>(c, a);
+  }
   return prompt_run<T, DP, 1, EXACT>(c, a);
 }
 

@@ -11,8 +11,9 @@
 //                 through transposing LDS reads, four keys of a column each
 //
 // The softmax is that of xs_attend.h: one pass, a running reference which is one
-// of the row's own scores, products that start from it, moved only when the best
-// has grown by 2^8.
+// of the row's own scores, products that start from it.  It moves when a lane's
+// weights of a step add up to more than 2^8, which their sum, needed anyway, says
+// without a maximum (@MAX@).
 #pragma once
 
 #include "xs_attend.h"
@@ -118,13 +119,13 @@ struct Rows32 {
   static constexpr int KC = DP / 16, DT = DP / 32;
   u32x4 q[NQ][KC];
   f32x16 o[DT], base;  // base: minus the reference, which the products start from
-  float most, l;       // the x above which the reference moves: NaN until the row's first score
+  float most, l;       // the sum of a step's weights above which the reference moves: -1 until the row's first score
 
   XS_DEV void init() {
     base = fill16(-0.0f);
 #pragma unroll
     for (int d = 0; d < DT; d++) o[d] = fill16(0.0f);
-    most = __builtin_nanf("");
+    most = -1.0f;
     l = 0.0f;
   }
   XS_DEV float reference() const { return -base[0]; }
@@ -139,39 +140,64 @@ struct Rows32 {
     f32x16 s[U];
 #pragma unroll
     for (int u = 0; u < U; u++) s[u] = base;
+    // fragments AHEAD of their products, so that LDS answers beside the others'
+    constexpr int AHEAD = 2, STEPS = KN * KC;
+    u32x4 k[AHEAD + 1][U];
 #pragma unroll
-    for (int m = 0; m < KN; m++)
+    for (int i = 0; i < AHEAD; i++)
 #pragma unroll
-      for (int c = 0; c < KC; c++)
+      for (int u = 0; u < U; u++) k[i][u] = at.key(ks[i / KC], kt, u, i % KC);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-          const u32x4 k = at.key(ks[m], kt, u, c);
+    for (int i = 0; i < STEPS; i++) {
+      if (i + AHEAD < STEPS) {
 #pragma unroll
-          for (int n = 0; n < NQ; n++) s[u] = mfma32(M{}, k, q[n][c], s[u]);
-        }
-    float x[U][16], top;
+        for (int u = 0; u < U; u++) k[(i + AHEAD) % (AHEAD + 1)][u] = at.key(ks[(i + AHEAD) / KC], kt, u, (i + AHEAD) % KC);
+      }
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int n = 0; n < NQ; n++) s[u] = mfma32(M{}, k[i % (AHEAD + 1)][u], q[n][i % KC], s[u]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    u32x4 v[2][U][2];
+    auto values = [&](int i) {
+#pragma unroll
+      for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int c = 0; c < 2; c++) v[i & 1][u][c] = at.value(vs[i / DT], vt, i % DT, u, c);
+    };
+    values(0);
+    __builtin_amdgcn_sched_barrier(0);
+    // (the other wave of the SIMD, in its products, needs an issue only every 32 cycles)
+    __builtin_amdgcn_s_setprio(1);
+    float p[U][16], sum;
     auto weigh = [&](bool from0, float ref, const On& on) {
 #pragma unroll
       for (int u = 0; u < U; u++)
 #pragma unroll
         for (int r = 0; r < 16; r++) {
           const float v = from0 ? s[u][r] - ref : s[u][r];
-          x[u][r] = OFF == 0.0f ? v * scale : __builtin_fmaf(v, scale, OFF);
+          p[u][r] = OFF == 0.0f ? v * scale : __builtin_fmaf(v, scale, OFF);
         }
       if (masked) {
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
-          for (int r = 0; r < 16; r++) x[u][r] = on(32 * u + 8 * (r / 4) + r % 4) ? x[u][r] : NEG_INF;
+          for (int r = 0; r < 16; r++) p[u][r] = on(32 * u + 8 * (r / 4) + r % 4) ? p[u][r] : NEG_INF;
       }
-      top = NEG_INF;
+      sum = 0.0f;
 #pragma unroll
       for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) top = fmaxf(top, x[u][r]);
+        for (int r = 0; r < 16; r += 4) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) p[u][r + e] = __builtin_amdgcn_exp2f(p[u][r + e]);
+          sum += (p[u][r] + p[u][r + 1]) + (p[u][r + 2] + p[u][r + 3]);
+        }
     };
     weigh(false, 0.0f, on);
-    if (__any(!(top <= most))) [[unlikely]] {
+    if (__any(sum > most)) [[unlikely]] {  // (a NaN does not move it: the row is lost)
       // the references of the rows that have grown move to their best scores
       const On rare = on.again();
       asm volatile("" : "+v"(kt));
@@ -189,7 +215,7 @@ struct Rows32 {
           }
       }
       const float sign = scale < 0.0f ? -1.0f : 1.0f, old = reference();
-      const bool unset = most != most;
+      const bool unset = most < 0.0f;
       // never below the old one (a product that starts elsewhere rounds elsewhere)
       float best = unset ? NEG_INF : old * sign;
 #pragma unroll
@@ -205,41 +231,40 @@ struct Rows32 {
         ref = scale == 0.0f ? 0.0f : best * sign;
         const float keep = unset ? 0.0f : __builtin_amdgcn_exp2f((old - ref) * scale);
         base = fill16(-ref);
-        most = LAZY + OFF;
+        most = OFF == 0.0f ? 0x1p8f : 0x1p14f;  // (2^(8 + OFF))
         l *= keep;
 #pragma unroll
         for (int d = 0; d < DT; d++) o[d] *= keep;
       }
       weigh(true, ref, rare.again());
     }
+    l += sum;
     u32x4 pf[NQ][U][2];
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
       for (int c = 0; c < 2; c++) {
-        float p[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) p[e] = __builtin_amdgcn_exp2f(x[u][8 * c + e]);
-        l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          pf[0][u][c][e] = pack2(M{}, p[2 * e], p[2 * e + 1]);
+          const float y0 = p[u][8 * c + 2 * e], y1 = p[u][8 * c + 2 * e + 1];
+          pf[0][u][c][e] = pack2(M{}, y0, y1);
           if constexpr (NQ == 2)
-            pf[1][u][c][e] = pack2(M{}, p[2 * e] - M::widen((uint16_t)pf[0][u][c][e]), p[2 * e + 1] - M::widen((uint16_t)(pf[0][u][c][e] >> 16)));
+            pf[1][u][c][e] = pack2(M{}, y0 - M::widen((uint16_t)pf[0][u][c][e]), y1 - M::widen((uint16_t)(pf[0][u][c][e] >> 16)));
         }
       }
+    __builtin_amdgcn_s_setprio(0);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int m = 0; m < KN; m++)
+    for (int i = 0; i < KN * DT; i++) {
+      if (i + 1 < KN * DT) values(i + 1);
 #pragma unroll
-      for (int d = 0; d < DT; d++)
+      for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int u = 0; u < U; u++)
+        for (int c = 0; c < 2; c++)
 #pragma unroll
-          for (int c = 0; c < 2; c++) {
-            const u32x4 v = at.value(vs[m], vt, d, u, c);
-#pragma unroll
-            for (int n = 0; n < NQ; n++) o[d] = mfma32(M{}, v, pf[n][u][c], o[d]);
-          }
+          for (int n = 0; n < NQ; n++) o[i % DT] = mfma32(M{}, v[i & 1][u][c], pf[n][u][c], o[i % DT]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   }
 };
 
