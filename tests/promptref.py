@@ -163,3 +163,32 @@ class Cache:
             x = t.double().cpu()
             same = (x == byte) | (torch.isnan(x) & torch.isnan(byte))
             assert bool(same.all()), same.logical_not().nonzero()[:4].tolist()
+
+
+def prompt_wide(q, k, v, start, scale):
+    """prompt() of finite inputs on the device, a head's whole square of scores at a time."""
+    T, HQ, D = q.shape
+    H = k.shape[1]
+    u = half_step(q.dtype)
+    out = torch.full((T, HQ, D), math.nan, dtype=torch.float64)
+    lse = torch.full((T, HQ), math.nan, dtype=torch.float64)
+    tol, ltol = torch.zeros_like(out), torch.zeros_like(lse)
+    for first, last in zip(start, start[1:]):
+        n = last - first
+        if n == 0:
+            continue
+        seen = torch.ones((n, n), dtype=torch.bool, device=q.device).tril()
+        count = torch.arange(1, n + 1, dtype=torch.float64, device=q.device)[:, None]
+        for h in range(HQ):
+            x, kh, vh = q[first:last, h].double(), k[first:last, h // (HQ // H)].double(), v[first:last, h // (HQ // H)].double()
+            s = (x @ kh.T.contiguous() * scale).masked_fill_(~seen, -math.inf)
+            p = s.softmax(-1)
+            y, around, z = p @ vh, p @ vh.abs(), s.logsumexp(-1, keepdim=True)
+            off = (D + 4) * F32 * ((x.abs() @ kh.abs().T.contiguous()) * seen).amax(-1, keepdim=True) * abs(scale)
+            off = off + 8 * F32 * (1 + s.abs().masked_fill_(~seen, 0).amax(-1, keepdim=True))
+            t = u * y.abs() * 1.01 + around * (u * 1.01 + 2 * off + 2 * (count + 8) * F32)
+            if q.dtype == torch.float16:
+                t = t + 2.0**-25 * (1 + count)
+            out[first:last, h], lse[first:last, h], tol[first:last, h] = y.cpu(), z[:, 0].cpu(), t.cpu()
+            ltol[first:last, h] = (off + (count + 8) * F32 + 4 * F32 * z.abs())[:, 0].cpu()
+    return out, lse, tol, ltol

@@ -264,6 +264,31 @@ def test_attend_long(ctx, nodes, hq, h, d, dtype):
     agree(c, s, look(ctx, c, s, max_len=8000))
 
 
+@pytest.mark.parametrize("nodes", [1, 5, 20])
+@pytest.mark.parametrize("seqs,h", [(70, 1), (64, 16), (300, 1)])
+def test_attend_many_sequences(seqs, h, nodes):
+    """More than a wave of them, as many as the device has places, and too many to be split; long and
+    short ones, empty and failing ones among them."""
+    from xwen_amd import tree
+    big = tree.CacheContext(max_seqs=seqs, max_nodes=nodes, q_heads=4 * h, kv_heads=h, head_dim=64, capacity=1600)
+    rng = np.random.default_rng(seqs + nodes)
+    lens = rng.integers(0, 40, seqs).tolist()
+    lens[3], lens[seqs // 2], lens[-1] = 1500, 700, 600
+    c = filled(lens, h, 64, cap=1600)
+    used = rng.integers(0, nodes + 1, seqs).tolist()
+    used[3], used[seqs // 2], used[-1] = nodes, nodes, 1
+    s = step(rng, c, nodes, 4 * h, BF, used=used)
+    agree(c, s, look(big, c, s))
+    got, bad = look(big, c, s), seqs // 2 - 1
+    c["len"][bad], c["len"][5] = -1, 1601
+    again = look(big, c, s)
+    assert [i for i, x in enumerate(again.seq_status.tolist()) if x] == sorted([5, bad])
+    # the others' shares may be cut elsewhere now: two roundings of a mean of values below 4 in
+    # bf16 (2^-8 of it at most each), and of its weights (as much again, averaged)
+    keep = [i for i in range(seqs) if i not in (5, bad)]
+    assert bool((again.out[5] == 7).all()) and bool(((again.out[keep].float() - got.out[keep].float()).abs() <= 2.0**-5).all())
+
+
 @pytest.mark.parametrize("dtype", [BF, HF])
 def test_attend_scales_of_any_size(ctx, dtype):
     """Blocks whose values differ by many powers of two (past f16's range), keys' and values'."""

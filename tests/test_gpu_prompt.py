@@ -76,6 +76,27 @@ def test_long_with_large_scores(ctx, hq, h, d, dtype):
     agree(c, run(ctx, c))
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("d", [64, 72, 96, 128])
+def test_enough_rows_to_fill_the_device(ctx, d, dtype):
+    """128 rows a workgroup: from 65,536 rows (tokens times q heads) on."""
+    c = case([1700, 0, 1, 333, 70], 32, 4, d, dtype, packed=True, spread=1.5, front=1)
+    got = run(ctx, c)
+    assert got.seq_status.tolist() == [0] * 5
+    promptref.agree(got.out, got.lse, promptref.prompt_wide(c["q"], c["k"], c["v"], c["start"], float(np.float32(1 / math.sqrt(d)))), left=7.0)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_what_is_not_finite_with_many_rows(ctx, dtype):
+    c = case([1000, 1100], 32, 2, 128, dtype)
+    clean = run(ctx, c)
+    c["v"][500, 0, 3], c["v"][501, 1, 4], c["k"][700, 0, 5] = math.inf, math.nan, math.nan
+    got = run(ctx, c)
+    assert torch.equal(got.out[:500], clean.out[:500]) and torch.equal(got.out[1000:], clean.out[1000:])
+    assert bool((got.out[500:700, :16, 3] == math.inf).all()) and bool(torch.isnan(got.out[501:1000, 16:, 4]).all())
+    assert bool(torch.isnan(got.out[700:1000, :16]).all()) and torch.equal(got.out[500:1000, 16:, 5:], clean.out[500:1000, 16:, 5:])
+
+
 def test_many_sequences(ctx):
     """More than a wave of them, empty ones among them."""
     rng = np.random.default_rng(1)
