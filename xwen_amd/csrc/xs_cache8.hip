@@ -437,17 +437,17 @@ XS_DEV void tree_block(Tile<T, DP, RT>& z, const uint16_t* kp, const uint16_t* v
 // is one for all sequences, so that long and short ones' workgroups end together:
 // the smallest that leaves no more splits than the device holds at once, `room`
 // for each head and row tile, so that no workgroup starts when the others end (as
-// many splits for every sequence instead, 32 of 327 to 8,192 slots: @RAG0@ us for
-// @RAG2@).  The lengths are on the device, so every workgroup finds the share and
+// many splits for every sequence instead, 32 of 327 to 8,192 slots: 87 us for
+// 81).  The lengths are on the device, so every workgroup finds the share and
 // its place among the sequences itself.
 struct Cut8 {
   int32_t G, tiles, units, room;  // units: (sequence, split) that the launch has; room 0: nothing is split
   float scale;
   float* part;                    // [units, kv heads, tiles] partial results
+  int32_t* plan;                  // [seqs] first unit << 16 and splits, for the join
 };
 struct Place8 {
   int b, split, share, n;  // b < 0: none; n: splits of the sequence
-  int unit;                // place among the units
   int len, nodes;          // of the sequence; nodes < 0: bad
 };
 
@@ -456,15 +456,13 @@ struct Place8 {
 template <int UNIT>
 XS_DEV int units_of(const Seq& sq) { return sq.bad ? 0 : (sq.len + UNIT - 1) / UNIT + (sq.n + UNIT - 1) / UNIT; }
 
-// The place of unit `want`, or (want < 0) the first of sequence `seq`.
 template <int UNIT, int LEAST, int WHOLE>
-XS_DEV Place8 place8(const xs_tree_attend_args& a, const Cut8& cut, int want, int seq) {
+XS_DEV Place8 place8(const xs_tree_attend_args& a, const Cut8& cut, int want) {
   const int lane = threadIdx.x & 63, seqs = (int)a.seqs;
   if (cut.room == 0) {
-    const int b = want < 0 ? seq : want;
-    if (b >= seqs) return {-1, 0, 1, 1, 0, 0, 0};
-    const Seq sq(a, b);
-    return {b, 0, 1, 1, b, sq.len, sq.bad ? -1 : sq.n};
+    if (want >= seqs) return {-1, 0, 1, 1, 0, 0};
+    const Seq sq(a, want);
+    return {want, 0, 1, 1, sq.len, sq.bad ? -1 : sq.n};
   }
   uint32_t u = 0;  // of the lane's sequence (of the last 64)
   int len = 0, nodes = -1;
@@ -502,15 +500,14 @@ XS_DEV Place8 place8(const xs_tree_attend_args& a, const Cut8& cut, int want, in
   for (int b0 = 0; b0 < seqs; b0 += 64) {
     if (seqs > 64) load(b0);
     const uint32_t n = splits(b0, share), upto = wave_scan(n) + before;
-    const uint64_t hit = want >= 0 ? __ballot(b0 + lane < seqs && upto > (uint32_t)want) : seq < b0 + 64 ? 1ull << (seq - b0) : 0ull;
+    const uint64_t hit = __ballot(b0 + lane < seqs && upto > (uint32_t)want);
     before = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
     if (!hit) continue;
     const int who = __ffsll((unsigned long long)hit) - 1, parts = __builtin_amdgcn_readlane((int)n, who);
     const int first = __builtin_amdgcn_readlane((int)upto, who) - parts;
-    return {b0 + who, want >= 0 ? want - first : 0, (int)share, parts, want >= 0 ? want : first,
-            __builtin_amdgcn_readlane(len, who), __builtin_amdgcn_readlane(nodes, who)};
+    return {b0 + who, want - first, (int)share, parts, __builtin_amdgcn_readlane(len, who), __builtin_amdgcn_readlane(nodes, who)};
   }
-  return {-1, 0, 1, 1, 0, 0, 0};
+  return {-1, 0, 1, 1, 0, 0};
 }
 
 // Workgroup i's part: groups of eight (kv head, sequence, split), each group's row
@@ -539,13 +536,16 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
   int tile, kh, unit;
   deal(cut, &tile, &kh, &unit);
   if (kh >= (int)a.kv_heads) return;
-  const Place8 pl = place8<KB, 2 * NW, 4 * NW>(a, cut, unit, 0);
+  const Place8 pl = place8<KB, 2 * NW, 4 * NW>(a, cut, unit);
   const int b = __builtin_amdgcn_readfirstlane(pl.b), split = __builtin_amdgcn_readfirstlane(pl.split);
   const int splits = __builtin_amdgcn_readfirstlane(pl.n);
   if (b < 0) return;
   const int share = __builtin_amdgcn_readfirstlane(pl.share), bh = b * (int)a.kv_heads + kh;
   const int len = __builtin_amdgcn_readfirstlane(pl.len), n = __builtin_amdgcn_readfirstlane(pl.nodes);
-  if (split == 0 && tile == 0 && kh == 0 && threadIdx.x == 0) a.seq_status[b] = n < 0 ? XS_ROW_BAD_PARAM : XS_ROW_OK;
+  if (split == 0 && tile == 0 && kh == 0 && threadIdx.x == 0) {
+    a.seq_status[b] = n < 0 ? XS_ROW_BAD_PARAM : XS_ROW_OK;
+    if (cut.room) cut.plan[b] = unit << 16 | splits;
+  }
   const int R = n * cut.G, row0 = tile * RT * 16;
   const int cached = (len + KB - 1) / KB, total = cached + (n + KB - 1) / KB;
   const int first = split * share, last = splits == 1 ? total : min(first + share, total);  // (one split: share says nothing)
@@ -705,13 +705,24 @@ __global__ __launch_bounds__((join8_threads<DP, SHARES>())) void join8_kernel(co
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pair = wave % PAIRS, share = wave / PAIRS;
   const int h = blockIdx.x % S::VH, tile = blockIdx.x / S::VH % cut.tiles, bh = blockIdx.x / (S::VH * cut.tiles);
   const int kh = bh % (int)a.kv_heads, b = bh / (int)a.kv_heads;
-  const Place8 pl = place8<KB, 2 * NW, 4 * NW>(a, cut, -1, b);
-  const int n = __builtin_amdgcn_readfirstlane(pl.n), nodes = __builtin_amdgcn_readfirstlane(pl.nodes), R = nodes * cut.G, row0 = 16 * tile;
+  const int plan = __builtin_amdgcn_readfirstlane(cut.plan[b]), n = plan & 0xFFFF;
+  const Seq sq(a, b);
+  const int nodes = __builtin_amdgcn_readfirstlane(sq.bad ? -1 : sq.n), R = nodes * cut.G, row0 = 16 * tile;
   if (row0 >= R || n <= 1) return;
   if (threadIdx.x == 0) odd = 0;
   __syncthreads();
-  const float* part = cut.part + (((int64_t)__builtin_amdgcn_readfirstlane((int)pl.unit) * a.kv_heads + kh) * cut.tiles + tile) * S::PART;
+  const float* part = cut.part + (((int64_t)(plan >> 16) * a.kv_heads + kh) * cut.tiles + tile) * S::PART;
   const int64_t step = a.kv_heads * cut.tiles * S::PART;
+  // the first fragments, on their way while the weights are formed
+  constexpr int AHEAD = 4;
+  const int f0 = h * S::VE + 2 * pair;
+  f32x4 y[AHEAD][2];
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) {
+    const f32x4* p = (const f32x4*)(part + min(share + SHARES * i, n - 1) * step) + f0 * 64 + lane;
+    y[i][0] = p[0];
+    y[i][1] = p[64];
+  }
   // a quarter of a wave takes a split's rows
   float top = NEG_INF, all = 0.0f;
   for (int s = 4 * wave + g; s < n; s += 4 * WAVES) {
@@ -731,14 +742,20 @@ __global__ __launch_bounds__((join8_threads<DP, SHARES>())) void join8_kernel(co
   }
   stat[1][4 * wave + g][x] = all;
   __syncthreads();
-  const int f0 = h * S::VE + 2 * pair;
   f32x4 o[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) {
+    if (share + SHARES * i >= n) break;
+    const float f = weight[share + SHARES * i][x];
+    o[0] += y[i][0] * f;
+    o[1] += y[i][1] * f;
+  }
 #pragma unroll 4
-  for (int s = share; s < n; s += SHARES) {
+  for (int s = share + SHARES * AHEAD; s < n; s += SHARES) {
     const f32x4* p = (const f32x4*)(part + s * step) + f0 * 64 + lane;
-    const float y = weight[s][x];
-    o[0] += p[0] * y;
-    o[1] += p[64] * y;
+    const float f = weight[s][x];
+    o[0] += p[0] * f;
+    o[1] += p[64] * f;
   }
   sum[share][2 * pair][lane] = o[0];
   sum[share][2 * pair + 1][lane] = o[1];
@@ -809,13 +826,16 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void attend8_wide_kerne
   int tile, kh, unit;
   deal(cut, &tile, &kh, &unit);
   if (kh >= (int)a.kv_heads) return;
-  const Place8 pl = place8<SK, STAGES_LEAST, STAGES_WHOLE>(a, cut, unit, 0);
+  const Place8 pl = place8<SK, STAGES_LEAST, STAGES_WHOLE>(a, cut, unit);
   const int b = __builtin_amdgcn_readfirstlane(pl.b), split = __builtin_amdgcn_readfirstlane(pl.split);
   const int splits = __builtin_amdgcn_readfirstlane(pl.n);
   if (b < 0) return;
   const int share = __builtin_amdgcn_readfirstlane(pl.share), bh = b * (int)a.kv_heads + kh;
   const int len = __builtin_amdgcn_readfirstlane(pl.len), n = __builtin_amdgcn_readfirstlane(pl.nodes);
-  if (split == 0 && tile == 0 && kh == 0 && threadIdx.x == 0) a.seq_status[b] = n < 0 ? XS_ROW_BAD_PARAM : XS_ROW_OK;
+  if (split == 0 && tile == 0 && kh == 0 && threadIdx.x == 0) {
+    a.seq_status[b] = n < 0 ? XS_ROW_BAD_PARAM : XS_ROW_OK;
+    if (cut.room) cut.plan[b] = unit << 16 | splits;
+  }
   const int R = n * cut.G, row = tile * S::ROWS + 32 * wr + x;
   const int cached = (len + SK - 1) / SK, total = cached + (n > 0 ? 1 : 0), first = split * share, last = splits == 1 ? total : min(first + share, total);
   if (tile * S::ROWS >= R || first >= total) return;  // (nodes below 0 too)
@@ -1011,13 +1031,19 @@ __global__ __launch_bounds__(256 * SHARES) void join32_kernel(const xs_tree_atte
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), share = wave / 4;
   const int f = blockIdx.x % S::DT * 4 + wave % 4, wr = blockIdx.x / S::DT % S::WR, tile = blockIdx.x / (S::DT * S::WR) % cut.tiles;
   const int bh = blockIdx.x / (S::DT * S::WR * cut.tiles), kh = bh % (int)a.kv_heads, b = bh / (int)a.kv_heads;
-  const Place8 pl = place8<SK, STAGES_LEAST, STAGES_WHOLE>(a, cut, -1, b);
-  const int n = __builtin_amdgcn_readfirstlane(pl.n), nodes = __builtin_amdgcn_readfirstlane(pl.nodes), R = nodes * cut.G, row = tile * S::ROWS + 32 * wr + x;
+  const int plan = __builtin_amdgcn_readfirstlane(cut.plan[b]), n = plan & 0xFFFF;
+  const Seq sq(a, b);
+  const int nodes = __builtin_amdgcn_readfirstlane(sq.bad ? -1 : sq.n), R = nodes * cut.G, row = tile * S::ROWS + 32 * wr + x;
   if (tile * S::ROWS + 32 * wr >= R || n <= 1) return;
   if (threadIdx.x == 0) odd = 0;
   __syncthreads();
-  const float* part = cut.part + (((int64_t)__builtin_amdgcn_readfirstlane((int)pl.unit) * a.kv_heads + kh) * cut.tiles + tile) * S::PART;
+  const float* part = cut.part + (((int64_t)(plan >> 16) * a.kv_heads + kh) * cut.tiles + tile) * S::PART;
   const int64_t step = a.kv_heads * cut.tiles * S::PART;
+  // the first fragments, on their way while the weights are formed
+  constexpr int AHEAD = SHARES > 1 ? 16 : 4;
+  f32x4 y[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) y[i] = ((const f32x4*)(part + min(share + SHARES * i, n - 1) * step))[(wr * S::NF + f) * 64 + lane];
   // half a wave takes a split's rows
   float top = NEG_INF, all = 0.0f;
   for (int s = 2 * wave + g; s < n; s += 2 * WAVES) {
@@ -1038,8 +1064,13 @@ __global__ __launch_bounds__(256 * SHARES) void join32_kernel(const xs_tree_atte
   stat[1][2 * wave + g][x] = all;
   __syncthreads();
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) {
+    if (share + SHARES * i >= n) break;
+    o += y[i] * weight[share + SHARES * i][x];
+  }
 #pragma unroll 8
-  for (int s = share; s < n; s += SHARES) o += ((const f32x4*)(part + s * step))[(wr * S::NF + f) * 64 + lane] * weight[s][x];
+  for (int s = share + SHARES * AHEAD; s < n; s += SHARES) o += ((const f32x4*)(part + s * step))[(wr * S::NF + f) * 64 + lane] * weight[s][x];
   sum[share][wave % 4][lane] = o;
   __syncthreads();
   if (share != 0) return;
@@ -1069,6 +1100,7 @@ bool cut8(xs_cache_context* c, const xs_tree_attend_args& a, int rows, int64_t s
   cut->tiles = (int32_t)((a.nodes * cut->G + rows - 1) / rows);
   cut->scale = a.scale * xst::LOG2E;
   cut->part = c->part;
+  cut->plan = c->evict.moves;  // (of max_seqs entries and more; an eviction fills it anew)
   const int64_t limit = a.max_len ? a.max_len : a.capacity, units = (limit + unit - 1) / unit + (a.nodes + unit - 1) / unit;
   const int64_t heads = a.kv_heads * cut->tiles;
   const int64_t places = c->part_floats / (heads * part);
