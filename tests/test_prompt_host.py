@@ -3,7 +3,9 @@ before the device is touched, the Python mirror's refusals, and what the calls l
 thread's current device."""
 import ctypes as C
 import os
+import shutil
 import subprocess
+import sys
 
 import pytest
 
@@ -157,6 +159,53 @@ def test_attend8_checks(host):
     assert chk(cache=kv8(v=None)) == E and chk(cache=kv8(k_exp=None)) == E and chk(cache=kv8(slot_stride=8)) == E and chk(cache=kv8(exp_ld=1)) == E
     assert chk(cache=kv8(slot_stride=(1 << 25) + 16)) == CAP and chk(cache=kv8(slot_stride=1 << 25)) == OK
     assert chk(cache=kv8(slot_stride=0)) == OK and chk(fresh=kv(v=DEV + 4)) == E and chk(fresh=kv(0)) == OK
+
+
+def test_the_checks_under_asan_and_ubsan():
+    """The checks above against the sanitized host build, in a child process."""
+    if os.environ.get("XS_HOST_LIB"):
+        pytest.skip("this is the child")
+    rt = subprocess.run(["gcc", "-print-file-name=libasan.so"], capture_output=True, text=True).stdout.strip() if shutil.which("gcc") else ""
+    if not os.path.isabs(rt) or not os.path.exists(rt) or not shutil.which("make"):
+        pytest.skip("gcc's AddressSanitizer runtime is not installed")
+    oracle = os.path.join(_lib.ROOT, "oracle")
+    subprocess.run(["make", "-s", "-C", oracle, "asan"], check=True)
+    env = dict(os.environ, LD_PRELOAD=rt, ASAN_OPTIONS="detect_leaks=0:halt_on_error=1:abort_on_error=1",
+               UBSAN_OPTIONS="halt_on_error=1:print_stacktrace=1",
+               XS_ORACLE_LIB=os.path.join(oracle, "_build", "asan", "libxs_oracle.so"),
+               XS_HOST_LIB=os.path.join(oracle, "_build", "asan", "libxs_host.so"))
+    r = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-p", "no:cacheprovider", "-k", "checks and not asan",
+                        os.path.abspath(__file__)], cwd=_lib.ROOT, env=env, capture_output=True, text=True, timeout=600)
+    tail = (r.stdout + r.stderr)[-4000:]
+    assert r.returncode == 0 and " passed" in r.stdout, tail
+    assert "AddressSanitizer" not in r.stderr and "runtime error:" not in r.stderr, tail
+
+
+def test_the_mirror_refuses_what_does_not_fit():
+    torch = pytest.importorskip("torch")
+    from xwen_amd import cache8, prompt as px
+
+    class Ctx:
+        device = 0
+
+    t = torch.zeros((3, 4, 64), dtype=torch.bfloat16)
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="not on the context's device"):
+        px.qk_rotate(Ctx(), t, t)
+    with pytest.raises(ValueError, match="bfloat16 or float16"):
+        px.qk_rotate(Ctx(), t.float(), t.float())
+    with pytest.raises(ValueError, match="both None"):
+        px.qk_rotate(Ctx(), None, None)
+    with pytest.raises(ValueError, match="go together"):
+        px.qk_rotate(Ctx(), t, t, i)
+    with pytest.raises(ValueError, match="not on the context's device"):
+        px.prompt_attend(Ctx(), t, t, t, i)
+    c8, e8 = torch.zeros((2, 64, 4, 64), dtype=torch.float8_e4m3fn), torch.zeros((2, 4, 2), dtype=torch.uint8)
+    f = torch.zeros((2, 3, 4, 64), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="not on the context's device"):
+        cache8.cache_append8(Ctx(), c8, c8, e8, e8, i, f, f)
+    with pytest.raises(ValueError, match="not on the context's device"):
+        cache8.tree_attend8(Ctx(), f, c8, c8, e8, e8, i, f, f, i)
 
 
 def test_calls_without_a_context():
