@@ -35,7 +35,8 @@ XS_DEV float pow2(int e) { return __uint_as_float((uint32_t)min(max(e + 127, 1),
 // (448 is 7/8 of 2^9).  A power of two loses nothing where the element type is
 // itself a float, but for the lowest of its subnormals, and makes both the
 // products and a later change of the scale exact.  Bound by reading the rows and
-// writing the bytes.
+// writing the bytes: 4 prompts of 328 to 8,192 rows of 8 heads of 128 (112 MB) in
+// 25 us; a step's 5 rows for each of 16 sequences 4.5 us, latency.
 
 constexpr int AB = 256;  // threads
 
@@ -174,7 +175,10 @@ __global__ __launch_bounds__(AB) void append_kernel(const xs_cache_append8_args 
 // values, and the weights of f16 calls are sums of two bf16 (a float of 11 bits
 // is one exactly, a weight to 16 bits), each part a product of its own.
 // A lane loads 16 bytes of a key: elements 64 c + 16 g + 8 h .. + 8 are chunk
-// 2 c + h of the products, for queries and fresh keys too.
+// 2 c + h of the products, for queries and fresh keys too.  Bound by the one read
+// of the cache up to 16 rows a head: decoding 32 sequences of 327 to 8,192 slots, 8
+// kv heads of 128 (302 MB), 81 us, of which the join of the splits takes 5; without
+// starts and ends the keys come at 5.2 to 5.9 TB/s.
 
 struct E4m3 {};  // (weights carry no power of two)
 XS_DEV constexpr float offset_of(E4m3) { return 0.0f; }
@@ -776,7 +780,12 @@ __global__ __launch_bounds__((join8_threads<DP, SHARES>())) void join8_kernel(co
 // threads turn into bf16 on their way to LDS, in stages of 64 through two
 // buffers: while one is read, the next is written from registers and the one
 // after it on its way from memory.  WK waves share 32 rows, each with its half of
-// a stage's keys, and add up at the end; 128 / WK rows a workgroup.
+// a stage's keys, and add up at the end; 128 / WK rows a workgroup.  Bound by the
+// products and the vector work beside them (xs_rows32.h), the widening among it:
+// 8 x 64 nodes of 32 q and 8 kv heads of 128 over 16,384 slots 170 to 185 us (806 to 744
+// TFLOP/s) of which the join takes 12; by memory where rows are few: 16 nodes over
+// 131,072 slots 76 to 82 us (3.5 to 3.3 TB/s).  The 16-row kernel with four row tiles
+// instead takes 721 and 216 us: its waves widen every key for 64 rows each.
 template <int DP, int WK>
 struct Shape32 {
   static constexpr int ROWS = 32 * NW / WK, WR = NW / WK;

@@ -176,6 +176,16 @@ __global__ __launch_bounds__(RT, 8) void rotate_kernel(const xs_qk_rotate_args a
 // rows, 32 a wave (xs_rows32.h; WK waves share them, each with its half of a stage's
 // keys, and add up at the end), and walks the keys up to its last row's token in
 // stages of 64, through two LDS buffers that loads fill while the other is read.
+//
+// Bound by the matrix cores and the vector units beside them: a stage of a wave at
+// head size 128 is 32 products of 32 cycles and some 900 cycles of vector work
+// (32 exponentials of 16, then scaling, sums, packing), which two waves a SIMD lay
+// side by side: the products run 64 % of the time at the clock that the power
+// leaves (1.8 GHz).  A prompt of 16,384 tokens, 32 q and 8 kv heads of 128: 1,900
+// to 2,000 us by card (1,157 to 1,100 TFLOP/s; a large library product reaches 1,334
+// to 1,366); 16 prompts of 164 to 4,096: 957 to 1,048 us (964 to 880 TFLOP/s).  One wave's
+// exponentials laid by hand beside its own next products, scores of two stages in
+// registers, spills: 2,346 us.
 
 // The sequence and the row tile of a workgroup: tiles of the device's valid
 // sequences, those with the most keys first, sequences of more than 64 in order.
@@ -261,7 +271,7 @@ XS_DEV void load_lds(const uint16_t* base, uint32_t bytes, u32x4* to) {
 XS_DEV void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 template <typename T, int DP, int WK, bool EXACT>
-__global__ __launch_bounds__(64 * NW, DP <= 64 ? 3 : DP <= 128 ? 2 : 1) void prompt_kernel(const xs_prompt_attend_args a, float scale) {
+__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_kernel(const xs_prompt_attend_args a, float scale) {
   using K = Keys<DP>;
   constexpr int KC = DP / 16, DT = DP / 32, ROWS = 32 * NW / WK, CH = K::CH, STAGE = K::STAGE;
   constexpr int PER = STAGE / (64 * NW);             // of a thread

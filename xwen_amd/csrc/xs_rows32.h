@@ -14,6 +14,8 @@
 // of the row's own scores, products that start from it.  It moves when a lane's
 // weights of a step add up to more than 2^8, which their sum, needed anyway, says
 // without a maximum (a prompt of 16,384 tokens with one: 2,064 us, so 2,028).
+// Fragments are asked for two products ahead of theirs, the first values before
+// the exponentials, and those go before the other wave's products (2,013, so 1,900).
 #pragma once
 
 #include "xs_attend.h"
@@ -198,24 +200,27 @@ struct Rows32 {
     };
     weigh(false, 0.0f, on);
     if (__any(sum > most)) [[unlikely]] {  // (a NaN does not move it: the row is lost)
-      // the references of the rows that have grown move to their best scores
+      // The references of the rows that have grown move to their best scores: all
+      // rows', whose products are formed again from 0, or those that start there.
       const On rare = on.again();
-      asm volatile("" : "+v"(kt));
-#pragma unroll
-      for (int u = 0; u < U; u++) {
-        s[u] = fill16(0.0f);
-#pragma unroll
-        for (int m = 0; m < KN; m++)
-#pragma unroll
-          for (int c = 0; c < KC; c++) {
-            const u32x4 k = at.key(ks[m], kt, u, c);
-#pragma unroll
-            for (int n = 0; n < NQ; n++) s[u] = mfma32(M{}, k, q[n][c], s[u]);
-            __builtin_amdgcn_sched_barrier(0);  // (one chunk in registers at a time)
-          }
-      }
       const float sign = scale < 0.0f ? -1.0f : 1.0f, old = reference();
-      const bool unset = most < 0.0f;
+      const bool unset = most < 0.0f, far = __any(sum > most && old != 0.0f);
+      if (far) [[unlikely]] {
+        asm volatile("" : "+v"(kt));
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          s[u] = fill16(0.0f);
+#pragma unroll
+          for (int m = 0; m < KN; m++)
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+              const u32x4 k = at.key(ks[m], kt, u, c);
+#pragma unroll
+              for (int n = 0; n < NQ; n++) s[u] = mfma32(M{}, k, q[n][c], s[u]);
+              __builtin_amdgcn_sched_barrier(0);  // (one chunk in registers at a time)
+            }
+        }
+      }
       // never below the old one (a product that starts elsewhere rounds elsewhere)
       float best = unset ? NEG_INF : old * sign;
 #pragma unroll
@@ -226,8 +231,8 @@ struct Rows32 {
           best = fmaxf(best, !masked || rare(32 * u + 8 * (r / 4) + r % 4) ? y : NEG_INF);
         }
       best = pair_max(best);
-      float ref = old;
-      if (best > NEG_INF) {
+      float ref = far ? old : 0.0f;  // (of a row that does not move: what its s lacks)
+      if ((far || old == 0.0f) && best > NEG_INF) {
         ref = scale == 0.0f ? 0.0f : best * sign;
         const float keep = unset ? 0.0f : __builtin_amdgcn_exp2f((old - ref) * scale);
         base = fill16(-ref);
