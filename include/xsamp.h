@@ -657,7 +657,8 @@ typedef struct {
  *               row start[b] + r, and n = start[b + 1] - start[b]
  * A block's e is the least with |x| <= 448 * 2^e for all its finite elements,
  * -100 at least; x is held as x * 2^-e, rounded once to e4m3 (nearest, ties to
- * even), a NaN or an infinity as NaN.  In a block that held slots already e
+ * even), a NaN or an infinity as NaN (bf16 from 248 * 2^120 on is thus held as
+ * 2^128, infinite to what reads it).  In a block that held slots already e
  * grows where the new rows ask for it, never shrinks, and the old slots are
  * then rounded again at the new e (exact but for what falls below e4m3's normal
  * numbers).  Results do not depend on how rows are cut into calls but for that
