@@ -780,15 +780,17 @@ __global__ __launch_bounds__((join8_threads<DP, SHARES>())) void join8_kernel(co
 // threads turn into bf16 on their way to LDS, in stages of 64 through two
 // buffers: while one is read, the next is written from registers and the one
 // after it on its way from memory.  WK waves share 32 rows, each with its half of
-// a stage's keys, and add up at the end; 128 / WK rows a workgroup.  Bound by the
-// products and the vector work beside them (xs_rows32.h), the widening among it:
-// 8 x 64 nodes of 32 q and 8 kv heads of 128 over 16,384 slots 170 to 185 us (806 to 744
+// a stage's keys, and add up at the end; 32 W / WK rows a workgroup of W waves.  Bound
+// by the products and the vector work beside them (xs_rows32.h), the widening among
+// it, which eight waves share where rows fill them (four, two workgroups a CU: 181
+// us for 170):
+// 8 x 64 nodes of 32 q and 8 kv heads of 128 over 16,384 slots 158 to 170 us (870 to 810
 // TFLOP/s) of which the join takes 12; by memory where rows are few: 16 nodes over
 // 131,072 slots 76 to 82 us (3.5 to 3.3 TB/s).  The 16-row kernel with four row tiles
 // instead takes 721 and 216 us: its waves widen every key for 64 rows each.
-template <int DP, int WK>
+template <int DP, int WK, int W>
 struct Shape32 {
-  static constexpr int ROWS = 32 * NW / WK, WR = NW / WK;
+  static constexpr int ROWS = 32 * W / WK, WR = W / WK;
   static constexpr int DT = DP / 32, NF = 4 * DT;    // fragments of four elements a lane
   static constexpr int STAT = WR * NF * 256;         // floats of a partial result: fragments,
   static constexpr int ODD = STAT + 2 * ROWS;        // then m and l of each row,
@@ -821,12 +823,13 @@ XS_DEV void store_four(const xs_tree_attend_args& a, int G, int b, int kh, int r
   if (a.lse && f == 0 && g == 0) a.lse[(b * a.nodes + node) * a.q_heads + head] = lse_of<E4m3>(a, ref, l);
 }
 
-template <typename T, int DP, int WK, bool EXACT>
-__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void attend8_wide_kernel(const xs_tree_attend_args a, const xs_kv8 c8, const Cut8 cut) {
-  using S = Shape32<DP, WK>;
+template <typename T, int DP, int WK, int W, bool EXACT>
+__global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend8_wide_kernel(const xs_tree_attend_args a, const xs_kv8 c8, const Cut8 cut) {
+  using S = Shape32<DP, WK, W>;
   using K = Keys<DP>;
-  constexpr int N = Parts<T>::N, CH = K::CH, KC = DP / 16, DT = DP / 32, TH = 64 * NW;
+  constexpr int N = Parts<T>::N, CH = K::CH, KC = DP / 16, DT = DP / 32, TH = 64 * W;
   constexpr int PER = SK * (DP / 16) / TH;  // 16-byte pieces of the cache that a thread moves, of k and of v
+  static_assert(SK * (DP / 16) % TH == 0, "a stage is whole pieces of every thread");
   __shared__ u32x4 lk[2][K::STAGE];
   __shared__ u32x4 lv[2][K::STAGE];
   __shared__ int odds;
@@ -1028,9 +1031,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void attend8_wide_kerne
 
 // Joins the splits of 32 rows, four fragments a workgroup: each wave one of them
 // over one of SHARES shares of the splits.
-template <typename T, int DP, int WK, int SHARES>
+template <typename T, int DP, int WK, int W, int SHARES>
 __global__ __launch_bounds__(256 * SHARES) void join32_kernel(const xs_tree_attend_args a, const Cut8 cut) {
-  using S = Shape32<DP, WK>;
+  using S = Shape32<DP, WK, W>;
   constexpr int WAVES = 4 * SHARES;
   __shared__ float weight[SPLITS][32];
   __shared__ float stat[2][2 * WAVES][32];
@@ -1120,7 +1123,7 @@ bool cut8(xs_cache_context* c, const xs_tree_attend_args& a, int rows, int64_t s
   cut->room = (int32_t)room;
   cut->units = (int32_t)(!room ? a.seqs : std::min(room > a.seqs ? room : room + a.seqs, a.seqs * ((units + least - 1) / least)));
   *grid = ((int64_t)cut->units * a.kv_heads + 7) / 8 * 8 * cut->tiles;
-  return xs_host_launch_fits(*grid, 64 * xst::NW);
+  return xs_host_launch_fits(*grid, 128 * xst::NW);
 }
 
 // Shares of the splits that a join goes through side by side: several where a
@@ -1142,18 +1145,18 @@ int attend8_run(xs_cache_context* c, const xs_tree_attend_args& a, const xs_kv8&
   return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
 }
 
-template <typename T, int DP, int WK, bool EXACT>
+template <typename T, int DP, int WK, int W, bool EXACT>
 int attend8_wide_run(xs_cache_context* c, const xs_tree_attend_args& a, const xs_kv8& c8) {
-  using S = xs8::Shape32<DP, WK>;
+  using S = xs8::Shape32<DP, WK, W>;
   xs8::Cut8 cut;
   int64_t grid;
   // (as many workgroups as a CU's LDS holds)
-  if (!cut8(c, a, S::ROWS, c->n_cu * (DP <= 128 ? 2 : 1), S::PART, xst::SK, xs8::STAGES_LEAST, xs8::STAGES_WHOLE, &cut, &grid)) return XS_ERR_CAPACITY;
+  if (!cut8(c, a, S::ROWS, c->n_cu * (DP <= 128 && W == xst::NW ? 2 : 1), S::PART, xst::SK, xs8::STAGES_LEAST, xs8::STAGES_WHOLE, &cut, &grid)) return XS_ERR_CAPACITY;
   const int64_t join = a.seqs * a.kv_heads * cut.tiles * S::WR * S::DT;
   if (cut.room && !xs_host_launch_fits(join, 1024)) return XS_ERR_CAPACITY;
-  hipLaunchKernelGGL((xs8::attend8_wide_kernel<T, DP, WK, EXACT>), dim3((unsigned)grid), dim3(64 * xst::NW), 0, c->stream, a, c8, cut);
-  if (cut.room && many8(cut, a)) hipLaunchKernelGGL((xs8::join32_kernel<T, DP, WK, 4>), dim3((unsigned)join), dim3(1024), 0, c->stream, a, cut);
-  else if (cut.room) hipLaunchKernelGGL((xs8::join32_kernel<T, DP, WK, 1>), dim3((unsigned)join), dim3(256), 0, c->stream, a, cut);
+  hipLaunchKernelGGL((xs8::attend8_wide_kernel<T, DP, WK, W, EXACT>), dim3((unsigned)grid), dim3(64 * W), 0, c->stream, a, c8, cut);
+  if (cut.room && many8(cut, a)) hipLaunchKernelGGL((xs8::join32_kernel<T, DP, WK, W, 4>), dim3((unsigned)join), dim3(1024), 0, c->stream, a, cut);
+  else if (cut.room) hipLaunchKernelGGL((xs8::join32_kernel<T, DP, WK, W, 1>), dim3((unsigned)join), dim3(256), 0, c->stream, a, cut);
   return hipGetLastError() == hipSuccess ? XS_OK : XS_ERR_HIP;
 }
 
@@ -1161,8 +1164,11 @@ template <typename T, int DP, bool EXACT>
 int attend8_rows(xs_cache_context* c, const xs_tree_attend_args& a, const xs_kv8& c8) {
   const int64_t rows = a.nodes * (a.q_heads / a.kv_heads);
   if (rows <= 16) return attend8_run<T, DP, EXACT>(c, a, c8);
-  if (rows <= 64) return attend8_wide_run<T, DP, 2, EXACT>(c, a, c8);
-  return attend8_wide_run<T, DP, 1, EXACT>(c, a, c8);
+  if (rows <= 64) return attend8_wide_run<T, DP, 2, xst::NW, EXACT>(c, a, c8);
+  if constexpr (DP == 128) {  // (heads of 64 have half a piece a thread, heads of 256 registers for one wave a SIMD)
+    if ((rows + 127) / 128 % 2 == 0) return attend8_wide_run<T, DP, 1, 2 * xst::NW, EXACT>(c, a, c8);
+  }
+  return attend8_wide_run<T, DP, 1, xst::NW, EXACT>(c, a, c8);
 }
 
 template <typename T, int DP>
