@@ -264,6 +264,17 @@ def test_attend_long(ctx, nodes, hq, h, d, dtype):
     agree(c, s, look(ctx, c, s, max_len=8000))
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("nodes,g,d", [(43, 3, 128), (64, 4, 80), (52, 5, 96), (64, 6, 112), (64, 8, 128), (64, 4, 64)])
+def test_attend_many_rows(ctx, nodes, g, d, dtype):
+    """129 to 512 rows of a head, odd and even numbers of 128 of them, with an infinity that one row sees."""
+    rng = np.random.default_rng(nodes * g + d)
+    c = filled([2600, 0, 63, 700], 2, d)
+    s = step(rng, c, nodes, 2 * g, dtype, used=[nodes, nodes, nodes - 1, nodes // 2])
+    s["fv"][:, nodes - 1, :, ::2] = math.inf
+    agree(c, s, look(ctx, c, s))
+
+
 @pytest.mark.parametrize("nodes", [1, 5, 20])
 @pytest.mark.parametrize("seqs,h", [(70, 1), (64, 16), (300, 1)])
 def test_attend_many_sequences(seqs, h, nodes):

@@ -783,11 +783,11 @@ __global__ __launch_bounds__((join8_threads<DP, SHARES>())) void join8_kernel(co
 // a stage's keys, and add up at the end; 32 W / WK rows a workgroup of W waves.  Bound
 // by the products and the vector work beside them (xs_rows32.h), the widening among
 // it, which eight waves share where rows fill them (four, two workgroups a CU: 181
-// us for 170):
-// 8 x 64 nodes of 32 q and 8 kv heads of 128 over 16,384 slots 158 to 170 us (870 to 810
-// TFLOP/s) of which the join takes 12; by memory where rows are few: 16 nodes over
-// 131,072 slots 76 to 82 us (3.5 to 3.3 TB/s).  The 16-row kernel with four row tiles
-// instead takes 721 and 216 us: its waves widen every key for 64 rows each.
+// us for 170): 8 x 64 nodes of 32 q and 8 kv heads of 128 over 16,384 slots 157 to
+// 170 us by card (880 to 810 TFLOP/s), of which the join takes 12.  By memory where
+// rows are few: 16 nodes over 131,072 slots 76 to 82 us (3.5 to 3.3 TB/s).  The
+// 16-row kernel with four row tiles instead takes 721 and 216 us: its waves widen
+// every key for 64 rows each.
 template <int DP, int WK, int W>
 struct Shape32 {
   static constexpr int ROWS = 32 * W / WK, WR = W / WK;
