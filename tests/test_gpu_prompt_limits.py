@@ -32,7 +32,7 @@ def test_prompt_rows_past_32_bits(ctx):
         v = room.as_strided(t.shape, (stride, 64, 1), i * 1024)
         v.copy_(t)
         views.append(v)
-    out = prompt.PromptAttended(out=room.as_strided((n, 2, 64), (stride, 64, 1), 3072), lse=torch.zeros((n, 2), device="cuda"),
+    out = prompt.PromptAttended(out=room.as_strided((n, 2, 64), (stride, 64, 1), 2560), lse=torch.zeros((n, 2), device="cuda"),
                                 seq_status=torch.zeros(1, dtype=torch.int32, device="cuda"))
     start = torch.tensor([0, n], dtype=torch.int32).cuda()
     prompt.prompt_attend(ctx, *views, start, out=out)
