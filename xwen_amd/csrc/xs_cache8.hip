@@ -171,9 +171,11 @@ __global__ __launch_bounds__(AB) void append_kernel(const xs_cache_append8_args 
 //
 // That of xs_attend.h with keys and values as bf16, which holds byte * 2^e
 // exactly: a block of 32 keys is one block of the cache, its scales two uniform
-// exponents, applied by the conversion itself.  f16 queries, fresh keys and
-// values, and the weights of f16 calls are sums of two bf16 (a float of 11 bits
-// is one exactly, a weight to 16 bits), each part a product of its own.
+// exponents, applied by the conversion itself.  f16 queries and fresh values, and
+// the weights of f16 calls are sums of two bf16 (a float of 11 bits is one
+// exactly, a weight to 16 bits), each part a product of its own.  The tree's own
+// scores are products of f16 as they stand: parts of an infinity times parts of a
+// query would not add up to it (0 times -inf, or -inf and +inf).
 // A lane loads 16 bytes of a key: elements 64 c + 16 g + 8 h .. + 8 are chunk
 // 2 c + h of the products, for queries and fresh keys too.  Bound by the one read
 // of the cache up to 16 rows a head: decoding 32 sequences of 327 to 8,192 slots, 8
@@ -230,26 +232,25 @@ XS_DEV void weights8(Tile<T, DP, RT>& z, int t, const float (&x)[8], u32x4 (&pf)
   }
 }
 
-// The weights of 32 keys: keys(u, c, m) is part m of chunk c of 16 of them,
-// again(u, c, m) the same formed anew where references move.
-template <typename T, int DP, int RT, bool MASKED, int KN, typename Keys, typename Again>
+// The weights of 32 keys, from products of type M with the first QN parts of the
+// queries: keys(u, c) is chunk c of 16 of them, again(u, c) the same formed anew
+// where references move.
+template <typename T, int DP, int RT, bool MASKED, typename M, int QN, typename Keys, typename Again>
 XS_DEV void softmax8(Tile<T, DP, RT>& z, float scale, const uint32_t* on, u32x4 (&pf)[Parts<T>::N][RT], Keys keys, Again again) {
   using S = Shape<DP, RT>;
   f32x4 s[RT][2];
 #pragma unroll
   for (int t = 0; t < RT; t++) s[t][0] = s[t][1] = z.w.start(t);
 #pragma unroll
-  for (int m = 0; m < KN; m++)
+  for (int c = 0; c < S::KC; c++)
 #pragma unroll
-    for (int c = 0; c < S::KC; c++)
+    for (int u = 0; u < 2; u++) {
+      const u32x4 k = keys(u, c);
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const u32x4 k = keys(u, c, m);
+      for (int t = 0; t < RT; t++)
 #pragma unroll
-        for (int t = 0; t < RT; t++)
-#pragma unroll
-          for (int n = 0; n < Parts<T>::N; n++) s[t][u] = mfma(Bf16{}, k, z.q[n][t][c], s[t][u]);
-      }
+        for (int n = 0; n < QN; n++) s[t][u] = mfma(M{}, k, z.q[n][t][c], s[t][u]);
+    }
 #pragma unroll
   for (int t = 0; t < RT; t++) {
     float x[8];
@@ -259,16 +260,14 @@ XS_DEV void softmax8(Tile<T, DP, RT>& z, float scale, const uint32_t* on, u32x4 
       if (far) [[unlikely]] {
         s[t][0] = s[t][1] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int m = 0; m < KN; m++)
+        for (int c = 0; c < S::KC; c++)
 #pragma unroll
-          for (int c = 0; c < S::KC; c++)
+          for (int u = 0; u < 2; u++) {
+            const u32x4 k = again(u, c);
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-              const u32x4 k = again(u, c, m);
-#pragma unroll
-              for (int n = 0; n < Parts<T>::N; n++) s[t][u] = mfma(Bf16{}, k, z.q[n][t][c], s[t][u]);
-              __builtin_amdgcn_sched_barrier(0);  // (one chunk in registers at a time)
-            }
+            for (int n = 0; n < QN; n++) s[t][u] = mfma(M{}, k, z.q[n][t][c], s[t][u]);
+            __builtin_amdgcn_sched_barrier(0);  // (one chunk in registers at a time)
+          }
       }
       z.w.template rebase<MASKED>(t, s[t], far, scale, MASKED ? on[t] : 0u, x);
     }
@@ -345,9 +344,9 @@ template <typename T, int DP, int RT, bool MASKED>
 XS_DEV void cache_weights(Tile<T, DP, RT>& z, const Raw<DP>& r, float scale, const uint32_t* on, u32x4 (&pf)[Parts<T>::N][RT]) {
   const float kscale = pow2((int)r.ke - 127);
   auto widen = [](uint32_t a, uint32_t b, float s) { return (u32x4){wide2(a, s, false), wide2(a, s, true), wide2(b, s, false), wide2(b, s, true)}; };
-  softmax8<T, DP, RT, MASKED, 1>(
-      z, scale, on, pf, [&](int u, int c, int) { return widen(r.k[u][c / 2][2 * (c % 2)], r.k[u][c / 2][2 * (c % 2) + 1], kscale); },
-      [&](int u, int c, int) {
+  softmax8<T, DP, RT, MASKED, Bf16, Parts<T>::N>(
+      z, scale, on, pf, [&](int u, int c) { return widen(r.k[u][c / 2][2 * (c % 2)], r.k[u][c / 2][2 * (c % 2) + 1], kscale); },
+      [&](int u, int c) {
         uint32_t a = r.k[u][c / 2][2 * (c % 2)], b = r.k[u][c / 2][2 * (c % 2) + 1];
         asm volatile("" : "+v"(a), "+v"(b));  // (not the first products' operands, kept)
         return widen(a, b, kscale);
@@ -381,7 +380,8 @@ XS_DEV void cache_product(Tile<T, DP, RT>& z, const Raw<DP>& r, const u32x4 (&pf
     }
 }
 
-// A block of the tree's own keys, in the inputs' type.
+// A block of the tree's own keys, in the inputs' type, as the queries are here
+// (z.q[0]).
 template <typename T, int DP, int RT, bool EXACT>
 XS_DEV void tree_block(Tile<T, DP, RT>& z, const uint16_t* kp, const uint16_t* vp, int64_t stride, int key0, int limit, int D, float scale,
                        const uint32_t* on) {
@@ -389,13 +389,11 @@ XS_DEV void tree_block(Tile<T, DP, RT>& z, const uint16_t* kp, const uint16_t* v
   constexpr int N = Parts<T>::N;
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
   u32x4 pf[N][RT];
-  auto keys = [&](int u, int c, int m) {
+  auto keys = [&](int u, int c) {
     const int key = min(key0 + 16 * u + x, limit - 1), d = 64 * (c / 2) + 16 * g + 8 * (c % 2);
-    u32x4 y[N];
-    split8(T{}, EXACT || d < D ? *(const u32x4*)(kp + key * stride + d) : (u32x4){0, 0, 0, 0}, y);
-    return y[m];
+    return EXACT || d < D ? *(const u32x4*)(kp + key * stride + d) : (u32x4){0, 0, 0, 0};
   };
-  softmax8<T, DP, RT, true, N>(z, scale, on, pf, keys, keys);
+  softmax8<T, DP, RT, true, T, 1>(z, scale, on, pf, keys, keys);
   __builtin_amdgcn_sched_barrier(0);  // (the values' registers not beside the keys')
   uint32_t v[N][8][S::VH][S::VE / 2];
 #pragma unroll
@@ -567,16 +565,21 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
   const int parent = parent_of(a, b);
   Tile<T, DP, RT> z;
   z.w.init();
+  auto query = [&](int row) {
+    const int r = min(row, R - 1);  // (rows past the last are not stored)
+    return (const uint16_t*)a.q + b * a.q_seq_stride + r / cut.G * a.q_node_stride + (kh * cut.G + r % cut.G) * a.q_head_stride + 16 * g;
+  };
+  auto chunk = [&](const uint16_t* p, int c) {
+    const int d = 64 * (c / 2) + 8 * (c % 2);
+    return EXACT || d + 16 * g < a.head_dim ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0};
+  };
 #pragma unroll
   for (int t = 0; t < RT; t++) {
-    const int row = min(row0 + 16 * t + x, R - 1);  // (rows past the last are not stored)
-    const int node = row / cut.G, head = kh * cut.G + row % cut.G;
-    const uint16_t* p = (const uint16_t*)a.q + b * a.q_seq_stride + node * a.q_node_stride + head * a.q_head_stride;
+    const uint16_t* p = query(row0 + 16 * t + x);
 #pragma unroll
     for (int c = 0; c < S::KC; c++) {
-      const int d = 64 * (c / 2) + 16 * g + 8 * (c % 2);
       u32x4 y[Tile<T, DP, RT>::N];
-      split8(T{}, EXACT || d < a.head_dim ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0}, y);
+      split8(T{}, chunk(p, c), y);
 #pragma unroll
       for (int m = 0; m < Tile<T, DP, RT>::N; m++) z.q[m][t][c] = y[m];
     }
@@ -609,27 +612,38 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
     if (row >= R) mine[t] = 0;
   }
 #pragma unroll 1
-  for (; i < last; i += NW) {
+  for (; i < min(last, cached); i += NW) {
+    const int limit = len - i * KB;
     uint32_t on[RT];
-    if (i < cached) {
-      const int limit = len - i * KB;
 #pragma unroll
-      for (int t = 0; t < RT; t++) on[t] = (1u << limit) - 1u;
-      load_keys8<DP, EXACT, true>(r, c8, at, eat, i, limit, a.head_dim);
-      u32x4 pf[Parts<T>::N][RT];
-      load_values8<DP, EXACT, true>(r, c8, at, eat, i, limit, a.head_dim);
-      __builtin_amdgcn_sched_barrier(0);
-      cache_weights<T, DP, RT, true>(z, r, cut.scale, on, pf);
-      __builtin_amdgcn_sched_barrier(0);
-      cache_product<T, DP, RT>(z, r, pf);
-    } else {
-      const int key0 = (i - cached) * KB;
+    for (int t = 0; t < RT; t++) on[t] = (1u << limit) - 1u;
+    load_keys8<DP, EXACT, true>(r, c8, at, eat, i, limit, a.head_dim);
+    u32x4 pf[Parts<T>::N][RT];
+    load_values8<DP, EXACT, true>(r, c8, at, eat, i, limit, a.head_dim);
+    __builtin_amdgcn_sched_barrier(0);
+    cache_weights<T, DP, RT, true>(z, r, cut.scale, on, pf);
+    __builtin_amdgcn_sched_barrier(0);
+    cache_product<T, DP, RT>(z, r, pf);
+  }
+  if (Parts<T>::N == 2 && i < last) {  // (whole queries, read again rather than kept)
 #pragma unroll
-      for (int t = 0; t < RT; t++) on[t] = (uint32_t)(mine[t] >> key0);
-      const int64_t f = b * a.fresh.seq_stride + kh * a.fresh.head_stride;
-      tree_block<T, DP, RT, EXACT>(z, (const uint16_t*)a.fresh.k + f, (const uint16_t*)a.fresh.v + f, a.fresh.slot_stride, key0, n,
-                                   a.head_dim, cut.scale, on);
+    for (int t = 0; t < RT; t++) {
+      int row = row0 + 16 * t + x;
+      asm volatile("" : "+v"(row));
+      const uint16_t* p = query(row);
+#pragma unroll
+      for (int c = 0; c < S::KC; c++) z.q[0][t][c] = chunk(p, c);
     }
+  }
+#pragma unroll 1
+  for (; i < last; i += NW) {
+    const int key0 = (i - cached) * KB;
+    uint32_t on[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) on[t] = (uint32_t)(mine[t] >> key0);
+    const int64_t f = b * a.fresh.seq_stride + kh * a.fresh.head_stride;
+    tree_block<T, DP, RT, EXACT>(z, (const uint16_t*)a.fresh.k + f, (const uint16_t*)a.fresh.v + f, a.fresh.slot_stride, key0, n, a.head_dim,
+                                 cut.scale, on);
   }
 
   // the waves' sums, brought to one reference; rows that see nothing of the
@@ -855,14 +869,20 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend8_wide_kernel
   const int parent = parent_of(a, b);
   Rows32<Bf16, DP, N> w;
   w.init();
+  auto query = [&](int r) {
+    const int node = min(r, R - 1) / cut.G, head = kh * cut.G + min(r, R - 1) % cut.G;
+    return (const uint16_t*)a.q + b * a.q_seq_stride + node * a.q_node_stride + head * a.q_head_stride;
+  };
+  auto chunk = [&](const uint16_t* p, int c) {
+    const int d = 16 * c + 8 * g;
+    return row < R && (EXACT || d < a.head_dim) ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0};
+  };
   {
-    const int node = min(row, R - 1) / cut.G, head = kh * cut.G + min(row, R - 1) % cut.G;
-    const uint16_t* p = (const uint16_t*)a.q + b * a.q_seq_stride + node * a.q_node_stride + head * a.q_head_stride;
+    const uint16_t* p = query(row);
 #pragma unroll
     for (int c = 0; c < KC; c++) {
-      const int d = 16 * c + 8 * g;
       u32x4 y[N];
-      split8(T{}, row < R && (EXACT || d < a.head_dim) ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0}, y);
+      split8(T{}, chunk(p, c), y);
 #pragma unroll
       for (int m = 0; m < N; m++) w.q[m][c] = y[m];
     }
@@ -918,7 +938,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend8_wide_kernel
     for (int i = 0; i < STEPS; i++) {
       const int u = WK == 1 ? i : wk;
       const uint64_t bits = on >> (32 * u + 4 * g);
-      w.template step<U, 1>(reads, {ks + 32 * u * CH}, {vs + 32 * u * CH}, cut.scale, masked, Bits{(uint32_t)bits, (uint32_t)(bits >> 32)});
+      w.template step<U, 1>(reads, ks + 32 * u * CH, {vs + 32 * u * CH}, cut.scale, masked, Bits{(uint32_t)bits, (uint32_t)(bits >> 32)});
     }
   };
   if (first < end) {
@@ -934,7 +954,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend8_wide_kernel
     const int limit = len - s * SK;
     step(lk[s & 1], lv[s & 1], limit < SK, limit < SK ? (1ull << limit) - 1ull : ~0ull);
   }
-  // the tree: parts in a buffer each
+  // the tree: keys and queries as they are, parts of the values in a buffer each
   int odd = 0;
   if (last == total) {
     if (threadIdx.x == 0) odds = 0;
@@ -955,16 +975,20 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend8_wide_kernel
         if ((v[i] & 0x7FFFu) >= inf_of(T{})) v[i] &= 0xFFFF0000u, odds = 1;
         if (((v[i] >> 16) & 0x7FFFu) >= inf_of(T{})) v[i] &= 0xFFFFu, odds = 1;
       }
-      u32x4 ks[N], vs[N];
-      split8(T{}, k, ks);
+      lk[0][r * CH + (c ^ K::turn_k(r))] = k;
+      u32x4 vs[N];
       split8(T{}, v, vs);
 #pragma unroll
-      for (int m = 0; m < N; m++) {
-        lk[m][r * CH + (c ^ K::turn_k(r))] = ks[m];
-        lv[m][r * CH + (c ^ K::turn_v(r))] = vs[m];
-      }
+      for (int m = 0; m < N; m++) lv[m][r * CH + (c ^ K::turn_v(r))] = vs[m];
     }
     __syncthreads();
+    if constexpr (N == 2) {
+      int again = row;
+      asm volatile("" : "+v"(again));  // (whole queries, read again rather than kept)
+      const uint16_t* p = query(again);
+#pragma unroll
+      for (int c = 0; c < KC; c++) w.q[0][c] = chunk(p, c);
+    }
     odd = odds;
 #pragma unroll 1
     for (int i = 0; i < 2 / WK; i++) {
@@ -972,8 +996,8 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend8_wide_kernel
       const uint64_t bits = mine >> (32 * u + 4 * g);
       const Bits on = {(uint32_t)bits, (uint32_t)(bits >> 32)};
       if (32 * u >= n) continue;
-      if constexpr (N == 1) w.template step<1, 1>(reads, {lk[0] + 32 * u * CH}, {lv[0] + 32 * u * CH}, cut.scale, true, on);
-      else w.template step<1, 2>(reads, {lk[0] + 32 * u * CH, lk[1] + 32 * u * CH}, {lv[0] + 32 * u * CH, lv[1] + 32 * u * CH}, cut.scale, true, on);
+      if constexpr (N == 1) w.template step<1, 1>(reads, lk[0] + 32 * u * CH, {lv[0] + 32 * u * CH}, cut.scale, true, on);
+      else w.template step<1, 2, 1, F16>(reads, lk[0] + 32 * u * CH, {lv[0] + 32 * u * CH, lv[1] + 32 * u * CH}, cut.scale, true, on);
     }
   }
 

@@ -369,13 +369,13 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_kernel(cons
     if (live && s * SK <= top_token) {
       const bool masked = s * SK + SK - 1 > low;
       if constexpr (WK == 1 && DP <= 128) {
-        w.template step<2, 1>(reads, {lds[s & 1][0]}, {lds[s & 1][1]}, scale, masked, Upto{token - s * SK - 4 * g});
+        w.template step<2, 1>(reads, lds[s & 1][0], {lds[s & 1][1]}, scale, masked, Upto{token - s * SK - 4 * g});
       } else {
         // a tile of 32 keys at a time: a wave's own, or what the registers hold
 #pragma unroll
         for (int i = 0; i < 2 / WK; i++) {
           const int u = WK == 1 ? i : wk;
-          w.template step<1, 1>(reads, {lds[s & 1][0] + 32 * u * CH}, {lds[s & 1][1] + 32 * u * CH}, scale, masked, Upto{token - s * SK - 32 * u - 4 * g});
+          w.template step<1, 1>(reads, lds[s & 1][0] + 32 * u * CH, {lds[s & 1][1] + 32 * u * CH}, scale, masked, Upto{token - s * SK - 32 * u - 4 * g});
         }
       }
     }

@@ -115,7 +115,8 @@ struct Bits {
 };
 
 // Rows of inputs T; queries are NQ parts that add up (of type M, as keys and
-// weights are for the products), weights NQ parts too.
+// weights are for the products), weights NQ parts too.  A step may instead take
+// q[0] alone, with keys of a type of their own (QN, QM).
 template <typename M, int DP, int NQ>
 struct Rows32 {
   static constexpr int KC = DP / 16, DT = DP / 32;
@@ -132,10 +133,10 @@ struct Rows32 {
   }
   XS_DEV float reference() const { return -base[0]; }
 
-  // A step of U tiles of 32 keys, the first of the stages ks and vs (KN parts that add up):
+  // A step of U tiles of 32 keys, the first of the stages ks and vs (VN parts that add up):
   // on (Upto, Bits) is asked for key 32 u + 8 (r / 4) + r % 4 where `masked`.
-  template <int U, int KN, typename On>
-  XS_DEV void step(const Reads<DP>& at, const u32x4* const (&ks)[KN], const u32x4* const (&vs)[KN], float scale, bool masked, const On on) {
+  template <int U, int VN, int QN = NQ, typename QM = M, typename On>
+  XS_DEV void step(const Reads<DP>& at, const u32x4* ks, const u32x4* const (&vs)[VN], float scale, bool masked, const On on) {
     constexpr float OFF = offset_of(M{});
     int kt = at.kturn, vt = at.vturn;
     asm volatile("" : "+v"(kt), "+v"(vt));
@@ -143,23 +144,23 @@ struct Rows32 {
 #pragma unroll
     for (int u = 0; u < U; u++) s[u] = base;
     // fragments AHEAD of their products, so that LDS answers beside the others'
-    constexpr int AHEAD = 2, STEPS = KN * KC;
+    constexpr int AHEAD = 2;
     u32x4 k[AHEAD + 1][U];
 #pragma unroll
     for (int i = 0; i < AHEAD; i++)
 #pragma unroll
-      for (int u = 0; u < U; u++) k[i][u] = at.key(ks[i / KC], kt, u, i % KC);
+      for (int u = 0; u < U; u++) k[i][u] = at.key(ks, kt, u, i);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < STEPS; i++) {
-      if (i + AHEAD < STEPS) {
+    for (int i = 0; i < KC; i++) {
+      if (i + AHEAD < KC) {
 #pragma unroll
-        for (int u = 0; u < U; u++) k[(i + AHEAD) % (AHEAD + 1)][u] = at.key(ks[(i + AHEAD) / KC], kt, u, (i + AHEAD) % KC);
+        for (int u = 0; u < U; u++) k[(i + AHEAD) % (AHEAD + 1)][u] = at.key(ks, kt, u, i + AHEAD);
       }
 #pragma unroll
       for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int n = 0; n < NQ; n++) s[u] = mfma32(M{}, k[i % (AHEAD + 1)][u], q[n][i % KC], s[u]);
+        for (int n = 0; n < QN; n++) s[u] = mfma32(QM{}, k[i % (AHEAD + 1)][u], q[n][i], s[u]);
       __builtin_amdgcn_sched_barrier(0);
     }
     u32x4 v[2][U][2];
@@ -211,14 +212,12 @@ struct Rows32 {
         for (int u = 0; u < U; u++) {
           s[u] = fill16(0.0f);
 #pragma unroll
-          for (int m = 0; m < KN; m++)
+          for (int c = 0; c < KC; c++) {
+            const u32x4 k = at.key(ks, kt, u, c);
 #pragma unroll
-            for (int c = 0; c < KC; c++) {
-              const u32x4 k = at.key(ks[m], kt, u, c);
-#pragma unroll
-              for (int n = 0; n < NQ; n++) s[u] = mfma32(M{}, k, q[n][c], s[u]);
-              __builtin_amdgcn_sched_barrier(0);  // (one chunk in registers at a time)
-            }
+            for (int n = 0; n < QN; n++) s[u] = mfma32(QM{}, k, q[n][c], s[u]);
+            __builtin_amdgcn_sched_barrier(0);  // (one chunk in registers at a time)
+          }
         }
       }
       // never below the old one (a product that starts elsewhere rounds elsewhere)
@@ -260,8 +259,8 @@ struct Rows32 {
     __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < KN * DT; i++) {
-      if (i + 1 < KN * DT) values(i + 1);
+    for (int i = 0; i < VN * DT; i++) {
+      if (i + 1 < VN * DT) values(i + 1);
 #pragma unroll
       for (int u = 0; u < U; u++)
 #pragma unroll
