@@ -586,7 +586,7 @@ typedef struct {
   int64_t q_token_stride, q_head_stride;
   const void* k;         /* [tokens, kv_heads, head_dim] */
   int64_t k_token_stride, k_head_stride;
-  const float* q_weight; /* [head_dim], 16-byte aligned; both weights or none (that of an absent side may be NULL) */
+  const float* q_weight; /* [head_dim], 16-byte aligned; both weights or none (that of an absent side is not read) */
   const float* k_weight;
   float eps;
   int32_t rot_dim;       /* 0..head_dim: a multiple of 16 (halves) or 8 (neighbours) */

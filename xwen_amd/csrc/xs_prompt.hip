@@ -521,8 +521,11 @@ int xs_qk_rotate(xs_cache_context* c, const xs_qk_rotate_args* in) {
   if (in->tokens == 0 || in->q_heads + in->kv_heads == 0) return XS_OK;
   const OnDevice on(c->device);
   if (!on.ok) return XS_ERR_HIP;
-  if (in->dtype == XS_BF16) return rotate_dim<xst::Bf16>(c, *in);
-  return rotate_dim<xst::F16>(c, *in);
+  xs_qk_rotate_args a = *in;  // (whether there is a norm is for the sides that have heads to say)
+  if (a.q_heads == 0) a.q_weight = nullptr;
+  if (a.kv_heads == 0) a.k_weight = nullptr;
+  if (a.dtype == XS_BF16) return rotate_dim<xst::Bf16>(c, a);
+  return rotate_dim<xst::F16>(c, a);
 }
 
 int xs_prompt_attend(xs_cache_context* c, const xs_prompt_attend_args* in) {
