@@ -111,15 +111,30 @@ __global__ __launch_bounds__(RT, 8) void rotate_kernel(const xs_qk_rotate_args a
     }
     if (i + 1 < passes) fetch(raw);
     if (norm) {
-      float sum = 0.0f;
+      auto squares = [&](float by) {
+        float sum = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 8; e++) sum = __builtin_fmaf(x[1][e], x[1][e], __builtin_fmaf(x[0][e], x[0][e], sum));
+        for (int e = 0; e < 8; e++) {
+          const float u = x[0][e] * by, v = x[1][e] * by;
+          sum = __builtin_fmaf(v, v, __builtin_fmaf(u, u, sum));
+        }
 #pragma unroll
-      for (int m = 1; m < LPH; m *= 2) sum += __shfl_xor(sum, m);
-      // (a square root's reciprocal to a step or so; below the normal numbers, of 2^48 times as much)
-      const float mean = sum / (float)D + a.eps;
-      const bool tiny = mean < 0x1p-100f;
-      const float inv = __builtin_amdgcn_rsqf(tiny ? mean * 0x1p48f : mean) * (tiny ? 0x1p24f : 1.0f);
+        for (int m = 1; m < LPH; m *= 2) sum += __shfl_xor(sum, m);
+        return sum / (float)D;
+      };
+      const float mean = squares(1.0f) + a.eps;
+      float inv = __builtin_amdgcn_rsqf(mean);  // (to a step or so)
+      const bool tiny = mean < 0x1p-80f;
+      if (__any(tiny || mean == -NEG_INF)) {  // (rare) squares past f32's range: those of elements 2^96 times as large, or as small
+        const float by = tiny ? 0x1p96f : 0x1p-96f, far = __builtin_amdgcn_rsqf(squares(by) + a.eps * by * by);
+        if (tiny || mean == -NEG_INF) {
+#pragma unroll
+          for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[j][e] = tiny ? x[j][e] * by * far : x[j][e] * far * by;
+          inv = 1.0f;
+        }
+      }
       const float* w = shared + (key ? D : 0);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
