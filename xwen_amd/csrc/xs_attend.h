@@ -132,6 +132,27 @@ XS_DEV constexpr float offset_of(F16) { return 6.0f; }
 XS_DEV constexpr uint32_t inf_of(Bf16) { return 0x7F80u; }
 XS_DEV constexpr uint32_t inf_of(F16) { return 0x7C00u; }
 
+// A value that is not finite reaches the rows that give it weight, which a product
+// does not see to (0 times it is NaN).  Where a result is not finite, and its row's
+// weights are numbers, the keys are walked again, three times: with 1 in the place
+// of every value that is inf or NaN and 0 in the others', so that a result above 0
+// says that such a value has weight; so for -inf or NaN; and with the finite values
+// alone.  Two elements of V as a pass takes them:
+enum { WALK = 0, ABOVE = 1, BELOW = 2, FINITE = 3 };
+XS_DEV constexpr uint32_t one_of(Bf16) { return 0x3F80u; }
+XS_DEV constexpr uint32_t one_of(F16) { return 0x3C00u; }
+template <typename T>
+XS_DEV uint32_t passed(T, uint32_t two, int pass) {
+  uint32_t y = 0;
+#pragma unroll
+  for (int i = 0; i < 32; i += 16) {
+    const uint32_t v = (two >> i) & 0xFFFFu, size = v & 0x7FFFu;
+    const bool odd = size >= inf_of(T{}), has = size > inf_of(T{}) || (v >> 15) == (pass == BELOW ? 1u : 0u);
+    y |= (pass == FINITE ? (odd ? 0u : v) : odd && has ? one_of(T{}) : 0u) << i;
+  }
+  return y;
+}
+
 // Over the four lanes of a row (x, 16 + x, 32 + x, 48 + x).
 XS_DEV float row_max(float v) {
   const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));

@@ -191,6 +191,7 @@ __global__ __launch_bounds__(RT, 8) void rotate_kernel(const xs_qk_rotate_args a
 // rows, 32 a wave (xs_rows32.h; WK waves share them, each with its half of a stage's
 // keys, and add up at the end), and walks the keys up to its last row's token in
 // stages of 64, through two LDS buffers that loads fill while the other is read.
+// Results that are not finite are walked for again (xs_attend.h, passed).
 //
 // Bound by the matrix cores and the vector units beside them: a stage of a wave at
 // head size 128 is 32 products of 32 cycles and some 900 cycles of vector work
@@ -292,7 +293,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_kernel(cons
   constexpr int PER = STAGE / (64 * NW);             // of a thread
   static_assert(STAGE % (64 * NW) == 0, "a stage is whole chunks of every thread");
   __shared__ u32x4 lds[2][2][STAGE];                  // [buffer][k, v]
-  __shared__ int odds;
+  __shared__ uint16_t marks[2][DT][64 * NW];          // [above, below] a lane's elements that an infinity reaches
+  __shared__ int odds;                                // a result is not finite
   const int lane = threadIdx.x & 63, x = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / WK, wk = wave % WK;
   const int G = (int)(a.q_heads / a.kv_heads);
@@ -305,7 +307,6 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_kernel(cons
   const int row0 = __builtin_amdgcn_readfirstlane(at.tile) * ROWS, wrow = row0 + 32 * wr;
   const int row = wrow + x, token = min(row, R - 1) / G, head = kh * G + min(row, R - 1) % G;
   const int low = min(wrow, R - 1) / G, top_token = min(wrow + 31, R - 1) / G;  // of the wave's rows
-  const int wg_low = row0 / G;                                                 // of the workgroup's
   const int end = min(row0 + ROWS - 1, R - 1) / G + 1;                         // keys that it needs
   const int stages = (end + SK - 1) / SK;
   const bool live = wrow < R;
@@ -314,11 +315,12 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_kernel(cons
   // the head's end are zero from the start.
   const uint16_t* kp = (const uint16_t*)a.k + (int64_t)t0 * a.kv_token_stride + kh * a.kv_head_stride;
   const uint16_t* vp = (const uint16_t*)a.v + (int64_t)t0 * a.kv_token_stride + kh * a.kv_head_stride;
-  if (!EXACT) {
+  auto clear = [&] {
+    if (EXACT) return;
 #pragma unroll
     for (int i = 0; i < 4 * PER; i++) (&lds[0][0][0])[i * 64 * NW + threadIdx.x] = (u32x4){0, 0, 0, 0};
     __syncthreads();
-  }
+  };
   auto fetch = [&](int s) {
     const int64_t o = (int64_t)s * SK * a.kv_token_stride;
     const int last = n - 1 - s * SK;
@@ -333,13 +335,12 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_kernel(cons
     }
   };
 
+  clear();
   fetch(0);
   const Reads<DP> reads;
-  int odd = 0;
   if (threadIdx.x == 0) odds = 0;
 
   Rows32<T, DP, 1> w;
-  w.init();
   {
     const uint16_t* p = (const uint16_t*)a.q + (int64_t)(t0 + token) * a.q_token_stride + head * a.q_head_stride;
 #pragma unroll
@@ -349,95 +350,101 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_kernel(cons
     }
   }
   __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the rows' loads too, which the loop would wait for at every stage
-  for (int s = 0; s < stages; s++) {
-    arrived();
-    __syncthreads();
-    if (s + 1 < stages) fetch(s + 1);
-    const bool masked_wg = s * SK + SK - 1 > wg_low;
-    if (masked_wg) {
-      // A NaN or an infinity of V would, through the product, reach rows that do
-      // not see its token: taken out here, and added at the end to the rows that do.
-      bool found = false;
-#pragma unroll
-      for (int i = 0; i < PER; i++) {
-        const u32x4 v = lds[s & 1][1][i * 64 * NW + threadIdx.x];
-#pragma unroll
-        for (int j = 0; j < 4; j++) found |= (v[j] & 0x7FFFu) >= inf_of(T{}) || ((v[j] >> 16) & 0x7FFFu) >= inf_of(T{});
-      }
-      if (__any(found) && lane == 0) odds = 1;
+  float l, ref;
+  f32x16(&o)[DT] = w.o;
+#pragma unroll 1
+  for (int pass = WALK;; pass++) {
+    w.init();
+    for (int s = 0; s < stages; s++) {
+      arrived();
       __syncthreads();
-      if (odds) {  // (rare; uniform)
-        odd = 1;
+      if (s + 1 < stages) fetch(s + 1);
+      if (pass != WALK) {  // (rare)
 #pragma unroll
         for (int i = 0; i < PER; i++) {
           u32x4 v = lds[s & 1][1][i * 64 * NW + threadIdx.x];
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            if ((v[j] & 0x7FFFu) >= inf_of(T{})) v[j] &= 0xFFFF0000u;
-            if (((v[j] >> 16) & 0x7FFFu) >= inf_of(T{})) v[j] &= 0xFFFFu;
-          }
+          for (int j = 0; j < 4; j++) v[j] = passed(T{}, v[j], pass);
           lds[s & 1][1][i * 64 * NW + threadIdx.x] = v;
         }
         __syncthreads();
       }
-    }
-    if (live && s * SK <= top_token) {
-      const bool masked = s * SK + SK - 1 > low;
-      if constexpr (WK == 1 && DP <= 128) {
-        w.template step<2, 1>(reads, lds[s & 1][0], {lds[s & 1][1]}, scale, masked, Upto{token - s * SK - 4 * g});
-      } else {
-        // a tile of 32 keys at a time: a wave's own, or what the registers hold
+      if (live && s * SK <= top_token) {
+        const bool masked = s * SK + SK - 1 > low;
+        if constexpr (WK == 1 && DP <= 128) {
+          w.template step<2, 1>(reads, lds[s & 1][0], {lds[s & 1][1]}, scale, masked, Upto{token - s * SK - 4 * g});
+        } else {
+          // a tile of 32 keys at a time: a wave's own, or what the registers hold
 #pragma unroll
-        for (int i = 0; i < 2 / WK; i++) {
-          const int u = WK == 1 ? i : wk;
-          w.template step<1, 1>(reads, lds[s & 1][0] + 32 * u * CH, {lds[s & 1][1] + 32 * u * CH}, scale, masked, Upto{token - s * SK - 32 * u - 4 * g});
+          for (int i = 0; i < 2 / WK; i++) {
+            const int u = WK == 1 ? i : wk;
+            w.template step<1, 1>(reads, lds[s & 1][0] + 32 * u * CH, {lds[s & 1][1] + 32 * u * CH}, scale, masked, Upto{token - s * SK - 32 * u - 4 * g});
+          }
         }
       }
     }
-  }
 
-  float l = pair_sum(w.l), ref = l == 0.0f ? NEG_INF : scale < 0.0f ? -w.reference() : w.reference();
-  f32x16(&o)[DT] = w.o;
-  if constexpr (WK == 2) {  // the two waves of the rows add up
-    __syncthreads();        // (the last stage's readers)
-    f32x16* sum = (f32x16*)&lds[0][0][0] + wr * DT * 64;
-    float* stat = (float*)&lds[1][0][0] + wr * 128;
-    if (wk == 1) {
+    l = pair_sum(w.l), ref = l == 0.0f ? NEG_INF : scale < 0.0f ? -w.reference() : w.reference();
+    if constexpr (WK == 2) {  // the two waves of the rows add up
+      __syncthreads();        // (the last stage's readers)
+      f32x16* sum = (f32x16*)&lds[0][0][0] + wr * DT * 64;
+      float* stat = (float*)&lds[1][0][0] + wr * 128;
+      if (wk == 1) {
 #pragma unroll
-      for (int d = 0; d < DT; d++) sum[d * 64 + lane] = o[d];
-      stat[lane] = ref;
-      stat[64 + lane] = l;
+        for (int d = 0; d < DT; d++) sum[d * 64 + lane] = o[d];
+        stat[lane] = ref;
+        stat[64 + lane] = l;
+      }
+      __syncthreads();
+      if (wk == 0) {
+        const float ref1 = stat[lane], l1 = stat[64 + lane], top = fmaxf(ref, ref1), mag = fabsf(scale);
+        // (a half without weights may hold what its masked products left)
+        const float f0 = ref == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((ref - top) * mag), f1 = ref1 == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((ref1 - top) * mag);
+        l = (ref == NEG_INF ? 0.0f : l * f0) + (ref1 == NEG_INF ? 0.0f : l1 * f1);
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+          const f32x16 y = sum[d * 64 + lane];
+#pragma unroll
+          for (int i = 0; i < 16; i++) o[d][i] = (ref == NEG_INF ? 0.0f : o[d][i] * f0) + (ref1 == NEG_INF ? 0.0f : y[i] * f1);
+        }
+        ref = top;
+      }
     }
-    __syncthreads();
-    if (wk == 1) return;
-    const float ref1 = stat[lane], l1 = stat[64 + lane], top = fmaxf(ref, ref1), mag = fabsf(scale);
-    // (a half without weights may hold what its masked products left)
-    const float f0 = ref == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((ref - top) * mag), f1 = ref1 == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((ref1 - top) * mag);
-    l = (ref == NEG_INF ? 0.0f : l * f0) + (ref1 == NEG_INF ? 0.0f : l1 * f1);
-#pragma unroll
-    for (int d = 0; d < DT; d++) {
-      const f32x16 y = sum[d * 64 + lane];
-#pragma unroll
-      for (int i = 0; i < 16; i++) o[d][i] = (ref == NEG_INF ? 0.0f : o[d][i] * f0) + (ref1 == NEG_INF ? 0.0f : y[i] * f1);
-    }
-    ref = top;
-  }
-  if (row >= R) return;
-  if (l == 0.0f) {  // every score -inf
-#pragma unroll
-    for (int d = 0; d < DT; d++) o[d] = fill16(0.0f);
-  }
-  if (odd && l != 0.0f) {  // (rare) the NaNs and infinities that were taken out, of the tokens that the row sees
-#pragma unroll 1
-    for (int j = wg_low / SK * SK; j <= token; j++)
+    if (pass == WALK) {
+      float z = 0.0f;
 #pragma unroll
       for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-          const int e = 32 * d + 8 * (r / 4) + 4 * g + r % 4;
-          const uint16_t v = e < a.head_dim ? vp[(int64_t)j * a.kv_token_stride + e] : 0;
-          if ((v & 0x7FFFu) >= inf_of(T{})) o[d][r] += T::widen(v);
+        for (int i = 0; i < 16; i++) z = __builtin_fmaf(o[d][i], 0.0f, z);
+      if (wk == 0 && row < R && l > 0.0f && z != z) odds = 1;
+      __syncthreads();
+      if (!odds) [[likely]] break;
+    } else if (pass == FINITE) {
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          if ((marks[0][d][threadIdx.x] >> i) & 1u) o[d][i] += -NEG_INF;
+          if ((marks[1][d][threadIdx.x] >> i) & 1u) o[d][i] += NEG_INF;
         }
+      break;
+    } else {
+#pragma unroll
+      for (int d = 0; d < DT; d++) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i++) m |= (o[d][i] > 0.0f ? 1u : 0u) << i;
+        marks[pass - ABOVE][d][threadIdx.x] = (uint16_t)m;
+      }
+      __syncthreads();  // (the stages' readers)
+    }
+    clear();
+    fetch(0);
+  }
+  if (wk == 1 || row >= R) return;
+  if (l == 0.0f) {  // every score -inf
+#pragma unroll
+    for (int d = 0; d < DT; d++) o[d] = fill16(0.0f);
   }
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint16_t* out = (uint16_t*)a.out + (int64_t)(t0 + token) * a.out_token_stride + head * a.out_head_stride;
