@@ -143,14 +143,22 @@ XS_DEV constexpr uint32_t one_of(Bf16) { return 0x3F80u; }
 XS_DEV constexpr uint32_t one_of(F16) { return 0x3C00u; }
 template <typename T>
 XS_DEV uint32_t passed(T, uint32_t two, int pass) {
-  uint32_t y = 0;
+  uint32_t y = 0, inf = inf_of(T{}), one = one_of(T{});
+  asm volatile("" : "+s"(inf), "+s"(one));  // (formed here, not kept in registers of the loops around)
 #pragma unroll
   for (int i = 0; i < 32; i += 16) {
     const uint32_t v = (two >> i) & 0xFFFFu, size = v & 0x7FFFu;
-    const bool odd = size >= inf_of(T{}), has = size > inf_of(T{}) || (v >> 15) == (pass == BELOW ? 1u : 0u);
-    y |= (pass == FINITE ? (odd ? 0u : v) : odd && has ? one_of(T{}) : 0u) << i;
+    const bool odd = size >= inf, has = size > inf || (v >> 15) == (pass == BELOW ? 1u : 0u);
+    y |= (pass == FINITE ? (odd ? 0u : v) : odd && has ? one : 0u) << i;
   }
   return y;
+}
+// y as marks say: inf where a value above has weight, -inf, or NaN where both have.
+XS_DEV float marked(float y, uint32_t above, uint32_t below, int i) {
+  uint32_t inf = 0x7F800000u;
+  asm volatile("" : "+s"(inf));
+  y += __uint_as_float(inf & (0u - ((above >> i) & 1u)));
+  return y - __uint_as_float(inf & (0u - ((below >> i) & 1u)));
 }
 
 // Over the four lanes of a row (x, 16 + x, 32 + x, 48 + x).
@@ -202,8 +210,8 @@ struct Shape {
   static constexpr int VE = DP >= 128 ? 8 : 4;       // value elements a lane loads of a half
   static constexpr int NF = VH * VE;                 // A fragments of V^T
   static constexpr int STAT = RT * NF * 256;         // floats of a partial result: fragments,
-  static constexpr int ODD = STAT + RT * 32;         // then m and l of each row,
-  static constexpr int PART = ODD + 4;               // then whether odd values are left out
+  static constexpr int PART = STAT + RT * 32 + 4;    // then m and l of each row, and 16 bytes to spare: what contexts are sized by
+  static constexpr int MARKS = (RT * NF + 7) / 8;    // words of a bit for each of a lane's elements
 };
 
 template <typename T, int DP, int RT>
@@ -220,7 +228,6 @@ struct Wave {
   std::conditional_t<ONCE, float, f32x4> c[RT];
   float most[RT];  // the x above which the reference moves: NaN until the row's first score
   float l[RT];
-  int odd;         // a node's values held a NaN or an infinity
 
   XS_DEV float minus(float v) const { return v; }
   XS_DEV float minus(const f32x4& v) const { return v[0]; }
@@ -234,7 +241,6 @@ struct Wave {
   }
 
   XS_DEV void init() {
-    odd = 0;
 #pragma unroll
     for (int t = 0; t < RT; t++) {
       refer(t, -0.0f);
@@ -309,6 +315,47 @@ struct Wave {
   XS_DEV float reference(int t, float scale) const { return scale < 0.0f ? minus(c[t]) : -minus(c[t]); }
 };
 
+// After a wave's pass over its keys (passed): whether it was the last.  `mine`: what
+// the lane's rows see of the tree, 0 where they count for nothing; marks: 2 MARKS
+// words of the lane, 64 apart.
+template <typename T, int DP, int RT>
+XS_DEV bool finished(Wave<T, DP, RT>& w, int pass, const uint64_t (&mine)[RT], uint32_t* marks) {
+  using S = Shape<DP, RT>;
+  if (pass == WALK) {
+    bool bad = false;
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+      float z = 0.0f;
+#pragma unroll
+      for (int f = 0; f < S::NF; f++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) z = __builtin_fmaf(w.o[t][f][r], 0.0f, z);
+      bad |= row_sum(w.l[t]) > 0.0f && z != z && mine[t] != 0;
+    }
+    if (!__any(bad)) [[likely]] return true;
+  } else {
+#pragma unroll
+    for (int i = 0; i < S::MARKS; i++) {
+      auto element = [&](int j) -> f32x4& { return w.o[(8 * i + j / 4) / S::NF][(8 * i + j / 4) % S::NF]; };
+      constexpr int LAST = 4 * RT * S::NF;
+      if (pass == FINITE) {
+        const uint32_t above = marks[64 * i], below = marks[64 * (S::MARKS + i)];
+#pragma unroll
+        for (int j = 0; j < 32 && 32 * i + j < LAST; j++) element(j)[j % 4] = marked(element(j)[j % 4], above, below, j);
+      } else {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 31; j >= 0; j--)
+          if (32 * i + j < LAST) m = m << 1 | (element(j)[j % 4] > 0.0f ? 1u : 0u);
+        marks[64 * (pass == BELOW ? S::MARKS + i : i)] = m;
+      }
+    }
+    if (pass == FINITE) return true;
+  }
+  w.init();
+  return false;
+}
+
 // O^T += V^T P^T over a block: v holds 16 bytes of each of the lane's eight
 // keys, pf the weights.
 template <typename T, int DP, int RT>
@@ -329,10 +376,10 @@ XS_DEV void accumulate(Wave<T, DP, RT>& w, const uint32_t (&v)[8][Shape<DP, RT>:
 
 // One block of 32 keys from base pointers (elements of one kv head): `limit`
 // keys of the source exist, `on` is the lane's mask of the block's keys for
-// each row tile (masked blocks only).
+// each row tile, `pass` what is made of the values (passed; masked blocks only).
 template <typename T, int DP, int RT, bool EXACT, bool MASKED>
 XS_DEV void block(Wave<T, DP, RT>& w, const uint16_t* kp, const uint16_t* vp, int64_t stride, int key0, int limit, int D, float scale,
-                  const uint32_t* on, bool in_tree) {
+                  const uint32_t* on, int pass) {
   using S = Shape<DP, RT>;
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
   u32x4 k[2][S::KC];
@@ -407,29 +454,21 @@ XS_DEV void block(Wave<T, DP, RT>& w, const uint16_t* kp, const uint16_t* vp, in
   }
   if (MASKED) {
     // Values of keys past the source count for nothing, whatever they hold.
-    // A NaN or an infinity of a node would, through the product (0 times it),
-    // reach the rows that do not see the node: it is taken out here, and
-    // store_pair adds it to the rows that do.
-    u16x2 top = {0, 0};
 #pragma unroll
     for (int e = 0; e < 8; e++)
 #pragma unroll
       for (int h = 0; h < S::VH; h++)
 #pragma unroll
-        for (int i = 0; i < S::VE / 2; i++) {
+        for (int i = 0; i < S::VE / 2; i++)
           if (key0 + 4 * g + (e & 3) + 16 * (e >> 2) >= limit) v[e][h][i] = 0;
-          top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, v[e][h][i] & 0x7FFF7FFFu));
-        }
-    if (in_tree && __any(max(top[0], top[1]) >= inf_of(T{}))) {
-      w.odd = 1;
+    if (pass != WALK) [[unlikely]] {
 #pragma unroll
       for (int e = 0; e < 8; e++)
 #pragma unroll
         for (int h = 0; h < S::VH; h++)
 #pragma unroll
           for (int i = 0; i < S::VE / 2; i++) {
-            if ((v[e][h][i] & 0x7FFFu) >= inf_of(T{})) v[e][h][i] &= 0xFFFF0000u;
-            if (((v[e][h][i] >> 16) & 0x7FFFu) >= inf_of(T{})) v[e][h][i] &= 0xFFFFu;
+            v[e][h][i] = passed(T{}, v[e][h][i], pass);
             __builtin_amdgcn_sched_barrier(0);
           }
     }
@@ -456,29 +495,18 @@ XS_DEV float lse_of(const xs_tree_attend_args& a, float ref, float l) {
   return l == 0.0f ? NEG_INF : __builtin_fmaf(ref, fabsf(a.scale), LN2 * (__builtin_amdgcn_logf(l) - offset_of(W{})));
 }
 
+// A result times what its weights are brought to another reference by; nothing,
+// whatever it is, where that is 0.
+XS_DEV f32x4 times(f32x4 y, float f) { return f == 0.0f ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : y * f; }
+
 // Two fragments (2 pair and 2 pair + 1 of half h) of a row tile's result: the
 // accumulators over l.  Lane (x, g) holds row x, elements 128 h + VE (4 g + r)
 // + 2 pair of each r.
 template <typename T, int DP, typename W = T>
-XS_DEV void store_pair(const xs_tree_attend_args& a, int G, int b, int kh, int row, int R, int h, int pair, f32x4 o0, f32x4 o1, float ref, float l, int odd,
-                       int n) {
+XS_DEV void store_pair(const xs_tree_attend_args& a, int G, int b, int kh, int row, int R, int h, int pair, f32x4 o0, f32x4 o1, float ref, float l) {
   constexpr int VE = Shape<DP, 1>::VE;
   const int g = (threadIdx.x & 63) >> 4;
   const int node = min(row, R - 1) / G, head = kh * G + min(row, R - 1) % G;
-  if (odd) {  // (rare) the NaNs and infinities among the values of the nodes that the row sees, but of an empty row's
-    const uint64_t sees = __shfl(ancestors(parent_of(a, b), n), node);
-    const uint16_t* v = (const uint16_t*)a.fresh.v + b * a.fresh.seq_stride + kh * a.fresh.head_stride;
-#pragma unroll 1
-    for (int j = 0; j < n; j++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int d = 128 * h + VE * (4 * g + r) + 2 * pair;
-        const uint32_t two = *(const uint32_t*)(v + j * a.fresh.slot_stride + min(d, a.head_dim - 2));
-        const uint16_t lo = (uint16_t)two, hi = (uint16_t)(two >> 16);
-        if (((sees >> j) & 1ull) && l != 0.0f && (lo & 0x7FFFu) >= inf_of(T{})) o0[r] += T::widen(lo);
-        if (((sees >> j) & 1ull) && l != 0.0f && (hi & 0x7FFFu) >= inf_of(T{})) o1[r] += T::widen(hi);
-      }
-  }
   if (row >= R) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint16_t* out = (uint16_t*)a.out + b * a.out_seq_stride + node * a.out_node_stride + head * a.out_head_stride;
@@ -535,7 +563,6 @@ __global__ __launch_bounds__(join_threads<DP>(FEWER)) void join_kernel(const xs_
   constexpr int MOST = FEWER ? FEW : SPLITS, TURNS = (MOST + 4 * WAVES - 1) / (4 * WAVES);
   __shared__ float weight[TURNS * 4 * WAVES][16];
   __shared__ float stat[2][WAVES][16];
-  __shared__ int odd;
   __shared__ f32x4 sum[SHARES][S::VE][64];
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -546,8 +573,6 @@ __global__ __launch_bounds__(join_threads<DP>(FEWER)) void join_kernel(const xs_
   const int R = sq.n * cut.G, row0 = (tile * RT + t) * 16;
   const int n = (sq.blocks() + cut.chunk - 1) / cut.chunk;
   if (sq.bad || row0 >= R || n <= 1) return;
-  if (threadIdx.x == 0) odd = 0;
-  __syncthreads();
   const float* part = cut.part + ((int64_t)bh * cut.nsplit * cut.tiles + tile) * S::PART;
   const int64_t step = (int64_t)cut.tiles * S::PART;
   // the first fragments, on their way while the weights are formed
@@ -569,7 +594,6 @@ __global__ __launch_bounds__(join_threads<DP>(FEWER)) void join_kernel(const xs_
     m[i] = s < n ? p[0] : NEG_INF;
     l[i] = p[16];
     top = fmaxf(top, m[i]);
-    if (p[S::ODD - S::STAT - 32 * t - x] != 0.0f) odd = 1;  // (any of them)
   }
   top = row_max(top);
   if (g == 0) stat[0][wave][x] = top;
@@ -590,15 +614,15 @@ __global__ __launch_bounds__(join_threads<DP>(FEWER)) void join_kernel(const xs_
   for (int i = 0; i < AHEAD; i++) {
     if (share + SHARES * i >= n) break;
     const float f = weight[share + SHARES * i][x];
-    o[0] += y[i][0] * f;
-    o[1] += y[i][1] * f;
+    o[0] += times(y[i][0], f);
+    o[1] += times(y[i][1], f);
   }
 #pragma unroll 8
   for (int s = share + SHARES * AHEAD; s < n; s += SHARES) {
     const f32x4* p = (const f32x4*)(part + s * step) + (t * S::NF + f0) * 64 + lane;
     const float f = weight[s][x];
-    o[0] += p[0] * f;
-    o[1] += p[64] * f;
+    o[0] += times(p[0], f);
+    o[1] += times(p[64], f);
   }
   all = 0.0f;
 #pragma unroll
@@ -614,7 +638,7 @@ __global__ __launch_bounds__(join_threads<DP>(FEWER)) void join_kernel(const xs_
       o[1] += sum[j][2 * pair + 1][lane];
     }
   }
-  store_pair<T, DP, W>(a, cut.G, b, kh, row0 + x, R, h, pair, o[0], o[1], top, all, odd, sq.n);
+  store_pair<T, DP, W>(a, cut.G, b, kh, row0 + x, R, h, pair, o[0], o[1], top, all);
 }
 
 }  // namespace xst

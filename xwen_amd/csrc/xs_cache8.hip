@@ -353,9 +353,9 @@ XS_DEV void cache_weights(Tile<T, DP, RT>& z, const Raw<DP>& r, float scale, con
       });
 }
 
-// Its second product.
+// Its second product, of values as `pass` takes them (xs_attend.h, passed).
 template <typename T, int DP, int RT>
-XS_DEV void cache_product(Tile<T, DP, RT>& z, const Raw<DP>& r, const u32x4 (&pf)[Parts<T>::N][RT]) {
+XS_DEV void cache_product(Tile<T, DP, RT>& z, const Raw<DP>& r, const u32x4 (&pf)[Parts<T>::N][RT], int pass) {
   using S = Shape<DP, RT>;
   const float vscale = pow2((int)r.ve - 127);
 #pragma unroll
@@ -365,6 +365,10 @@ XS_DEV void cache_product(Tile<T, DP, RT>& z, const Raw<DP>& r, const u32x4 (&pf
       uint32_t y[8];
 #pragma unroll
       for (int e = 0; e < 8; e++) y[e] = wide2(r.v[e][h][j / 4], vscale, j / 2 % 2);
+      if (pass != WALK) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = passed(Bf16{}, y[e], pass);
+      }
       u32x4 a[2];
 #pragma unroll
       for (int i = 0; i < 4; i++) {
@@ -384,7 +388,7 @@ XS_DEV void cache_product(Tile<T, DP, RT>& z, const Raw<DP>& r, const u32x4 (&pf
 // (z.q[0]).
 template <typename T, int DP, int RT, bool EXACT>
 XS_DEV void tree_block(Tile<T, DP, RT>& z, const uint16_t* kp, const uint16_t* vp, int64_t stride, int key0, int limit, int D, float scale,
-                       const uint32_t* on) {
+                       const uint32_t* on, int pass) {
   using S = Shape<DP, RT>;
   constexpr int N = Parts<T>::N;
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
@@ -411,13 +415,10 @@ XS_DEV void tree_block(Tile<T, DP, RT>& z, const uint16_t* kp, const uint16_t* v
         r[0] = y[0];
         r[1] = y[1];
       }
-      // What is not finite would, through the product, reach the rows that do not
-      // see the node: taken out here, added by store_pair to the rows that do.
 #pragma unroll
       for (int i = 0; i < S::VE / 2; i++) {
         if (slot >= limit) r[i] = 0;
-        if ((r[i] & 0x7FFFu) >= inf_of(T{})) r[i] &= 0xFFFF0000u, z.w.odd = 1;
-        if (((r[i] >> 16) & 0x7FFFu) >= inf_of(T{})) r[i] &= 0xFFFFu, z.w.odd = 1;
+        if (pass != WALK) r[i] = passed(T{}, r[i], pass);
       }
       u32x4 y[N];
       split8(T{}, r, y);
@@ -427,7 +428,6 @@ XS_DEV void tree_block(Tile<T, DP, RT>& z, const uint16_t* kp, const uint16_t* v
         for (int i = 0; i < S::VE / 2; i++) v[n][e][h][i] = y[n][i];
     }
   }
-  z.w.odd = __any(z.w.odd);
 #pragma unroll
   for (int m = 0; m < N; m++)
 #pragma unroll
@@ -532,7 +532,6 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
   using S = Shape<DP, RT>;
   __shared__ float stat[NW][RT][2][16];
   __shared__ f32x4 sum[NW][RT][S::NF][64];
-  __shared__ int odds[NW];
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int tile, kh, unit;
@@ -573,17 +572,20 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
     const int d = 64 * (c / 2) + 8 * (c % 2);
     return EXACT || d + 16 * g < a.head_dim ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0};
   };
+  auto queries = [&]() __attribute__((always_inline)) {
 #pragma unroll
-  for (int t = 0; t < RT; t++) {
-    const uint16_t* p = query(row0 + 16 * t + x);
+    for (int t = 0; t < RT; t++) {
+      const uint16_t* p = query(row0 + 16 * t + x);
 #pragma unroll
-    for (int c = 0; c < S::KC; c++) {
-      u32x4 y[Tile<T, DP, RT>::N];
-      split8(T{}, chunk(p, c), y);
+      for (int c = 0; c < S::KC; c++) {
+        u32x4 y[Tile<T, DP, RT>::N];
+        split8(T{}, chunk(p, c), y);
 #pragma unroll
-      for (int m = 0; m < Tile<T, DP, RT>::N; m++) z.q[m][t][c] = y[m];
+        for (int m = 0; m < Tile<T, DP, RT>::N; m++) z.q[m][t][c] = y[m];
+      }
     }
-  }
+  };
+  queries();
 
   // whole blocks of the cache: a block's registers take the next one's keys once
   // its scores are formed, and the next one's values after its second product (a
@@ -597,7 +599,7 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
     __builtin_amdgcn_sched_barrier(0);  // (the loads leave here, not where the last ones have come)
     load_keys8<DP, EXACT, false>(r, c8, at, eat, next, KB, a.head_dim);
     __builtin_amdgcn_sched_barrier(0);
-    cache_product<T, DP, RT>(z, r, pf);
+    cache_product<T, DP, RT>(z, r, pf, WALK);
     __builtin_amdgcn_sched_barrier(0);
     load_values8<DP, EXACT, false>(r, c8, at, eat, next, KB, a.head_dim);
     __builtin_amdgcn_sched_barrier(0);
@@ -611,45 +613,56 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
     mine[t] = __shfl(sees, min(row / cut.G, 63));
     if (row >= R) mine[t] = 0;
   }
+  auto rest = [&](int i, auto pass) __attribute__((always_inline)) {
 #pragma unroll 1
-  for (; i < min(last, cached); i += NW) {
-    const int limit = len - i * KB;
-    uint32_t on[RT];
+    for (; i < min(last, cached); i += NW) {
+      const int limit = len - i * KB;
+      uint32_t on[RT];
 #pragma unroll
-    for (int t = 0; t < RT; t++) on[t] = (1u << limit) - 1u;
-    load_keys8<DP, EXACT, true>(r, c8, at, eat, i, limit, a.head_dim);
-    u32x4 pf[Parts<T>::N][RT];
-    load_values8<DP, EXACT, true>(r, c8, at, eat, i, limit, a.head_dim);
-    __builtin_amdgcn_sched_barrier(0);
-    cache_weights<T, DP, RT, true>(z, r, cut.scale, on, pf);
-    __builtin_amdgcn_sched_barrier(0);
-    cache_product<T, DP, RT>(z, r, pf);
-  }
-  if (Parts<T>::N == 2 && i < last) {  // (whole queries, read again rather than kept)
-#pragma unroll
-    for (int t = 0; t < RT; t++) {
-      int row = row0 + 16 * t + x;
-      asm volatile("" : "+v"(row));
-      const uint16_t* p = query(row);
-#pragma unroll
-      for (int c = 0; c < S::KC; c++) z.q[0][t][c] = chunk(p, c);
+      for (int t = 0; t < RT; t++) on[t] = limit >= KB ? ~0u : (1u << limit) - 1u;
+      load_keys8<DP, EXACT, true>(r, c8, at, eat, i, limit, a.head_dim);
+      u32x4 pf[Parts<T>::N][RT];
+      load_values8<DP, EXACT, true>(r, c8, at, eat, i, limit, a.head_dim);
+      __builtin_amdgcn_sched_barrier(0);
+      cache_weights<T, DP, RT, true>(z, r, cut.scale, on, pf);
+      __builtin_amdgcn_sched_barrier(0);
+      cache_product<T, DP, RT>(z, r, pf, pass);
     }
-  }
-#pragma unroll 1
-  for (; i < last; i += NW) {
-    const int key0 = (i - cached) * KB;
-    uint32_t on[RT];
+    if (Parts<T>::N == 2 && i < last) {  // (whole queries, read again rather than kept)
 #pragma unroll
-    for (int t = 0; t < RT; t++) on[t] = (uint32_t)(mine[t] >> key0);
-    const int64_t f = b * a.fresh.seq_stride + kh * a.fresh.head_stride;
-    tree_block<T, DP, RT, EXACT>(z, (const uint16_t*)a.fresh.k + f, (const uint16_t*)a.fresh.v + f, a.fresh.slot_stride, key0, n, a.head_dim,
-                                 cut.scale, on);
+      for (int t = 0; t < RT; t++) {
+        int row = row0 + 16 * t + x;
+        asm volatile("" : "+v"(row));
+        const uint16_t* p = query(row);
+#pragma unroll
+        for (int c = 0; c < S::KC; c++) z.q[0][t][c] = chunk(p, c);
+      }
+    }
+#pragma unroll 1
+    for (; i < last; i += NW) {
+      const int key0 = (i - cached) * KB;
+      uint32_t on[RT];
+#pragma unroll
+      for (int t = 0; t < RT; t++) on[t] = (uint32_t)(mine[t] >> key0);
+      const int64_t f = b * a.fresh.seq_stride + kh * a.fresh.head_stride;
+      tree_block<T, DP, RT, EXACT>(z, (const uint16_t*)a.fresh.k + f, (const uint16_t*)a.fresh.v + f, a.fresh.slot_stride, key0, n, a.head_dim,
+                                   cut.scale, on, pass);
+    }
+  };
+  rest(i, std::integral_constant<int, WALK>{});
+  uint32_t* marked = (uint32_t*)&sum[wave] + lane;
+  if (!finished(z.w, WALK, mine, marked)) [[unlikely]] {
+    int pass = ABOVE;
+#pragma unroll 1
+    do {
+      if constexpr (Parts<T>::N == 2) queries();
+      rest(first + wave, pass);
+    } while (!finished(z.w, pass++, mine, marked));
   }
 
   // the waves' sums, brought to one reference; rows that see nothing of the
   // tree see nothing of the cache either
   float ref[RT];
-  if (lane == 0) odds[wave] = z.w.odd;
 #pragma unroll
   for (int t = 0; t < RT; t++) {
     z.w.l[t] = row_sum(z.w.l[t]);
@@ -669,13 +682,12 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
     for (int j = 0; j < NW; j++) top = fmaxf(top, stat[j][t][0][x]);
     const float f = ref[t] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((ref[t] - top) * mag);
 #pragma unroll
-    for (int k = 0; k < S::NF; k++) sum[wave][t][k][lane] = ref[t] == NEG_INF ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : z.w.o[t][k] * f;
+    for (int k = 0; k < S::NF; k++) sum[wave][t][k][lane] = times(z.w.o[t][k], f);
   }
   __syncthreads();
   // a wave takes every fourth pair of fragments
   constexpr int PAIRS = S::VE / 2;
   const bool whole = first == 0 && last == total;
-  const int odd = odds[0] | odds[1] | odds[2] | odds[3];
   float* part = cut.part + (((int64_t)unit * a.kv_heads + kh) * cut.tiles + tile) * S::PART;
 #pragma unroll 1
   for (int u = wave; u < RT * S::VH * PAIRS; u += NW) {
@@ -692,7 +704,7 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
       o[1] += sum[j][t][f0 + 1][lane];
     }
     if (whole) {
-      store_pair<T, DP, E4m3>(a, cut.G, b, kh, row0 + 16 * t + x, R, h, pair, o[0], o[1], top, all, odd, n);
+      store_pair<T, DP, E4m3>(a, cut.G, b, kh, row0 + 16 * t + x, R, h, pair, o[0], o[1], top, all);
     } else {
       f32x4* p = (f32x4*)part + (t * S::NF + f0) * 64 + lane;
       p[0] = o[0];
@@ -700,7 +712,6 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
       if (h == 0 && pair == 0 && g == 0) {
         part[S::STAT + 32 * t + x] = top;
         part[S::STAT + 32 * t + 16 + x] = all;
-        part[S::ODD] = odd ? 1.0f : 0.0f;
       }
     }
   }
@@ -717,7 +728,6 @@ __global__ __launch_bounds__((join8_threads<DP, SHARES>())) void join8_kernel(co
   constexpr int PAIRS = S::VE / 2, WAVES = PAIRS * SHARES;
   __shared__ float weight[SPLITS][16];
   __shared__ float stat[2][4 * WAVES][16];
-  __shared__ int odd;
   __shared__ f32x4 sum[SHARES][S::VE][64];
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), pair = wave % PAIRS, share = wave / PAIRS;
@@ -727,8 +737,6 @@ __global__ __launch_bounds__((join8_threads<DP, SHARES>())) void join8_kernel(co
   const Seq sq(a, b);
   const int nodes = __builtin_amdgcn_readfirstlane(sq.bad ? -1 : sq.n), R = nodes * cut.G, row0 = 16 * tile;
   if (row0 >= R || n <= 1) return;
-  if (threadIdx.x == 0) odd = 0;
-  __syncthreads();
   const float* part = cut.part + (((int64_t)(plan >> 16) * a.kv_heads + kh) * cut.tiles + tile) * S::PART;
   const int64_t step = a.kv_heads * cut.tiles * S::PART;
   // the first fragments, on their way while the weights are formed
@@ -746,7 +754,6 @@ __global__ __launch_bounds__((join8_threads<DP, SHARES>())) void join8_kernel(co
   for (int s = 4 * wave + g; s < n; s += 4 * WAVES) {
     const float* p = part + s * step;
     top = fmaxf(top, p[S::STAT + x]);
-    if (p[S::ODD] != 0.0f) odd = 1;  // (any of them)
   }
   stat[0][4 * wave + g][x] = top;
   __syncthreads();
@@ -765,15 +772,15 @@ __global__ __launch_bounds__((join8_threads<DP, SHARES>())) void join8_kernel(co
   for (int i = 0; i < AHEAD; i++) {
     if (share + SHARES * i >= n) break;
     const float f = weight[share + SHARES * i][x];
-    o[0] += y[i][0] * f;
-    o[1] += y[i][1] * f;
+    o[0] += times(y[i][0], f);
+    o[1] += times(y[i][1], f);
   }
 #pragma unroll 4
   for (int s = share + SHARES * AHEAD; s < n; s += SHARES) {
     const f32x4* p = (const f32x4*)(part + s * step) + f0 * 64 + lane;
     const float f = weight[s][x];
-    o[0] += p[0] * f;
-    o[1] += p[64] * f;
+    o[0] += times(p[0], f);
+    o[1] += times(p[64], f);
   }
   sum[share][2 * pair][lane] = o[0];
   sum[share][2 * pair + 1][lane] = o[1];
@@ -787,7 +794,7 @@ __global__ __launch_bounds__((join8_threads<DP, SHARES>())) void join8_kernel(co
     o[0] += sum[j][2 * pair][lane];
     o[1] += sum[j][2 * pair + 1][lane];
   }
-  store_pair<T, DP, E4m3>(a, cut.G, b, kh, row0 + x, R, h, pair, o[0], o[1], top, all, odd, nodes);
+  store_pair<T, DP, E4m3>(a, cut.G, b, kh, row0 + x, R, h, pair, o[0], o[1], top, all);
 }
 
 // More rows than that: 32 a wave (xs_rows32.h), of keys that the workgroup's
@@ -807,8 +814,7 @@ struct Shape32 {
   static constexpr int ROWS = 32 * W / WK, WR = W / WK;
   static constexpr int DT = DP / 32, NF = 4 * DT;    // fragments of four elements a lane
   static constexpr int STAT = WR * NF * 256;         // floats of a partial result: fragments,
-  static constexpr int ODD = STAT + 2 * ROWS;        // then m and l of each row,
-  static constexpr int PART = ODD + 4;               // then whether odd values are left out
+  static constexpr int PART = STAT + 2 * ROWS;       // then m and l of each row
 };
 
 // Stages of a sequence: the cache's, and the tree's one.
@@ -816,20 +822,9 @@ constexpr int STAGES_LEAST = 4, STAGES_WHOLE = 8;
 
 // Fragment f (elements e .. e + 4 of row `row`, e = 8 f + 4 g) of the result.
 template <typename T>
-XS_DEV void store_four(const xs_tree_attend_args& a, int G, int b, int kh, int row, int R, int f, f32x4 o, float ref, float l, int odd, int n) {
+XS_DEV void store_four(const xs_tree_attend_args& a, int G, int b, int kh, int row, int R, int f, f32x4 o, float ref, float l) {
   const int g = (threadIdx.x & 63) >> 5, e = 8 * f + 4 * g;
   const int node = min(row, R - 1) / G, head = kh * G + min(row, R - 1) % G;
-  if (odd) {  // (rare) the NaNs and infinities among the values of the nodes that the row sees, but of an empty row's
-    const uint64_t sees = __shfl(ancestors(parent_of(a, b), n), node);
-    const uint16_t* v = (const uint16_t*)a.fresh.v + b * a.fresh.seq_stride + kh * a.fresh.head_stride;
-#pragma unroll 1
-    for (int j = 0; j < n; j++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const uint16_t y = v[j * a.fresh.slot_stride + min(e + i, a.head_dim - 1)];
-        if (((sees >> j) & 1ull) && l != 0.0f && (y & 0x7FFFu) >= inf_of(T{})) o[i] += T::widen(y);
-      }
-  }
   if (row >= R) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   uint16_t* out = (uint16_t*)a.out + b * a.out_seq_stride + node * a.out_node_stride + head * a.out_head_stride;
@@ -844,10 +839,11 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend8_wide_kernel
   constexpr int N = Parts<T>::N, CH = K::CH, KC = DP / 16, DT = DP / 32, TH = 64 * W;
   constexpr int PER = SK * (DP / 16) / TH;  // 16-byte pieces of the cache that a thread moves, of k and of v
   static_assert(SK * (DP / 16) % TH == 0, "a stage is whole pieces of every thread");
+  constexpr int NE = PER < SK / KB ? PER : SK / KB;  // a thread's exponents: its pieces j of PER / NE lie in one block
   __shared__ u32x4 lk[2][K::STAGE];
   __shared__ u32x4 lv[2][K::STAGE];
-  __shared__ int odds;
-  const int lane = threadIdx.x & 63, x = lane & 31, g = lane >> 5;
+  __shared__ uint16_t marks[2][DT][TH];  // [above, below] a lane's elements that an infinity reaches
+  __shared__ int odds;                   // a result is not finite
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = wave / WK, wk = wave % WK;
   int tile, kh, unit;
   deal(cut, &tile, &kh, &unit);
@@ -862,194 +858,242 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend8_wide_kernel
     a.seq_status[b] = n < 0 ? XS_ROW_BAD_PARAM : XS_ROW_OK;
     if (cut.room) cut.plan[b] = unit << 16 | splits;
   }
-  const int R = n * cut.G, row = tile * S::ROWS + 32 * wr + x;
+  const int R = n * cut.G;
   const int cached = (len + SK - 1) / SK, total = cached + (n > 0 ? 1 : 0), first = split * share, last = splits == 1 ? total : min(first + share, total);
   if (tile * S::ROWS >= R || first >= total) return;  // (nodes below 0 too)
-
-  const int parent = parent_of(a, b);
-  Rows32<Bf16, DP, N> w;
-  w.init();
-  auto query = [&](int r) {
-    const int node = min(r, R - 1) / cut.G, head = kh * cut.G + min(r, R - 1) % cut.G;
-    return (const uint16_t*)a.q + b * a.q_seq_stride + node * a.q_node_stride + head * a.q_head_stride;
-  };
-  auto chunk = [&](const uint16_t* p, int c) {
-    const int d = 16 * c + 8 * g;
-    return row < R && (EXACT || d < a.head_dim) ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0};
-  };
-  {
-    const uint16_t* p = query(row);
-#pragma unroll
-    for (int c = 0; c < KC; c++) {
-      u32x4 y[N];
-      split8(T{}, chunk(p, c), y);
-#pragma unroll
-      for (int m = 0; m < N; m++) w.q[m][c] = y[m];
-    }
-  }
-  const uint64_t seen = ancestors(parent, n);
-  const uint64_t mine = __shfl(seen, min(row / cut.G, 63)) & (row < R ? ~0ull : 0ull);  // what the lane's row sees of the tree
-  const Reads<DP> reads;
 
   // whole and part stages of the cache
   const int end = min(last, cached);
   const int64_t at = b * c8.seq_stride + kh * c8.head_stride, eat = (int64_t)bh * c8.exp_ld;
   const uint32_t stride = (uint32_t)c8.slot_stride;
-  u32x4 rk[PER], rv[PER];
-  uint32_t ek[PER], ev[PER];
-  auto fetch = [&](int s) {
-    const int64_t base = at + (int64_t)s * SK * c8.slot_stride;
-    const int most = len - 1 - s * SK;
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-      const int p = j * TH + threadIdx.x, r = min(p / (DP / 16), most), c = p % (DP / 16);
-      const uint32_t off = (uint32_t)r * stride + 16 * c;
-      const bool in = EXACT || 16 * c < a.head_dim;
-      rk[j] = in ? *(const u32x4*)(c8.k + base + off) : (u32x4){0, 0, 0, 0};
-      rv[j] = in ? *(const u32x4*)(c8.v + base + off) : (u32x4){0, 0, 0, 0};
-      ek[j] = c8.k_exp[eat + s * (SK / KB) + r / KB];
-      ev[j] = c8.v_exp[eat + s * (SK / KB) + r / KB];
-    }
-  };
-  auto put = [&](int s) {
-    const int most = len - 1 - s * SK;
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-      const int p = j * TH + threadIdx.x, r = p / (DP / 16), c = p % (DP / 16);
-      const float ks = pow2((int)ek[j] - 127), vs = pow2((int)ev[j] - 127);
-      const u32x4 y = r <= most ? rv[j] : (u32x4){0, 0, 0, 0};  // (past the length: nothing, whatever it holds)
-#pragma unroll
-      for (int h = 0; h < 2; h++) {
-        u32x4 k, v;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          k[i] = wide2(rk[j][2 * h + i / 2], ks, i % 2);
-          v[i] = wide2(y[2 * h + i / 2], vs, i % 2);
-        }
-        lk[s & 1][r * CH + ((2 * c + h) ^ K::turn_k(r))] = k;
-        lv[s & 1][r * CH + ((2 * c + h) ^ K::turn_v(r))] = v;
-      }
-    }
-  };
-  auto step = [&](const u32x4* ks, const u32x4* vs, bool masked, uint64_t on) {
-    // (f16: a tile at a time, which the registers hold beside two parts of each row)
-    constexpr int U = N == 1 && WK == 1 ? 2 : 1, STEPS = 2 / (U * WK);
-#pragma unroll
-    for (int i = 0; i < STEPS; i++) {
-      const int u = WK == 1 ? i : wk;
-      const uint64_t bits = on >> (32 * u + 4 * g);
-      w.template step<U, 1>(reads, ks + 32 * u * CH, {vs + 32 * u * CH}, cut.scale, masked, Bits{(uint32_t)bits, (uint32_t)(bits >> 32)});
-    }
-  };
-  if (first < end) {
-    fetch(first);
-    put(first);
-    if (first + 1 < end) fetch(first + 1);
-  }
+  Rows32<Bf16, DP, N> w;
+  float l, ref;
+  int row;
+  if (threadIdx.x == 0) odds = 0;
 #pragma unroll 1
-  for (int s = first; s < end; s++) {
-    __syncthreads();
-    if (s + 1 < end) put(s + 1);
-    if (s + 2 < end) fetch(s + 2);
-    const int limit = len - s * SK;
-    step(lk[s & 1], lv[s & 1], limit < SK, limit < SK ? (1ull << limit) - 1ull : ~0ull);
-  }
-  // the tree: keys and queries as they are, parts of the values in a buffer each
-  int odd = 0;
-  if (last == total) {
-    if (threadIdx.x == 0) odds = 0;
-    __syncthreads();
-    const int64_t f = b * a.fresh.seq_stride + kh * a.fresh.head_stride;
-#pragma unroll 1
-    for (int p = threadIdx.x; p < K::STAGE; p += TH) {
-      const int r = p / CH, c = p % CH;
-      u32x4 k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
-      if (r < n && (EXACT || 8 * c < a.head_dim)) {
-        k = *(const u32x4*)((const uint16_t*)a.fresh.k + f + r * a.fresh.slot_stride + 8 * c);
-        v = *(const u32x4*)((const uint16_t*)a.fresh.v + f + r * a.fresh.slot_stride + 8 * c);
-      }
-      // What is not finite would, through the product, reach the rows that do not
-      // see the node: taken out here, added by store_four to the rows that do.
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        if ((v[i] & 0x7FFFu) >= inf_of(T{})) v[i] &= 0xFFFF0000u, odds = 1;
-        if (((v[i] >> 16) & 0x7FFFu) >= inf_of(T{})) v[i] &= 0xFFFFu, odds = 1;
-      }
-      lk[0][r * CH + (c ^ K::turn_k(r))] = k;
-      u32x4 vs[N];
-      split8(T{}, v, vs);
-#pragma unroll
-      for (int m = 0; m < N; m++) lv[m][r * CH + (c ^ K::turn_v(r))] = vs[m];
-    }
-    __syncthreads();
-    if constexpr (N == 2) {
-      int again = row;
-      asm volatile("" : "+v"(again));  // (whole queries, read again rather than kept)
-      const uint16_t* p = query(again);
+  for (int pass = WALK;; pass++) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // (nothing of a lane's is kept from pass to pass)
+    const int lane = tid & 63, x = lane & 31, g = lane >> 5;
+    row = tile * S::ROWS + 32 * wr + x;
+    const int parent = parent_of(a, b);
+    auto query = [&](int r) {
+      const int node = min(r, R - 1) / cut.G, head = kh * cut.G + min(r, R - 1) % cut.G;
+      return (const uint16_t*)a.q + b * a.q_seq_stride + node * a.q_node_stride + head * a.q_head_stride;
+    };
+    auto chunk = [&](const uint16_t* p, int c) {
+      const int d = 16 * c + 8 * g;
+      return row < R && (EXACT || d < a.head_dim) ? *(const u32x4*)(p + d) : (u32x4){0, 0, 0, 0};
+    };
+    {
+      const uint16_t* p = query(row);
 #pragma unroll
       for (int c = 0; c < KC; c++) w.q[0][c] = chunk(p, c);
+      if constexpr (N == 2) {
+#pragma unroll
+        for (int c = 0; c < KC; c++) {
+          __builtin_amdgcn_sched_barrier(0);  // (one chunk's comparisons at a time)
+          u32x4 y[N];
+          split8(T{}, w.q[0][c], y);
+          w.q[0][c] = y[0];
+          w.q[1][c] = y[1];
+        }
+      }
     }
-    odd = odds;
-#pragma unroll 1
-    for (int i = 0; i < 2 / WK; i++) {
-      const int u = WK == 1 ? i : wk;
-      const uint64_t bits = mine >> (32 * u + 4 * g);
-      const Bits on = {(uint32_t)bits, (uint32_t)(bits >> 32)};
-      if (32 * u >= n) continue;
-      if constexpr (N == 1) w.template step<1, 1>(reads, lk[0] + 32 * u * CH, {lv[0] + 32 * u * CH}, cut.scale, true, on);
-      else w.template step<1, 2, 1, F16>(reads, lk[0] + 32 * u * CH, {lv[0] + 32 * u * CH, lv[1] + 32 * u * CH}, cut.scale, true, on);
-    }
-  }
+    const uint64_t seen = ancestors(parent, n);
+    const uint64_t mine = __shfl(seen, min(row / cut.G, 63)) & (row < R ? ~0ull : 0ull);  // what the lane's row sees of the tree
+    const Reads<DP> reads(lane);
 
-  // rows that see nothing of the tree see nothing of the cache either
-  float l = mine == 0 ? 0.0f : pair_sum(w.l);
-  float ref = l == 0.0f ? NEG_INF : cut.scale < 0.0f ? -w.reference() : w.reference();
-  if (l == 0.0f) {
+    u32x4 rk[PER], rv[PER];
+    uint32_t ek[NE], ev[NE];
+    auto fetch = [&](int s) {
+      const int64_t base = at + (int64_t)s * SK * c8.slot_stride;
+      const int most = len - 1 - s * SK;
 #pragma unroll
-    for (int d = 0; d < DT; d++) w.o[d] = fill16(0.0f);
-  }
-  if constexpr (WK == 2) {
-    __syncthreads();  // (the stages' last readers)
-    f32x4* sum = (f32x4*)&lk[0][0] + wr * S::NF * 64;
-    float* stat = (float*)&lv[0][0] + wr * 64;
-    if (wk == 1) {
-#pragma unroll
-      for (int f = 0; f < S::NF; f++) {
-        const f32x16 o = w.o[f / 4];
-        sum[f * 64 + lane] = (f32x4){o[4 * (f % 4)], o[4 * (f % 4) + 1], o[4 * (f % 4) + 2], o[4 * (f % 4) + 3]};
+      for (int j = 0; j < PER; j++) {
+        const int p = j * TH + tid, r = min(p / (DP / 16), most), c = p % (DP / 16);
+        const uint32_t off = (uint32_t)r * stride + 16 * c;
+        const bool in = EXACT || 16 * c < a.head_dim;
+        rk[j] = in ? *(const u32x4*)(c8.k + base + off) : (u32x4){0, 0, 0, 0};
+        rv[j] = in ? *(const u32x4*)(c8.v + base + off) : (u32x4){0, 0, 0, 0};
+        if (j % (PER / NE) == 0) {
+          ek[j / (PER / NE)] = c8.k_exp[eat + s * (SK / KB) + r / KB];
+          ev[j / (PER / NE)] = c8.v_exp[eat + s * (SK / KB) + r / KB];
+        }
       }
-      if (g == 0) {
-        stat[x] = ref;
-        stat[32 + x] = l;
+    };
+    auto put = [&](int s) {
+      const int most = len - 1 - s * SK;
+#pragma unroll
+      for (int j = 0; j < PER; j++) {
+        const int p = j * TH + tid, r = p / (DP / 16), c = p % (DP / 16);
+        const float ks = pow2((int)ek[j / (PER / NE)] - 127), vs = pow2((int)ev[j / (PER / NE)] - 127);
+        const u32x4 y = r <= most ? rv[j] : (u32x4){0, 0, 0, 0};  // (past the length: nothing, whatever it holds)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          u32x4 k, v;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            k[i] = wide2(rk[j][2 * h + i / 2], ks, i % 2);
+            v[i] = wide2(y[2 * h + i / 2], vs, i % 2);
+          }
+          lk[s & 1][r * CH + ((2 * c + h) ^ K::turn_k(r))] = k;
+          lv[s & 1][r * CH + ((2 * c + h) ^ K::turn_v(r))] = v;
+        }
+      }
+      if (pass != WALK) [[unlikely]] {  // (the thread's own pieces)
+#pragma unroll 1
+        for (int i = 0; i < 2 * PER; i++) {
+          const int p = i / 2 * TH + tid, r = p / (DP / 16);
+          u32x4* v = &lv[s & 1][r * CH + ((2 * (p % (DP / 16)) + i % 2) ^ K::turn_v(r))];
+#pragma unroll
+          for (int e = 0; e < 4; e++) (*v)[e] = passed(Bf16{}, (*v)[e], pass);
+        }
+      }
+    };
+    auto step = [&](const u32x4* ks, const u32x4* vs, bool masked, uint64_t on) {
+      // (f16: a tile at a time, which the registers hold beside two parts of each row)
+      constexpr int U = N == 1 && WK == 1 ? 2 : 1, STEPS = 2 / (U * WK);
+#pragma unroll
+      for (int i = 0; i < STEPS; i++) {
+        const int u = WK == 1 ? i : wk;
+        const uint64_t bits = on >> (32 * u + 4 * g);
+        w.template step<U, 1>(reads, ks + 32 * u * CH, {vs + 32 * u * CH}, cut.scale, masked, Bits{(uint32_t)bits, (uint32_t)(bits >> 32)});
+      }
+    };
+
+    w.init();
+    if (first < end) {
+      fetch(first);
+      put(first);
+      if (first + 1 < end) fetch(first + 1);
+    }
+#pragma unroll 1
+    for (int s = first; s < end; s++) {
+      __syncthreads();
+      if (s + 1 < end) put(s + 1);
+      if (s + 2 < end) fetch(s + 2);
+      const int limit = len - s * SK;
+      step(lk[s & 1], lv[s & 1], limit < SK, limit < SK ? (1ull << limit) - 1ull : ~0ull);
+    }
+    // the tree: keys and queries as they are, parts of the values in a buffer each
+    if (last == total) {
+      __syncthreads();
+      const int64_t f = b * a.fresh.seq_stride + kh * a.fresh.head_stride;
+#pragma unroll 1
+      for (int p = tid; p < K::STAGE; p += TH) {
+        const int r = p / CH, c = p % CH;
+        u32x4 k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
+        if (r < n && (EXACT || 8 * c < a.head_dim)) {
+          k = *(const u32x4*)((const uint16_t*)a.fresh.k + f + r * a.fresh.slot_stride + 8 * c);
+          v = *(const u32x4*)((const uint16_t*)a.fresh.v + f + r * a.fresh.slot_stride + 8 * c);
+        }
+        if (pass != WALK) [[unlikely]] {
+#pragma unroll
+          for (int i = 0; i < 4; i++) v[i] = passed(T{}, v[i], pass);
+        }
+        lk[0][r * CH + (c ^ K::turn_k(r))] = k;
+        u32x4 vs[N];
+        split8(T{}, v, vs);
+#pragma unroll
+        for (int m = 0; m < N; m++) lv[m][r * CH + (c ^ K::turn_v(r))] = vs[m];
+      }
+      __syncthreads();
+      if constexpr (N == 2) {
+        int again = row;
+        asm volatile("" : "+v"(again));  // (whole queries, read again rather than kept)
+        const uint16_t* p = query(again);
+#pragma unroll
+        for (int c = 0; c < KC; c++) w.q[0][c] = chunk(p, c);
+      }
+#pragma unroll 1
+      for (int i = 0; i < 2 / WK; i++) {
+        const int u = WK == 1 ? i : wk;
+        const uint64_t bits = mine >> (32 * u + 4 * g);
+        const Bits on = {(uint32_t)bits, (uint32_t)(bits >> 32)};
+        if (32 * u >= n) continue;
+        if constexpr (N == 1) w.template step<1, 1>(reads, lk[0] + 32 * u * CH, {lv[0] + 32 * u * CH}, cut.scale, true, on);
+        else w.template step<1, 2, 1, F16>(reads, lk[0] + 32 * u * CH, {lv[0] + 32 * u * CH, lv[1] + 32 * u * CH}, cut.scale, true, on);
       }
     }
-    __syncthreads();
-    if (wk == 1) return;
-    const float ref1 = stat[x], l1 = stat[32 + x], top = fmaxf(ref, ref1), mag = fabsf(cut.scale);
-    const float f0 = ref == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((ref - top) * mag);
-    const float f1 = ref1 == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((ref1 - top) * mag);
-    l = (ref == NEG_INF ? 0.0f : l * f0) + (ref1 == NEG_INF ? 0.0f : l1 * f1);
-    ref = top;
+
+    // rows that see nothing of the tree see nothing of the cache either
+    l = mine == 0 ? 0.0f : pair_sum(w.l);
+    ref = l == 0.0f ? NEG_INF : cut.scale < 0.0f ? -w.reference() : w.reference();
+    if (l == 0.0f) {
 #pragma unroll
-    for (int f = 0; f < S::NF; f++) {
-      const f32x4 y = sum[f * 64 + lane];
+      for (int d = 0; d < DT; d++) w.o[d] = fill16(0.0f);
+    }
+    if constexpr (WK == 2) {
+      __syncthreads();  // (the stages' last readers)
+      f32x4* sum = (f32x4*)&lk[0][0] + wr * S::NF * 64;
+      float* stat = (float*)&lv[0][0] + wr * 64;
+      if (wk == 1) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) w.o[f / 4][4 * (f % 4) + i] = __builtin_fmaf(w.o[f / 4][4 * (f % 4) + i], f0, y[i] * f1);
+        for (int f = 0; f < S::NF; f++) {
+          const f32x16 o = w.o[f / 4];
+          sum[f * 64 + lane] = (f32x4){o[4 * (f % 4)], o[4 * (f % 4) + 1], o[4 * (f % 4) + 2], o[4 * (f % 4) + 3]};
+        }
+        if (g == 0) {
+          stat[x] = ref;
+          stat[32 + x] = l;
+        }
+      }
+      __syncthreads();
+      if (wk == 0) {
+        const float ref1 = stat[x], l1 = stat[32 + x], top = fmaxf(ref, ref1), mag = fabsf(cut.scale);
+        const float f0 = ref == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((ref - top) * mag);
+        const float f1 = ref1 == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((ref1 - top) * mag);
+        l = (ref == NEG_INF ? 0.0f : l * f0) + (ref1 == NEG_INF ? 0.0f : l1 * f1);
+        ref = top;
+#pragma unroll
+        for (int f = 0; f < S::NF; f++) {
+          const f32x4 y = sum[f * 64 + lane];
+#pragma unroll
+          for (int i = 0; i < 4; i++) w.o[f / 4][4 * (f % 4) + i] = __builtin_fmaf(w.o[f / 4][4 * (f % 4) + i], f0, y[i] * f1);
+        }
+      }
+    }
+    if (pass == WALK) {
+      float z = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) z = __builtin_fmaf(w.o[d][i], 0.0f, z);
+      if (wk == 0 && row < R && l > 0.0f && z != z) odds = 1;
+      __syncthreads();
+      if (!__builtin_amdgcn_readfirstlane(odds)) [[likely]] break;
+    } else if (pass == FINITE) {
+#pragma unroll
+      for (int d = 0; d < DT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) w.o[d][i] = marked(w.o[d][i], marks[0][d][tid], marks[1][d][tid], i);
+      break;
+    } else {
+#pragma unroll
+      for (int d = 0; d < DT; d++) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 15; i >= 0; i--) m = m << 1 | (w.o[d][i] > 0.0f ? 1u : 0u);
+        marks[pass - ABOVE][d][tid] = (uint16_t)m;
+      }
+      __syncthreads();  // (the stages' readers)
     }
   }
+  if (wk == 1) return;
+  const int lane = threadIdx.x & 63, x = lane & 31, g = lane >> 5;
   const bool whole = first == 0 && last == total;
   float* part = cut.part + (((int64_t)unit * a.kv_heads + kh) * cut.tiles + tile) * S::PART;
 #pragma unroll
   for (int f = 0; f < S::NF; f++) {
     const f32x16 o = w.o[f / 4];
     const f32x4 y = {o[4 * (f % 4)], o[4 * (f % 4) + 1], o[4 * (f % 4) + 2], o[4 * (f % 4) + 3]};
-    if (whole) store_four<T>(a, cut.G, b, kh, row, R, f, y, ref, l, odd, n);
+    if (whole) store_four<T>(a, cut.G, b, kh, row, R, f, y, ref, l);
     else ((f32x4*)part)[(wr * S::NF + f) * 64 + lane] = y;
   }
   if (!whole && g == 0) {
     part[S::STAT + 32 * wr + x] = ref;
     part[S::STAT + S::ROWS + 32 * wr + x] = l;
-    if (wr == 0) part[S::ODD] = odd ? 1.0f : 0.0f;
   }
 }
 
@@ -1061,7 +1105,6 @@ __global__ __launch_bounds__(256 * SHARES) void join32_kernel(const xs_tree_atte
   constexpr int WAVES = 4 * SHARES;
   __shared__ float weight[SPLITS][32];
   __shared__ float stat[2][2 * WAVES][32];
-  __shared__ int odd;
   __shared__ f32x4 sum[SHARES][4][64];
   const int lane = threadIdx.x & 63, x = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), share = wave / 4;
@@ -1071,8 +1114,6 @@ __global__ __launch_bounds__(256 * SHARES) void join32_kernel(const xs_tree_atte
   const Seq sq(a, b);
   const int nodes = __builtin_amdgcn_readfirstlane(sq.bad ? -1 : sq.n), R = nodes * cut.G, row = tile * S::ROWS + 32 * wr + x;
   if (tile * S::ROWS + 32 * wr >= R || n <= 1) return;
-  if (threadIdx.x == 0) odd = 0;
-  __syncthreads();
   const float* part = cut.part + (((int64_t)(plan >> 16) * a.kv_heads + kh) * cut.tiles + tile) * S::PART;
   const int64_t step = a.kv_heads * cut.tiles * S::PART;
   // the first fragments, on their way while the weights are formed
@@ -1085,7 +1126,6 @@ __global__ __launch_bounds__(256 * SHARES) void join32_kernel(const xs_tree_atte
   for (int s = 2 * wave + g; s < n; s += 2 * WAVES) {
     const float* p = part + s * step;
     top = fmaxf(top, p[S::STAT + 32 * wr + x]);
-    if (p[S::ODD] != 0.0f) odd = 1;  // (any of them)
   }
   stat[0][2 * wave + g][x] = top;
   __syncthreads();
@@ -1103,10 +1143,10 @@ __global__ __launch_bounds__(256 * SHARES) void join32_kernel(const xs_tree_atte
 #pragma unroll
   for (int i = 0; i < AHEAD; i++) {
     if (share + SHARES * i >= n) break;
-    o += y[i] * weight[share + SHARES * i][x];
+    o += times(y[i], weight[share + SHARES * i][x]);
   }
 #pragma unroll 8
-  for (int s = share + SHARES * AHEAD; s < n; s += SHARES) o += ((const f32x4*)(part + s * step))[(wr * S::NF + f) * 64 + lane] * weight[s][x];
+  for (int s = share + SHARES * AHEAD; s < n; s += SHARES) o += times(((const f32x4*)(part + s * step))[(wr * S::NF + f) * 64 + lane], weight[s][x]);
   sum[share][wave % 4][lane] = o;
   __syncthreads();
   if (share != 0) return;
@@ -1115,7 +1155,7 @@ __global__ __launch_bounds__(256 * SHARES) void join32_kernel(const xs_tree_atte
   for (int j = 0; j < 2 * WAVES; j++) all += stat[1][j][x];
 #pragma unroll
   for (int j = 1; j < SHARES; j++) o += sum[j][wave % 4][lane];
-  store_four<T>(a, cut.G, b, kh, row, R, f, o, top, all, odd, nodes);
+  store_four<T>(a, cut.G, b, kh, row, R, f, o, top, all);
 }
 
 }  // namespace xs8

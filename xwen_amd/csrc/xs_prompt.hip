@@ -337,7 +337,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_kernel(cons
 
   clear();
   fetch(0);
-  const Reads<DP> reads;
+  const Reads<DP> reads(lane);
   if (threadIdx.x == 0) odds = 0;
 
   Rows32<T, DP, 1> w;
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_kernel(cons
       arrived();
       __syncthreads();
       if (s + 1 < stages) fetch(s + 1);
-      if (pass != WALK) {  // (rare)
+      if (pass != WALK) [[unlikely]] {
 #pragma unroll
         for (int i = 0; i < PER; i++) {
           u32x4 v = lds[s & 1][1][i * 64 * NW + threadIdx.x];
@@ -418,22 +418,19 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void prompt_kernel(cons
         for (int i = 0; i < 16; i++) z = __builtin_fmaf(o[d][i], 0.0f, z);
       if (wk == 0 && row < R && l > 0.0f && z != z) odds = 1;
       __syncthreads();
-      if (!odds) [[likely]] break;
+      if (!__builtin_amdgcn_readfirstlane(odds)) [[likely]] break;
     } else if (pass == FINITE) {
 #pragma unroll
       for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          if ((marks[0][d][threadIdx.x] >> i) & 1u) o[d][i] += -NEG_INF;
-          if ((marks[1][d][threadIdx.x] >> i) & 1u) o[d][i] += NEG_INF;
-        }
+        for (int i = 0; i < 16; i++) o[d][i] = marked(o[d][i], marks[0][d][threadIdx.x], marks[1][d][threadIdx.x], i);
       break;
     } else {
 #pragma unroll
       for (int d = 0; d < DT; d++) {
         uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 16; i++) m |= (o[d][i] > 0.0f ? 1u : 0u) << i;
+        for (int i = 15; i >= 0; i--) m = m << 1 | (o[d][i] > 0.0f ? 1u : 0u);
         marks[pass - ABOVE][d][threadIdx.x] = (uint16_t)m;
       }
       __syncthreads();  // (the stages' readers)

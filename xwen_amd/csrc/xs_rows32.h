@@ -65,8 +65,8 @@ struct Reads {
   using K = Keys<DP>;
   static constexpr int CH = K::CH;
   int krow, kturn, vrow, vturn;
-  XS_DEV Reads() {
-    const int lane = threadIdx.x & 63, x = lane & 31, g = lane >> 5, i = lane & 15, vr = 4 * g + (i >> 2);
+  XS_DEV explicit Reads(int lane) {
+    const int x = lane & 31, g = lane >> 5, i = lane & 15, vr = 4 * g + (i >> 2);
     krow = x * CH * 16;
     kturn = 16 * (g ^ K::turn_k(x));
     vrow = vr * CH * 16 + 8 * (i & 1);

@@ -25,7 +25,6 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
   using S = Shape<DP, RT>;
   __shared__ float stat[NW][RT][2][16];
   __shared__ f32x4 sum[NW][RT][S::NF][64];
-  __shared__ int odds[NW];
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tile = (blockIdx.x >> 3) % cut.tiles;
@@ -63,7 +62,7 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
   int i = first + wave;
   // whole blocks of the cache
   for (; i < last && (i + 1) * KB <= sq.len; i += NW)
-    block<T, DP, RT, EXACT, false>(w, ck, cv, a.cache.slot_stride, i * KB, sq.len, a.head_dim, cut.scale, nullptr, false);
+    block<T, DP, RT, EXACT, false>(w, ck, cv, a.cache.slot_stride, i * KB, sq.len, a.head_dim, cut.scale, nullptr, WALK);
   // its last one, and the tree's
   const uint64_t sees = ancestors(parent, sq.n);
   uint64_t mine[RT];  // what the lane's rows see of the tree
@@ -73,23 +72,33 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
     mine[t] = __shfl(sees, min(row / cut.G, 63));
     if (row >= R) mine[t] = 0;
   }
+  auto rest = [&](int i, auto pass) __attribute__((always_inline)) {
 #pragma unroll 1
-  for (; i < last; i += NW) {
-    const bool in_tree = i >= cached;
-    const int key0 = (in_tree ? i - cached : i) * KB, limit = in_tree ? sq.n : sq.len;
-    const xs_kv& kv = in_tree ? a.fresh : a.cache;
-    const int64_t at = b * kv.seq_stride + kh * kv.head_stride;
-    uint32_t on[RT];
+    for (; i < last; i += NW) {
+      const bool in_tree = i >= cached;
+      const int key0 = (in_tree ? i - cached : i) * KB, limit = in_tree ? sq.n : sq.len;
+      const xs_kv& kv = in_tree ? a.fresh : a.cache;
+      const int64_t at = b * kv.seq_stride + kh * kv.head_stride;
+      uint32_t on[RT];
 #pragma unroll
-    for (int t = 0; t < RT; t++) on[t] = in_tree ? (uint32_t)(mine[t] >> key0) : (1u << (sq.len - key0)) - 1u;
-    block<T, DP, RT, EXACT, true>(w, (const uint16_t*)kv.k + at, (const uint16_t*)kv.v + at, kv.slot_stride, key0, limit, a.head_dim,
-                                  cut.scale, on, in_tree);
+      for (int t = 0; t < RT; t++)
+        on[t] = in_tree ? (uint32_t)(mine[t] >> key0) : sq.len - key0 >= KB ? ~0u : (1u << (sq.len - key0)) - 1u;
+      block<T, DP, RT, EXACT, true>(w, (const uint16_t*)kv.k + at, (const uint16_t*)kv.v + at, kv.slot_stride, key0, limit, a.head_dim,
+                                    cut.scale, on, pass);
+    }
+  };
+  rest(i, std::integral_constant<int, WALK>{});
+  uint32_t* marked = (uint32_t*)&sum[wave] + lane;
+  if (!finished(w, WALK, mine, marked)) [[unlikely]] {
+    int pass = ABOVE;
+#pragma unroll 1
+    do rest(first + wave, pass);
+    while (!finished(w, pass++, mine, marked));
   }
 
   // the waves' sums, brought to one reference; rows that see nothing of the
   // tree see nothing of the cache either
   float ref[RT];
-  if (lane == 0) odds[wave] = w.odd;
 #pragma unroll
   for (int t = 0; t < RT; t++) {
     w.l[t] = row_sum(w.l[t]);
@@ -109,13 +118,12 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
     for (int j = 0; j < NW; j++) top = fmaxf(top, stat[j][t][0][x]);
     const float f = ref[t] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f((ref[t] - top) * mag);
 #pragma unroll
-    for (int k = 0; k < S::NF; k++) sum[wave][t][k][lane] = ref[t] == NEG_INF ? (f32x4){0.0f, 0.0f, 0.0f, 0.0f} : w.o[t][k] * f;
+    for (int k = 0; k < S::NF; k++) sum[wave][t][k][lane] = times(w.o[t][k], f);
   }
   __syncthreads();
   // a wave takes every fourth pair of fragments
   constexpr int PAIRS = S::VE / 2;
   const bool whole = first == 0 && last == total;
-  const int odd = odds[0] | odds[1] | odds[2] | odds[3];
   float* part = cut.part + (((int64_t)bh * cut.nsplit + split) * cut.tiles + tile) * S::PART;
 #pragma unroll 1
   for (int u = wave; u < RT * S::VH * PAIRS; u += NW) {
@@ -132,7 +140,7 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
       o[1] += sum[j][t][f0 + 1][lane];
     }
     if (whole) {
-      store_pair<T, DP>(a, cut.G, b, kh, row0 + 16 * t + x, R, h, pair, o[0], o[1], top, all, odd, sq.n);
+      store_pair<T, DP>(a, cut.G, b, kh, row0 + 16 * t + x, R, h, pair, o[0], o[1], top, all);
     } else {
       f32x4* p = (f32x4*)part + (t * S::NF + f0) * 64 + lane;
       p[0] = o[0];
@@ -140,7 +148,6 @@ __global__ __launch_bounds__(64 * NW, DP * RT <= 64 ? 4 : DP * RT <= 128 ? 3 : D
       if (h == 0 && pair == 0 && g == 0) {
         part[S::STAT + 32 * t + x] = top;
         part[S::STAT + 32 * t + 16 + x] = all;
-        part[S::ODD] = odd ? 1.0f : 0.0f;
       }
     }
   }
@@ -172,6 +179,7 @@ __global__ __launch_bounds__(64 * NW, 1) void attend_wide_kernel(const xs_tree_a
   using G = Stage<DP>;
   __shared__ u32x4 lk[3][G::SK * G::CH];
   __shared__ u32x4 lv[3][G::SK * G::CH];
+  __shared__ uint32_t marks[NW][2 * S::MARKS][64];
   const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wgs = cut.tiles / NW;  // workgroups of a split: NW tiles each
@@ -326,20 +334,29 @@ __global__ __launch_bounds__(64 * NW, 1) void attend_wide_kernel(const xs_tree_a
     if (row >= R) mine[t] = 0;
   }
   if (row0 >= R) return;
+  auto rest = [&](int i, auto pass) __attribute__((always_inline)) {
 #pragma unroll 1
-  for (int i = first + stages * SB; i < last; i++) {
-    const bool in_tree = i >= cached;
-    const int key0 = (in_tree ? i - cached : i) * KB, limit = in_tree ? sq.n : sq.len;
-    const xs_kv& kv = in_tree ? a.fresh : a.cache;
-    const int64_t at = b * kv.seq_stride + kh * kv.head_stride;
-    uint32_t on[RT];
+    for (; i < last; i++) {
+      const bool in_tree = i >= cached;
+      const int key0 = (in_tree ? i - cached : i) * KB, limit = in_tree ? sq.n : sq.len;
+      const xs_kv& kv = in_tree ? a.fresh : a.cache;
+      const int64_t at = b * kv.seq_stride + kh * kv.head_stride;
+      uint32_t on[RT];
 #pragma unroll
-    for (int t = 0; t < RT; t++)
-      on[t] = in_tree ? (uint32_t)(mine[t] >> key0) : sq.len - key0 >= KB ? ~0u : (1u << (sq.len - key0)) - 1u;
-    block<T, DP, RT, EXACT, true>(w, (const uint16_t*)kv.k + at, (const uint16_t*)kv.v + at, kv.slot_stride, key0, limit, a.head_dim,
-                                  cut.scale, on, in_tree);
+      for (int t = 0; t < RT; t++)
+        on[t] = in_tree ? (uint32_t)(mine[t] >> key0) : sq.len - key0 >= KB ? ~0u : (1u << (sq.len - key0)) - 1u;
+      block<T, DP, RT, EXACT, true>(w, (const uint16_t*)kv.k + at, (const uint16_t*)kv.v + at, kv.slot_stride, key0, limit, a.head_dim,
+                                    cut.scale, on, pass);
+    }
+  };
+  rest(first + stages * SB, std::integral_constant<int, WALK>{});
+  uint32_t* marked = &marks[wave][0][lane];
+  if (!finished(w, WALK, mine, marked)) [[unlikely]] {
+    int pass = ABOVE;
+#pragma unroll 1
+    do rest(first, pass);
+    while (!finished(w, pass++, mine, marked));
   }
-  constexpr int PAIRS = S::VE / 2;
   const bool whole = first == 0 && last == total;
   float* part = cut.part + (((int64_t)bh * cut.nsplit + split) * cut.tiles + tile) * S::PART;
 #pragma unroll
@@ -350,23 +367,15 @@ __global__ __launch_bounds__(64 * NW, 1) void attend_wide_kernel(const xs_tree_a
 #pragma unroll
     for (int f = 0; f < S::NF; f++)
       if (l == 0.0f) w.o[t][f] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    if (whole && !w.odd) {
+    if (whole) {
 #pragma unroll
       for (int h = 0; h < S::VH; h++) store_half<T, DP, RT>(a, cut.G, b, kh, row0 + 16 * t + x, R, h, w.o[t], ref, l);
-    } else if (whole) {
-#pragma unroll
-      for (int h = 0; h < S::VH; h++)
-#pragma unroll
-        for (int pair = 0; pair < PAIRS; pair++)
-          store_pair<T, DP>(a, cut.G, b, kh, row0 + 16 * t + x, R, h, pair, w.o[t][h * S::VE + 2 * pair], w.o[t][h * S::VE + 2 * pair + 1], ref,
-                            l, w.odd, sq.n);
     } else {
 #pragma unroll
       for (int f = 0; f < S::NF; f++) ((f32x4*)part)[(t * S::NF + f) * 64 + lane] = w.o[t][f];
       if (g == 0) {
         part[S::STAT + 32 * t + x] = ref;
         part[S::STAT + 32 * t + 16 + x] = l;
-        part[S::ODD] = w.odd ? 1.0f : 0.0f;
       }
     }
   }
