@@ -521,7 +521,7 @@ XS_DEV void store_pair(const xs_tree_attend_args& a, int G, int b, int kh, int r
 
 // All fragments of half h, VE elements of each r at a time (pairs of 4 bytes
 // instead: 19 us of a workgroup's 58 where 32 sequences of 500 slots have 256 rows each).
-template <typename T, int DP, int RT, typename W = T>
+template <typename T, int DP, int RT>
 XS_DEV void store_half(const xs_tree_attend_args& a, int G, int b, int kh, int row, int R, int h, const f32x4 (&o)[Shape<DP, RT>::NF], float ref,
                        float l) {
   constexpr int VE = Shape<DP, 1>::VE;
@@ -535,13 +535,13 @@ XS_DEV void store_half(const xs_tree_attend_args& a, int G, int b, int kh, int r
     const int d = 128 * h + VE * (4 * g + r);
     uint32_t y[VE / 2];
 #pragma unroll
-    for (int i = 0; i < VE / 2; i++) y[i] = pack2(T{}, ended<T, W>(o[h * VE + 2 * i][r] * inv), ended<T, W>(o[h * VE + 2 * i + 1][r] * inv));
+    for (int i = 0; i < VE / 2; i++) y[i] = pack2(T{}, within(T{}, o[h * VE + 2 * i][r] * inv), within(T{}, o[h * VE + 2 * i + 1][r] * inv));
     if (d < a.head_dim) {
       if constexpr (VE == 8) *(u32x4*)(out + d) = (u32x4){y[0], y[1], y[2], y[3]};
       else *(u32x2*)(out + d) = (u32x2){y[0], y[1]};
     }
   }
-  if (a.lse && h == 0 && g == 0) a.lse[(b * a.nodes + node) * a.q_heads + head] = lse_of<W>(a, ref, l);
+  if (a.lse && h == 0 && g == 0) a.lse[(b * a.nodes + node) * a.q_heads + head] = lse_of<T>(a, ref, l);
 }
 
 // Joins the splits of 16 rows and one half of the head: each wave two
@@ -556,7 +556,7 @@ constexpr int join_shares(bool few) { return few ? 1 : 16 / (Shape<DP, 1>::VE / 
 template <int DP>
 constexpr int join_threads(bool few) { return 64 * (Shape<DP, 1>::VE / 2) * join_shares<DP>(few); }
 
-template <typename T, int DP, int RT, bool FEWER, typename W = T>
+template <typename T, int DP, int RT, bool FEWER>
 __global__ __launch_bounds__(join_threads<DP>(FEWER)) void join_kernel(const xs_tree_attend_args a, const Cut cut) {
   using S = Shape<DP, RT>;
   constexpr int PAIRS = S::VE / 2, SHARES = join_shares<DP>(FEWER), WAVES = PAIRS * SHARES;
@@ -638,7 +638,7 @@ __global__ __launch_bounds__(join_threads<DP>(FEWER)) void join_kernel(const xs_
       o[1] += sum[j][2 * pair + 1][lane];
     }
   }
-  store_pair<T, DP, W>(a, cut.G, b, kh, row0 + x, R, h, pair, o[0], o[1], top, all);
+  store_pair<T, DP>(a, cut.G, b, kh, row0 + x, R, h, pair, o[0], o[1], top, all);
 }
 
 }  // namespace xst
