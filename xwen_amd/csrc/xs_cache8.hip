@@ -839,7 +839,6 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend8_wide_kernel
   constexpr int N = Parts<T>::N, CH = K::CH, KC = DP / 16, DT = DP / 32, TH = 64 * W;
   constexpr int PER = SK * (DP / 16) / TH;  // 16-byte pieces of the cache that a thread moves, of k and of v
   static_assert(SK * (DP / 16) % TH == 0, "a stage is whole pieces of every thread");
-  constexpr int NE = PER < SK / KB ? PER : SK / KB;  // a thread's exponents: its pieces j of PER / NE lie in one block
   __shared__ u32x4 lk[2][K::STAGE];
   __shared__ u32x4 lv[2][K::STAGE];
   __shared__ uint16_t marks[2][DT][TH];  // [above, below] a lane's elements that an infinity reaches
@@ -905,10 +904,11 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend8_wide_kernel
     const Reads<DP> reads(lane);
 
     u32x4 rk[PER], rv[PER];
-    uint32_t ek[NE], ev[NE];
+    uint32_t ex;  // a stage's exponents: of the keys' two blocks, then of the values', by lane & 3
     auto fetch = [&](int s) {
       const int64_t base = at + (int64_t)s * SK * c8.slot_stride;
       const int most = len - 1 - s * SK;
+      ex = ((lane & 2) ? c8.v_exp : c8.k_exp)[eat + min(s * (SK / KB) + (lane & 1), (len - 1) / KB)];
 #pragma unroll
       for (int j = 0; j < PER; j++) {
         const int p = j * TH + tid, r = min(p / (DP / 16), most), c = p % (DP / 16);
@@ -916,10 +916,6 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend8_wide_kernel
         const bool in = EXACT || 16 * c < a.head_dim;
         rk[j] = in ? *(const u32x4*)(c8.k + base + off) : (u32x4){0, 0, 0, 0};
         rv[j] = in ? *(const u32x4*)(c8.v + base + off) : (u32x4){0, 0, 0, 0};
-        if (j % (PER / NE) == 0) {
-          ek[j / (PER / NE)] = c8.k_exp[eat + s * (SK / KB) + r / KB];
-          ev[j / (PER / NE)] = c8.v_exp[eat + s * (SK / KB) + r / KB];
-        }
       }
     };
     auto put = [&](int s) {
@@ -927,7 +923,9 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend8_wide_kernel
 #pragma unroll
       for (int j = 0; j < PER; j++) {
         const int p = j * TH + tid, r = p / (DP / 16), c = p % (DP / 16);
-        const float ks = pow2((int)ek[j / (PER / NE)] - 127), vs = pow2((int)ev[j / (PER / NE)] - 127);
+        // (a wave's pieces j lie in one block)
+        const int block = PER > 1 ? j * (TH / (DP / 16)) / KB : __builtin_amdgcn_readfirstlane(r / KB);
+        const float ks = pow2(__builtin_amdgcn_readlane((int)ex, block) - 127), vs = pow2(__builtin_amdgcn_readlane((int)ex, 2 + block) - 127);
         const u32x4 y = r <= most ? rv[j] : (u32x4){0, 0, 0, 0};  // (past the length: nothing, whatever it holds)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
