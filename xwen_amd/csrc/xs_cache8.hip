@@ -969,6 +969,7 @@ __global__ __launch_bounds__(64 * W, DP <= 128 ? 2 : 1) void attend8_wide_kernel
 #pragma unroll 1
     for (int s = first; s < end; s++) {
       __syncthreads();
+      if constexpr (N == 2) asm volatile("" : "+v"(tid));  // (its addresses, formed anew, need no registers)
       if (s + 1 < end) put(s + 1);
       if (s + 2 < end) fetch(s + 2);
       const int limit = len - s * SK;
