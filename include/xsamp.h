@@ -570,12 +570,14 @@ int xs_cache_evict(xs_cache_context* ctx, const xs_cache_evict_args* args);
 
 /* Norms and positions of queries and keys, each head of each token on its own:
  *   y = x / sqrt(mean(x^2) + eps) * weight   (weights NULL: y = x)
+ * (elements of any size: their squares may pass f32),
  * and of y the first rot_dim elements in pairs (a, b), i < rot_dim / 2:
  *   (a cos t - b sin t, b cos t + a sin t),  t = pos * inv_freq[i]
  * with (a, b) elements i and i + rot_dim / 2 (XS_ROT_HALVES) or 2 i and 2 i + 1
  * (XS_ROT_NEIGHBOURS).  Angles are formed in f64 (any int32 position), the rest
  * in f32, rounded once.  An output may be its input itself (same strides), and
- * overlaps no other input or output. */
+ * overlaps no other input or output.  Either side has at most 65,536 heads
+ * (XS_ERR_CAPACITY). */
 #define XS_ROT_HALVES 0
 #define XS_ROT_NEIGHBOURS 1
 typedef struct {
@@ -612,8 +614,9 @@ int xs_qk_rotate(xs_cache_context* ctx, const xs_qk_rotate_args* args);
  * it holds.  A sequence may be empty.  One whose start lies below 0 or below an
  * earlier entry of start, or whose end lies below its start or past `tokens`,
  * gets XS_ROW_BAD_PARAM and nothing else; rows of no sequence are left as they
- * were.  kv_token_stride is at most 2^24, a kv head's rows (tokens times its
- * q heads) at most 2^30 (XS_ERR_CAPACITY). */
+ * were.  There are at most 65,536 sequences and 4,096 q heads, kv_token_stride
+ * is at most 2^24, a kv head's rows (tokens times its q heads) at most 2^30
+ * (XS_ERR_CAPACITY).  A sequence sees its own tokens of this call only, no cache. */
 typedef struct {
   int32_t dtype;         /* XS_BF16 or XS_F16: q, k, v and out */
   int32_t head_dim;      /* a multiple of 8, 8..256 */
@@ -638,7 +641,7 @@ int xs_prompt_attend(xs_cache_context* ctx, const xs_prompt_attend_args* args);
  * fraction, largest 448, no infinities), [seqs, slots, kv_heads, head_dim] like
  * xs_kv with strides in bytes, multiples of 16.  Every XS_CACHE8_BLOCK slots of
  * a head share a power of two, for keys and for values: element = byte * 2^e,
- * with e + 127 held in a byte of k_exp or v_exp [seqs, kv_heads, exp_ld].  The
+ * with e + 127, of 1 to 254, held in a byte of k_exp or v_exp [seqs, kv_heads, exp_ld].  The
  * exponents of blocks that hold no slot in use need no values. */
 #define XS_CACHE8_BLOCK 32
 typedef struct {
@@ -691,7 +694,8 @@ int xs_cache_append8(xs_cache_context* ctx, const xs_cache_append8_args* args);
  * (fresh) are in the inputs' type.  Weights are rounded to bf16 where q is bf16;
  * where it is f16, to the sum of two bf16 (16 bits), since an element of the
  * cache may pass f16's range (and a mean of such elements f16's end: an
- * infinity then).  slot_stride is at most 2^25 (XS_ERR_CAPACITY). */
+ * infinity then; a key's element held as 2^128 may make the scores of an f16 row
+ * NaN).  slot_stride is at most 2^25 (XS_ERR_CAPACITY). */
 typedef struct {
   int32_t dtype;         /* XS_BF16 or XS_F16: q, fresh and out */
   int32_t head_dim;      /* a multiple of 16, 16..256 */

@@ -5,7 +5,8 @@ Elements are e4m3 (torch.float8_e4m3fn) times a power of two that BLOCK slots of
 share, its exponent + 127 in a uint8.  Cache8 holds one layer's buffers and makes the
 calls of a sequence's life: prompt() attends a prompt to itself and appends it; per step
 attend() is the draft tree's attention and commit() appends the accepted path.  It takes
-half of tree.TreeCache's bytes and keeps every token (nothing is evicted).
+half of tree.TreeCache's bytes and keeps every token (nothing is evicted).  A prompt sees
+nothing of the cache: one that continues a sequence is not for prompt().
 
 Calls run on torch's current stream and are asynchronous; statuses are device tensors,
 raised by tree.check().
@@ -133,8 +134,11 @@ class Cache8:
     def prompt(self, q, k, v, start, *, scale: float | None = None, max_len: int = 0,
                out: PromptAttended | None = None) -> PromptAttended:
         """Prompts packed as prompt_attend takes them: their attention, each to itself (in 16
-        bits), and their keys and values appended.  max_len: a bound on the prompts' lengths (0:
-        none; it sizes the append's launch)."""
+        bits), and their keys and values appended.  What a sequence's cache holds already is not
+        attended to: a second turn, a shared prefix or a part of a prompt after the first gets
+        the attention of a text of its own.  max_len: a bound on the prompts' lengths (0: none; it
+        sizes the append's launch, and a longer prompt is attended but not appended:
+        append_status)."""
         a = prompt_attend(self.ctx, q, k, v, start, scale=scale, out=out)
         self._append(k, v, start=start, rows=max_len)
         return a

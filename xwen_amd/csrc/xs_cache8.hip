@@ -179,8 +179,8 @@ __global__ __launch_bounds__(AB) void append_kernel(const xs_cache_append8_args 
 // A lane loads 16 bytes of a key: elements 64 c + 16 g + 8 h .. + 8 are chunk
 // 2 c + h of the products, for queries and fresh keys too.  Bound by the one read
 // of the cache up to 16 rows a head: decoding 32 sequences of 327 to 8,192 slots, 8
-// kv heads of 128 (302 MB), 81 us, of which the join of the splits takes 5; without
-// starts and ends the keys come at 5.2 to 5.9 TB/s.
+// kv heads of 128 (302 MB), 77 to 80 us by card, of which the join of the splits takes
+// 5; without starts and ends the keys come at 5.2 to 5.9 TB/s.
 
 struct E4m3 {};  // (weights carry no power of two)
 XS_DEV constexpr float offset_of(E4m3) { return 0.0f; }
@@ -437,10 +437,12 @@ XS_DEV void tree_block(Tile<T, DP, RT>& z, const uint16_t* kp, const uint16_t* v
 // How a call is cut.  The keys are counted in units (blocks of 32, stages of 64),
 // and a sequence of u units is split in u / share of them, rounded up.  The share
 // is one for all sequences, so that long and short ones' workgroups end together:
-// the smallest that leaves no more splits than the device holds at once, `room`
-// for each head and row tile, so that no workgroup starts when the others end (as
-// many splits for every sequence instead, 32 of 327 to 8,192 slots: 87 us for
-// 81).  The lengths are on the device, so every workgroup finds the share and
+// the smallest that leaves no more splits than `room` for each head and row tile:
+// as many as the device holds at once, so that no workgroup starts when the others
+// end (as many splits for every sequence instead, 32 of 327 to 8,192 slots: 87 us for
+// 81), but no more than a join takes of one sequence (SPLITS: of one kv head of 128,
+// single rows then fill a third of the device) or than the context has partial
+// results for.  The lengths are on the device, so every workgroup finds the share and
 // its place among the sequences itself.
 struct Cut8 {
   int32_t G, tiles, units, room;  // units: (sequence, split) that the launch has; room 0: nothing is split
@@ -804,9 +806,9 @@ __global__ __launch_bounds__((join8_threads<DP, SHARES>())) void join8_kernel(co
 // a stage's keys, and add up at the end; 32 W / WK rows a workgroup of W waves.  Bound
 // by the products and the vector work beside them (xs_rows32.h), the widening among
 // it, which eight waves share where rows fill them (four, two workgroups a CU: 181
-// us for 170): 8 x 64 nodes of 32 q and 8 kv heads of 128 over 16,384 slots 157 to
-// 170 us by card (880 to 810 TFLOP/s), of which the join takes 12.  By memory where
-// rows are few: 16 nodes over 131,072 slots 76 to 82 us (3.5 to 3.3 TB/s).  The
+// us for 170): 8 x 64 nodes of 32 q and 8 kv heads of 128 over 16,384 slots 160 to
+// 187 us by card (856 to 733 TFLOP/s), of which the join takes 12.  By memory where
+// rows are few: 16 nodes over 131,072 slots 72 to 88 us (3.7 to 3.1 TB/s).  The
 // 16-row kernel with four row tiles instead takes 721 and 216 us: its waves widen
 // every key for 64 rows each.
 template <int DP, int WK, int W>

@@ -28,7 +28,7 @@ using namespace xst;
 // RT / LPH heads in a row (tokens outermost, a token's q heads before its kv
 // heads), a pass's pieces on their way while the last one is worked on; the
 // angles of its tokens, and the weights, are in LDS.  Bound by the one read and
-// write of the heads: 16,384 tokens of 40 heads of 128 (336 MB) in 80 us.
+// write of the heads: 16,384 tokens of 40 heads of 128 (336 MB) in 80 to 86 us by card.
 // All passes' pieces in registers at once take 204 of them, which leaves two
 // waves a SIMD: 186 us.
 
@@ -196,10 +196,11 @@ __global__ __launch_bounds__(RT, 8) void rotate_kernel(const xs_qk_rotate_args a
 // Bound by the matrix cores and the vector units beside them: a stage of a wave at
 // head size 128 is 32 products of 32 cycles and some 900 cycles of vector work
 // (32 exponentials of 16, then scaling, sums, packing), which two waves a SIMD lay
-// side by side: the products run 64 % of the time at the clock that the power
-// leaves (1.8 GHz).  A prompt of 16,384 tokens, 32 q and 8 kv heads of 128: 1,900
-// to 2,000 us by card (1,157 to 1,100 TFLOP/s; a large library product reaches 1,334
-// to 1,366); 16 prompts of 164 to 4,096: 957 to 1,048 us (964 to 880 TFLOP/s).  One wave's
+// side by side: the products run 62 to 64 % of the time at the clock that the power
+// leaves (1.8 GHz).  A prompt of 16,384 tokens, 32 q and 8 kv heads of 128: 1,870
+// to 2,080 us by card (1,176 to 1,057 TFLOP/s; a large library product reaches 1,334
+// to 1,366); 16 prompts of 164 to 4,096: 944 to 1,054 us (977 to 875 TFLOP/s).
+// With NaN among the values, walked for again, 4.9 times as long.  One wave's
 // exponentials laid by hand beside its own next products, scores of two stages in
 // registers, spills: 2,346 us.
 
