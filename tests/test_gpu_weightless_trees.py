@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from tests import treeref
-from tests.test_gpu_cache8 import empty_cache, look, put, step
+from tests.test_gpu_cache8 import empty_cache, filled, look, put, step
 from tests.test_gpu_tree_attend import blank, case, run
 from tests.test_gpu_weightless_values import BF, HF, INF, LOWS, agree, definition, spoil
 
@@ -109,3 +109,46 @@ def test_trees_over_8_bits(ctx, nodes, group, d, dtype, low):
         x = c[n].double() * torch.exp2(e.double())
         held.append(torch.where(x.abs() >= 2.0**128, torch.copysign(torch.full_like(x, INF), x), x))
     check_trees(got, s["q"], *held, LENS, s["fk"], s["fv"], s["parent"], s["used"])
+
+
+@pytest.mark.parametrize("nodes,group,d", [(5, 3, 64), (12, 4, 128), (24, 4, 128), (50, 4, 256)])
+def test_rows_of_nan_beside(ctx, nodes, group, d):
+    """A NaN query's row, and rows whose masked tokens' values are not finite, in one tile."""
+    rng = np.random.default_rng(nodes)
+    g = torch.Generator().manual_seed(nodes)
+    c = case(rng, LENS, nodes, 2 * group, 2, d, BF)
+    masked_nodes(c, "v", -INF, g)
+    c["q"][:, nodes // 2, 1, 5] = math.nan
+    got = run(ctx, c, out=blank(c))
+    check_trees(got, c["q"], c["k"], c["v"], LENS, c["fk"], c["fv"], c["parent"], c["used"])
+
+
+@pytest.mark.parametrize("nodes,group", [(1, 4), (12, 4), (50, 4)])
+def test_a_graph_replays_with_values_that_come_and_go(ctx, nodes, group):
+    """Captured with finite values; replayed with NaN and infinities in the cache, then without."""
+    from xwen_amd import cache8, tree
+    rng = np.random.default_rng(nodes)
+    c = filled([4000, 70], 2, 128, seed=nodes)
+    s = step(rng, c, nodes, 2 * group, BF)
+    s["q"][..., 0], s["fk"][..., 0] = 1.0, 0.0
+    clean = look(ctx, c, s)
+    out = tree.Attended(*(torch.zeros_like(t) for t in (clean.out, clean.lse, clean.seq_status)))
+    parent = s["parent"].cuda()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache8.tree_attend8(ctx, s["q"], c["k"], c["v"], c["k_exp"], c["v_exp"], c["len"], s["fk"], s["fv"], parent, out=out)
+    fine = c["v"].view(torch.uint8).clone()
+    for i in range(4):
+        c["v"].view(torch.uint8).copy_(fine)
+        s["fv"][:, 0, :, 3] = (math.nan, 1.0, -INF, 1.0)[i]
+        if i % 2 == 0:
+            c["v"].view(torch.uint8)[:, 33, :, 7] = 127
+        out.out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = look(ctx, c, s)
+        same = (out.out == want.out) | (out.out.isnan() & want.out.isnan())
+        assert bool(same.all()) and torch.equal(out.lse, want.lse)
+        assert bool(torch.isnan(out.out[0, 0, :, 7]).all()) == (i % 2 == 0) and bool(torch.isfinite(out.out[0, 0, :, 20]).all())
+        torch.cuda.synchronize()
